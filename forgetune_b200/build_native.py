@@ -11,9 +11,12 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
+import time
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
@@ -21,6 +24,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libforgetune_b200.so")
+OBJ_DIR = os.path.join(LIB_DIR, "obj")
 
 SOURCES = ["runtime.cu", "engine.cpp"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -33,33 +37,65 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found (set NVCC or put CUDA on PATH)")
 
 
-def _inputs():
-    files = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".cpp", ".hpp", ".h"))]
-    files.append(os.path.join(INCLUDE, "forgetune_b200.h"))
+def _inputs(source=None):
+    """The source (default: all sources) and every project header it includes, transitively."""
+    todo = [os.path.join(CSRC, s) for s in ([source] if source else SOURCES)]
+    files = []
+    while todo:
+        path = todo.pop()
+        if path in files:
+            continue
+        files.append(path)
+        with open(path, encoding="utf-8") as f:
+            for name in re.findall(r'^\s*#include\s+"([^"]+)"', f.read(), re.M):
+                for d in (CSRC, INCLUDE):
+                    if os.path.isfile(os.path.join(d, name)):
+                        todo.append(os.path.join(d, name))
     return files
 
 
-def up_to_date() -> bool:
-    if not os.path.isfile(LIB_PATH):
+def _newer(target, files) -> bool:
+    if not os.path.isfile(target):
         return False
-    t = os.path.getmtime(LIB_PATH)
-    return all(os.path.getmtime(f) <= t for f in _inputs())
+    t = os.path.getmtime(target)
+    return all(os.path.getmtime(f) <= t for f in files)
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
-        return LIB_PATH
-    os.makedirs(LIB_DIR, exist_ok=True)
-    tmp = LIB_PATH + ".tmp%d" % os.getpid()
-    cmd = [nvcc(), "-std=c++17", "-O3", "-lineinfo"] + ARCH_FLAGS + [
-        "-I", INCLUDE, "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
-        "-o", tmp] + [os.path.join(CSRC, s) for s in SOURCES]
+def up_to_date() -> bool:
+    return _newer(LIB_PATH, _inputs())
+
+
+def _run(cmd, target, verbose) -> None:
+    """Run ``cmd`` + ["-o", file] and put the file in place of ``target``, dated when the command began: an
+    input edited meanwhile stays newer."""
+    began = time.time()
+    tmp = target + ".tmp%d" % os.getpid()
+    cmd = cmd + ["-o", tmp]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("nvcc failed (%d):\n%s\n%s" % (r.returncode, r.stdout[-4000:], r.stderr[-8000:]))
-    os.replace(tmp, LIB_PATH)
+    os.utime(tmp, (began, began))
+    os.replace(tmp, target)
+
+
+def _compile(source, force, verbose) -> str:
+    obj = os.path.join(OBJ_DIR, source + ".o")
+    if force or not _newer(obj, _inputs(source)):
+        _run([nvcc(), "-std=c++17", "-O3", "-lineinfo"] + ARCH_FLAGS + [
+            "-I", INCLUDE, "-Xcompiler", "-fPIC,-fvisibility=hidden", "-c", os.path.join(CSRC, source)], obj, verbose)
+    return obj
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile what changed (the sources side by side) and link the library."""
+    if not force and up_to_date():
+        return LIB_PATH
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        objs = list(pool.map(lambda s: _compile(s, force, verbose), SOURCES))
+    _run([nvcc()] + ARCH_FLAGS + ["-shared"] + objs, LIB_PATH, verbose)
     return LIB_PATH
 
 

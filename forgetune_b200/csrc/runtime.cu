@@ -30,41 +30,18 @@
 #include "philox.cuh"
 #include "simt_gemm.cuh"
 #include "splitk_gemv.cuh"
+#include "status.hpp"
 #include "tc_pair_gemm.cuh"
 #include "tc_mlp_pair.cuh"
 #include "chain_gemv.cuh"
 #include "tc_conv.cuh"
 #include "narrow_gemm.cuh"
 
-#define FTB_API extern "C" __attribute__((visibility("default")))
-
 namespace ftb {
-
-// ---------------------------------------------------------------------------
-// status codes (include/forgetune_b200.h)
-// ---------------------------------------------------------------------------
-enum Status : int {
-  ST_OK = 0,
-  ST_NULL = -1,
-  ST_INPUT = -2,
-  ST_OUTPUT = -3,
-  ST_ALLOC = -4,
-  ST_DEVICE = -5,
-  ST_CONFIG = -6,
-};
 
 static thread_local std::string t_last_error;
 
-static void set_error(const std::string& s) { t_last_error = s; }
-
-#define CUDA_TRY(expr)                                                                 \
-  do {                                                                                 \
-    cudaError_t _e = (expr);                                                           \
-    if (_e != cudaSuccess) {                                                           \
-      set_error(std::string(#expr) + ": " + cudaGetErrorString(_e));                  \
-      return ST_DEVICE;                                                                \
-    }                                                                                  \
-  } while (0)
+void set_error(const std::string& s) { t_last_error = s; }
 
 struct DeviceGuard {
   int prev = -1;

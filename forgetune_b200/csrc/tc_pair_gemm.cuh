@@ -36,73 +36,6 @@
 
 namespace ftb {
 
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t cluster_index() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t cluster_count() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%nclusterid.x;" : "=r"(r));
-  return r;
-}
-
-// shared::cluster address of the shared variable `p` in CTA `rank` of this cluster
-__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
-
-// Arrive on an mbarrier of this CTA or the peer (default release semantics,
-// as for a local arrive: what the arrival publishes to the pair's MMAs is
-// shared memory already made visible to the async proxy by
-// fence.proxy.async).
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t caddr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
-}
-
-__device__ __forceinline__ void st_cluster_u32(uint32_t caddr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(caddr), "r"(v) : "memory");
-}
-
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// Bounded wait (arrivals may come from the peer CTA).  On timeout it raises
-// this CTA's and the peer's abort flags.
-__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t peer_abort,
-                                          int* err, int code, bool ignore_abort = false) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
-  for (uint32_t it = 1;; ++it) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 255u) == 0) {
-      if (!ignore_abort && *abort_flag) return false;
-      if (global_ns() - t0 > kTcWaitLimitNs) {
-        *abort_flag = 1;
-        st_cluster_u32(peer_abort, 1u);
-        atomicCAS(err, 0, code);
-        return false;
-      }
-    }
-  }
-}
-
-__device__ __forceinline__ bool pair_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                               uint32_t peer_abort, int* err, int code, bool ignore_abort = false) {
-  const bool ok = pair_wait(bar, parity, abort_flag, peer_abort, err, code, ignore_abort);
-  return __all_sync(0xffffffffu, ok);
-}
-
 // D[256 x N] (+)= A[256 x 8] B[8 x N] over the SM pair, tf32 operands from
 // the shared memory of both CTAs at the same offsets.
 __device__ __forceinline__ void umma2_tf32(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -112,13 +45,6 @@ __device__ __forceinline__ void umma2_tf32(uint32_t d_tmem, uint64_t a, uint64_t
       "tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
-}
-
-// Arrive once on the mbarrier at shared::cluster address `caddr` (this CTA's
-// or the peer's) when every MMA this thread issued so far has completed.
-__device__ __forceinline__ void umma2_commit(uint32_t caddr) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(caddr)
-               : "memory");
 }
 
 // Instruction descriptor: D f32, A/B tf32, both K-major, M=256, N=n (a
