@@ -26,7 +26,7 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libforgetune_b200.so")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 
-SOURCES = ["runtime.cu", "engine.cpp"]
+SOURCES = ["runtime.cu", "fp8.cu", "engine.cpp"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,336 @@
+"""Block-scaled 8-bit operators on CUDA tensors.
+
+A dense layer in 8 bits is a chain of three operators, each one call of the
+engine library's C ABI (``ftb_quantize_rows``, ``ftb_quantize_weight``,
+``ftb_rms_norm``, ``ftb_fp8_linear``; include/forgetune_b200.h) on the current
+torch stream::
+
+    w1 = quantize_weight(layer1.weight)                 # once, [n, k]
+    h, res = rms_norm(x, norm.weight, residual=res, quantize=True)
+    h = fp8_linear(h, w1, bias=layer1.bias, relu=True, quantize=True)
+    x = fp8_linear(h, w2, bias=layer2.bias)
+
+The format is e4m3 values with one power-of-two scale (ue8m0, the format the
+tensor cores take) for each block of 128 along a row of activations and for
+each 128 x 128 block of a weight: the smallest power of two with
+``max|x| / scale <= 448``, 1 for a block of zeros.  Values that are not finite
+are stored as NaN.  Products are accumulated in fp32.
+
+Inputs are 2-D; a plain input whose rows are not contiguous is copied first,
+as ``CompiledModel.run_device`` does.  The operators are for inference: they
+return tensors without gradients.  The first call on a device sets it up, so
+make it before capturing a CUDA graph.  The reference has no counterpart (its
+models are float32 only).
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _native
+from .errors import ForgeTuneRuntimeError, InvalidShapeError
+
+__all__ = ["Fp8Rows", "Fp8Weight", "quantize_rows", "quantize_weight", "rms_norm", "fp8_linear"]
+
+BLOCK = 128
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # FTB_F32, FTB_F16, FTB_BF16
+_FTB_E4M3 = 3
+_FP8_RELU = 1
+
+
+def _blocks(n: int) -> int:
+    return (n + BLOCK - 1) // BLOCK
+
+
+def _rows(shape, unit: int, dtype, device) -> torch.Tensor:
+    """An uninitialised matrix whose rows start on multiples of ``unit`` elements."""
+    ld = (shape[1] + unit - 1) // unit * unit
+    return torch.empty_strided(shape, (ld, 1), dtype=dtype, device=device)
+
+
+class _Fp8:
+    """8-bit values [rows, k] with their block scales."""
+
+    __slots__ = ("data", "scales")
+    _row_block = 1
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        name = type(self).__name__
+        if not (isinstance(data, torch.Tensor) and data.dtype == _E4M3):
+            raise TypeError("%s: data must be a torch.float8_e4m3fn tensor" % name)
+        if not (isinstance(scales, torch.Tensor) and scales.dtype == _E8M0):
+            raise TypeError("%s: scales must be a torch.float8_e8m0fnu tensor" % name)
+        if data.dim() != 2 or data.shape[1] < 1:
+            raise InvalidShapeError("%s: data must be [rows, k] with k >= 1, got %s" % (name, tuple(data.shape)))
+        b = self._row_block
+        want = ((data.shape[0] + b - 1) // b, _blocks(data.shape[1]))
+        if tuple(scales.shape) != want:
+            raise InvalidShapeError("%s: scales of data %s must be %s, got %s"
+                                    % (name, tuple(data.shape), want, tuple(scales.shape)))
+        if data.device != scales.device:
+            raise ValueError("%s: data and scales are on different devices" % name)
+        self.data = data
+        self.scales = scales
+
+    @classmethod
+    def pack(cls, data: torch.Tensor, scales: torch.Tensor):
+        """The same values in rows laid out as the operators need them (copied where they are not)."""
+        r = cls(data, scales)
+        if _ld8(r.data, 16) is None:
+            r.data = _rows(data.shape, 16, _E4M3, data.device).copy_(data)
+        if _ld8(r.scales, 4) is None:
+            r.scales = _rows(scales.shape, 4, _E8M0, scales.device).copy_(scales)
+        return r
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.data.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values the blocks stand for."""
+        rows, k = self.data.shape
+        f = self.scales.float().repeat_interleave(BLOCK, 1)[:, :k]
+        if self._row_block > 1:
+            f = f.repeat_interleave(self._row_block, 0)[:rows]
+        return (self.data.float() * f).to(dtype)
+
+
+class Fp8Rows(_Fp8):
+    """Quantised activations [m, k]: e4m3 ``data`` and ue8m0 ``scales`` [m, ceil(k / 128)].
+
+    Rows of ``data`` start on 16-byte and rows of ``scales`` on 4-byte
+    boundaries; :meth:`pack` lays out tensors that do not."""
+
+    __slots__ = ()
+
+
+class Fp8Weight(_Fp8):
+    """A quantised weight [n, k]: e4m3 ``data`` and ue8m0 ``scales`` [ceil(n / 128), ceil(k / 128)],
+    laid out like :class:`Fp8Rows`."""
+
+    __slots__ = ()
+    _row_block = BLOCK
+
+
+def _ld8(t: torch.Tensor, unit: int) -> Optional[int]:
+    """Row stride of an 8-bit matrix, or None where its rows are not laid out in units of ``unit`` bytes."""
+    rows, cols = t.shape
+    if (cols > 1 and t.stride(1) != 1) or t.data_ptr() % unit:
+        return None
+    if rows <= 1:
+        return (cols + unit - 1) // unit * unit
+    ld = t.stride(0)
+    return ld if ld >= cols and ld % unit == 0 else None
+
+
+def _quantized(q: _Fp8, what: str) -> Tuple[int, int, int, int]:
+    """(data pointer, stride, scales pointer, stride) of quantised rows."""
+    ld, s_ld = _ld8(q.data, 16), _ld8(q.scales, 4)
+    if ld is None or s_ld is None:
+        raise InvalidShapeError("%s: rows of data must start on 16-byte and rows of scales on 4-byte boundaries "
+                                "(see %s.pack)" % (what, type(q).__name__))
+    return q.data.data_ptr(), ld, q.scales.data_ptr(), s_ld
+
+
+def _plain_ld(t: torch.Tensor) -> Optional[int]:
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        return None
+    if rows <= 1:
+        return cols
+    return t.stride(0) if t.stride(0) >= cols else None
+
+
+def _plain_in(t, what: str, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPES):
+        raise TypeError("%s must be a float32, float16 or bfloat16 CUDA tensor" % what)
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (what, dtype, t.dtype))
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise InvalidShapeError("%s must be 2-D with at least one column, got %s" % (what, tuple(t.shape)))
+    return t if _plain_ld(t) is not None else t.contiguous()
+
+
+def _plain_out(t, what: str, shape, dtype: torch.dtype, device) -> torch.Tensor:
+    """A caller's output tensor, checked."""
+    if not (isinstance(t, torch.Tensor) and t.dtype == dtype):
+        raise TypeError("%s must be a %s tensor" % (what, dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise InvalidShapeError("%s must be %s, got %s" % (what, tuple(shape), tuple(t.shape)))
+    if t.device != device:
+        raise ValueError("%s is on %s, the input on %s" % (what, t.device, device))
+    if _plain_ld(t) is None:
+        raise InvalidShapeError("%s: rows must be contiguous and must not overlap" % what)
+    return t
+
+
+def _rows_out(out, what: str, shape, device) -> Fp8Rows:
+    if out is None:
+        return _new(Fp8Rows, _rows(shape, 16, _E4M3, device), _rows((shape[0], _blocks(shape[1])), 4, _E8M0, device))
+    if not isinstance(out, Fp8Rows):
+        raise TypeError("%s must be an Fp8Rows" % what)
+    if tuple(out.shape) != tuple(shape):
+        raise InvalidShapeError("%s must be %s, got %s" % (what, tuple(shape), tuple(out.shape)))
+    if out.device != device:
+        raise ValueError("%s is on %s, the input on %s" % (what, out.device, device))
+    return out
+
+
+def _new(cls, data, scales):
+    """An instance of tensors that are right by construction."""
+    r = cls.__new__(cls)
+    r.data = data
+    r.scales = scales
+    return r
+
+
+def _vector(t, what: str, n: int, device) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.float32):
+        raise TypeError("%s must be a float32 tensor" % what)
+    if tuple(t.shape) != (n,):
+        raise InvalidShapeError("%s must be [%d], got %s" % (what, n, tuple(t.shape)))
+    if t.device != device:
+        raise ValueError("%s is on %s, the input on %s" % (what, t.device, device))
+    return t if n == 1 or t.stride(0) == 1 else t.contiguous()
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    """One C call on the current stream of ``device``."""
+    fn = getattr(_native.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        raise ForgeTuneRuntimeError("%s failed (%d): %s" % (name, rc, _native.last_error()))
+
+
+def quantize_rows(x: torch.Tensor, out: Optional[Fp8Rows] = None) -> Fp8Rows:
+    """Activations [m, k] (float32, float16, bfloat16) to 8 bits with a scale for each 128 along a row."""
+    x = _plain_in(x, "quantize_rows: x")
+    r = _rows_out(out, "quantize_rows: out", x.shape, x.device)
+    q = _quantized(r, "quantize_rows: out")
+    m, k = x.shape
+    _call("ftb_quantize_rows", x.device, x.data_ptr(), _TYPES[x.dtype], _plain_ld(x), *q, m, k)
+    return r
+
+
+def quantize_weight(w: torch.Tensor) -> Fp8Weight:
+    """A weight [n, k] (``nn.Linear``'s layout; float32, float16, bfloat16) to 8 bits with a scale for each
+    128 x 128 block.  Done once, where a model is loaded."""
+    w = _plain_in(w, "quantize_weight: w")
+    n, k = w.shape
+    if n < 1:
+        raise InvalidShapeError("quantize_weight: w must have at least one row")
+    r = _new(Fp8Weight, _rows((n, k), 16, _E4M3, w.device), _rows((_blocks(n), _blocks(k)), 4, _E8M0, w.device))
+    _call("ftb_quantize_weight", w.device, w.data_ptr(), _TYPES[w.dtype], _plain_ld(w),
+          *_quantized(r, "quantize_weight"), n, k)
+    return r
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+             residual: Optional[torch.Tensor] = None, quantize: bool = False,
+             out: Union[torch.Tensor, Fp8Rows, None] = None, residual_out: Optional[torch.Tensor] = None):
+    """``y = h / sqrt(mean(h^2) + eps) * weight`` over the rows of ``h = x + residual``.
+
+    ``x`` and ``residual`` are [m, k] of one type (float32, float16,
+    bfloat16), ``weight`` float32 [k] or None.  The sum, the mean and the norm
+    are computed in fp32 and ``y`` is rounded once: to ``x``'s type, or to an
+    :class:`Fp8Rows` with ``quantize``.  Without a residual returns ``y``; with
+    one returns ``(y, h)``, ``h`` in ``x``'s type.  ``out`` and
+    ``residual_out`` receive them in place of new tensors; ``residual_out``
+    may be ``x`` or ``residual``, ``out`` may be ``x``.
+    """
+    x = _plain_in(x, "rms_norm: x")
+    m, k = x.shape
+    dev, t = x.device, _TYPES[x.dtype]
+    weight = _vector(weight, "rms_norm: weight", k, dev)
+    h = None
+    if residual is not None:
+        residual = _plain_in(residual, "rms_norm: residual", x.dtype)
+        if residual.shape != x.shape:
+            raise InvalidShapeError("rms_norm: residual must be %s, got %s" % (tuple(x.shape), tuple(residual.shape)))
+        if residual.device != dev:
+            raise ValueError("rms_norm: residual is on %s, the input on %s" % (residual.device, dev))
+        h = torch.empty((m, k), dtype=x.dtype, device=dev) if residual_out is None else \
+            _plain_out(residual_out, "rms_norm: residual_out", x.shape, x.dtype, dev)
+    elif residual_out is not None:
+        raise ValueError("rms_norm: residual_out needs a residual")
+    if quantize:
+        y = _rows_out(out, "rms_norm: out", x.shape, dev)
+        q, q_ld, s, s_ld = _quantized(y, "rms_norm: out")
+        target = (q, _FTB_E4M3, q_ld, s, s_ld)
+    else:
+        y = torch.empty((m, k), dtype=x.dtype, device=dev) if out is None else \
+            _plain_out(out, "rms_norm: out", x.shape, x.dtype, dev)
+        target = (y.data_ptr(), t, _plain_ld(y), None, 0)
+    _call("ftb_rms_norm", dev, x.data_ptr(), t, _plain_ld(x),
+          residual.data_ptr() if residual is not None else None, _plain_ld(residual) if residual is not None else 0,
+          weight.data_ptr() if weight is not None else None, float(eps),
+          h.data_ptr() if h is not None else None, _plain_ld(h) if h is not None else 0, *target, m, k)
+    return y if residual is None else (y, h)
+
+
+def fp8_linear(x: Union[Fp8Rows, torch.Tensor], weight: Fp8Weight, bias: Optional[torch.Tensor] = None,
+               relu: bool = False, residual: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None, quantize: bool = False,
+               out: Union[torch.Tensor, Fp8Rows, None] = None) -> Union[torch.Tensor, Fp8Rows]:
+    """``relu(x @ weight.T + bias) + residual`` with 8-bit operands: [m, k] and [n, k] to [m, n].
+
+    ``x`` is an :class:`Fp8Rows`, or a plain tensor that is quantised first.
+    ``bias`` is float32 [n]; ``relu`` keeps NaN; ``residual`` is [m, n] of any
+    plain type.  The result has ``out_dtype`` (default: the plain ``x``'s type,
+    else the residual's, else float32), or is an :class:`Fp8Rows` with
+    ``quantize``.  ``out`` receives it in place of a new tensor and may be
+    ``residual``.
+    """
+    if not isinstance(weight, Fp8Weight):
+        raise TypeError("fp8_linear: weight must be an Fp8Weight (see quantize_weight)")
+    if not isinstance(x, Fp8Rows):
+        if out_dtype is None and isinstance(x, torch.Tensor):
+            out_dtype = x.dtype
+        x = quantize_rows(_plain_in(x, "fp8_linear: x"))
+    m, k = x.shape
+    n = weight.shape[0]
+    dev = x.device
+    if weight.shape[1] != k:
+        raise InvalidShapeError("fp8_linear: x is %s, weight %s: their depths differ"
+                                % (tuple(x.shape), tuple(weight.shape)))
+    if not x.data.is_cuda:
+        raise TypeError("fp8_linear: x must be on a CUDA device")
+    if weight.device != dev:
+        raise ValueError("fp8_linear: weight is on %s, the input on %s" % (weight.device, dev))
+    bias = _vector(bias, "fp8_linear: bias", n, dev)
+    res = (None, 0, 0)
+    if residual is not None:
+        residual = _plain_in(residual, "fp8_linear: residual")
+        if tuple(residual.shape) != (m, n):
+            raise InvalidShapeError("fp8_linear: residual must be %s, got %s" % ((m, n), tuple(residual.shape)))
+        if residual.device != dev:
+            raise ValueError("fp8_linear: residual is on %s, the input on %s" % (residual.device, dev))
+        res = (residual.data_ptr(), _TYPES[residual.dtype], _plain_ld(residual))
+    if quantize:
+        y = _rows_out(out, "fp8_linear: out", (m, n), dev)
+        q, q_ld, s, s_ld = _quantized(y, "fp8_linear: out")
+        target = (q, _FTB_E4M3, q_ld, s, s_ld)
+    else:
+        if out_dtype is None:
+            out_dtype = residual.dtype if residual is not None else torch.float32
+        if out_dtype not in _TYPES:
+            raise TypeError("fp8_linear: out_dtype must be float32, float16 or bfloat16, got %s" % (out_dtype,))
+        y = torch.empty((m, n), dtype=out_dtype, device=dev) if out is None else \
+            _plain_out(out, "fp8_linear: out", (m, n), out_dtype, dev)
+        target = (y.data_ptr(), _TYPES[out_dtype], _plain_ld(y), None, 0)
+    _call("ftb_fp8_linear", dev, *_quantized(x, "fp8_linear: x"), *_quantized(weight, "fp8_linear: weight"),
+          bias.data_ptr() if bias is not None else None, *res, *target, m, n, k, _FP8_RELU if relu else 0)
+    return y

@@ -221,6 +221,59 @@ FORGETUNE_EXPORT int ftb_small_gemm_noalloc(const float* d_x, const float* d_w, 
                                             const float* d_residual, float* d_y, int64_t m, int64_t k, int64_t n,
                                             uint32_t flags, void* stream);
 
+/* Block-scaled 8-bit operators.  No counterpart in the reference (fp32 only):
+ * a dense layer whose operands are held in 8 bits, the quantisation that
+ * feeds it, and the RMS norm that precedes such layers.
+ *
+ * The format: e4m3 values and, for each block of 128 along a row, one
+ * power-of-two scale 2^e stored as the byte e + 127; the block stands for
+ * value * scale.  Weights [n, k] share a scale per 128 x 128 block.  The scale
+ * is the smallest power of two with max|x| / scale <= 448, and 1 for a block
+ * of zeros.  Values that are not finite are stored as NaN; the scale comes
+ * from the finite values of the block.
+ *
+ * Matrices are row-major device arrays on the current device, rows `*_ld`
+ * elements apart.  8-bit values need 16-byte aligned rows (base and stride),
+ * scales [rows, ceil(k / 128)] 4-byte aligned rows, plain types the alignment
+ * of an element.  Only the k values and ceil(k / 128) scales of each row are
+ * read or written.  Everything is enqueued on `stream` (NULL = the legacy
+ * default stream) without synchronising or allocating; there is no workspace,
+ * so calls may overlap, and calls may be captured into CUDA graphs.  The
+ * first call on each device sets it up (and loads the library's device code):
+ * make it outside stream capture.  m = 0 returns 0 without a launch.
+ *
+ * Status codes as above: -1 null pointer, -2 sizes, strides, alignment or
+ * types, -5 launch error, or an earlier call's kernel on this device gave up
+ * a wait (reported once, by the next call). */
+#define FTB_F32 0
+#define FTB_F16 1
+#define FTB_BF16 2
+#define FTB_E4M3 3 /* outputs only: block-scaled, with a scale array */
+
+/* x [m, k] of a plain type -> q [m, k] and scales [m, ceil(k / 128)]. */
+FORGETUNE_EXPORT int ftb_quantize_rows(const void* x, int x_type, int64_t x_ld, uint8_t* q, int64_t q_ld,
+                                       uint8_t* scales, int64_t s_ld, int64_t m, int64_t k, void* stream);
+/* w [n, k] of a plain type -> q [n, k] and scales [ceil(n / 128), ceil(k / 128)]. */
+FORGETUNE_EXPORT int ftb_quantize_weight(const void* w, int w_type, int64_t w_ld, uint8_t* q, int64_t q_ld,
+                                         uint8_t* scales, int64_t s_ld, int64_t n, int64_t k, void* stream);
+/* h = x + residual (x alone when residual is null); y = h / sqrt(mean(h^2) + eps) * weight, the mean over
+ * the row, all in fp32.  weight [k] may be null (ones).  h, if not null, receives the sum in x's type; it
+ * may be x or residual themselves (same pointer and stride), as may a plain y.  y has x's type, or is
+ * quantised (y_type FTB_E4M3, scales not null) from the fp32 values. */
+FORGETUNE_EXPORT int ftb_rms_norm(const void* x, int x_type, int64_t x_ld, const void* residual, int64_t r_ld,
+                                  const float* weight, float eps, void* h, int64_t h_ld, void* y, int y_type,
+                                  int64_t y_ld, uint8_t* scales, int64_t s_ld, int64_t m, int64_t k, void* stream);
+/* y[m, n] = epi(sum_k a[m, k] w[n, k]) with a [m, k] quantised by rows and w [n, k] as a weight; epi adds
+ * bias[n] (null: none), applies ReLU (FTB_FP8_RELU; keeps NaN), then adds residual[m, n] (null: none) of any
+ * plain type.  y is plain, or quantised (FTB_E4M3, y_scales not null).  A plain y may be residual itself
+ * (same pointer, type and stride). */
+#define FTB_FP8_RELU 1u
+FORGETUNE_EXPORT int ftb_fp8_linear(const uint8_t* a, int64_t a_ld, const uint8_t* a_scales, int64_t as_ld,
+                                    const uint8_t* w, int64_t w_ld, const uint8_t* w_scales, int64_t ws_ld,
+                                    const float* bias, const void* residual, int r_type, int64_t r_ld, void* y,
+                                    int y_type, int64_t y_ld, uint8_t* y_scales, int64_t ys_ld, int64_t m, int64_t n,
+                                    int64_t k, uint32_t flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,135 @@
+"""Block-scaled 8-bit operators without a GPU: refusals of the C ABI and of
+the Python entry points, and the format's container."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from forgetune_b200 import (Fp8Rows, Fp8Weight, InvalidShapeError, _native, fp8_linear, quantize_rows,
+                            quantize_weight, rms_norm)
+
+from . import fp8_reference as ref
+
+P = 1 << 20  # a well aligned address that no refused call touches
+
+
+def rc(name, *args):
+    return getattr(_native.lib(), name)(*args)
+
+
+def test_quantize_rows_refusals():
+    def call(x=P, t=0, x_ld=200, q=P, q_ld=208, s=P, s_ld=4, m=3, k=200):
+        return rc("ftb_quantize_rows", x, t, x_ld, q, q_ld, s, s_ld, m, k, None)
+    assert call(m=0) == 0
+    assert call(x=None) == call(q=None) == call(s=None) == -1
+    for bad in (dict(m=-1), dict(k=0), dict(k=1 << 31), dict(t=3), dict(t=-1), dict(x=P + 2), dict(x_ld=199),
+                dict(q=P + 8), dict(q_ld=200), dict(q_ld=192), dict(s=P + 2), dict(s_ld=2), dict(s_ld=0)):
+        assert call(**bad) == -2, bad
+        assert "ftb_quantize_rows" in _native.last_error()
+
+
+def test_quantize_weight_refusals():
+    def call(w=P, t=0, w_ld=200, q=P, q_ld=208, s=P, s_ld=4, n=3, k=200):
+        return rc("ftb_quantize_weight", w, t, w_ld, q, q_ld, s, s_ld, n, k, None)
+    assert call(w=None) == call(q=None) == call(s=None) == -1
+    for bad in (dict(n=0), dict(k=0), dict(n=1 << 31), dict(t=3), dict(w=P + 1), dict(w_ld=1), dict(q=P + 4),
+                dict(q_ld=201), dict(s=P + 1), dict(s_ld=6)):
+        assert call(**bad) == -2, bad
+
+
+def test_rms_norm_refusals():
+    def call(x=P, t=2, x_ld=200, r=P, r_ld=200, w=P, eps=1e-6, h=P, h_ld=200, y=P, yt=2, y_ld=208, s=P, s_ld=4, m=3,
+             k=200):
+        return rc("ftb_rms_norm", x, t, x_ld, r, r_ld, w, eps, h, h_ld, y, yt, y_ld, s, s_ld, m, k, None)
+    assert call(m=0) == 0
+    assert call(x=None) == call(y=None) == call(yt=3, s=None) == -1
+    for bad in (dict(m=-1), dict(k=0), dict(t=3), dict(t=9), dict(yt=0), dict(r=None), dict(eps=-1.0),
+                dict(eps=float("nan")), dict(x=P + 1), dict(x_ld=1), dict(r=P + 1), dict(r_ld=7), dict(w=P + 2),
+                dict(h=P + 1), dict(h_ld=0), dict(y=P + 1), dict(y_ld=199), dict(yt=3, y=P + 8), dict(yt=3, y_ld=200),
+                dict(yt=3, s=P + 3), dict(yt=3, s_ld=1)):
+        assert call(**bad) == -2, bad
+
+
+def test_linear_refusals():
+    def call(a=P, a_ld=208, sa=P, sa_ld=4, w=P, w_ld=208, sw=P, sw_ld=4, bias=P, res=P, rt=0, r_ld=130, y=P, yt=0,
+             y_ld=144, ys=P, ys_ld=4, m=3, n=130, k=200, flags=1):
+        return rc("ftb_fp8_linear", a, a_ld, sa, sa_ld, w, w_ld, sw, sw_ld, bias, res, rt, r_ld, y, yt, y_ld, ys,
+                  ys_ld, m, n, k, flags, None)
+    assert call(m=0) == 0
+    for bad in ("a", "sa", "w", "sw", "y"):
+        assert call(**{bad: None}) == -1
+    assert call(yt=3, ys=None) == -1
+    for bad in (dict(m=-1), dict(n=0), dict(k=0), dict(m=1 << 31), dict(flags=2), dict(yt=4), dict(rt=3),
+                dict(a=P + 8), dict(a_ld=200), dict(sa=P + 1), dict(sa_ld=5), dict(w=P + 1), dict(w_ld=192),
+                dict(sw=P + 2), dict(sw_ld=0), dict(bias=P + 2), dict(res=P + 2), dict(r_ld=129), dict(y=P + 2),
+                dict(y_ld=129), dict(yt=3, y=P + 8), dict(yt=3, y_ld=130), dict(yt=3, ys=P + 2), dict(yt=3, ys_ld=1)):
+        assert call(**bad) == -2, bad
+
+
+def fp8(*shape):
+    return torch.zeros(*shape).to(torch.float8_e4m3fn)
+
+
+def scale(*shape):
+    return torch.ones(*shape).to(torch.float8_e8m0fnu)
+
+
+def test_containers_check_their_parts():
+    Fp8Rows(fp8(3, 200), scale(3, 2))
+    Fp8Weight(fp8(130, 200), scale(2, 2))
+    with pytest.raises(TypeError):
+        Fp8Rows(torch.zeros(3, 200), scale(3, 2))
+    with pytest.raises(TypeError):
+        Fp8Rows(fp8(3, 200), torch.ones(3, 2))
+    for cls, d, s in ((Fp8Rows, fp8(3, 200), scale(3, 1)), (Fp8Weight, fp8(130, 200), scale(130, 2)),
+                      (Fp8Rows, fp8(200), scale(2)), (Fp8Rows, fp8(3, 0), scale(3, 0))):
+        with pytest.raises(InvalidShapeError):
+            cls(d, s)
+
+
+def test_pack_lays_rows_out_and_keeps_the_values():
+    g = torch.Generator().manual_seed(0)
+    d = torch.randn(5, 77, generator=g).to(torch.float8_e4m3fn)
+    s = (2.0 ** torch.randint(-3, 3, (5, 1), generator=g).float()).to(torch.float8_e8m0fnu)
+    q = Fp8Rows.pack(d, s)
+    assert q.data.stride() == (80, 1) and q.scales.stride() == (4, 1)
+    assert np.array_equal(q.dequantize().numpy(), d.float().numpy() * s.float().numpy())
+    again = Fp8Rows.pack(q.data, q.scales)
+    assert again.data.data_ptr() == q.data.data_ptr() and again.scales.data_ptr() == q.scales.data_ptr()
+    t = Fp8Weight.pack(fp8(77, 5).t(), scale(1, 1))  # columns in place of rows
+    assert t.data.stride() == (80, 1)
+
+
+def test_entry_points_refuse_host_tensors():
+    x = torch.zeros(2, 128)
+    q, w = Fp8Rows.pack(fp8(2, 128), scale(2, 1)), Fp8Weight.pack(fp8(128, 128), scale(1, 1))
+    for call in (lambda: quantize_rows(x), lambda: quantize_weight(x), lambda: rms_norm(x), lambda: fp8_linear(x, w),
+                 lambda: fp8_linear(q, w), lambda: quantize_rows(None), lambda: fp8_linear(q, x)):
+        with pytest.raises(TypeError):
+            call()
+
+
+def test_reference_rounds_to_the_nearest_e4m3_value():
+    """The reference's rounding against torch's conversion on every border between two e4m3 values."""
+    bits = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    mid = (bits[1:] + bits[:-1]) / 2
+    v = np.concatenate([bits, mid, np.nextafter(mid.astype(np.float32), np.float32(0)).astype(np.float64),
+                        np.nextafter(mid.astype(np.float32), np.float32(999)).astype(np.float64)])
+    v = np.concatenate([v, -v])
+    want = torch.from_numpy(v).float().to(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(ref.e4m3(v), want)
+    assert ref.scale_exponent(np.array([0.0, 448.0, 448.1, 1.0, 1e-45, 3.4e38])).tolist() == [0, 0, 1, -8, -127, 120]
+
+
+def test_abi_constants_match_the_header():
+    import os
+    import re
+    from forgetune_b200 import fp8 as mod
+    header = open(os.path.join(os.path.dirname(__file__), "..", "include", "forgetune_b200.h")).read()
+    val = {n: int(v) for n, v in re.findall(r"#define (FTB_(?:F32|F16|BF16|E4M3)) (\d)", header)}
+    assert [mod._TYPES[t] for t in (torch.float32, torch.float16, torch.bfloat16)] == \
+        [val["FTB_F32"], val["FTB_F16"], val["FTB_BF16"]]
+    assert mod._FTB_E4M3 == val["FTB_E4M3"] and "#define FTB_FP8_RELU 1u" in header
+    assert ctypes.sizeof(ctypes.c_int64) == 8
