@@ -50,15 +50,11 @@ _SIGS = {
     "ftb_philox_normal": ([c_void_p, c_uint64, c_uint64, c_uint64, c_void_p], c_int),
     "ftb_small_gemm_noalloc": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                 ctypes.c_uint32, c_void_p], c_int),
-    "ftb_quantize_rows": ([c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
-                           c_void_p], c_int),
-    "ftb_quantize_weight": ([c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
-                             c_void_p], c_int),
-    "ftb_rms_norm": ([c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, ctypes.c_float, c_void_p, c_int64,
-                      c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p], c_int),
-    "ftb_fp8_linear": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                        c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_int64,
-                        c_int64, ctypes.c_uint32, c_void_p], c_int),
+    # the arguments' structs, packed by fp8.py
+    "ftb_quantize_rows": ([c_char_p, c_void_p], c_int),
+    "ftb_quantize_weight": ([c_char_p, c_void_p], c_int),
+    "ftb_rms_norm": ([c_char_p, c_void_p], c_int),
+    "ftb_fp8_linear": ([c_char_p, c_void_p], c_int),
 }
 
 EXPORTED = sorted(_SIGS)

@@ -86,24 +86,26 @@ static int fp8_device(const char* fn, Fp8Device** out) {
   return ST_OK;
 }
 
-static bool is_plain(int type) { return type == FTB_F32 || type == FTB_F16 || type == FTB_BF16; }
+static bool is_plain(int64_t type) { return type == FTB_F32 || type == FTB_F16 || type == FTB_BF16; }
 static bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-static int64_t type_size(int type) { return type == FTB_F32 ? 4 : type == FTB_E4M3 ? 1 : 2; }
 
 // Rows of `cols` elements `ld` apart: enough room, and the alignment of the
 // element type (plain) or of the copy engine (quantised).  "" when fine.
-static std::string check_plain(const char* what, const void* p, int type, int64_t cols, int64_t ld) {
-  if (!aligned(p, (uintptr_t)type_size(type))) return std::string(what) + " is not aligned to its type";
-  if (ld < cols) return std::string(what) + " rows overlap (stride below the row length)";
+static std::string check(const char* what, const ftb_matrix& x, int64_t cols) {
+  if (!is_plain(x.type)) return std::string(what) + " must be float32, float16 or bfloat16";
+  if (!aligned(x.data, x.type == FTB_F32 ? 4 : 2)) return std::string(what) + " is not aligned to its type";
+  if (x.ld < cols) return std::string(what) + " rows overlap (stride below the row length)";
   return "";
 }
-static std::string check_quantized(const char* what, const void* q, int64_t q_ld, const void* s, int64_t s_ld,
-                                   int64_t cols) {
-  if (!aligned(q, 16) || q_ld % 16 || q_ld < cols)
+static std::string check(const char* what, const ftb_fp8_matrix& q, int64_t cols) {
+  if (!aligned(q.data, 16) || q.ld % 16 || q.ld < cols)
     return std::string(what) + " values need 16-byte aligned rows (base and stride) of at least their length";
-  if (!aligned(s, 4) || s_ld % 4 || s_ld < fp8_blocks(cols))
+  if (!aligned(q.scales, 4) || q.scales_ld % 4 || q.scales_ld < fp8_blocks(cols))
     return std::string(what) + " scales need 4-byte aligned rows (base and stride) of at least their length";
   return "";
+}
+static bool sizes_ok(int64_t m, int64_t n, int64_t k) {
+  return m >= 0 && m <= kFp8MaxDim && n >= 1 && n <= kFp8MaxDim && k >= 1 && k <= kFp8MaxDim;
 }
 
 static int launched(const char* fn, cudaError_t e) {
@@ -129,147 +131,144 @@ static int guarded(const char* fn, F&& body) noexcept {
 
 using namespace ftb;
 
-FTB_API int ftb_quantize_rows(const void* x, int x_type, int64_t x_ld, uint8_t* q, int64_t q_ld, uint8_t* scales,
-                              int64_t s_ld, int64_t m, int64_t k, void* stream) {
+FTB_API int ftb_quantize_rows(const ftb_quantize_args* args, void* stream) {
   static const char fn[] = "ftb_quantize_rows";
   return guarded(fn, [&]() -> int {
-    if (m == 0) return ST_OK;
-    if (!x || !q || !scales) return refuse(fn, "null pointer", ST_NULL);
-    if (m < 0 || m > kFp8MaxDim || k < 1 || k > kFp8MaxDim) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^30");
-    if (!is_plain(x_type)) return refuse(fn, "x is float32, float16 or bfloat16");
-    std::string why = check_plain("x", x, x_type, k, x_ld);
-    if (why.empty()) why = check_quantized("output", q, q_ld, scales, s_ld, k);
+    if (!args) return refuse(fn, "null arguments", ST_NULL);
+    const ftb_quantize_args& a = *args;
+    if (a.m == 0) return ST_OK;
+    if (!a.x.data || !a.q.data || !a.q.scales) return refuse(fn, "null pointer", ST_NULL);
+    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^30");
+    std::string why = check("x", a.x, a.k);
+    if (why.empty()) why = check("q", a.q, a.k);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
     RowsParams p{};
-    p.x = x;
-    p.x_ld = x_ld;
-    p.q = q;
-    p.q_ld = q_ld;
-    p.s = scales;
-    p.s_ld = s_ld;
-    p.m = m;
-    p.k = k;
-    return launched(fn, launch_quantize_rows(p, x_type, d->sm_count, static_cast<cudaStream_t>(stream)));
+    p.x = a.x.data;
+    p.x_ld = a.x.ld;
+    p.q = a.q.data;
+    p.q_ld = a.q.ld;
+    p.s = a.q.scales;
+    p.s_ld = a.q.scales_ld;
+    p.m = a.m;
+    p.k = a.k;
+    return launched(fn, launch_quantize_rows(p, (int)a.x.type, static_cast<cudaStream_t>(stream)));
   });
 }
 
-FTB_API int ftb_quantize_weight(const void* w, int w_type, int64_t w_ld, uint8_t* q, int64_t q_ld, uint8_t* scales,
-                                int64_t s_ld, int64_t n, int64_t k, void* stream) {
+FTB_API int ftb_quantize_weight(const ftb_quantize_args* args, void* stream) {
   static const char fn[] = "ftb_quantize_weight";
   return guarded(fn, [&]() -> int {
-    if (!w || !q || !scales) return refuse(fn, "null pointer", ST_NULL);
-    if (n < 1 || n > kFp8MaxDim || k < 1 || k > kFp8MaxDim) return refuse(fn, "needs 1 <= n and 1 <= k, at most 2^30");
-    if (!is_plain(w_type)) return refuse(fn, "w is float32, float16 or bfloat16");
-    std::string why = check_plain("w", w, w_type, k, w_ld);
-    if (why.empty()) why = check_quantized("output", q, q_ld, scales, s_ld, k);
+    if (!args) return refuse(fn, "null arguments", ST_NULL);
+    const ftb_quantize_args& a = *args;
+    if (a.m == 0) return ST_OK;
+    if (!a.x.data || !a.q.data || !a.q.scales) return refuse(fn, "null pointer", ST_NULL);
+    if (!sizes_ok(a.m, 1, a.k) || fp8_blocks(a.m) > 65535)
+      return refuse(fn, "needs 0 <= m <= 128 * 65535 and 1 <= k <= 2^30");
+    std::string why = check("x", a.x, a.k);
+    if (why.empty()) why = check("q", a.q, a.k);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
     RowsParams p{};
-    p.x = w;
-    p.x_ld = w_ld;
-    p.q = q;
-    p.q_ld = q_ld;
-    p.s = scales;
-    p.s_ld = s_ld;
-    p.m = n;
-    p.k = k;
-    return launched(fn, launch_quantize_weight(p, w_type, static_cast<cudaStream_t>(stream)));
+    p.x = a.x.data;
+    p.x_ld = a.x.ld;
+    p.q = a.q.data;
+    p.q_ld = a.q.ld;
+    p.s = a.q.scales;
+    p.s_ld = a.q.scales_ld;
+    p.m = a.m;
+    p.k = a.k;
+    return launched(fn, launch_quantize_weight(p, (int)a.x.type, static_cast<cudaStream_t>(stream)));
   });
 }
 
-FTB_API int ftb_rms_norm(const void* x, int x_type, int64_t x_ld, const void* residual, int64_t r_ld,
-                         const float* weight, float eps, void* h, int64_t h_ld, void* y, int y_type, int64_t y_ld,
-                         uint8_t* scales, int64_t s_ld, int64_t m, int64_t k, void* stream) {
+FTB_API int ftb_rms_norm(const ftb_rms_norm_args* args, void* stream) {
   static const char fn[] = "ftb_rms_norm";
   return guarded(fn, [&]() -> int {
-    if (m == 0) return ST_OK;
-    if (!x || !y || (y_type == FTB_E4M3 && !scales)) return refuse(fn, "null pointer", ST_NULL);
-    if (h && !residual) return refuse(fn, "h is the sum with a residual: pass one");
-    if (m < 0 || m > kFp8MaxDim || k < 1 || k > kFp8MaxDim) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^30");
-    if (!is_plain(x_type)) return refuse(fn, "x is float32, float16 or bfloat16");
-    if (y_type != x_type && y_type != FTB_E4M3) return refuse(fn, "y has x's type or is quantised");
-    if (!(eps >= 0.0f)) return refuse(fn, "eps must not be negative");
-    std::string why = check_plain("x", x, x_type, k, x_ld);
-    if (why.empty() && residual) why = check_plain("residual", residual, x_type, k, r_ld);
-    if (why.empty() && h) why = check_plain("h", h, x_type, k, h_ld);
-    if (why.empty() && weight && !aligned(weight, 4)) why = "weight is not aligned to its type";
-    if (why.empty())
-      why = y_type == FTB_E4M3 ? check_quantized("output", y, y_ld, scales, s_ld, k)
-                               : check_plain("y", y, y_type, k, y_ld);
+    if (!args) return refuse(fn, "null arguments", ST_NULL);
+    const ftb_rms_norm_args& a = *args;
+    if (a.m == 0) return ST_OK;
+    if (!a.x.data || (!a.y.data && !a.q.data) || (a.q.data && !a.q.scales)) return refuse(fn, "null pointer", ST_NULL);
+    if (a.y.data && a.q.data) return refuse(fn, "y and q are both set");
+    if (a.h.data && !a.residual.data) return refuse(fn, "h is the sum with a residual: pass one");
+    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^30");
+    if (!(a.eps >= 0.0)) return refuse(fn, "eps must not be negative");
+    std::string why = check("x", a.x, a.k);
+    const ftb_matrix* others[3] = {&a.residual, &a.h, &a.y};
+    const char* names[3] = {"residual", "h", "y"};
+    for (int i = 0; i < 3 && why.empty(); ++i) {
+      if (!others[i]->data) continue;
+      why = check(names[i], *others[i], a.k);
+      if (why.empty() && others[i]->type != a.x.type) why = std::string(names[i]) + " must have x's type";
+    }
+    if (why.empty() && a.weight && !aligned(a.weight, 4)) why = "weight is not aligned to its type";
+    if (why.empty() && a.q.data) why = check("q", a.q, a.k);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
     RowsParams p{};
-    p.x = x;
-    p.x_ld = x_ld;
-    p.residual = residual;
-    p.r_ld = r_ld;
-    p.weight = weight;
-    p.eps = eps;
-    p.h = h;
-    p.h_ld = h_ld;
-    if (y_type == FTB_E4M3) {
-      p.q = static_cast<uint8_t*>(y);
-      p.q_ld = y_ld;
-      p.s = scales;
-      p.s_ld = s_ld;
-    } else {
-      p.y = y;
-      p.y_ld = y_ld;
-    }
-    p.m = m;
-    p.k = k;
-    return launched(fn, launch_rms_norm(p, x_type, d->sm_count, static_cast<cudaStream_t>(stream)));
+    p.x = a.x.data;
+    p.x_ld = a.x.ld;
+    p.residual = a.residual.data;
+    p.r_ld = a.residual.ld;
+    p.weight = a.weight;
+    p.eps = (float)a.eps;
+    p.h = a.h.data;
+    p.h_ld = a.h.ld;
+    p.y = a.y.data;
+    p.y_ld = a.y.ld;
+    p.q = a.q.data;
+    p.q_ld = a.q.ld;
+    p.s = a.q.scales;
+    p.s_ld = a.q.scales_ld;
+    p.m = a.m;
+    p.k = a.k;
+    return launched(fn, launch_rms_norm(p, (int)a.x.type, d->sm_count, static_cast<cudaStream_t>(stream)));
   });
 }
 
-FTB_API int ftb_fp8_linear(const uint8_t* a, int64_t a_ld, const uint8_t* a_scales, int64_t as_ld, const uint8_t* w,
-                           int64_t w_ld, const uint8_t* w_scales, int64_t ws_ld, const float* bias,
-                           const void* residual, int r_type, int64_t r_ld, void* y, int y_type, int64_t y_ld,
-                           uint8_t* y_scales, int64_t ys_ld, int64_t m, int64_t n, int64_t k, uint32_t flags,
-                           void* stream) {
+FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
   static const char fn[] = "ftb_fp8_linear";
   return guarded(fn, [&]() -> int {
-    if (m == 0) return ST_OK;
-    if (!a || !a_scales || !w || !w_scales || !y || (y_type == FTB_E4M3 && !y_scales))
+    if (!args) return refuse(fn, "null arguments", ST_NULL);
+    const ftb_fp8_linear_args& a = *args;
+    if (a.m == 0) return ST_OK;
+    if (!a.a.data || !a.a.scales || !a.w.data || !a.w.scales || (!a.y.data && !a.q.data) ||
+        (a.q.data && !a.q.scales))
       return refuse(fn, "null pointer", ST_NULL);
-    if (m < 0 || m > kFp8MaxDim || n < 1 || n > kFp8MaxDim || k < 1 || k > kFp8MaxDim)
-      return refuse(fn, "needs 0 <= m, 1 <= n and 1 <= k, at most 2^30");
-    if (flags & ~(uint32_t)FTB_FP8_RELU) return refuse(fn, "unknown flags");
-    if (!is_plain(y_type) && y_type != FTB_E4M3) return refuse(fn, "y is float32, float16, bfloat16 or quantised");
-    if (residual && !is_plain(r_type)) return refuse(fn, "residual is float32, float16 or bfloat16");
-    std::string why = check_quantized("a", a, a_ld, a_scales, as_ld, k);
-    if (why.empty()) why = check_quantized("w", w, w_ld, w_scales, ws_ld, k);
-    if (why.empty() && bias && !aligned(bias, 4)) why = "bias is not aligned to its type";
-    if (why.empty() && residual) why = check_plain("residual", residual, r_type, n, r_ld);
-    if (why.empty())
-      why = y_type == FTB_E4M3 ? check_quantized("output", y, y_ld, y_scales, ys_ld, n)
-                               : check_plain("y", y, y_type, n, y_ld);
+    if (a.y.data && a.q.data) return refuse(fn, "y and q are both set");
+    if (!sizes_ok(a.m, a.n, a.k)) return refuse(fn, "needs 0 <= m, 1 <= n and 1 <= k, at most 2^30");
+    if (a.flags & ~(int64_t)FTB_FP8_RELU) return refuse(fn, "unknown flags");
+    std::string why = check("a", a.a, a.k);
+    if (why.empty()) why = check("w", a.w, a.k);
+    if (why.empty() && a.bias && !aligned(a.bias, 4)) why = "bias is not aligned to its type";
+    if (why.empty() && a.residual.data) why = check("residual", a.residual, a.n);
+    if (why.empty() && a.y.data) why = check("y", a.y, a.n);
+    if (why.empty() && a.q.data) why = check("q", a.q, a.n);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
-    Fp8Operands o{a, a_ld, w, w_ld};
+    Fp8Operands o{a.a.data, a.a.ld, a.w.data, a.w.ld};
     Fp8Params p{};
-    p.M = (int)m;
-    p.N = (int)n;
-    p.K = (int)k;
-    p.sa = a_scales;
-    p.sa_ld = as_ld;
-    p.sw = w_scales;
-    p.sw_ld = ws_ld;
-    p.e.bias = bias;
-    p.e.residual = residual;
-    p.e.res_ld = r_ld;
-    p.e.res_type = r_type;
-    p.e.relu = (flags & FTB_FP8_RELU) != 0;
-    p.e.y = y;
-    p.e.y_ld = y_ld;
-    p.e.y_type = y_type;
-    p.e.ys = y_scales;
-    p.e.ys_ld = ys_ld;
+    p.M = (int)a.m;
+    p.N = (int)a.n;
+    p.K = (int)a.k;
+    p.sa = a.a.scales;
+    p.sa_ld = a.a.scales_ld;
+    p.sw = a.w.scales;
+    p.sw_ld = a.w.scales_ld;
+    p.e.bias = a.bias;
+    p.e.residual = a.residual.data;
+    p.e.res_ld = a.residual.ld;
+    p.e.res_type = (int)a.residual.type;
+    p.e.relu = (a.flags & FTB_FP8_RELU) != 0;
+    p.e.y = a.q.data ? a.q.data : a.y.data;
+    p.e.y_ld = a.q.data ? a.q.ld : a.y.ld;
+    p.e.y_type = a.q.data ? kFp8Type : (int)a.y.type;
+    p.e.ys = a.q.scales;
+    p.e.ys_ld = a.q.scales_ld;
     p.err = d->fault_dev;
     return launched(fn, launch_fp8_linear(o, p, static_cast<cudaStream_t>(stream)));
   });

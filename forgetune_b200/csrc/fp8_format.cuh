@@ -23,6 +23,7 @@
 namespace ftb {
 
 constexpr int kFp8Block = 128;
+constexpr int kFp8Type = 3;  // beside FTB_F32 .. FTB_BF16: a quantised output
 
 inline int64_t fp8_blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 
@@ -62,14 +63,16 @@ __device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax_bits) {
 // 1 / scale = 2^(127 - byte), exact: the byte is at most 247.
 __device__ __forceinline__ float fp8_inv_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
-// Four values over the scale as e4m3, the first in the lowest byte.  v 0 + v
-// keeps every finite v (signed zeros too) and turns infinities into NaN,
+// Keeps every finite v (signed zeros too) and turns infinities into NaN,
 // which the saturating conversion would make 448.
+__device__ __forceinline__ float nan_unless_finite(float v) { return __fmaf_rn(v, 0.0f, v); }
+
+// Four values (finite or NaN) over the scale as e4m3, the first in the lowest byte.
 __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inv) {
-  a = __fmaf_rn(a, 0.0f, a) * inv;
-  b = __fmaf_rn(b, 0.0f, b) * inv;
-  c = __fmaf_rn(c, 0.0f, c) * inv;
-  d = __fmaf_rn(d, 0.0f, d) * inv;
+  a *= inv;
+  b *= inv;
+  c *= inv;
+  d *= inv;
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));

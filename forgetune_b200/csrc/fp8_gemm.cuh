@@ -40,7 +40,7 @@ struct Fp8Epilogue {
   int64_t res_ld;
   int res_type;
   int relu;
-  void* y;                // [M, N] of y_type (FTB_E4M3: quantised)
+  void* y;                // [M, N] of y_type (kFp8Type: quantised)
   int64_t y_ld;
   int y_type;
   uint8_t* ys;            // scales of a quantised output
@@ -141,11 +141,13 @@ __device__ __forceinline__ void fp8_finish(const Fp8Epilogue& e, int64_t m, int 
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(v[i], r[i]);
   }
-  if (e.y_type == FTB_E4M3) {
+  if (e.y_type == kFp8Type) {
     uint32_t a = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
       if (i < cnt) a = max(a, finite_abs_bits(v[i]));
+      v[i] = nan_unless_finite(v[i]);
+    }
     const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, a));
     const uint32_t w = fp8_pack4(v[0], v[1], v[2], v[3], fp8_inv_scale(byte));
     uint8_t* q = static_cast<uint8_t*>(e.y) + m * e.y_ld + n;

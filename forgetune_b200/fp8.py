@@ -25,6 +25,7 @@ models are float32 only).
 
 from __future__ import annotations
 
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
@@ -37,18 +38,25 @@ __all__ = ["Fp8Rows", "Fp8Weight", "quantize_rows", "quantize_weight", "rms_norm
 BLOCK = 128
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # FTB_F32, FTB_F16, FTB_BF16
-_FTB_E4M3 = 3
 _FP8_RELU = 1
+
+# The argument structs of include/forgetune_b200.h: every field has eight
+# bytes.  A matrix is (pointer, stride, type), a quantised one (pointer,
+# stride, scales pointer, stride).
+_QUANTIZE_ARGS = struct.Struct("=9q")  # x, q, m, k
+_RMS_NORM_ARGS = struct.Struct("=7qd12q")  # x, residual, weight, eps, h, y, q, m, k
+_LINEAR_ARGS = struct.Struct("=23q")  # a, w, bias, residual, y, q, m, n, k, flags
+_NO_MATRIX = (0, 0, 0)
+_NO_FP8 = (0, 0, 0, 0)
 
 
 def _blocks(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK
 
 
-def _rows(shape, unit: int, dtype, device) -> torch.Tensor:
+def _rows(m: int, k: int, unit: int, dtype, device) -> torch.Tensor:
     """An uninitialised matrix whose rows start on multiples of ``unit`` elements."""
-    ld = (shape[1] + unit - 1) // unit * unit
-    return torch.empty_strided(shape, (ld, 1), dtype=dtype, device=device)
+    return torch.empty_strided((m, k), ((k + unit - 1) // unit * unit, 1), dtype=dtype, device=device)
 
 
 class _Fp8:
@@ -80,9 +88,9 @@ class _Fp8:
         """The same values in rows laid out as the operators need them (copied where they are not)."""
         r = cls(data, scales)
         if _ld8(r.data, 16) is None:
-            r.data = _rows(data.shape, 16, _E4M3, data.device).copy_(data)
+            r.data = _rows(*data.shape, 16, _E4M3, data.device).copy_(data)
         if _ld8(r.scales, 4) is None:
-            r.scales = _rows(scales.shape, 4, _E8M0, scales.device).copy_(scales)
+            r.scales = _rows(*scales.shape, 4, _E8M0, scales.device).copy_(scales)
         return r
 
     @property
@@ -122,16 +130,16 @@ class Fp8Weight(_Fp8):
 def _ld8(t: torch.Tensor, unit: int) -> Optional[int]:
     """Row stride of an 8-bit matrix, or None where its rows are not laid out in units of ``unit`` bytes."""
     rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or t.data_ptr() % unit:
+    ld, step = t.stride()
+    if (step != 1 and cols > 1) or t.data_ptr() % unit:
         return None
     if rows <= 1:
         return (cols + unit - 1) // unit * unit
-    ld = t.stride(0)
     return ld if ld >= cols and ld % unit == 0 else None
 
 
-def _quantized(q: _Fp8, what: str) -> Tuple[int, int, int, int]:
-    """(data pointer, stride, scales pointer, stride) of quantised rows."""
+def _fp8(q: _Fp8, what: str) -> Tuple[int, int, int, int]:
+    """Quantised rows as the C ABI takes them."""
     ld, s_ld = _ld8(q.data, 16), _ld8(q.scales, 4)
     if ld is None or s_ld is None:
         raise InvalidShapeError("%s: rows of data must start on 16-byte and rows of scales on 4-byte boundaries "
@@ -139,48 +147,57 @@ def _quantized(q: _Fp8, what: str) -> Tuple[int, int, int, int]:
     return q.data.data_ptr(), ld, q.scales.data_ptr(), s_ld
 
 
-def _plain_ld(t: torch.Tensor) -> Optional[int]:
+def _ld(t: torch.Tensor) -> Optional[int]:
+    """Row stride of a plain matrix, or None where its rows are not contiguous or overlap."""
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
         return None
     if rows <= 1:
         return cols
-    return t.stride(0) if t.stride(0) >= cols else None
+    return ld if ld >= cols else None
 
 
-def _plain_in(t, what: str, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+def _input(t, what: str) -> Tuple[torch.Tensor, int]:
+    """A plain 2-D CUDA input (copied where its rows are not contiguous) and its row stride."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPES):
         raise TypeError("%s must be a float32, float16 or bfloat16 CUDA tensor" % what)
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError("%s must be %s, got %s" % (what, dtype, t.dtype))
     if t.dim() != 2 or t.shape[1] < 1:
         raise InvalidShapeError("%s must be 2-D with at least one column, got %s" % (what, tuple(t.shape)))
-    return t if _plain_ld(t) is not None else t.contiguous()
+    ld = _ld(t)
+    return (t, ld) if ld is not None else (t.contiguous(), t.shape[1])
 
 
-def _plain_out(t, what: str, shape, dtype: torch.dtype, device) -> torch.Tensor:
-    """A caller's output tensor, checked."""
-    if not (isinstance(t, torch.Tensor) and t.dtype == dtype):
-        raise TypeError("%s must be a %s tensor" % (what, dtype))
-    if tuple(t.shape) != tuple(shape):
+def _check(t: torch.Tensor, what: str, shape, device) -> None:
+    if t.shape != shape:
         raise InvalidShapeError("%s must be %s, got %s" % (what, tuple(shape), tuple(t.shape)))
     if t.device != device:
         raise ValueError("%s is on %s, the input on %s" % (what, t.device, device))
-    if _plain_ld(t) is None:
-        raise InvalidShapeError("%s: rows must be contiguous and must not overlap" % what)
-    return t
 
 
-def _rows_out(out, what: str, shape, device) -> Fp8Rows:
+def _output(out, what: str, shape, dtype: torch.dtype, device) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
+    """A new plain output, or the caller's, and the matrix the C ABI takes."""
     if out is None:
-        return _new(Fp8Rows, _rows(shape, 16, _E4M3, device), _rows((shape[0], _blocks(shape[1])), 4, _E8M0, device))
-    if not isinstance(out, Fp8Rows):
-        raise TypeError("%s must be an Fp8Rows" % what)
-    if tuple(out.shape) != tuple(shape):
-        raise InvalidShapeError("%s must be %s, got %s" % (what, tuple(shape), tuple(out.shape)))
-    if out.device != device:
-        raise ValueError("%s is on %s, the input on %s" % (what, out.device, device))
-    return out
+        out = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+        return out, (out.data_ptr(), shape[1], _TYPES[dtype])
+    if not (isinstance(out, torch.Tensor) and out.dtype == dtype):
+        raise TypeError("%s must be a %s tensor" % (what, dtype))
+    _check(out, what, shape, device)
+    ld = _ld(out)
+    if ld is None:
+        raise InvalidShapeError("%s: rows must be contiguous and must not overlap" % what)
+    return out, (out.data_ptr(), ld, _TYPES[dtype])
+
+
+def _fp8_output(out, what: str, m: int, k: int, device) -> Tuple[Fp8Rows, Tuple[int, int, int, int]]:
+    """A new quantised output, or the caller's, and the matrix the C ABI takes."""
+    if out is not None:
+        if not isinstance(out, Fp8Rows):
+            raise TypeError("%s must be an Fp8Rows" % what)
+        _check(out, what, (m, k), device)
+        return out, _fp8(out, what)
+    r = _new(Fp8Rows, _rows(m, k, 16, _E4M3, device), _rows(m, _blocks(k), 4, _E8M0, device))
+    return r, (r.data.data_ptr(), (k + 15) // 16 * 16, r.scales.data_ptr(), (_blocks(k) + 3) // 4 * 4)
 
 
 def _new(cls, data, scales):
@@ -196,45 +213,45 @@ def _vector(t, what: str, n: int, device) -> Optional[torch.Tensor]:
         return None
     if not (isinstance(t, torch.Tensor) and t.dtype == torch.float32):
         raise TypeError("%s must be a float32 tensor" % what)
-    if tuple(t.shape) != (n,):
-        raise InvalidShapeError("%s must be [%d], got %s" % (what, n, tuple(t.shape)))
-    if t.device != device:
-        raise ValueError("%s is on %s, the input on %s" % (what, t.device, device))
+    _check(t, what, (n,), device)
     return t if n == 1 or t.stride(0) == 1 else t.contiguous()
 
 
-def _call(name: str, device: torch.device, *args) -> None:
+def _call(name: str, device: torch.device, args: bytes) -> None:
     """One C call on the current stream of ``device``."""
     fn = getattr(_native.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(args, stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(args, stream)
     if rc != 0:
         raise ForgeTuneRuntimeError("%s failed (%d): %s" % (name, rc, _native.last_error()))
 
 
 def quantize_rows(x: torch.Tensor, out: Optional[Fp8Rows] = None) -> Fp8Rows:
     """Activations [m, k] (float32, float16, bfloat16) to 8 bits with a scale for each 128 along a row."""
-    x = _plain_in(x, "quantize_rows: x")
-    r = _rows_out(out, "quantize_rows: out", x.shape, x.device)
-    q = _quantized(r, "quantize_rows: out")
+    x, ld = _input(x, "quantize_rows: x")
     m, k = x.shape
-    _call("ftb_quantize_rows", x.device, x.data_ptr(), _TYPES[x.dtype], _plain_ld(x), *q, m, k)
+    dev = x.device
+    r, q = _fp8_output(out, "quantize_rows: out", m, k, dev)
+    _call("ftb_quantize_rows", dev, _QUANTIZE_ARGS.pack(x.data_ptr(), ld, _TYPES[x.dtype], *q, m, k))
     return r
 
 
 def quantize_weight(w: torch.Tensor) -> Fp8Weight:
     """A weight [n, k] (``nn.Linear``'s layout; float32, float16, bfloat16) to 8 bits with a scale for each
     128 x 128 block.  Done once, where a model is loaded."""
-    w = _plain_in(w, "quantize_weight: w")
+    w, ld = _input(w, "quantize_weight: w")
     n, k = w.shape
     if n < 1:
         raise InvalidShapeError("quantize_weight: w must have at least one row")
-    r = _new(Fp8Weight, _rows((n, k), 16, _E4M3, w.device), _rows((_blocks(n), _blocks(k)), 4, _E8M0, w.device))
-    _call("ftb_quantize_weight", w.device, w.data_ptr(), _TYPES[w.dtype], _plain_ld(w),
-          *_quantized(r, "quantize_weight"), n, k)
+    dev = w.device
+    r = _new(Fp8Weight, _rows(n, k, 16, _E4M3, dev), _rows(_blocks(n), _blocks(k), 4, _E8M0, dev))
+    _call("ftb_quantize_weight", dev,
+          _QUANTIZE_ARGS.pack(w.data_ptr(), ld, _TYPES[w.dtype], *_fp8(r, "quantize_weight"), n, k))
     return r
 
 
@@ -251,33 +268,28 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     ``residual_out`` receive them in place of new tensors; ``residual_out``
     may be ``x`` or ``residual``, ``out`` may be ``x``.
     """
-    x = _plain_in(x, "rms_norm: x")
-    m, k = x.shape
-    dev, t = x.device, _TYPES[x.dtype]
+    x, ld = _input(x, "rms_norm: x")
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    m, k = shape
+    t = _TYPES[dtype]
     weight = _vector(weight, "rms_norm: weight", k, dev)
-    h = None
+    r_arg = h_arg = y_arg = _NO_MATRIX
+    q_arg = _NO_FP8
     if residual is not None:
-        residual = _plain_in(residual, "rms_norm: residual", x.dtype)
-        if residual.shape != x.shape:
-            raise InvalidShapeError("rms_norm: residual must be %s, got %s" % (tuple(x.shape), tuple(residual.shape)))
-        if residual.device != dev:
-            raise ValueError("rms_norm: residual is on %s, the input on %s" % (residual.device, dev))
-        h = torch.empty((m, k), dtype=x.dtype, device=dev) if residual_out is None else \
-            _plain_out(residual_out, "rms_norm: residual_out", x.shape, x.dtype, dev)
+        residual, r_ld = _input(residual, "rms_norm: residual")
+        if residual.dtype != dtype:
+            raise TypeError("rms_norm: residual must be %s, got %s" % (dtype, residual.dtype))
+        _check(residual, "rms_norm: residual", shape, dev)
+        r_arg = (residual.data_ptr(), r_ld, t)
+        h, h_arg = _output(residual_out, "rms_norm: residual_out", shape, dtype, dev)
     elif residual_out is not None:
         raise ValueError("rms_norm: residual_out needs a residual")
     if quantize:
-        y = _rows_out(out, "rms_norm: out", x.shape, dev)
-        q, q_ld, s, s_ld = _quantized(y, "rms_norm: out")
-        target = (q, _FTB_E4M3, q_ld, s, s_ld)
+        y, q_arg = _fp8_output(out, "rms_norm: out", m, k, dev)
     else:
-        y = torch.empty((m, k), dtype=x.dtype, device=dev) if out is None else \
-            _plain_out(out, "rms_norm: out", x.shape, x.dtype, dev)
-        target = (y.data_ptr(), t, _plain_ld(y), None, 0)
-    _call("ftb_rms_norm", dev, x.data_ptr(), t, _plain_ld(x),
-          residual.data_ptr() if residual is not None else None, _plain_ld(residual) if residual is not None else 0,
-          weight.data_ptr() if weight is not None else None, float(eps),
-          h.data_ptr() if h is not None else None, _plain_ld(h) if h is not None else 0, *target, m, k)
+        y, y_arg = _output(out, "rms_norm: out", shape, dtype, dev)
+    _call("ftb_rms_norm", dev, _RMS_NORM_ARGS.pack(
+        x.data_ptr(), ld, t, *r_arg, 0 if weight is None else weight.data_ptr(), eps, *h_arg, *y_arg, *q_arg, m, k))
     return y if residual is None else (y, h)
 
 
@@ -297,40 +309,34 @@ def fp8_linear(x: Union[Fp8Rows, torch.Tensor], weight: Fp8Weight, bias: Optiona
     if not isinstance(weight, Fp8Weight):
         raise TypeError("fp8_linear: weight must be an Fp8Weight (see quantize_weight)")
     if not isinstance(x, Fp8Rows):
-        if out_dtype is None and isinstance(x, torch.Tensor):
-            out_dtype = x.dtype
-        x = quantize_rows(_plain_in(x, "fp8_linear: x"))
-    m, k = x.shape
-    n = weight.shape[0]
-    dev = x.device
-    if weight.shape[1] != k:
-        raise InvalidShapeError("fp8_linear: x is %s, weight %s: their depths differ"
-                                % (tuple(x.shape), tuple(weight.shape)))
-    if not x.data.is_cuda:
+        x, _ = _input(x, "fp8_linear: x")
+        out_dtype = out_dtype or x.dtype
+        x = quantize_rows(x)
+    elif not x.data.is_cuda:
         raise TypeError("fp8_linear: x must be on a CUDA device")
-    if weight.device != dev:
-        raise ValueError("fp8_linear: weight is on %s, the input on %s" % (weight.device, dev))
+    dev = x.data.device
+    m, k = x.data.shape
+    n, wk = weight.data.shape
+    if wk != k:
+        raise InvalidShapeError("fp8_linear: x is %s, weight %s: their depths differ" % ((m, k), (n, wk)))
+    if weight.data.device != dev:
+        raise ValueError("fp8_linear: weight is on %s, the input on %s" % (weight.data.device, dev))
     bias = _vector(bias, "fp8_linear: bias", n, dev)
-    res = (None, 0, 0)
+    r_arg = y_arg = _NO_MATRIX
+    q_arg = _NO_FP8
     if residual is not None:
-        residual = _plain_in(residual, "fp8_linear: residual")
-        if tuple(residual.shape) != (m, n):
-            raise InvalidShapeError("fp8_linear: residual must be %s, got %s" % ((m, n), tuple(residual.shape)))
-        if residual.device != dev:
-            raise ValueError("fp8_linear: residual is on %s, the input on %s" % (residual.device, dev))
-        res = (residual.data_ptr(), _TYPES[residual.dtype], _plain_ld(residual))
+        residual, r_ld = _input(residual, "fp8_linear: residual")
+        _check(residual, "fp8_linear: residual", (m, n), dev)
+        r_arg = (residual.data_ptr(), r_ld, _TYPES[residual.dtype])
     if quantize:
-        y = _rows_out(out, "fp8_linear: out", (m, n), dev)
-        q, q_ld, s, s_ld = _quantized(y, "fp8_linear: out")
-        target = (q, _FTB_E4M3, q_ld, s, s_ld)
+        y, q_arg = _fp8_output(out, "fp8_linear: out", m, n, dev)
     else:
         if out_dtype is None:
-            out_dtype = residual.dtype if residual is not None else torch.float32
-        if out_dtype not in _TYPES:
+            out_dtype = torch.float32 if residual is None else residual.dtype
+        elif out_dtype not in _TYPES:
             raise TypeError("fp8_linear: out_dtype must be float32, float16 or bfloat16, got %s" % (out_dtype,))
-        y = torch.empty((m, n), dtype=out_dtype, device=dev) if out is None else \
-            _plain_out(out, "fp8_linear: out", (m, n), out_dtype, dev)
-        target = (y.data_ptr(), _TYPES[out_dtype], _plain_ld(y), None, 0)
-    _call("ftb_fp8_linear", dev, *_quantized(x, "fp8_linear: x"), *_quantized(weight, "fp8_linear: weight"),
-          bias.data_ptr() if bias is not None else None, *res, *target, m, n, k, _FP8_RELU if relu else 0)
+        y, y_arg = _output(out, "fp8_linear: out", (m, n), out_dtype, dev)
+    _call("ftb_fp8_linear", dev, _LINEAR_ARGS.pack(
+        *_fp8(x, "fp8_linear: x"), *_fp8(weight, "fp8_linear: weight"), 0 if bias is None else bias.data_ptr(),
+        *r_arg, *y_arg, *q_arg, m, n, k, _FP8_RELU if relu else 0))
     return y

@@ -232,7 +232,7 @@ FORGETUNE_EXPORT int ftb_small_gemm_noalloc(const float* d_x, const float* d_w, 
  * of zeros.  Values that are not finite are stored as NaN; the scale comes
  * from the finite values of the block.
  *
- * Matrices are row-major device arrays on the current device, rows `*_ld`
+ * Matrices are row-major device arrays on the current device, rows `ld`
  * elements apart.  8-bit values need 16-byte aligned rows (base and stride),
  * scales [rows, ceil(k / 128)] 4-byte aligned rows, plain types the alignment
  * of an element.  Only the k values and ceil(k / 128) scales of each row are
@@ -248,31 +248,58 @@ FORGETUNE_EXPORT int ftb_small_gemm_noalloc(const float* d_x, const float* d_w, 
 #define FTB_F32 0
 #define FTB_F16 1
 #define FTB_BF16 2
-#define FTB_E4M3 3 /* outputs only: block-scaled, with a scale array */
 
-/* x [m, k] of a plain type -> q [m, k] and scales [m, ceil(k / 128)]. */
-FORGETUNE_EXPORT int ftb_quantize_rows(const void* x, int x_type, int64_t x_ld, uint8_t* q, int64_t q_ld,
-                                       uint8_t* scales, int64_t s_ld, int64_t m, int64_t k, void* stream);
-/* w [n, k] of a plain type -> q [n, k] and scales [ceil(n / 128), ceil(k / 128)]. */
-FORGETUNE_EXPORT int ftb_quantize_weight(const void* w, int w_type, int64_t w_ld, uint8_t* q, int64_t q_ld,
-                                         uint8_t* scales, int64_t s_ld, int64_t n, int64_t k, void* stream);
-/* h = x + residual (x alone when residual is null); y = h / sqrt(mean(h^2) + eps) * weight, the mean over
- * the row, all in fp32.  weight [k] may be null (ones).  h, if not null, receives the sum in x's type; it
- * may be x or residual themselves (same pointer and stride), as may a plain y.  y has x's type, or is
- * quantised (y_type FTB_E4M3, scales not null) from the fp32 values. */
-FORGETUNE_EXPORT int ftb_rms_norm(const void* x, int x_type, int64_t x_ld, const void* residual, int64_t r_ld,
-                                  const float* weight, float eps, void* h, int64_t h_ld, void* y, int y_type,
-                                  int64_t y_ld, uint8_t* scales, int64_t s_ld, int64_t m, int64_t k, void* stream);
-/* y[m, n] = epi(sum_k a[m, k] w[n, k]) with a [m, k] quantised by rows and w [n, k] as a weight; epi adds
- * bias[n] (null: none), applies ReLU (FTB_FP8_RELU; keeps NaN), then adds residual[m, n] (null: none) of any
- * plain type.  y is plain, or quantised (FTB_E4M3, y_scales not null).  A plain y may be residual itself
- * (same pointer, type and stride). */
-#define FTB_FP8_RELU 1u
-FORGETUNE_EXPORT int ftb_fp8_linear(const uint8_t* a, int64_t a_ld, const uint8_t* a_scales, int64_t as_ld,
-                                    const uint8_t* w, int64_t w_ld, const uint8_t* w_scales, int64_t ws_ld,
-                                    const float* bias, const void* residual, int r_type, int64_t r_ld, void* y,
-                                    int y_type, int64_t y_ld, uint8_t* y_scales, int64_t ys_ld, int64_t m, int64_t n,
-                                    int64_t k, uint32_t flags, void* stream);
+typedef struct {
+  void* data;
+  int64_t ld;
+  int64_t type; /* FTB_F32, FTB_F16 or FTB_BF16 */
+} ftb_matrix;
+
+typedef struct {
+  uint8_t* data;   /* e4m3 values */
+  int64_t ld;
+  uint8_t* scales; /* e + 127 each */
+  int64_t scales_ld;
+} ftb_fp8_matrix;
+
+/* x [m, k] -> q [m, k] with scales [m, ceil(k / 128)] (ftb_quantize_rows) or
+ * [ceil(m / 128), ceil(k / 128)] (ftb_quantize_weight, x = w [n, k], m = n). */
+typedef struct {
+  ftb_matrix x;
+  ftb_fp8_matrix q;
+  int64_t m, k;
+} ftb_quantize_args;
+FORGETUNE_EXPORT int ftb_quantize_rows(const ftb_quantize_args* args, void* stream);
+FORGETUNE_EXPORT int ftb_quantize_weight(const ftb_quantize_args* args, void* stream);
+
+/* h = x + residual (x alone where residual.data is null); y = h / sqrt(mean(h^2) + eps) * weight, the mean
+ * over the row, all in fp32.  weight [k] may be null (ones).  h, where not null, receives the sum in x's
+ * type; it may be x or residual themselves (same pointer and stride), as may a plain y.  All plain matrices
+ * have x's type.  Exactly one of y.data and q.data is set: q is quantised from the fp32 values. */
+typedef struct {
+  ftb_matrix x, residual;
+  const float* weight;
+  double eps;
+  ftb_matrix h, y;
+  ftb_fp8_matrix q;
+  int64_t m, k;
+} ftb_rms_norm_args;
+FORGETUNE_EXPORT int ftb_rms_norm(const ftb_rms_norm_args* args, void* stream);
+
+/* y[m, n] = epi(sum_k a[m, k] w[n, k]), a [m, k] quantised by rows, w [n, k] as a weight.  epi adds bias[n]
+ * (null: none), applies ReLU (FTB_FP8_RELU; keeps NaN), then adds residual[m, n] (null: none) of any plain
+ * type.  Exactly one of y.data (plain) and q.data (quantised by rows) is set.  A plain y may be residual
+ * itself (same pointer, type and stride). */
+#define FTB_FP8_RELU 1
+typedef struct {
+  ftb_fp8_matrix a, w;
+  const float* bias;
+  ftb_matrix residual, y;
+  ftb_fp8_matrix q;
+  int64_t m, n, k;
+  int64_t flags;
+} ftb_fp8_linear_args;
+FORGETUNE_EXPORT int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream);
 
 #ifdef __cplusplus
 }

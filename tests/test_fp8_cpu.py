@@ -1,7 +1,8 @@
 """Block-scaled 8-bit operators without a GPU: refusals of the C ABI and of
 the Python entry points, and the format's container."""
 
-import ctypes
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -9,62 +10,63 @@ import torch
 
 from forgetune_b200 import (Fp8Rows, Fp8Weight, InvalidShapeError, _native, fp8_linear, quantize_rows,
                             quantize_weight, rms_norm)
+from forgetune_b200 import fp8 as mod
 
 from . import fp8_reference as ref
 
 P = 1 << 20  # a well aligned address that no refused call touches
 
 
-def rc(name, *args):
-    return getattr(_native.lib(), name)(*args)
+def rc(name, fmt, *args):
+    return getattr(_native.lib(), name)(fmt.pack(*args), None)
 
 
-def test_quantize_rows_refusals():
-    def call(x=P, t=0, x_ld=200, q=P, q_ld=208, s=P, s_ld=4, m=3, k=200):
-        return rc("ftb_quantize_rows", x, t, x_ld, q, q_ld, s, s_ld, m, k, None)
+@pytest.mark.parametrize("name", ["ftb_quantize_rows", "ftb_quantize_weight"])
+def test_quantize_refusals(name):
+    def call(x=P, x_ld=200, t=0, q=P, q_ld=208, s=P, s_ld=4, m=3, k=200):
+        return rc(name, mod._QUANTIZE_ARGS, x, x_ld, t, q, q_ld, s, s_ld, m, k)
     assert call(m=0) == 0
-    assert call(x=None) == call(q=None) == call(s=None) == -1
-    for bad in (dict(m=-1), dict(k=0), dict(k=1 << 31), dict(t=3), dict(t=-1), dict(x=P + 2), dict(x_ld=199),
-                dict(q=P + 8), dict(q_ld=200), dict(q_ld=192), dict(s=P + 2), dict(s_ld=2), dict(s_ld=0)):
+    assert getattr(_native.lib(), name)(None, None) == -1
+    assert call(x=0) == call(q=0) == call(s=0) == -1
+    for bad in (dict(m=-1), dict(k=0), dict(m=1 << 31), dict(k=1 << 31), dict(t=3), dict(t=-1), dict(x=P + 2),
+                dict(x_ld=199), dict(q=P + 8), dict(q_ld=200), dict(q_ld=192), dict(s=P + 2), dict(s_ld=2),
+                dict(s_ld=0), dict(s_ld=6)):
         assert call(**bad) == -2, bad
-        assert "ftb_quantize_rows" in _native.last_error()
-
-
-def test_quantize_weight_refusals():
-    def call(w=P, t=0, w_ld=200, q=P, q_ld=208, s=P, s_ld=4, n=3, k=200):
-        return rc("ftb_quantize_weight", w, t, w_ld, q, q_ld, s, s_ld, n, k, None)
-    assert call(w=None) == call(q=None) == call(s=None) == -1
-    for bad in (dict(n=0), dict(k=0), dict(n=1 << 31), dict(t=3), dict(w=P + 1), dict(w_ld=1), dict(q=P + 4),
-                dict(q_ld=201), dict(s=P + 1), dict(s_ld=6)):
-        assert call(**bad) == -2, bad
+        assert name in _native.last_error()
 
 
 def test_rms_norm_refusals():
-    def call(x=P, t=2, x_ld=200, r=P, r_ld=200, w=P, eps=1e-6, h=P, h_ld=200, y=P, yt=2, y_ld=208, s=P, s_ld=4, m=3,
-             k=200):
-        return rc("ftb_rms_norm", x, t, x_ld, r, r_ld, w, eps, h, h_ld, y, yt, y_ld, s, s_ld, m, k, None)
+    def call(x=P, x_ld=200, t=2, r=P, r_ld=200, rt=2, w=P, eps=1e-6, h=P, h_ld=200, ht=2, y=P, y_ld=208, yt=2, q=0,
+             q_ld=208, s=0, s_ld=4, m=3, k=200):
+        return rc("ftb_rms_norm", mod._RMS_NORM_ARGS, x, x_ld, t, r, r_ld, rt, w, eps, h, h_ld, ht, y, y_ld, yt, q,
+                  q_ld, s, s_ld, m, k)
+    fp8_out = dict(y=0, q=P, s=P)
     assert call(m=0) == 0
-    assert call(x=None) == call(y=None) == call(yt=3, s=None) == -1
-    for bad in (dict(m=-1), dict(k=0), dict(t=3), dict(t=9), dict(yt=0), dict(r=None), dict(eps=-1.0),
-                dict(eps=float("nan")), dict(x=P + 1), dict(x_ld=1), dict(r=P + 1), dict(r_ld=7), dict(w=P + 2),
-                dict(h=P + 1), dict(h_ld=0), dict(y=P + 1), dict(y_ld=199), dict(yt=3, y=P + 8), dict(yt=3, y_ld=200),
-                dict(yt=3, s=P + 3), dict(yt=3, s_ld=1)):
+    assert _native.lib().ftb_rms_norm(None, None) == -1
+    assert call(x=0) == call(y=0) == call(y=0, q=P) == -1
+    for bad in (dict(m=-1), dict(k=0), dict(t=3), dict(t=9), dict(yt=0), dict(rt=1), dict(ht=7), dict(r=0),
+                dict(eps=-1.0), dict(eps=float("nan")), dict(x=P + 1), dict(x_ld=1), dict(r=P + 1), dict(r_ld=7),
+                dict(w=P + 2), dict(h=P + 1), dict(h_ld=0), dict(y=P + 1), dict(y_ld=199), dict(q=P, s=P),
+                dict(fp8_out, q=P + 8), dict(fp8_out, q_ld=200), dict(fp8_out, s=P + 3), dict(fp8_out, s_ld=1)):
         assert call(**bad) == -2, bad
 
 
 def test_linear_refusals():
-    def call(a=P, a_ld=208, sa=P, sa_ld=4, w=P, w_ld=208, sw=P, sw_ld=4, bias=P, res=P, rt=0, r_ld=130, y=P, yt=0,
-             y_ld=144, ys=P, ys_ld=4, m=3, n=130, k=200, flags=1):
-        return rc("ftb_fp8_linear", a, a_ld, sa, sa_ld, w, w_ld, sw, sw_ld, bias, res, rt, r_ld, y, yt, y_ld, ys,
-                  ys_ld, m, n, k, flags, None)
+    def call(a=P, a_ld=208, sa=P, sa_ld=4, w=P, w_ld=208, sw=P, sw_ld=4, bias=P, res=P, r_ld=130, rt=0, y=P,
+             y_ld=144, yt=0, q=0, q_ld=144, s=0, s_ld=4, m=3, n=130, k=200, flags=1):
+        return rc("ftb_fp8_linear", mod._LINEAR_ARGS, a, a_ld, sa, sa_ld, w, w_ld, sw, sw_ld, bias, res, r_ld, rt, y,
+                  y_ld, yt, q, q_ld, s, s_ld, m, n, k, flags)
+    fp8_out = dict(y=0, q=P, s=P)
     assert call(m=0) == 0
+    assert _native.lib().ftb_fp8_linear(None, None) == -1
     for bad in ("a", "sa", "w", "sw", "y"):
-        assert call(**{bad: None}) == -1
-    assert call(yt=3, ys=None) == -1
+        assert call(**{bad: 0}) == -1
+    assert call(y=0, q=P) == -1
     for bad in (dict(m=-1), dict(n=0), dict(k=0), dict(m=1 << 31), dict(flags=2), dict(yt=4), dict(rt=3),
                 dict(a=P + 8), dict(a_ld=200), dict(sa=P + 1), dict(sa_ld=5), dict(w=P + 1), dict(w_ld=192),
                 dict(sw=P + 2), dict(sw_ld=0), dict(bias=P + 2), dict(res=P + 2), dict(r_ld=129), dict(y=P + 2),
-                dict(y_ld=129), dict(yt=3, y=P + 8), dict(yt=3, y_ld=130), dict(yt=3, ys=P + 2), dict(yt=3, ys_ld=1)):
+                dict(y_ld=129), dict(q=P, s=P), dict(fp8_out, q=P + 8), dict(fp8_out, q_ld=130),
+                dict(fp8_out, s=P + 2), dict(fp8_out, s_ld=1)):
         assert call(**bad) == -2, bad
 
 
@@ -123,13 +125,15 @@ def test_reference_rounds_to_the_nearest_e4m3_value():
     assert ref.scale_exponent(np.array([0.0, 448.0, 448.1, 1.0, 1e-45, 3.4e38])).tolist() == [0, 0, 1, -8, -127, 120]
 
 
-def test_abi_constants_match_the_header():
-    import os
-    import re
-    from forgetune_b200 import fp8 as mod
-    header = open(os.path.join(os.path.dirname(__file__), "..", "include", "forgetune_b200.h")).read()
-    val = {n: int(v) for n, v in re.findall(r"#define (FTB_(?:F32|F16|BF16|E4M3)) (\d)", header)}
-    assert [mod._TYPES[t] for t in (torch.float32, torch.float16, torch.bfloat16)] == \
-        [val["FTB_F32"], val["FTB_F16"], val["FTB_BF16"]]
-    assert mod._FTB_E4M3 == val["FTB_E4M3"] and "#define FTB_FP8_RELU 1u" in header
-    assert ctypes.sizeof(ctypes.c_int64) == 8
+def test_argument_structs_match_the_header(tmp_path):
+    """The packed arguments have the header's sizes and constants, as a C compiler sees them."""
+    src = tmp_path / "t.c"
+    src.write_text('#include <stdio.h>\n#include "forgetune_b200.h"\nint main(void) { printf("%d %d %d %d %d %d %d\\n", '
+                   "(int)sizeof(ftb_quantize_args), (int)sizeof(ftb_rms_norm_args), (int)sizeof(ftb_fp8_linear_args), "
+                   "FTB_F32, FTB_F16, FTB_BF16, FTB_FP8_RELU); return 0; }\n")
+    include = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "include")
+    subprocess.run(["gcc", "-I", include, str(src), "-o", str(tmp_path / "t")], check=True)
+    got = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()
+    types = [mod._TYPES[t] for t in (torch.float32, torch.float16, torch.bfloat16)]
+    assert [int(v) for v in got] == [mod._QUANTIZE_ARGS.size, mod._RMS_NORM_ARGS.size, mod._LINEAR_ARGS.size] + \
+        types + [mod._FP8_RELU]
