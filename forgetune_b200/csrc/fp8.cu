@@ -3,25 +3,30 @@
 // launches.
 #include <cuda_runtime.h>
 
-#include <atomic>
+#include <algorithm>
+#include <cmath>
+#include <exception>
 #include <mutex>
 #include <string>
 
 #include "forgetune_b200.h"
 #include "fp8_gemm.cuh"
+#include "fp8_pair.cuh"
 #include "fp8_rows.cuh"
 #include "status.hpp"
 
 namespace ftb {
 
 constexpr int kFp8MaxDevices = 64;
-constexpr int64_t kFp8MaxDim = int64_t(1) << 30;
+constexpr int64_t kFp8MaxDim = int64_t(1) << 28;
 
 struct Fp8Device {
   std::once_flag once;
   int rc = ST_OK;
   std::string err;
   int sm_count = 0;
+  int pairs = 0;  // SM pairs resident at once
+  int tile_slots[4] = {0, 0, 0, 0};  // CTAs of the tile kernel resident at once, in clusters of 1, 2, 4 and 8
   // set by a kernel whose bounded wait gave up: mapped host memory, so the
   // next call reads it without a copy
   volatile int* fault = nullptr;
@@ -54,6 +59,8 @@ static void fp8_setup(int dev, Fp8Device* d) {
   if (e == cudaSuccess) e = fp8_tile_attributes<32>();
   if (e == cudaSuccess) e = fp8_tile_attributes<64>();
   if (e == cudaSuccess) e = fp8_tile_attributes<128>();
+  if (e == cudaSuccess) e = fp8_tile_slots(d->tile_slots);
+  if (e == cudaSuccess) e = fp8_pair_prepare(&d->pairs);
   if (e != cudaSuccess) {
     d->rc = ST_DEVICE;
     d->err = std::string("set-up failed: ") + cudaGetErrorString(e);
@@ -104,6 +111,10 @@ static std::string check(const char* what, const ftb_fp8_matrix& q, int64_t cols
     return std::string(what) + " scales need 4-byte aligned rows (base and stride) of at least their length";
   return "";
 }
+// Base and rows on 16-byte boundaries.
+static bool rows_aligned(const ftb_matrix& x) {
+  return aligned(x.data, 16) && (x.ld * (x.type == FTB_F32 ? 4 : 2)) % 16 == 0;
+}
 static bool sizes_ok(int64_t m, int64_t n, int64_t k) {
   return m >= 0 && m <= kFp8MaxDim && n >= 1 && n <= kFp8MaxDim && k >= 1 && k <= kFp8MaxDim;
 }
@@ -112,6 +123,60 @@ static int launched(const char* fn, cudaError_t e) {
   if (e == cudaSuccess) return ST_OK;
   cudaGetLastError();
   return refuse(fn, std::string("launch failed: ") + cudaGetErrorString(e), ST_DEVICE);
+}
+
+// The kernel for a product: the tile kernel with NT tokens per tile and a
+// cluster of `split` CTAs per tile, or the pair kernel (nt = 0).
+struct Fp8Choice {
+  int nt, split;
+};
+
+// Picks by an estimate of the time in microseconds.  A CTA of the tile kernel
+// takes 0.40 per k-block when it waits for its loads, and an SM at least
+// 0.0097 per KB that its CTAs load; finishing costs 0.016 per token of a tile,
+// 0.008 more per token that is not shared out over the cluster; a cluster
+// costs 0.5.  A pair takes 0.28 per k-block and 1.2 per tile, and 6 more than
+// a tile before and after.  The constants are a fit to 72 shapes (m 1..4096, k and
+// n 64..8192) timed with every choice on a B200; over those shapes the pick
+// is 1.5 % slower than the best choice in the mean (geometric), 14 % at most
+// but for one.  Examples, best and next kinds: 1 x 4096 x 4096 (m, k, n): 16
+// tokens, split 4: 5.4 us, split 1: 12.2 us; 512 x 512 x 512: 16 tokens: 3.5,
+// 128 tokens: 6.8 us; 512 x 4096 x 4096: 128 tokens, split 2: 16.2, pair:
+// 17.8 us; 1024 x 4096 x 4096: pair 18.6, 128 tokens 22.6 us.
+static Fp8Choice choose_fp8(int64_t m, int64_t n, int64_t k, const Fp8Device& d) {
+  const double sms = d.sm_count;
+  const int64_t nk = (k + 127) / 128, nt128 = (n + 127) / 128;
+  const int64_t pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
+  Fp8Choice best{0, 1};
+  double best_us = 7.9 + std::ceil((double)pair_tiles / d.pairs) * ((double)nk * 0.28 + 1.2);
+  for (int nt = 16; nt <= 128; nt *= 2) {
+    const int64_t tiles = nt128 * ((m + nt - 1) / nt);
+    for (int i = 0, split = 1; i < 4; ++i, split *= 2) {
+      if (split > 1 && nk < split * 2) break;  // a CTA without a k-block of its own
+      const double ctas = (double)tiles * split;
+      const double kb = (double)std::min<int64_t>(nk, ((nk + 3) / 4 + split - 1) / split * 4);
+      const double rounds = std::ceil(ctas / d.tile_slots[i]), per_sm = std::ceil(ctas / sms);
+      const double load = std::max(rounds * kb * 0.40, per_sm * kb * (16 + nt / 8) * 0.0097);
+      const double us = 2.0 + load + per_sm * nt * (0.016 + 0.008 / split) + (split > 1 ? 0.5 : 0.0);
+      if (us < best_us) {
+        best_us = us;
+        best = Fp8Choice{nt, split};
+      }
+    }
+    if (nt >= m) break;
+  }
+  return best;
+}
+
+static cudaError_t launch_fp8_linear(const Fp8Operands& o, const Fp8Params& p, const Fp8Device& d, cudaStream_t s) {
+  const Fp8Choice c = choose_fp8(p.M, p.N, p.K, d);
+  switch (c.nt) {
+    case 16: return launch_fp8_tile<16>(o, p, c.split, s);
+    case 32: return launch_fp8_tile<32>(o, p, c.split, s);
+    case 64: return launch_fp8_tile<64>(o, p, c.split, s);
+    case 128: return launch_fp8_tile<128>(o, p, c.split, s);
+    default: return launch_fp8_pair(o, p, d.pairs, 0, s);
+  }
 }
 
 template <typename F>
@@ -138,7 +203,7 @@ FTB_API int ftb_quantize_rows(const ftb_quantize_args* args, void* stream) {
     const ftb_quantize_args& a = *args;
     if (a.m == 0) return ST_OK;
     if (!a.x.data || !a.q.data || !a.q.scales) return refuse(fn, "null pointer", ST_NULL);
-    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^30");
+    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^28");
     std::string why = check("x", a.x, a.k);
     if (why.empty()) why = check("q", a.q, a.k);
     if (!why.empty()) return refuse(fn, why);
@@ -165,7 +230,7 @@ FTB_API int ftb_quantize_weight(const ftb_quantize_args* args, void* stream) {
     if (a.m == 0) return ST_OK;
     if (!a.x.data || !a.q.data || !a.q.scales) return refuse(fn, "null pointer", ST_NULL);
     if (!sizes_ok(a.m, 1, a.k) || fp8_blocks(a.m) > 65535)
-      return refuse(fn, "needs 0 <= m <= 128 * 65535 and 1 <= k <= 2^30");
+      return refuse(fn, "needs 0 <= m <= 128 * 65535 and 1 <= k <= 2^28");
     std::string why = check("x", a.x, a.k);
     if (why.empty()) why = check("q", a.q, a.k);
     if (!why.empty()) return refuse(fn, why);
@@ -193,7 +258,7 @@ FTB_API int ftb_rms_norm(const ftb_rms_norm_args* args, void* stream) {
     if (!a.x.data || (!a.y.data && !a.q.data) || (a.q.data && !a.q.scales)) return refuse(fn, "null pointer", ST_NULL);
     if (a.y.data && a.q.data) return refuse(fn, "y and q are both set");
     if (a.h.data && !a.residual.data) return refuse(fn, "h is the sum with a residual: pass one");
-    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^30");
+    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^28");
     if (!(a.eps >= 0.0)) return refuse(fn, "eps must not be negative");
     std::string why = check("x", a.x, a.k);
     const ftb_matrix* others[3] = {&a.residual, &a.h, &a.y};
@@ -239,7 +304,7 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
         (a.q.data && !a.q.scales))
       return refuse(fn, "null pointer", ST_NULL);
     if (a.y.data && a.q.data) return refuse(fn, "y and q are both set");
-    if (!sizes_ok(a.m, a.n, a.k)) return refuse(fn, "needs 0 <= m, 1 <= n and 1 <= k, at most 2^30");
+    if (!sizes_ok(a.m, a.n, a.k)) return refuse(fn, "needs 0 <= m, 1 <= n and 1 <= k, at most 2^28");
     if (a.flags & ~(int64_t)FTB_FP8_RELU) return refuse(fn, "unknown flags");
     std::string why = check("a", a.a, a.k);
     if (why.empty()) why = check("w", a.w, a.k);
@@ -269,7 +334,9 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
     p.e.y_type = a.q.data ? kFp8Type : (int)a.y.type;
     p.e.ys = a.q.scales;
     p.e.ys_ld = a.q.scales_ld;
+    p.e.res_vec = rows_aligned(a.residual);
+    p.e.y_vec = rows_aligned(a.y);
     p.err = d->fault_dev;
-    return launched(fn, launch_fp8_linear(o, p, static_cast<cudaStream_t>(stream)));
+    return launched(fn, launch_fp8_linear(o, p, *d, static_cast<cudaStream_t>(stream)));
   });
 }

@@ -24,7 +24,8 @@
 #pragma once
 
 #include <algorithm>
-#include <atomic>
+#include <cstring>
+#include <type_traits>
 
 #include "fp8_format.cuh"
 #include "tc_ptx.cuh"
@@ -32,6 +33,7 @@
 namespace ftb {
 
 constexpr int kFp8Threads = 256;
+constexpr int kFp8MaxSplit = 8;  // CTAs that share a tile's depth: the portable cluster size
 
 // What an epilogue reads and writes.
 struct Fp8Epilogue {
@@ -45,6 +47,7 @@ struct Fp8Epilogue {
   int y_type;
   uint8_t* ys;            // scales of a quantised output
   int64_t ys_ld;
+  int res_vec, y_vec;     // residual and plain output: bases and rows are aligned to 16 bytes
 };
 
 struct Fp8Params {
@@ -107,39 +110,67 @@ __device__ __forceinline__ void st_shared4(uint32_t addr, uint32_t a, uint32_t b
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// Four consecutive values of `src` (any of the plain types) from column n, of
-// which `cnt` exist.
+// Four consecutive values of a plain type, of which `cnt` exist; `vec`: rows
+// and bases are aligned to four elements.
 template <typename T>
-__device__ __forceinline__ void fp8_load4(const T* src, int cnt, float (&v)[4]) {
+__device__ __forceinline__ void fp8_load4(const T* src, int cnt, bool vec, float (&v)[4]) {
+  if (vec && cnt >= 4) {
+    T t[4];
+    if constexpr (sizeof(T) == 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src);
+      memcpy(t, &u, 16);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(src);
+      memcpy(t, &u, 8);
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = i < cnt ? to_f32(src[i]) : 0.0f;
+    for (int i = 0; i < 4; ++i) v[i] = to_f32(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < cnt ? to_f32(src[i]) : 0.0f;
+  }
 }
 
 template <typename T>
-__device__ __forceinline__ void fp8_store4(T* dst, int cnt, const float (&v)[4]) {
+__device__ __forceinline__ void fp8_store4(T* dst, int cnt, bool vec, const float (&v)[4]) {
+  if (vec && cnt >= 4) {
+    T t[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < cnt) dst[i] = from_f32<T>(v[i]);
+    for (int i = 0; i < 4; ++i) t[i] = from_f32<T>(v[i]);
+    if constexpr (sizeof(T) == 4) {
+      uint4 u;
+      memcpy(&u, t, 16);
+      *reinterpret_cast<uint4*>(dst) = u;
+    } else {
+      uint2 u;
+      memcpy(&u, t, 8);
+      *reinterpret_cast<uint2*>(dst) = u;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < cnt) dst[i] = from_f32<T>(v[i]);
+  }
 }
 
 // A warp finishes 128 outputs of token m: lane l has columns n .. n + 3,
-// n = n0 + 4 l.
-__device__ __forceinline__ void fp8_finish(const Fp8Epilogue& e, int64_t m, int n0, int N, int lane, float (&v)[4]) {
+// n = n0 + 4 l, their bias and residual; `cnt` = N - n columns exist from there.
+__device__ __forceinline__ void fp8_residual(const Fp8Epilogue& e, int64_t m, int n, int cnt, float (&r)[4]) {
+  const int64_t at = m * e.res_ld + n;
+  if (e.res_type == FTB_F32) fp8_load4(static_cast<const float*>(e.residual) + at, cnt, e.res_vec, r);
+  else if (e.res_type == FTB_F16) fp8_load4(static_cast<const __half*>(e.residual) + at, cnt, e.res_vec, r);
+  else fp8_load4(static_cast<const __nv_bfloat16*>(e.residual) + at, cnt, e.res_vec, r);
+}
+
+__device__ __forceinline__ void fp8_finish(const Fp8Epilogue& e, int64_t m, int n0, int N, int lane,
+                                           const float (&bias)[4], const float (&res)[4], float (&v)[4]) {
   const int n = n0 + 4 * lane;
-  const int cnt = min(4, N - n);  // below 1: no column
+  const int cnt = N - n;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (e.bias && i < cnt) v[i] = __fadd_rn(v[i], e.bias[n + i]);
+    if (e.bias) v[i] = __fadd_rn(v[i], bias[i]);
     if (e.relu) v[i] = (v[i] != v[i] || v[i] > 0.0f) ? v[i] : 0.0f;  // keeps NaN
-  }
-  if (e.residual && cnt > 0) {
-    float r[4];
-    const int64_t at = m * e.res_ld + n;
-    if (e.res_type == FTB_F32) fp8_load4(static_cast<const float*>(e.residual) + at, cnt, r);
-    else if (e.res_type == FTB_F16) fp8_load4(static_cast<const __half*>(e.residual) + at, cnt, r);
-    else fp8_load4(static_cast<const __nv_bfloat16*>(e.residual) + at, cnt, r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(v[i], r[i]);
+    if (e.residual) v[i] = __fadd_rn(v[i], res[i]);
   }
   if (e.y_type == kFp8Type) {
     uint32_t a = 0;
@@ -151,7 +182,7 @@ __device__ __forceinline__ void fp8_finish(const Fp8Epilogue& e, int64_t m, int 
     const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, a));
     const uint32_t w = fp8_pack4(v[0], v[1], v[2], v[3], fp8_inv_scale(byte));
     uint8_t* q = static_cast<uint8_t*>(e.y) + m * e.y_ld + n;
-    if (cnt == 4) {
+    if (cnt >= 4) {
       *reinterpret_cast<uint32_t*>(q) = w;
     } else {
       for (int i = 0; i < cnt; ++i) q[i] = (uint8_t)(w >> (8 * i));
@@ -161,9 +192,22 @@ __device__ __forceinline__ void fp8_finish(const Fp8Epilogue& e, int64_t m, int 
   }
   if (cnt < 1) return;
   const int64_t at = m * e.y_ld + n;
-  if (e.y_type == FTB_F32) fp8_store4(static_cast<float*>(e.y) + at, cnt, v);
-  else if (e.y_type == FTB_F16) fp8_store4(static_cast<__half*>(e.y) + at, cnt, v);
-  else fp8_store4(static_cast<__nv_bfloat16*>(e.y) + at, cnt, v);
+  if (e.y_type == FTB_F32) fp8_store4(static_cast<float*>(e.y) + at, cnt, e.y_vec, v);
+  else if (e.y_type == FTB_F16) fp8_store4(static_cast<__half*>(e.y) + at, cnt, e.y_vec, v);
+  else fp8_store4(static_cast<__nv_bfloat16*>(e.y) + at, cnt, e.y_vec, v);
+}
+
+// The address in CTA `rank` of the cluster of the shared variable at `addr`.
+__device__ __forceinline__ uint32_t cluster_map(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void ld_cluster4(uint32_t addr, float (&v)[4]) {
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+               : "r"(addr)
+               : "memory");
 }
 
 template <int NT>
@@ -181,7 +225,7 @@ struct Fp8TileSmem {
   static_assert(NT * 128 * 4 <= STAGES * STAGE_BYTES, "the result tile reuses the ring");
 };
 
-template <int NT>
+template <int NT, int SPLIT>
 __global__ void __launch_bounds__(kFp8Threads) fp8_tile_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                const __grid_constant__ CUtensorMap map_a,
                                                                const Fp8Params p) {
@@ -200,10 +244,15 @@ __global__ void __launch_bounds__(kFp8Threads) fp8_tile_kernel(const __grid_cons
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned n_tiles = (unsigned)(p.N + 127) / 128u;
-  const int n0 = (int)(blockIdx.x % n_tiles) * 128;
-  const int m0 = (int)(blockIdx.x / n_tiles) * NT;
+  const unsigned tile_id = blockIdx.x / SPLIT;
+  const int n0 = (int)(tile_id % n_tiles) * 128;
+  const int m0 = (int)(tile_id / n_tiles) * NT;
   const int nk = (p.K + kFp8Block - 1) / kFp8Block;
-  const int kb0 = 0, kb1 = nk;
+  // this CTA's k-blocks: whole groups of four, so that its scale words start
+  // at byte 0; the last CTAs of a cluster may have none
+  const int rank = SPLIT > 1 ? (int)cluster_ctarank() : 0;
+  const int per = ((nk + 3) / 4 + SPLIT - 1) / SPLIT * 4;
+  const int kb0 = min(nk, rank * per), kb1 = min(nk, kb0 + per);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -232,6 +281,12 @@ __global__ void __launch_bounds__(kFp8Threads) fp8_tile_kernel(const __grid_cons
   grid_dep_trigger();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_sf = tmem + L::D_COLS;
+  float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of this lane's outputs
+  if (p.e.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n0 + 4 * lane + i < p.N) bias[i] = __ldg(p.e.bias + n0 + 4 * lane + i);
+  }
 
   if (warp == 0) {
     bool ok = true;
@@ -308,13 +363,14 @@ __global__ void __launch_bounds__(kFp8Threads) fp8_tile_kernel(const __grid_cons
   }
   __syncwarp();
   float* tile = reinterpret_cast<float*>(smem);  // [NT][128]
-  if (warp >= 4) {
+  const int tokens = min(NT, p.M - m0);
+  if (warp >= 4 && kb0 < kb1) {
     const bool ok = mbar_wait_warp(done, 0, abort_flag, p.err, 7);
     tc_fence_after();
     if (ok) {
       const int q = warp & 3;
 #pragma unroll 1
-      for (int c0 = 0; c0 < NT; c0 += 32) {
+      for (int c0 = 0; c0 < tokens; c0 += 32) {
         uint32_t r[32];
         FTB_TMEM_LD32(tmem + c0 + ((uint32_t)(q * 32) << 16), r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -325,18 +381,50 @@ __global__ void __launch_bounds__(kFp8Threads) fp8_tile_kernel(const __grid_cons
     }
     tc_fence_before();
   }
-  __syncthreads();
+  if (SPLIT > 1) cluster_sync_all();
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::TMEM_COLS)
                  : "memory");
   }
-  if (*abort_flag) return;
-  for (int t = warp; t < NT && m0 + t < p.M; t += kFp8Threads / 32) {
-    const float4 f = *reinterpret_cast<const float4*>(tile + t * 128 + lane * 4);
-    float v[4] = {f.x, f.y, f.z, f.w};
-    fp8_finish(p.e, m0 + t, n0, p.N, lane, v);
+  // each CTA finishes its share of the tokens, U per warp at a time (all
+  // their loads in flight together): the partial sums in rank order, of the
+  // CTAs that had k-blocks
+  constexpr int U = SPLIT <= 2 ? 8 : 16 / SPLIT, STEP = SPLIT * (kFp8Threads / 32);
+  const int parts = (nk + per - 1) / per;
+  const int n = n0 + 4 * lane;
+  for (int t0 = rank + SPLIT * warp; t0 < tokens; t0 += U * STEP) {
+    float v[U][SPLIT][4], res[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * STEP;
+      if (t >= tokens) break;
+      const float* at = tile + t * 128 + lane * 4;
+      if constexpr (SPLIT == 1) {
+        const float4 f = *reinterpret_cast<const float4*>(at);
+        v[u][0][0] = f.x, v[u][0][1] = f.y, v[u][0][2] = f.z, v[u][0][3] = f.w;
+      } else {
+#pragma unroll
+        for (int r = 0; r < SPLIT; ++r)
+          if (r < parts) ld_cluster4(cluster_map(smem_u32(at), r), v[u][r]);
+      }
+      if (p.e.residual) fp8_residual(p.e, m0 + t, n, p.N - n, res[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * STEP;
+      if (t >= tokens) break;
+#pragma unroll
+      for (int r = 1; r < SPLIT; ++r)
+        if (r < parts) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[u][0][i] = __fadd_rn(v[u][0][i], v[u][r][i]);
+        }
+      fp8_finish(p.e, m0 + t, n0, p.N, lane, bias, res[u], v[u][0]);
+    }
   }
+  if (SPLIT > 1) cluster_sync_all();  // no CTA leaves while another reads its sums
 }
 
 // ---------------------------------------------------------------------------
@@ -363,27 +451,82 @@ struct Fp8Operands {
   int64_t w_ld;
 };
 
-template <int NT>
-inline cudaError_t fp8_tile_attributes() {
-  return cudaFuncSetAttribute(fp8_tile_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8TileSmem<NT>::TOTAL);
-}
-
-template <int NT>
+template <int NT, int SPLIT>
 inline cudaError_t launch_fp8_tile(const Fp8Operands& o, const Fp8Params& p, cudaStream_t s) {
   CUtensorMap map_w, map_a;
   if (!make_map_fp8(&map_w, o.w, p.N, p.K, o.w_ld, 128) || !make_map_fp8(&map_a, o.a, p.M, p.K, o.a_ld, NT))
     return cudaErrorInvalidValue;
-  const int64_t tiles = ((int64_t)(p.N + 127) / 128) * (((int64_t)p.M + NT - 1) / NT);
-  if (tiles > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  const dim3 grid((unsigned)tiles);
-  return pdl_launch(fp8_tile_kernel<NT>, grid, dim3(kFp8Threads), Fp8TileSmem<NT>::TOTAL, s, map_w, map_a, p);
+  const int64_t ctas = (((int64_t)p.N + 127) / 128) * (((int64_t)p.M + NT - 1) / NT) * SPLIT;
+  if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kFp8Threads);
+  cfg.dynamicSmemBytes = Fp8TileSmem<NT>::TOTAL;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = SPLIT;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = SPLIT > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, fp8_tile_kernel<NT, SPLIT>, map_w, map_a, p);
 }
 
-inline cudaError_t launch_fp8_linear(const Fp8Operands& o, const Fp8Params& p, cudaStream_t s) {
-  if (p.M <= 16) return launch_fp8_tile<16>(o, p, s);
-  if (p.M <= 32) return launch_fp8_tile<32>(o, p, s);
-  if (p.M <= 64) return launch_fp8_tile<64>(o, p, s);
-  return launch_fp8_tile<128>(o, p, s);
+// NT tokens per tile; `split` CTAs (1, 2, 4 or 8: a cluster) share its k-blocks.
+template <int NT>
+inline cudaError_t launch_fp8_tile(const Fp8Operands& o, const Fp8Params& p, int split, cudaStream_t s) {
+  switch (split) {
+    case 1: return launch_fp8_tile<NT, 1>(o, p, s);
+    case 2: return launch_fp8_tile<NT, 2>(o, p, s);
+    case 4: return launch_fp8_tile<NT, 4>(o, p, s);
+    default: return launch_fp8_tile<NT, 8>(o, p, s);
+  }
+}
+
+template <int NT, int SPLIT>
+inline cudaError_t fp8_tile_attribute() {
+  return cudaFuncSetAttribute(fp8_tile_kernel<NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Fp8TileSmem<NT>::TOTAL);
+}
+template <int NT>
+inline cudaError_t fp8_tile_attributes() {
+  cudaError_t e = fp8_tile_attribute<NT, 1>();
+  if (e == cudaSuccess) e = fp8_tile_attribute<NT, 2>();
+  if (e == cudaSuccess) e = fp8_tile_attribute<NT, 4>();
+  if (e == cudaSuccess) e = fp8_tile_attribute<NT, 8>();
+  return e;
+}
+
+// CTAs of the tile kernel resident at once in clusters of 1, 2, 4 and 8 (the
+// widest tile; the narrower ones have the same two CTAs per SM).
+template <int SPLIT>
+inline cudaError_t fp8_tile_slots1(int* slots) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(SPLIT);
+  cfg.blockDim = dim3(kFp8Threads);
+  cfg.dynamicSmemBytes = Fp8TileSmem<128>::TOTAL;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = SPLIT;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, fp8_tile_kernel<128, SPLIT>, &cfg);
+  if (e != cudaSuccess) return e;
+  *slots = clusters * SPLIT;
+  return clusters > 0 ? cudaSuccess : cudaErrorInvalidConfiguration;
+}
+inline cudaError_t fp8_tile_slots(int (&slots)[4]) {
+  cudaError_t e = fp8_tile_slots1<1>(&slots[0]);
+  if (e == cudaSuccess) e = fp8_tile_slots1<2>(&slots[1]);
+  if (e == cudaSuccess) e = fp8_tile_slots1<4>(&slots[2]);
+  if (e == cudaSuccess) e = fp8_tile_slots1<8>(&slots[3]);
+  return e;
 }
 
 }  // namespace ftb

@@ -1,0 +1,563 @@
+// Block-scaled 8-bit matrix product on SM pairs, for many tokens: the
+// arithmetic of fp8_gemm.cuh on 256 x 256 tiles (tcgen05 cta_group::2).
+//
+// CTA r of a pair holds token rows [128 r, 128 r + 128) and weight rows
+// [128 r, 128 r + 128) of the tile, so each SM loads 32 KB per k-block of 128
+// for 128 x 256 x 128 products, half of what two separate 128 x 256 tiles
+// would load; its tensor memory receives its 128 token rows.  Both CTAs need
+// the scales of their own tokens and of all 256 outputs.
+//
+// Tensor memory: accumulators at columns [0, 256) and [224, 480), scale
+// factors at [480, 512).  The two accumulators share columns 224 .. 255, so
+// that both fit beside the scale factors: the epilogue reads the shared
+// columns of a tile first, and the next tile's products wait for that alone.
+//
+// Persistent pairs walk the tiles in bands of eight row blocks (the pairs at
+// work then share 8 + 9 operand blocks of 256 rows through L2, not 2 + 37).
+// Twelve warps per CTA:
+//   warp 0     TMA producer of this CTA's rows (its own barriers);
+//   warp 1     tensor memory; in the leader CTA the MMAs of the pair;
+//   warp 2     scale factors of this CTA, four k-blocks at a time;
+//   warp 3     passes this CTA's landed stages on to the leader;
+//   warps 4-11 epilogue: a lane quarter and one half of the columns each,
+//              32 columns at a time through a staging box and a TMA store
+//              (plain row stores where the output's rows are not 16-byte
+//              aligned).  A quantised output needs the largest of its 128
+//              columns first: they are read from tensor memory twice.
+#pragma once
+
+#include "fp8_gemm.cuh"
+
+namespace ftb {
+
+constexpr int kFp8PairThreads = 384;
+constexpr int kFp8PairStages = 5;
+constexpr int kFp8Band = 8;
+
+struct Fp8PairSmem {
+  static constexpr int OPERAND_BYTES = 128 * 128;
+  static constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
+  static constexpr int SF_BYTES = 512 + 1024;
+  static constexpr int STAGING = 8 * 2 * 2048;  // two boxes per epilogue warp
+  static constexpr int SF_OFF = kFp8PairStages * STAGE_BYTES + STAGING;
+  static constexpr int BAR_OFF = SF_OFF + 2 * SF_BYTES;
+  static constexpr int NBAR = 3 * kFp8PairStages + 4 + 4 + 2;
+  static constexpr int TOTAL = 1024 + BAR_OFF + 8 * NBAR + 16;
+  static_assert(TOTAL <= 227 * 1024, "shared memory budget");
+};
+
+struct Fp8PairParams {
+  Fp8Params p;
+  int y_tma;     // the output has a TMA map
+  int bias_vec;  // bias is 16-byte aligned
+  int stall_test;
+};
+
+__device__ __forceinline__ void umma2_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+      : "memory");
+}
+
+// In both CTAs: 512 bytes of this CTA's scale factors into its tensor memory.
+__device__ __forceinline__ void tmem2_copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t smem) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(smem)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+
+// Tile number -> token and output block, in bands of kFp8Band token blocks.
+struct Fp8Tiles {
+  int tm, tn;
+  __device__ __forceinline__ void at(int t, int& m0, int& n0) const {
+    const int band = t / (kFp8Band * tn), in = t - band * kFp8Band * tn;
+    const int h = min(kFp8Band, tm - band * kFp8Band);
+    m0 = (band * kFp8Band + in % h) * 256;
+    n0 = in / h * 256;
+  }
+};
+
+// 32 consecutive columns of `row` from n as fp32 (zeros past N).
+template <typename T>
+__device__ __forceinline__ void add_residual32(const T* row, int n, int N, bool vec, float (&v)[32]) {
+  if (vec && n + 32 <= N) {
+    constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 32 / E; ++i) {
+      const uint4 u = reinterpret_cast<const uint4*>(row + n)[i];
+      T t[E];
+      memcpy(t, &u, 16);
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[i * E + j] = __fadd_rn(v[i * E + j], to_f32(t[j]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (n + i < N) v[i] = __fadd_rn(v[i], to_f32(row[n + i]));
+  }
+}
+
+// The epilogue's arithmetic on 32 columns of one token.
+__device__ __forceinline__ void fp8_epilogue32(const Fp8PairParams& q, int64_t m, int n, float (&v)[32]) {
+  const Fp8Epilogue& e = q.p.e;
+  const int N = q.p.N;
+  if (e.bias) {
+    if (q.bias_vec && n + 32 <= N) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>(e.bias + n) + i);
+        v[4 * i] = __fadd_rn(v[4 * i], b.x);
+        v[4 * i + 1] = __fadd_rn(v[4 * i + 1], b.y);
+        v[4 * i + 2] = __fadd_rn(v[4 * i + 2], b.z);
+        v[4 * i + 3] = __fadd_rn(v[4 * i + 3], b.w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (n + i < N) v[i] = __fadd_rn(v[i], __ldg(e.bias + n + i));
+    }
+  }
+  if (e.relu) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = (v[i] != v[i] || v[i] > 0.0f) ? v[i] : 0.0f;
+  }
+  if (e.residual && m < q.p.M) {
+    if (e.res_type == FTB_F32) add_residual32(static_cast<const float*>(e.residual) + m * e.res_ld, n, N, e.res_vec, v);
+    else if (e.res_type == FTB_F16)
+      add_residual32(static_cast<const __half*>(e.residual) + m * e.res_ld, n, N, e.res_vec, v);
+    else add_residual32(static_cast<const __nv_bfloat16*>(e.residual) + m * e.res_ld, n, N, e.res_vec, v);
+  }
+}
+
+// One epilogue warp's staging: two boxes of 32 rows x 64 bytes (64-byte
+// swizzle; a quantised output's rows are 32 bytes, unswizzled).
+struct Fp8Staging {
+  uint32_t base;
+  uint32_t count;  // boxes so far
+  int lane;
+  __device__ __forceinline__ uint32_t begin() {
+    if (lane == 0) bulk_wait_read1();
+    __syncwarp();
+    return base + (count & 1u) * 2048u;
+  }
+  __device__ __forceinline__ void put64(uint32_t box, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
+    st_shared4(box + lane * 64 + ((chunk ^ ((lane >> 1) & 3)) << 4), a, b, c, d);
+  }
+  __device__ __forceinline__ void end(const CUtensorMap* map, int n, int m, uint32_t box) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, n, m, box);
+      bulk_commit();
+    }
+    ++count;
+  }
+};
+
+// Rows of a staged box into an output without TMA: its rows are not 16-byte
+// aligned, or the box reaches past the last column (a TMA store clips columns
+// in units of 16 bytes only).  C columns from n, R rows at a time.
+template <typename U>
+__device__ __forceinline__ void store_box_rows(uint32_t box, U* y, int64_t ld, int m0, int n, int M, int N, int lane) {
+  constexpr int E = (int)sizeof(U), W = E == 1 ? 32 : 64, C = W / E, R = 32 / C;
+  __syncwarp();
+  for (int r0 = 0; r0 < 32; r0 += R) {
+    const int r = r0 + lane / C, c = lane % C;
+    const uint32_t swz = E == 1 ? 0u : (uint32_t)((r >> 1) & 3);
+    const uint32_t at = box + r * W + ((((uint32_t)(c * E) >> 4) ^ swz) << 4) + ((c * E) & 15);
+    uint32_t u;
+    if constexpr (E == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(at));
+    else if constexpr (E == 2) asm volatile("{ .reg .u16 t; ld.shared.u16 t, [%1]; cvt.u32.u16 %0, t; }" : "=r"(u) : "r"(at));
+    else asm volatile("ld.shared.u8 %0, [%1];" : "=r"(u) : "r"(at));
+    if (m0 + r < M && n + c < N) y[(int64_t)(m0 + r) * ld + n + c] = (U)u;
+  }
+  __syncwarp();
+}
+
+// 32 finished columns of 32 tokens (lane = token) into a plain output.
+template <typename T>
+__device__ __forceinline__ void store_plain32(const Fp8PairParams& q, const CUtensorMap* map, Fp8Staging& st, int m0,
+                                              int n, const float (&v)[32]) {
+  constexpr int C = 64 / (int)sizeof(T);  // columns per box
+#pragma unroll
+  for (int b = 0; b < 32 / C; ++b) {
+    if (n + b * C >= q.p.N) break;
+    const uint32_t box = st.begin();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      T t[C / 4];
+#pragma unroll
+      for (int j = 0; j < C / 4; ++j) t[j] = from_f32<T>(v[b * C + i * (C / 4) + j]);
+      uint32_t u[4];
+      memcpy(u, t, 16);
+      st.put64(box, i, u[0], u[1], u[2], u[3]);
+    }
+    if (q.y_tma && n + (b + 1) * C <= q.p.N) {
+      st.end(map, n + b * C, m0, box);
+    } else {
+      using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+      store_box_rows(box, static_cast<U*>(q.p.e.y), q.p.e.y_ld, m0, n + b * C, q.p.M, q.p.N, st.lane);
+    }
+  }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
+    fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                    const __grid_constant__ CUtensorMap map_y, const Fp8PairParams q) {
+  using L = Fp8PairSmem;
+  constexpr int STAGES = kFp8PairStages;
+  constexpr uint32_t kAcc1 = 224, kSf = 480;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* staging = smem + STAGES * L::STAGE_BYTES;
+  uint8_t* sf = smem + L::SF_OFF;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);  // this CTA's loads landed
+  uint64_t* ready = full + STAGES;      // leader: both CTAs' loads landed
+  uint64_t* empty = ready + STAGES;     // the pair's MMAs done with the stage
+  uint64_t* sf_full = empty + STAGES;   // [2] leader: both CTAs' scale factors staged
+  uint64_t* sf_empty = sf_full + 2;     // [2] the pair's MMAs done with them
+  uint64_t* accf = sf_empty + 2;        // [2] accumulator complete
+  uint64_t* acce = accf + 2;            // [2] leader: accumulator read (16 warps)
+  uint64_t* shared_cols = acce + 2;     // leader: the shared columns read (16 warps), once per tile
+  uint64_t* drain = shared_cols + 1;    // leader: MMAs retired after an abort
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 1) + 1;
+
+  const Fp8Params& p = q.p;
+  const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nk = (p.K + kFp8Block - 1) / kFp8Block;
+  Fp8Tiles tiles{(p.M + 255) / 256, (p.N + 255) / 256};
+  const int ntiles = tiles.tm * tiles.tn;
+  const int pair = (int)cluster_index(), npairs = (int)cluster_count();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&ready[s], 2);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sf_full[s], 2);
+      mbar_init(&sf_empty[s], 1);
+      mbar_init(&accf[s], 1);
+      mbar_init(&acce[s], 16);
+    }
+    mbar_init(shared_cols, 16);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(const_cast<uint32_t*>(tmem_slot))),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  grid_dep_wait();
+  grid_dep_trigger();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t peer_abort = cluster_addr(const_cast<int*>(abort_flag), peer);
+
+  if (warp == 0) {
+    bool ok = true;
+    uint32_t it = 0;
+    for (int t = pair; t < ntiles && ok; t += npairs) {
+      int m0, n0;
+      tiles.at(t, m0, n0);
+      m0 += (int)rank * 128;
+      n0 += (int)rank * 128;
+      for (int kb = 0; kb < nk; ++kb, ++it) {
+        const uint32_t s = it % STAGES;
+        if (!(ok = pair_wait_warp(&empty[s], ((it / STAGES) & 1u) ^ 1u, abort_flag, peer_abort, p.err, 11))) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&full[s], L::STAGE_BYTES);
+          tma_load_2d(smem + s * L::STAGE_BYTES, &map_a, kb * kFp8Block, m0, &full[s]);
+          tma_load_2d(smem + s * L::STAGE_BYTES + L::OPERAND_BYTES, &map_w, kb * kFp8Block, n0, &full[s]);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok)  // the copies in flight land before the CTA leaves
+      for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
+        pair_wait_warp(&full[j % STAGES], (j / STAGES) & 1u, abort_flag, peer_abort, p.err, 12, /*ignore_abort=*/true);
+  } else if (warp == 1) {
+    if (rank == 0) {
+      bool ok = true;
+      uint32_t it = 0, sg = 0, tc = 0;
+      if (q.stall_test) ok = pair_wait_warp(drain, 0, abort_flag, peer_abort, p.err, 13);
+      for (int t = pair; t < ntiles && ok; t += npairs, ++tc) {
+        const uint32_t b = tc & 1u;
+        if (!(ok = pair_wait_warp(&acce[b], ((tc >> 1) & 1u) ^ 1u, abort_flag, peer_abort, p.err, 14))) break;
+        if (tc > 0 &&
+            !(ok = pair_wait_warp(shared_cols, (tc - 1) & 1u, abort_flag, peer_abort, p.err, 15)))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem + b * kAcc1;
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const uint32_t slot = sg & 1u, byte = (uint32_t)kb & 3u;
+          const uint32_t sfa = tmem + kSf + slot * 16, sfb = sfa + 4;
+          if (byte == 0) {
+            if (!(ok = pair_wait_warp(&sf_full[slot], (sg >> 1) & 1u, abort_flag, peer_abort, p.err, 16))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t at = smem_u32(sf + slot * L::SF_BYTES);
+              tmem2_copy_scales(sfa, fp8_scale_desc(at));
+              tmem2_copy_scales(sfb, fp8_scale_desc(at + 512));
+              tmem2_copy_scales(sfb + 4, fp8_scale_desc(at + 1024));
+            }
+            __syncwarp();
+          }
+          const uint32_t s = it % STAGES;
+          if (!(ok = pair_wait_warp(&ready[s], (it / STAGES) & 1u, abort_flag, peer_abort, p.err, 17))) break;
+          tc_fence_after();
+          const bool last = kb + 1 == nk, group_end = byte == 3u || last;
+          const uint32_t empty_peer = cluster_addr(&empty[s], peer);
+          const uint32_t sf_empty_peer = cluster_addr(&sf_empty[slot], peer);
+          const uint32_t accf_peer = cluster_addr(&accf[b], peer);
+          if (elect_one()) {
+            const uint32_t a = smem_u32(smem + s * L::STAGE_BYTES), w = a + L::OPERAND_BYTES;
+            const uint32_t idesc = fp8_idesc(256, 256, (int)byte);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              umma2_fp8(d, fp8_operand_desc(a + j * 32), fp8_operand_desc(w + j * 32), idesc, sfa, sfb,
+                        (kb > 0 || j > 0) ? 1u : 0u);
+            umma2_commit(smem_u32(&empty[s]));
+            umma2_commit(empty_peer);
+            if (group_end) {
+              umma2_commit(smem_u32(&sf_empty[slot]));
+              umma2_commit(sf_empty_peer);
+            }
+            if (last) {
+              umma2_commit(smem_u32(&accf[b]));
+              umma2_commit(accf_peer);
+            }
+          }
+          __syncwarp();
+          if (group_end) ++sg;
+        }
+      }
+      if (!ok) {
+        if (elect_one()) umma2_commit(smem_u32(drain));
+        __syncwarp();
+        pair_wait_warp(drain, 0, abort_flag, peer_abort, p.err, 18, /*ignore_abort=*/true);
+      }
+    }
+  } else if (warp == 2) {
+    bool ok = true;
+    uint32_t sg = 0;
+    const int groups = (nk + 3) >> 2, nb = (p.N + kFp8Block - 1) / kFp8Block;
+    for (int t = pair; t < ntiles && ok; t += npairs) {
+      int m0, n0;
+      tiles.at(t, m0, n0);
+      const int r0 = m0 + (int)rank * 128 + lane, b0 = n0 / kFp8Block;
+      const uint8_t* w0 = p.sw + (int64_t)b0 * p.sw_ld;
+      const uint8_t* w1 = p.sw + (int64_t)min(b0 + 1, nb - 1) * p.sw_ld;
+      for (int g = 0; g < groups; ++g, ++sg) {
+        const uint32_t slot = sg & 1u;
+        const uint32_t x = fp8_scale_word(w0, g, nk), y = fp8_scale_word(w1, g, nk);
+        uint32_t a[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          a[j] = r0 + 32 * j < p.M ? fp8_scale_word(p.sa + (int64_t)(r0 + 32 * j) * p.sa_ld, g, nk) : 0u;
+        if (!(ok = pair_wait_warp(&sf_empty[slot], ((sg >> 1) & 1u) ^ 1u, abort_flag, peer_abort, p.err, 19))) break;
+        const uint32_t at = smem_u32(sf + slot * L::SF_BYTES) + lane * 16;
+        st_shared4(at, a[0], a[1], a[2], a[3]);
+        st_shared4(at + 512, x, x, x, x);
+        st_shared4(at + 1024, y, y, y, y);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(cluster_addr(&sf_full[slot], 0));
+      }
+    }
+  } else if (warp == 3) {
+    bool ok = true;
+    uint32_t it = 0;
+    for (int t = pair; t < ntiles && ok; t += npairs) {
+      for (int kb = 0; kb < nk; ++kb, ++it) {
+        const uint32_t s = it % STAGES;
+        if (!(ok = pair_wait_warp(&full[s], (it / STAGES) & 1u, abort_flag, peer_abort, p.err, 20))) break;
+        if (lane == 0) mbar_arrive_cluster(cluster_addr(&ready[s], 0));
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    Fp8Staging st{smem_u32(staging) + (uint32_t)(warp - 4) * 4096u, 0u, lane};
+    const uint32_t shared_leader = cluster_addr(shared_cols, 0);
+    uint32_t tc = 0;
+    for (int t = pair; t < ntiles; t += npairs, ++tc) {
+      const uint32_t b = tc & 1u;
+      if (!pair_wait_warp(&accf[b], (tc >> 1) & 1u, abort_flag, peer_abort, p.err, 21)) break;
+      tc_fence_after();
+      int m0, n0;
+      tiles.at(t, m0, n0);
+      m0 += (int)rank * 128 + quarter * 32;
+      n0 += half * 128;
+      const int64_t m = (int64_t)m0 + lane;
+      const uint32_t acc = tmem + b * kAcc1 + (uint32_t)half * 128 + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t acce_leader = cluster_addr(&acce[b], 0);
+      // the chunk that holds the shared columns comes first: the last of
+      // accumulator 0's upper half, the first of accumulator 1's lower half
+      auto chunk = [&](int j) { return half ? 3 - j : j; };
+      auto load = [&](int j, float (&v)[32]) {
+        uint32_t r[32];
+        FTB_TMEM_LD32(acc + 32 * chunk(j), r);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+      };
+      auto release = [&](uint32_t leader_bar) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(leader_bar);
+      };
+      if (p.e.y_type != kFp8Type) {
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+          float v[32];
+          load(j, v);
+          if (j == 0) release(shared_leader);
+          if (j == 3) release(acce_leader);
+          const int n = n0 + 32 * chunk(j);
+          if (n >= p.N || m0 >= p.M) continue;
+          fp8_epilogue32(q, m, n, v);
+          if (p.e.y_type == FTB_F32) store_plain32<float>(q, &map_y, st, m0, n, v);
+          else if (p.e.y_type == FTB_F16) store_plain32<__half>(q, &map_y, st, m0, n, v);
+          else store_plain32<__nv_bfloat16>(q, &map_y, st, m0, n, v);
+        }
+      } else {
+        const bool inside = n0 < p.N && m0 < p.M;
+        float first[32];
+        uint32_t amax = 0;
+        auto finish = [&](int j, float (&v)[32]) {
+          const int n = n0 + 32 * chunk(j);
+          if (inside && n < p.N) fp8_epilogue32(q, m, n, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (n + i >= p.N) v[i] = 0.0f;
+        };
+        load(0, first);
+        release(shared_leader);
+        finish(0, first);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) amax = max(amax, finite_abs_bits(first[i]));
+#pragma unroll 1
+        for (int j = 1; j < 4; ++j) {
+          float v[32];
+          load(j, v);
+          finish(j, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) amax = max(amax, finite_abs_bits(v[i]));
+        }
+        const uint32_t byte = fp8_scale_byte(amax);
+        const float inv = fp8_inv_scale(byte);
+        if (inside && m < p.M) p.e.ys[m * p.e.ys_ld + n0 / kFp8Block] = (uint8_t)byte;
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+          float v[32];
+          if (j == 0) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = first[i];
+          } else {
+            load(j, v);
+            if (j == 3) release(acce_leader);
+            finish(j, v);
+          }
+          const int n = n0 + 32 * chunk(j);
+          if (!inside || n >= p.N) continue;
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            w[i] = fp8_pack4(nan_unless_finite(v[4 * i]), nan_unless_finite(v[4 * i + 1]),
+                             nan_unless_finite(v[4 * i + 2]), nan_unless_finite(v[4 * i + 3]), inv);
+          const uint32_t box = st.begin();
+          st_shared4(box + lane * 32, w[0], w[1], w[2], w[3]);
+          st_shared4(box + lane * 32 + 16, w[4], w[5], w[6], w[7]);
+          if (n + 32 <= p.N) st.end(&map_y, n, m0, box);
+          else store_box_rows(box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, m0, n, p.M, p.N, lane);
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();  // this warp's stores are complete before the CTA leaves
+  }
+  tc_fence_before();
+  cluster_sync_all();  // no MMA of the pair and no remote arrival is still in flight
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// Shared-memory attribute and the number of pairs that are resident at once.
+inline cudaError_t fp8_pair_prepare(int* pairs) {
+  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8PairSmem::TOTAL);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2, 1, 1);
+  cfg.blockDim = dim3(kFp8PairThreads, 1, 1);
+  cfg.dynamicSmemBytes = Fp8PairSmem::TOTAL;
+  e = cudaOccupancyMaxActiveClusters(pairs, fp8_pair_kernel, &cfg);
+  if (e == cudaSuccess && *pairs <= 0) e = cudaErrorInvalidConfiguration;
+  return e;
+}
+
+// The output as TMA stores it: boxes of 32 rows x 64 bytes (64-byte swizzle),
+// of 32 x 32 bytes for a quantised one.  False where its rows are not 16-byte
+// aligned.
+inline bool make_map_fp8_out(CUtensorMap* map, const Fp8Epilogue& e, int64_t m, int64_t n) {
+  const int size = e.y_type == FTB_F32 ? 4 : e.y_type == kFp8Type ? 1 : 2;
+  if ((reinterpret_cast<uintptr_t>(e.y) & 15) || (e.y_ld * size) % 16) return false;
+  PFN_encodeTiled enc = tma_encoder();
+  if (!enc) return false;
+  const int bytes = e.y_type == kFp8Type ? 32 : 64;
+  cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)m};
+  cuuint64_t strides[1] = {(cuuint64_t)(e.y_ld * size)};
+  cuuint32_t box[2] = {(cuuint32_t)(bytes / size), 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = size == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  return enc(map, type, 2, e.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+inline cudaError_t launch_fp8_pair(const Fp8Operands& o, const Fp8Params& p, int max_pairs, int stall_test,
+                                   cudaStream_t s) {
+  CUtensorMap map_a, map_w, map_y;
+  if (!make_map_fp8(&map_a, o.a, p.M, p.K, o.a_ld, 128) || !make_map_fp8(&map_w, o.w, p.N, p.K, o.w_ld, 128))
+    return cudaErrorInvalidValue;
+  Fp8PairParams q{};
+  q.p = p;
+  memset(&map_y, 0, sizeof(map_y));
+  q.y_tma = make_map_fp8_out(&map_y, p.e, p.M, p.N) ? 1 : 0;
+  if (!q.y_tma && p.e.y_type == kFp8Type) return cudaErrorInvalidValue;
+  q.bias_vec = (reinterpret_cast<uintptr_t>(p.e.bias) & 15) == 0;
+  q.stall_test = stall_test;
+  const int64_t tiles = (((int64_t)p.M + 255) / 256) * (((int64_t)p.N + 255) / 256);
+  if (tiles > 0x3fffffff) return cudaErrorInvalidConfiguration;
+  const unsigned pairs = (unsigned)std::min<int64_t>(tiles, max_pairs);
+  return pdl_launch(fp8_pair_kernel, dim3(2 * pairs), dim3(kFp8PairThreads), Fp8PairSmem::TOTAL, s, map_a, map_w,
+                    map_y, q);
+}
+
+}  // namespace ftb

@@ -7,10 +7,12 @@
 // 16-bit type, 4 of fp32.  A quantisation block of 128 is then 16 or 32
 // neighbouring lanes, so its largest value is a few shuffles away.  Rows whose
 // base, stride or length keep them off 16-byte boundaries take the same
-// kernels with element-wise loads and stores (VECTOR false).
+// kernels with element-wise loads and stores.
 #pragma once
 
 #include <algorithm>
+#include <cstring>
+#include <type_traits>
 
 #include "fp8_format.cuh"
 #include "tc_ptx.cuh"
@@ -37,6 +39,13 @@ struct RowsParams {
 
 template <typename T>
 constexpr int kRowVec = 16 / (int)sizeof(T);
+
+// How a kernel's lanes meet its rows.
+enum RowMode : int {
+  ROW_ELEMENTS,  // element by element
+  ROW_VECTORS,   // 16 bytes at a time; a lane's vector is inside the row or past its end
+  ROW_WHOLE,     // and no lane's vector is past the end
+};
 
 // 16 bytes of T as fp32.
 __device__ __forceinline__ void unpack(const uint4& u, float (&v)[4]) {
@@ -83,12 +92,12 @@ __device__ __forceinline__ uint4 pack_vec(const float (&v)[VEC]) {
 }
 
 // A lane's vector at column c: zeros past k.
-template <typename T, bool VECTOR>
-__device__ __forceinline__ uint4 load_vec(const T* row, int64_t c, int64_t k) {
+template <typename T, RowMode MODE>
+__device__ __forceinline__ uint4 load_vec(const T* row, int c, int k) {
   constexpr int VEC = kRowVec<T>;
   uint4 u = make_uint4(0, 0, 0, 0);
-  if constexpr (VECTOR) {
-    if (c < k) u = *reinterpret_cast<const uint4*>(row + c);
+  if constexpr (MODE != ROW_ELEMENTS) {
+    if (MODE == ROW_WHOLE || c < k) u = *reinterpret_cast<const uint4*>(row + c);
   } else {
     T t[VEC];
 #pragma unroll
@@ -98,10 +107,10 @@ __device__ __forceinline__ uint4 load_vec(const T* row, int64_t c, int64_t k) {
   return u;
 }
 
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void store_vec(T* row, int64_t c, int64_t k, const float (&v)[kRowVec<T>]) {
-  if constexpr (VECTOR) {
-    if (c < k) *reinterpret_cast<uint4*>(row + c) = pack_vec<T>(v);
+template <typename T, RowMode MODE>
+__device__ __forceinline__ void store_vec(T* row, int c, int k, const float (&v)[kRowVec<T>]) {
+  if constexpr (MODE != ROW_ELEMENTS) {
+    if (MODE == ROW_WHOLE || c < k) *reinterpret_cast<uint4*>(row + c) = pack_vec<T>(v);
   } else {
 #pragma unroll
     for (int i = 0; i < kRowVec<T>; ++i)
@@ -109,73 +118,177 @@ __device__ __forceinline__ void store_vec(T* row, int64_t c, int64_t k, const fl
   }
 }
 
-// The largest of the block's 128 / VEC lanes.
-template <int VEC>
-__device__ __forceinline__ uint32_t block_max(uint32_t a) {
-  if constexpr (VEC == 4) return __reduce_max_sync(0xffffffffu, a);
-#pragma unroll
-  for (int o = 8; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-  return a;
+// The scale byte plus one of a lane's largest |x| (as bits), 0 where all are
+// zero, above 0xFF where one is not finite.  Adding 0x1FFFFF carries into the
+// exponent exactly where the mantissa is above 1.75 (see fp8_scale_byte).
+__device__ __forceinline__ uint32_t scale_code(uint32_t a) {
+  const int b = (int)((a + 0x1FFFFFu) >> 23) - 7;
+  const uint32_t c = (uint32_t)max(b, 1);
+  return a == 0u ? 0u : a >= 0x7F800000u ? 0x1FFu : c;
 }
 
-// A warp quantises its lanes' vectors (VEC 8: two blocks, VEC 4: one) and
-// stores values and scales; every lane takes part, also past k.
+// The largest code of each block: 128 / VEC neighbouring lanes.  For VEC 8 two
+// vectors' codes share a word, which halves the shuffles.
+template <int VEC, int N>
+__device__ __forceinline__ void block_codes(uint32_t (&code)[N]) {
+  if constexpr (VEC == 4) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) code[n] = __reduce_max_sync(0xffffffffu, code[n]);
+  } else {
+    constexpr int W = (N + 1) / 2;
+    uint32_t w[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = code[2 * i] | (2 * i + 1 < N ? code[(2 * i + 1) % N] << 16 : 0u);
+#pragma unroll
+    for (int o = 8; o; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = __vmaxu2(w[i], __shfl_xor_sync(0xffffffffu, w[i], o));
+#pragma unroll
+    for (int n = 0; n < N; ++n) code[n] = (n & 1) ? w[n / 2] >> 16 : w[n / 2] & 0xFFFFu;
+  }
+}
+
+// Where a lane's vector goes: its place in the row's values and its block's
+// place among the scales, and how many columns the row still has there.
+struct VecPlace {
+  uint8_t *q, *s;
+  int left;
+};
+
+// A warp quantises N vectors per lane at once (a vector's 32 lanes are two
+// blocks for VEC 8, one for VEC 4) and stores values and scales where at(n)
+// says.  Every lane takes part, also past the row's end.  `a`: the bits of
+// each vector's largest |x|.  WHOLE: every vector is inside its row.
+template <bool WHOLE, int VEC, int N, typename At>
+__device__ __forceinline__ void quantize_vecs(float (&v)[N][VEC], const uint32_t (&a)[N], At&& at) {
+  uint32_t code[N];
+  uint32_t most = 0;
+#pragma unroll
+  for (int n = 0; n < N; ++n) code[n] = scale_code(a[n]), most = max(most, code[n]);
+  if (__any_sync(0xffffffffu, most > 0xFFu)) {
+    // some value is not finite: the scales come from the others
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      uint32_t f = 0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        f = max(f, finite_abs_bits(v[n][i]));
+        v[n][i] = nan_unless_finite(v[n][i]);
+      }
+      code[n] = scale_code(f);
+    }
+  }
+  block_codes<VEC>(code);
+  const bool lead = (threadIdx.x & (kFp8Block / VEC - 1)) == 0;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const uint32_t byte = code[n] ? code[n] - 1u : 127u;
+    const float inv = fp8_inv_scale(byte);
+    const VecPlace o = at(n);
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      w[i] = fp8_pack4(v[n][4 * i], v[n][4 * i + 1], v[n][4 * i + 2], v[n][4 * i + 3], inv);
+    if (WHOLE || o.left >= VEC) {
+      if constexpr (VEC == 8) *reinterpret_cast<uint2*>(o.q) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(o.q) = w[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i < o.left) o.q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+    if (lead && (WHOLE || o.left > 0)) *o.s = (uint8_t)byte;
+  }
+}
+
 template <int VEC>
-__device__ __forceinline__ void quantize_vec(float (&v)[VEC], uint8_t* qrow, uint8_t* srow, int64_t c, int64_t k) {
+__device__ __forceinline__ uint32_t abs_max_bits(const float (&v)[VEC]) {
   uint32_t a = 0;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  a = block_max<VEC>(a);
-  if (__any_sync(0xffffffffu, a >= 0x7F800000u)) {
-    // some value is not finite: the scale comes from the others
-    a = 0;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      a = max(a, finite_abs_bits(v[i]));
-      v[i] = nan_unless_finite(v[i]);
-    }
-    a = block_max<VEC>(a);
-  }
-  const uint32_t byte = fp8_scale_byte(a);
-  const float inv = fp8_inv_scale(byte);
-  uint32_t w[VEC / 4];
-#pragma unroll
-  for (int i = 0; i < VEC / 4; ++i) w[i] = fp8_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
-  if (c + VEC <= k) {
-    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(qrow + c) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(qrow + c) = w[0];
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (c + i < k) qrow[c + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
-  }
-  if (c % kFp8Block == 0 && c < k) srow[c / kFp8Block] = (uint8_t)byte;
+  return a;
 }
 
-// One warp per chunk of kQuantUnits x 32 vectors of a row, its loads issued
-// together.
+// The same from 16 bytes of T: 16-bit types compare two at a time as integers.
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max_bits(const uint4& u) {
+  if constexpr (sizeof(T) == 4) {
+    return max(max(u.x & 0x7FFFFFFFu, u.y & 0x7FFFFFFFu), max(u.z & 0x7FFFFFFFu, u.w & 0x7FFFFFFFu));
+  } else {
+    const uint32_t m = 0x7FFF7FFFu;
+    const uint32_t w = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+    const uint32_t h = max(w >> 16, w & 0xFFFFu);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
+    else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+  }
+}
+
+// A row is cut into units of 32 vectors.  Long rows: grid (rows, CTAs per row),
+// a warp takes N units of a row, all in flight together.
 constexpr int kQuantUnits = 4;
 
-template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const RowsParams p, const uint32_t chunks) {
-  constexpr int VEC = kRowVec<T>;
+template <typename T, RowMode MODE>
+__global__ void __launch_bounds__(256, MODE != ROW_ELEMENTS ? 4 : 1) quantize_rows_kernel(const RowsParams p) {
+  constexpr int VEC = kRowVec<T>, N = kQuantUnits, STEP = 32 * VEC;
   grid_dep_wait();
   grid_dep_trigger();
-  const int64_t warp = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t row = (warp >> 32) == 0 ? (int64_t)((uint32_t)warp / chunks) : warp / chunks;
-  if (row >= p.m) return;
-  const int64_t c0 = ((warp - row * chunks) * kQuantUnits * 32 + (threadIdx.x & 31)) * VEC;
+  const int64_t row = blockIdx.x;
+  const int k = (int)p.k, chunk = (int)(blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5)) * N * STEP;
+  if (chunk >= k) return;
+  const int c = chunk + (int)(threadIdx.x & 31) * VEC;
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
-  uint4 u[kQuantUnits];
+  uint4 u[N];
 #pragma unroll
-  for (int j = 0; j < kQuantUnits; ++j) u[j] = load_vec<T, VECTOR>(x, c0 + j * 32 * VEC, p.k);
+  for (int n = 0; n < N; ++n) u[n] = load_vec<T, MODE>(x, c + n * STEP, k);
+  float v[N][VEC];
+  uint32_t a[N];
 #pragma unroll
-  for (int j = 0; j < kQuantUnits; ++j) {
-    const int64_t c = c0 + j * 32 * VEC;
-    float v[VEC];
-    unpack_vec<T>(u[j], v);
-    quantize_vec<VEC>(v, p.q + row * p.q_ld, p.s + row * p.s_ld, c, p.k);
+  for (int n = 0; n < N; ++n) {
+    a[n] = abs_max_bits<T>(u[n]);
+    unpack_vec<T>(u[n], v[n]);
   }
+  uint8_t *q = p.q + row * p.q_ld + c, *s = p.s + row * p.s_ld + c / kFp8Block;
+  auto at = [&](int n) { return VecPlace{q + n * STEP, s + n * (STEP / kFp8Block), k - c - n * STEP}; };
+  if (chunk + N * STEP <= k) quantize_vecs<true>(v, a, at);
+  else quantize_vecs<false>(v, a, at);
+}
+
+// Short rows, of `blocks` blocks: the lanes of a block take N blocks in turn,
+// counted through all rows.
+template <typename T, RowMode MODE>
+__global__ void __launch_bounds__(256) quantize_short_kernel(const RowsParams p, const uint32_t blocks) {
+  constexpr int VEC = kRowVec<T>, N = kQuantUnits, L = kFp8Block / VEC, B = 32 / L;  // L lanes per block
+  grid_dep_wait();
+  grid_dep_trigger();
+  const int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * N * B, row0 = first / blocks;
+  const int k = (int)p.k, lane = threadIdx.x & 31;
+  const uint32_t b0 = (uint32_t)(first - row0 * blocks) + lane / L;
+  auto place = [&](int n, int64_t& row, int& c) {
+    const uint32_t b = b0 + n * B, r = b / blocks;
+    row = row0 + r;
+    c = row < p.m ? (int)((b - r * blocks) * kFp8Block + lane % L * VEC) : k;
+  };
+  float v[N][VEC];
+  uint32_t a[N];
+  uint4 u[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    int64_t row;
+    int c;
+    place(n, row, c);
+    u[n] = load_vec<T, MODE>(static_cast<const T*>(p.x) + row * p.x_ld, c, k);
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    a[n] = abs_max_bits<T>(u[n]);
+    unpack_vec<T>(u[n], v[n]);
+  }
+  quantize_vecs<false>(v, a, [&](int n) {
+    int64_t row;
+    int c;
+    place(n, row, c);
+    return VecPlace{p.q + row * p.q_ld + c, p.s + row * p.s_ld + c / kFp8Block, k - c};
+  });
 }
 
 // One CTA per 128 x 128 block of a weight: the block's largest value first,
@@ -227,88 +340,99 @@ __device__ __forceinline__ float square_sum(const float (&v)[VEC]) {
   return t[0];
 }
 
-// What follows once a vector's h and its row's scale are known.
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void norm_finish(const RowsParams& p, int64_t row, int64_t c, float scale,
-                                            float (&v)[kRowVec<T>]) {
+// What follows once a row's h and scale are known: N vectors of it, vector n
+// at column c + n step; k = 0 past the last row.
+template <typename T, RowMode MODE, int N>
+__device__ __forceinline__ void norm_finish(const RowsParams& p, int64_t row, int c, int step, int k, float scale,
+                                            float (&v)[N][kRowVec<T>]) {
   constexpr int VEC = kRowVec<T>;
-  if (p.h) store_vec<T, VECTOR>(static_cast<T*>(p.h) + row * p.h_ld, c, p.k, v);
-  if (p.weight) {
-    if (VECTOR && c < p.k) {
+  if (p.h) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) store_vec<T, MODE>(static_cast<T*>(p.h) + row * p.h_ld, c + n * step, k, v[n]);
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int at = c + n * step;
+    if (!p.weight) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[n][i] *= scale;
+    } else if (MODE == ROW_WHOLE || (MODE == ROW_VECTORS && at < k)) {
 #pragma unroll
       for (int i = 0; i < VEC; i += 4) {
-        const float4 w = *reinterpret_cast<const float4*>(p.weight + c + i);
-        v[i] = v[i] * scale * w.x;
-        v[i + 1] = v[i + 1] * scale * w.y;
-        v[i + 2] = v[i + 2] * scale * w.z;
-        v[i + 3] = v[i + 3] * scale * w.w;
+        const float4 w = *reinterpret_cast<const float4*>(p.weight + at + i);
+        v[n][i] = v[n][i] * scale * w.x;
+        v[n][i + 1] = v[n][i + 1] * scale * w.y;
+        v[n][i + 2] = v[n][i + 2] * scale * w.z;
+        v[n][i + 3] = v[n][i + 3] * scale * w.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = c + i < p.k ? v[i] * scale * p.weight[c + i] : 0.0f;
+      for (int i = 0; i < VEC; ++i) v[n][i] = at + i < k ? v[n][i] * scale * p.weight[at + i] : 0.0f;
     }
+  }
+  if (p.q) {
+    uint32_t a[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) a[n] = abs_max_bits(v[n]);
+    uint8_t *q = p.q + row * p.q_ld + c, *s = p.s + row * p.s_ld + c / kFp8Block;
+    auto at = [&](int n) { return VecPlace{q + n * step, s + n * (step / kFp8Block), k - c - n * step}; };
+    quantize_vecs<MODE == ROW_WHOLE>(v, a, at);
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] *= scale;
+    for (int n = 0; n < N; ++n) store_vec<T, MODE>(static_cast<T*>(p.y) + row * p.y_ld, c + n * step, k, v[n]);
   }
-  if (p.q) quantize_vec<VEC>(v, p.q + row * p.q_ld, p.s + row * p.s_ld, c, p.k);
-  else store_vec<T, VECTOR>(static_cast<T*>(p.y) + row * p.y_ld, c, p.k, v);
 }
 
 //   h = x + residual (fp32),  y = h / sqrt(mean(h^2) + eps) weight
-// `warps` warps per row, which keep it in registers: NV vectors per lane.  A
-// CTA has one row, or several short ones.
-template <typename T, bool VECTOR, int NV>
-__global__ void __launch_bounds__(1024) rms_norm_kernel(const RowsParams p, const int warps) {
+// `lanes` threads per row, which keep it in registers: NV vectors per lane.  A
+// row has 8 or 16 lanes of a warp (rows that short), a warp or several; a CTA
+// has one row or several.
+template <typename T, RowMode MODE, int NV>
+__global__ void __launch_bounds__(1024) rms_norm_kernel(const RowsParams p, const int lanes) {
   constexpr int VEC = kRowVec<T>;
   __shared__ float part[32];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = w / warps * warps;  // the first warp of this one's row
-  const int64_t row = (int64_t)blockIdx.x * ((blockDim.x >> 5) / warps) + w / warps;
-  const int64_t c0 = (int64_t)((w - first) * 32 + lane) * VEC, step = (int64_t)warps * 32 * VEC;
+  const int in_row = threadIdx.x & (lanes - 1);  // lanes is a power of two
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+  const int c0 = in_row * VEC, step = lanes * VEC, k = row < p.m ? (int)p.k : 0;
   grid_dep_wait();
   grid_dep_trigger();
   float v[NV][VEC];
   float ss = 0.0f;
-  if (row < p.m) {
-    const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
-    const T* r = static_cast<const T*>(p.residual) + row * p.r_ld;
-    uint4 xu[NV], ru[NV];
+  const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
+  const T* r = static_cast<const T*>(p.residual) + row * p.r_ld;
+  uint4 xu[NV], ru[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) xu[j] = load_vec<T, VECTOR>(x, c0 + j * step, p.k);
-    if (p.residual) {
+  for (int j = 0; j < NV; ++j) xu[j] = load_vec<T, MODE>(x, c0 + j * step, k);
+  if (p.residual) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) ru[j] = load_vec<T, VECTOR>(r, c0 + j * step, p.k);
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      unpack_vec<T>(xu[j], v[j]);
-      if (p.residual) {
-        float t[VEC];
-        unpack_vec<T>(ru[j], t);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] += t[i];
-      }
-      ss += square_sum(v[j]);
-    }
+    for (int j = 0; j < NV; ++j) ru[j] = load_vec<T, MODE>(r, c0 + j * step, k);
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (warps > 1) {
+  for (int j = 0; j < NV; ++j) {
+    unpack_vec<T>(xu[j], v[j]);
+    if (p.residual) {
+      float t[VEC];
+      unpack_vec<T>(ru[j], t);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j][i] += t[i];
+    }
+    ss += square_sum(v[j]);
+  }
+  for (int o = min(lanes, 32) / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (lanes > 32) {
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = lanes >> 5, first = w & ~(warps - 1);
     if (lane == 0) part[w] = ss;
     __syncthreads();
     ss = lane < warps ? part[first + lane] : 0.0f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   }
-  if (row >= p.m) return;
   const float scale = rsqrtf(ss / (float)p.k + p.eps);
-#pragma unroll
-  for (int j = 0; j < NV; ++j) norm_finish<T, VECTOR>(p, row, c0 + j * step, scale, v[j]);
+  norm_finish<T, MODE>(p, row, c0, step, k, scale, v);
 }
 
 // Rows too long for registers: one CTA per row, which reads it twice.
-template <typename T, bool VECTOR>
+template <typename T, RowMode MODE>
 __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p) {
   constexpr int VEC = kRowVec<T>;
   __shared__ float part[32];
@@ -319,11 +443,12 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p)
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.r_ld : nullptr;
   const int64_t step = 1024 * VEC;
-  auto load = [&](int64_t c, float (&v)[VEC]) {
-    unpack_vec<T>(load_vec<T, VECTOR>(x, c, p.k), v);
+  const int k = (int)p.k;
+  auto load = [&](int c, float (&v)[VEC]) {
+    unpack_vec<T>(load_vec<T, MODE>(x, c, k), v);
     if (r) {
       float t[VEC];
-      unpack_vec<T>(load_vec<T, VECTOR>(r, c, p.k), t);
+      unpack_vec<T>(load_vec<T, MODE>(r, c, k), t);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[i] += t[i];
     }
@@ -331,7 +456,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p)
   float ss = 0.0f;
   for (int64_t c = (int64_t)threadIdx.x * VEC; c < p.k; c += step) {
     float v[VEC];
-    load(c, v);
+    load((int)c, v);
     ss += square_sum(v);
   }
 #pragma unroll
@@ -343,9 +468,10 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p)
   for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   const float scale = rsqrtf(ss / (float)p.k + p.eps);
   for (int64_t c0 = (int64_t)w * 32 * VEC; c0 < p.k; c0 += step) {  // whole warps: they quantise together
-    float v[VEC];
-    load(c0 + lane * VEC, v);
-    norm_finish<T, VECTOR>(p, row, c0 + lane * VEC, scale, v);
+    const int c = (int)c0 + lane * VEC;
+    float v[1][VEC];
+    load(c, v[0]);
+    norm_finish<T, MODE>(p, row, c, 0, k, scale, v);
   }
 }
 
@@ -361,13 +487,16 @@ inline bool rows_vector(const void* p, int64_t ld, int64_t rows) {
 
 template <typename T>
 inline cudaError_t launch_quantize_rows_t(const RowsParams& p, cudaStream_t s) {
-  const int64_t chunk = kQuantUnits * 32 * kRowVec<T>;
-  const int64_t chunks = (p.k + chunk - 1) / chunk;
-  const int64_t grid = (p.m * chunks + 7) / 8;
-  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const bool vec = p.k % kRowVec<T> == 0 && rows_vector<T>(p.x, p.x_ld, p.m);
-  return pdl_launch(vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)grid),
-                    dim3(256), 0, s, p, (uint32_t)chunks);
+  const int64_t units = (p.k + 32 * kRowVec<T> - 1) / (32 * kRowVec<T>);
+  if (units < kQuantUnits) {
+    const int64_t blocks = fp8_blocks(p.k), cta = 8 * kQuantUnits * 32 * kRowVec<T> / kFp8Block;
+    return pdl_launch(vec ? quantize_short_kernel<T, ROW_VECTORS> : quantize_short_kernel<T, ROW_ELEMENTS>,
+                      dim3((unsigned)((p.m * blocks + cta - 1) / cta)), dim3(256), 0, s, p, (uint32_t)blocks);
+  }
+  const int64_t warps = (units + kQuantUnits - 1) / kQuantUnits, ctas = (warps + 7) / 8;
+  return pdl_launch(vec ? quantize_rows_kernel<T, ROW_VECTORS> : quantize_rows_kernel<T, ROW_ELEMENTS>,
+                    dim3((unsigned)p.m, (unsigned)ctas), dim3((unsigned)(32 * ((warps + ctas - 1) / ctas))), 0, s, p);
 }
 inline cudaError_t launch_quantize_rows(const RowsParams& p, int type, cudaStream_t s) {
   if (type == FTB_F32) return launch_quantize_rows_t<float>(p, s);
@@ -383,28 +512,37 @@ inline cudaError_t launch_quantize_weight(const RowsParams& p, int type, cudaStr
                     grid, dim3(256), 0, s, p);
 }
 
-template <typename T, bool VECTOR>
-inline cudaError_t launch_rms_norm_v(const RowsParams& p, int sm_count, cudaStream_t s) {
-  const int64_t vectors = (p.k + kRowVec<T> - 1) / kRowVec<T>;
-  constexpr int64_t kMost = 1024 * 4;  // vectors of a row that the registers of 1024 threads hold
-  if (vectors > kMost)
-    return pdl_launch(rms_norm_long_kernel<T, VECTOR>, dim3((unsigned)p.m), dim3(1024), 0, s, p);
-  // Many rows: four vectors per lane, so that few warps share a row and many
-  // loads are in flight.  Few rows: one per lane, the shortest time.
-  const int nv = p.m >= 2 * sm_count || vectors > 1024 ? 4 : 1;
-  int warps = 1;
-  while (warps * 32 * nv < vectors) warps *= 2;
-  const int rows = std::max(1, 8 / warps);
+template <typename T, RowMode MODE>
+inline cudaError_t launch_rms_norm_m(const RowsParams& p, int nv, int lanes, cudaStream_t s) {
+  const int threads = std::max(256, lanes), rows = threads / lanes;
   const unsigned grid = (unsigned)((p.m + rows - 1) / rows);
-  return pdl_launch(nv == 4 ? rms_norm_kernel<T, VECTOR, 4> : rms_norm_kernel<T, VECTOR, 1>, dim3(grid),
-                    dim3(32 * warps * rows), 0, s, p, warps);
+  return pdl_launch(nv == 4   ? rms_norm_kernel<T, MODE, 4>
+                    : nv == 2 ? rms_norm_kernel<T, MODE, 2>
+                              : rms_norm_kernel<T, MODE, 1>,
+                    dim3(grid), dim3(threads), 0, s, p, lanes);
 }
 template <typename T>
 inline cudaError_t launch_rms_norm_t(const RowsParams& p, int sm_count, cudaStream_t s) {
   const bool vec = p.k % kRowVec<T> == 0 && rows_vector<T>(p.x, p.x_ld, p.m) &&
                    rows_vector<T>(p.residual, p.r_ld, p.m) && rows_vector<T>(p.h, p.h_ld, p.m) &&
                    rows_vector<T>(p.y, p.y_ld, p.m) && (reinterpret_cast<uintptr_t>(p.weight) & 15) == 0;
-  return vec ? launch_rms_norm_v<T, true>(p, sm_count, s) : launch_rms_norm_v<T, false>(p, sm_count, s);
+  const int64_t vectors = (p.k + kRowVec<T> - 1) / kRowVec<T>;
+  if (vectors > 1024 * 4)  // more than the registers of 1024 threads hold
+    return pdl_launch(vec ? rms_norm_long_kernel<T, ROW_VECTORS> : rms_norm_long_kernel<T, ROW_ELEMENTS>,
+                      dim3((unsigned)p.m), dim3(1024), 0, s, p);
+  // Many rows: up to four vectors per lane, so that few warps share a row and
+  // many loads are in flight (16384 x 8192 bf16, residual, quantised: 149 us
+  // with four, 200 with two, 241 with one).  Few rows: one per lane, the
+  // shortest time (1 x 4096: 2.5 us against 3.4 with four).
+  int nv = 1;
+  if (p.m >= 2 * sm_count || vectors > 1024) nv = vectors <= 32 ? 1 : vectors <= 64 ? 2 : 4;
+  // a quantisation block's lanes stay together
+  int lanes = p.q ? kFp8Block / kRowVec<T> : 8;
+  while ((int64_t)lanes * nv < vectors) lanes *= 2;
+  const int rows = std::max(256, lanes) / lanes;
+  if (!vec) return launch_rms_norm_m<T, ROW_ELEMENTS>(p, nv, lanes, s);
+  if ((int64_t)lanes * nv == vectors && p.m % rows == 0) return launch_rms_norm_m<T, ROW_WHOLE>(p, nv, lanes, s);
+  return launch_rms_norm_m<T, ROW_VECTORS>(p, nv, lanes, s);
 }
 inline cudaError_t launch_rms_norm(const RowsParams& p, int type, int sm_count, cudaStream_t s) {
   if (type == FTB_F32) return launch_rms_norm_t<float>(p, sm_count, s);

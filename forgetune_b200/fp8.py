@@ -50,10 +50,6 @@ _NO_MATRIX = (0, 0, 0)
 _NO_FP8 = (0, 0, 0, 0)
 
 
-def _blocks(n: int) -> int:
-    return (n + BLOCK - 1) // BLOCK
-
-
 def _rows(m: int, k: int, unit: int, dtype, device) -> torch.Tensor:
     """An uninitialised matrix whose rows start on multiples of ``unit`` elements."""
     return torch.empty_strided((m, k), ((k + unit - 1) // unit * unit, 1), dtype=dtype, device=device)
@@ -62,44 +58,80 @@ def _rows(m: int, k: int, unit: int, dtype, device) -> torch.Tensor:
 class _Fp8:
     """8-bit values [rows, k] with their block scales."""
 
-    __slots__ = ("data", "scales")
+    __slots__ = ("_data", "_scales", "_m", "_k", "_ld", "_scales_ld")
     _row_block = 1
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
         name = type(self).__name__
-        if not (isinstance(data, torch.Tensor) and data.dtype == _E4M3):
+        if not isinstance(data, torch.Tensor) or data.dtype is not _E4M3:
             raise TypeError("%s: data must be a torch.float8_e4m3fn tensor" % name)
-        if not (isinstance(scales, torch.Tensor) and scales.dtype == _E8M0):
+        if not isinstance(scales, torch.Tensor) or scales.dtype is not _E8M0:
             raise TypeError("%s: scales must be a torch.float8_e8m0fnu tensor" % name)
-        if data.dim() != 2 or data.shape[1] < 1:
-            raise InvalidShapeError("%s: data must be [rows, k] with k >= 1, got %s" % (name, tuple(data.shape)))
+        shape, s_shape = data.shape, scales.shape
+        if len(shape) != 2 or shape[1] < 1:
+            raise InvalidShapeError("%s: data must be [rows, k] with k >= 1, got %s" % (name, tuple(shape)))
+        m, k = shape
         b = self._row_block
-        want = ((data.shape[0] + b - 1) // b, _blocks(data.shape[1]))
-        if tuple(scales.shape) != want:
+        rows, kb = (m + b - 1) // b, (k + BLOCK - 1) // BLOCK
+        if s_shape != (rows, kb):
             raise InvalidShapeError("%s: scales of data %s must be %s, got %s"
-                                    % (name, tuple(data.shape), want, tuple(scales.shape)))
-        if data.device != scales.device:
+                                    % (name, (m, k), (rows, kb), tuple(s_shape)))
+        if data.get_device() != scales.get_device():
             raise ValueError("%s: data and scales are on different devices" % name)
-        self.data = data
-        self.scales = scales
+        self._data = data
+        self._scales = scales
+        self._m = m
+        self._k = k
+        self._ld = _ld8(m, k, data.stride(), 16)  # None: not laid out as the operators need it
+        self._scales_ld = _ld8(rows, kb, scales.stride(), 4)
 
     @classmethod
     def pack(cls, data: torch.Tensor, scales: torch.Tensor):
         """The same values in rows laid out as the operators need them (copied where they are not)."""
         r = cls(data, scales)
-        if _ld8(r.data, 16) is None:
-            r.data = _rows(*data.shape, 16, _E4M3, data.device).copy_(data)
-        if _ld8(r.scales, 4) is None:
-            r.scales = _rows(*scales.shape, 4, _E8M0, scales.device).copy_(scales)
+        if r._ld is None or data.data_ptr() % 16:
+            data = _rows(*data.shape, 16, _E4M3, data.device).copy_(data)
+        if r._scales_ld is None or scales.data_ptr() % 4:
+            scales = _rows(*scales.shape, 4, _E8M0, scales.device).copy_(scales)
+        return cls(data, scales)
+
+    @classmethod
+    def _empty(cls, m: int, k: int, device):
+        """Uninitialised values, laid out as the operators need them."""
+        kb = (k + BLOCK - 1) // BLOCK
+        r = cls.__new__(cls)
+        r._m = m
+        r._k = k
+        r._ld = ld = (k + 15) // 16 * 16
+        r._scales_ld = s_ld = (kb + 3) // 4 * 4
+        r._data = torch.empty_strided((m, k), (ld, 1), dtype=_E4M3, device=device)
+        r._scales = torch.empty_strided(((m + cls._row_block - 1) // cls._row_block, kb), (s_ld, 1), dtype=_E8M0,
+                                        device=device)
         return r
+
+    def _args(self, what: str) -> Tuple[int, int, int, int]:
+        """The matrix as the C ABI takes it."""
+        p, s = self._data.data_ptr(), self._scales.data_ptr()
+        if self._ld is None or self._scales_ld is None or p % 16 or s % 4:
+            raise InvalidShapeError("%s: rows of data must start on 16-byte and rows of scales on 4-byte boundaries "
+                                    "(see %s.pack)" % (what, type(self).__name__))
+        return p, self._ld, s, self._scales_ld
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     @property
     def shape(self) -> torch.Size:
-        return self.data.shape
+        return self._data.shape
 
     @property
     def device(self) -> torch.device:
-        return self.data.device
+        return self._data.device
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the blocks stand for."""
@@ -127,24 +159,14 @@ class Fp8Weight(_Fp8):
     _row_block = BLOCK
 
 
-def _ld8(t: torch.Tensor, unit: int) -> Optional[int]:
+def _ld8(rows: int, cols: int, stride, unit: int) -> Optional[int]:
     """Row stride of an 8-bit matrix, or None where its rows are not laid out in units of ``unit`` bytes."""
-    rows, cols = t.shape
-    ld, step = t.stride()
-    if (step != 1 and cols > 1) or t.data_ptr() % unit:
+    ld, step = stride
+    if step != 1 and cols > 1:
         return None
     if rows <= 1:
         return (cols + unit - 1) // unit * unit
     return ld if ld >= cols and ld % unit == 0 else None
-
-
-def _fp8(q: _Fp8, what: str) -> Tuple[int, int, int, int]:
-    """Quantised rows as the C ABI takes them."""
-    ld, s_ld = _ld8(q.data, 16), _ld8(q.scales, 4)
-    if ld is None or s_ld is None:
-        raise InvalidShapeError("%s: rows of data must start on 16-byte and rows of scales on 4-byte boundaries "
-                                "(see %s.pack)" % (what, type(q).__name__))
-    return q.data.data_ptr(), ld, q.scales.data_ptr(), s_ld
 
 
 def _ld(t: torch.Tensor) -> Optional[int]:
@@ -158,14 +180,17 @@ def _ld(t: torch.Tensor) -> Optional[int]:
     return ld if ld >= cols else None
 
 
-def _input(t, what: str) -> Tuple[torch.Tensor, int]:
-    """A plain 2-D CUDA input (copied where its rows are not contiguous) and its row stride."""
+def _input(t, what: str) -> Tuple[torch.Tensor, int, int, int, int]:
+    """A plain 2-D CUDA input (copied where its rows are not contiguous), its sizes, row stride and type."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _TYPES):
         raise TypeError("%s must be a float32, float16 or bfloat16 CUDA tensor" % what)
     if t.dim() != 2 or t.shape[1] < 1:
         raise InvalidShapeError("%s must be 2-D with at least one column, got %s" % (what, tuple(t.shape)))
+    rows, cols = t.shape
     ld = _ld(t)
-    return (t, ld) if ld is not None else (t.contiguous(), t.shape[1])
+    if ld is None:
+        t, ld = t.contiguous(), cols
+    return t, rows, cols, ld, _TYPES[t.dtype]
 
 
 def _check(t: torch.Tensor, what: str, shape, device) -> None:
@@ -189,23 +214,14 @@ def _output(out, what: str, shape, dtype: torch.dtype, device) -> Tuple[torch.Te
     return out, (out.data_ptr(), ld, _TYPES[dtype])
 
 
-def _fp8_output(out, what: str, m: int, k: int, device) -> Tuple[Fp8Rows, Tuple[int, int, int, int]]:
-    """A new quantised output, or the caller's, and the matrix the C ABI takes."""
-    if out is not None:
-        if not isinstance(out, Fp8Rows):
-            raise TypeError("%s must be an Fp8Rows" % what)
-        _check(out, what, (m, k), device)
-        return out, _fp8(out, what)
-    r = _new(Fp8Rows, _rows(m, k, 16, _E4M3, device), _rows(m, _blocks(k), 4, _E8M0, device))
-    return r, (r.data.data_ptr(), (k + 15) // 16 * 16, r.scales.data_ptr(), (_blocks(k) + 3) // 4 * 4)
-
-
-def _new(cls, data, scales):
-    """An instance of tensors that are right by construction."""
-    r = cls.__new__(cls)
-    r.data = data
-    r.scales = scales
-    return r
+def _fp8_output(out, what: str, m: int, k: int, device) -> Fp8Rows:
+    """A new quantised output, or the caller's."""
+    if out is None:
+        return Fp8Rows._empty(m, k, device)
+    if not isinstance(out, Fp8Rows):
+        raise TypeError("%s must be an Fp8Rows" % what)
+    _check(out, what, (m, k), device)
+    return out
 
 
 def _vector(t, what: str, n: int, device) -> Optional[torch.Tensor]:
@@ -233,25 +249,22 @@ def _call(name: str, device: torch.device, args: bytes) -> None:
 
 def quantize_rows(x: torch.Tensor, out: Optional[Fp8Rows] = None) -> Fp8Rows:
     """Activations [m, k] (float32, float16, bfloat16) to 8 bits with a scale for each 128 along a row."""
-    x, ld = _input(x, "quantize_rows: x")
-    m, k = x.shape
+    x, m, k, ld, t = _input(x, "quantize_rows: x")
     dev = x.device
-    r, q = _fp8_output(out, "quantize_rows: out", m, k, dev)
-    _call("ftb_quantize_rows", dev, _QUANTIZE_ARGS.pack(x.data_ptr(), ld, _TYPES[x.dtype], *q, m, k))
+    r = _fp8_output(out, "quantize_rows: out", m, k, dev)
+    _call("ftb_quantize_rows", dev, _QUANTIZE_ARGS.pack(x.data_ptr(), ld, t, *r._args("quantize_rows: out"), m, k))
     return r
 
 
 def quantize_weight(w: torch.Tensor) -> Fp8Weight:
     """A weight [n, k] (``nn.Linear``'s layout; float32, float16, bfloat16) to 8 bits with a scale for each
     128 x 128 block.  Done once, where a model is loaded."""
-    w, ld = _input(w, "quantize_weight: w")
-    n, k = w.shape
+    w, n, k, ld, t = _input(w, "quantize_weight: w")
     if n < 1:
         raise InvalidShapeError("quantize_weight: w must have at least one row")
-    dev = w.device
-    r = _new(Fp8Weight, _rows(n, k, 16, _E4M3, dev), _rows(_blocks(n), _blocks(k), 4, _E8M0, dev))
-    _call("ftb_quantize_weight", dev,
-          _QUANTIZE_ARGS.pack(w.data_ptr(), ld, _TYPES[w.dtype], *_fp8(r, "quantize_weight"), n, k))
+    r = Fp8Weight._empty(n, k, w.device)
+    _call("ftb_quantize_weight", w.device,
+          _QUANTIZE_ARGS.pack(w.data_ptr(), ld, t, *r._args("quantize_weight"), n, k))
     return r
 
 
@@ -268,26 +281,26 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     ``residual_out`` receive them in place of new tensors; ``residual_out``
     may be ``x`` or ``residual``, ``out`` may be ``x``.
     """
-    x, ld = _input(x, "rms_norm: x")
-    shape, dtype, dev = x.shape, x.dtype, x.device
-    m, k = shape
-    t = _TYPES[dtype]
+    x, m, k, ld, t = _input(x, "rms_norm: x")
+    dtype, dev = x.dtype, x.device
     weight = _vector(weight, "rms_norm: weight", k, dev)
     r_arg = h_arg = y_arg = _NO_MATRIX
     q_arg = _NO_FP8
     if residual is not None:
-        residual, r_ld = _input(residual, "rms_norm: residual")
-        if residual.dtype != dtype:
+        residual, rm, rk, r_ld, rt = _input(residual, "rms_norm: residual")
+        if rt != t:
             raise TypeError("rms_norm: residual must be %s, got %s" % (dtype, residual.dtype))
-        _check(residual, "rms_norm: residual", shape, dev)
+        if rm != m or rk != k or residual.device != dev:
+            _check(residual, "rms_norm: residual", (m, k), dev)
         r_arg = (residual.data_ptr(), r_ld, t)
-        h, h_arg = _output(residual_out, "rms_norm: residual_out", shape, dtype, dev)
+        h, h_arg = _output(residual_out, "rms_norm: residual_out", (m, k), dtype, dev)
     elif residual_out is not None:
         raise ValueError("rms_norm: residual_out needs a residual")
     if quantize:
-        y, q_arg = _fp8_output(out, "rms_norm: out", m, k, dev)
+        y = _fp8_output(out, "rms_norm: out", m, k, dev)
+        q_arg = y._args("rms_norm: out")
     else:
-        y, y_arg = _output(out, "rms_norm: out", shape, dtype, dev)
+        y, y_arg = _output(out, "rms_norm: out", (m, k), dtype, dev)
     _call("ftb_rms_norm", dev, _RMS_NORM_ARGS.pack(
         x.data_ptr(), ld, t, *r_arg, 0 if weight is None else weight.data_ptr(), eps, *h_arg, *y_arg, *q_arg, m, k))
     return y if residual is None else (y, h)
@@ -308,28 +321,30 @@ def fp8_linear(x: Union[Fp8Rows, torch.Tensor], weight: Fp8Weight, bias: Optiona
     """
     if not isinstance(weight, Fp8Weight):
         raise TypeError("fp8_linear: weight must be an Fp8Weight (see quantize_weight)")
+    if quantize and out_dtype is not None:
+        raise ValueError("fp8_linear: a quantised result has no out_dtype")
     if not isinstance(x, Fp8Rows):
-        x, _ = _input(x, "fp8_linear: x")
+        x = _input(x, "fp8_linear: x")[0]
         out_dtype = out_dtype or x.dtype
         x = quantize_rows(x)
-    elif not x.data.is_cuda:
+    elif not x._data.is_cuda:
         raise TypeError("fp8_linear: x must be on a CUDA device")
-    dev = x.data.device
-    m, k = x.data.shape
-    n, wk = weight.data.shape
-    if wk != k:
-        raise InvalidShapeError("fp8_linear: x is %s, weight %s: their depths differ" % ((m, k), (n, wk)))
-    if weight.data.device != dev:
-        raise ValueError("fp8_linear: weight is on %s, the input on %s" % (weight.data.device, dev))
+    m, k, n, dev = x._m, x._k, weight._m, x._data.device
+    if weight._k != k:
+        raise InvalidShapeError("fp8_linear: x is %s, weight %s: their depths differ" % ((m, k), (n, weight._k)))
+    if weight._data.device != dev:
+        raise ValueError("fp8_linear: weight is on %s, the input on %s" % (weight._data.device, dev))
     bias = _vector(bias, "fp8_linear: bias", n, dev)
     r_arg = y_arg = _NO_MATRIX
     q_arg = _NO_FP8
     if residual is not None:
-        residual, r_ld = _input(residual, "fp8_linear: residual")
-        _check(residual, "fp8_linear: residual", (m, n), dev)
-        r_arg = (residual.data_ptr(), r_ld, _TYPES[residual.dtype])
+        residual, rm, rn, r_ld, rt = _input(residual, "fp8_linear: residual")
+        if rm != m or rn != n or residual.device != dev:
+            _check(residual, "fp8_linear: residual", (m, n), dev)
+        r_arg = (residual.data_ptr(), r_ld, rt)
     if quantize:
-        y, q_arg = _fp8_output(out, "fp8_linear: out", m, n, dev)
+        y = _fp8_output(out, "fp8_linear: out", m, n, dev)
+        q_arg = y._args("fp8_linear: out")
     else:
         if out_dtype is None:
             out_dtype = torch.float32 if residual is None else residual.dtype
@@ -337,6 +352,6 @@ def fp8_linear(x: Union[Fp8Rows, torch.Tensor], weight: Fp8Weight, bias: Optiona
             raise TypeError("fp8_linear: out_dtype must be float32, float16 or bfloat16, got %s" % (out_dtype,))
         y, y_arg = _output(out, "fp8_linear: out", (m, n), out_dtype, dev)
     _call("ftb_fp8_linear", dev, _LINEAR_ARGS.pack(
-        *_fp8(x, "fp8_linear: x"), *_fp8(weight, "fp8_linear: weight"), 0 if bias is None else bias.data_ptr(),
+        *x._args("fp8_linear: x"), *weight._args("fp8_linear: weight"), 0 if bias is None else bias.data_ptr(),
         *r_arg, *y_arg, *q_arg, m, n, k, _FP8_RELU if relu else 0))
     return y
