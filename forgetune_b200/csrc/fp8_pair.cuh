@@ -12,8 +12,9 @@
 // that both fit beside the scale factors: the epilogue reads the shared
 // columns of a tile first, and the next tile's products wait for that alone.
 //
-// Persistent pairs walk the tiles in bands of eight row blocks (the pairs at
-// work then share 8 + 9 operand blocks of 256 rows through L2, not 2 + 37).
+// Persistent pairs walk the tiles in bands of 16 row blocks (74 pairs at work
+// then share 16 + 5 operand blocks of 256 rows through L2, not 2 + 37;
+// 8192^3: 385 us, with bands of 8 390, of 4 401).
 // Twelve warps per CTA:
 //   warp 0     TMA producer of this CTA's rows (its own barriers);
 //   warp 1     tensor memory; in the leader CTA the MMAs of the pair;
@@ -31,15 +32,16 @@
 namespace ftb {
 
 constexpr int kFp8PairThreads = 384;
-constexpr int kFp8PairStages = 5;
-constexpr int kFp8Band = 8;
+constexpr int kFp8PairStages = 6;
+constexpr int kFp8Band = 16;
 
 struct Fp8PairSmem {
   static constexpr int OPERAND_BYTES = 128 * 128;
   static constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
   static constexpr int SF_BYTES = 512 + 1024;
-  static constexpr int STAGING = 8 * 2 * 2048;  // two boxes per epilogue warp
-  static constexpr int SF_OFF = kFp8PairStages * STAGE_BYTES + STAGING;
+  static constexpr int STAGING = 8 * 2048;  // a box per epilogue warp
+  static constexpr int BIAS = 8 * 512;      // its columns' bias
+  static constexpr int SF_OFF = kFp8PairStages * STAGE_BYTES + STAGING + BIAS;
   static constexpr int BAR_OFF = SF_OFF + 2 * SF_BYTES;
   static constexpr int NBAR = 3 * kFp8PairStages + 4 + 4 + 2;
   static constexpr int TOTAL = 1024 + BAR_OFF + 8 * NBAR + 16;
@@ -74,7 +76,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int
                "r"(c0), "r"(c1), "r"(smem)
                : "memory");
 }
-__device__ __forceinline__ void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 
 // Tile number -> token and output block, in bands of kFp8Band token blocks.
 struct Fp8Tiles {
@@ -107,24 +108,19 @@ __device__ __forceinline__ void add_residual32(const T* row, int n, int N, bool 
   }
 }
 
-// The epilogue's arithmetic on 32 columns of one token.
-__device__ __forceinline__ void fp8_epilogue32(const Fp8PairParams& q, int64_t m, int n, float (&v)[32]) {
+// The epilogue's arithmetic on 32 columns of one token; their bias is at bias4.
+__device__ __forceinline__ void fp8_epilogue32(const Fp8PairParams& q, int64_t m, int n, const float4* bias4,
+                                               float (&v)[32]) {
   const Fp8Epilogue& e = q.p.e;
   const int N = q.p.N;
   if (e.bias) {
-    if (q.bias_vec && n + 32 <= N) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 b = __ldg(reinterpret_cast<const float4*>(e.bias + n) + i);
-        v[4 * i] = __fadd_rn(v[4 * i], b.x);
-        v[4 * i + 1] = __fadd_rn(v[4 * i + 1], b.y);
-        v[4 * i + 2] = __fadd_rn(v[4 * i + 2], b.z);
-        v[4 * i + 3] = __fadd_rn(v[4 * i + 3], b.w);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (n + i < N) v[i] = __fadd_rn(v[i], __ldg(e.bias + n + i));
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = bias4[i];
+      v[4 * i] = __fadd_rn(v[4 * i], b.x);
+      v[4 * i + 1] = __fadd_rn(v[4 * i + 1], b.y);
+      v[4 * i + 2] = __fadd_rn(v[4 * i + 2], b.z);
+      v[4 * i + 3] = __fadd_rn(v[4 * i + 3], b.w);
     }
   }
   if (e.relu) {
@@ -139,28 +135,25 @@ __device__ __forceinline__ void fp8_epilogue32(const Fp8PairParams& q, int64_t m
   }
 }
 
-// One epilogue warp's staging: two boxes of 32 rows x 64 bytes (64-byte
-// swizzle; a quantised output's rows are 32 bytes, unswizzled).
+// One epilogue warp's staging box: 32 rows x 64 bytes (64-byte swizzle; a
+// quantised output's rows are 32 bytes, unswizzled).
 struct Fp8Staging {
-  uint32_t base;
-  uint32_t count;  // boxes so far
+  uint32_t box;
   int lane;
-  __device__ __forceinline__ uint32_t begin() {
-    if (lane == 0) bulk_wait_read1();
+  __device__ __forceinline__ void begin() const {  // the last store has read it
+    if (lane == 0) bulk_wait_read();
     __syncwarp();
-    return base + (count & 1u) * 2048u;
   }
-  __device__ __forceinline__ void put64(uint32_t box, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
+  __device__ __forceinline__ void put64(int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
     st_shared4(box + lane * 64 + ((chunk ^ ((lane >> 1) & 3)) << 4), a, b, c, d);
   }
-  __device__ __forceinline__ void end(const CUtensorMap* map, int n, int m, uint32_t box) {
+  __device__ __forceinline__ void end(const CUtensorMap* map, int n, int m) const {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
       tma_store_2d(map, n, m, box);
       bulk_commit();
     }
-    ++count;
   }
 };
 
@@ -186,13 +179,13 @@ __device__ __forceinline__ void store_box_rows(uint32_t box, U* y, int64_t ld, i
 
 // 32 finished columns of 32 tokens (lane = token) into a plain output.
 template <typename T>
-__device__ __forceinline__ void store_plain32(const Fp8PairParams& q, const CUtensorMap* map, Fp8Staging& st, int m0,
+__device__ __forceinline__ void store_plain32(const Fp8PairParams& q, const CUtensorMap* map, const Fp8Staging& st, int m0,
                                               int n, const float (&v)[32]) {
   constexpr int C = 64 / (int)sizeof(T);  // columns per box
 #pragma unroll
   for (int b = 0; b < 32 / C; ++b) {
     if (n + b * C >= q.p.N) break;
-    const uint32_t box = st.begin();
+    st.begin();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       T t[C / 4];
@@ -200,13 +193,13 @@ __device__ __forceinline__ void store_plain32(const Fp8PairParams& q, const CUte
       for (int j = 0; j < C / 4; ++j) t[j] = from_f32<T>(v[b * C + i * (C / 4) + j]);
       uint32_t u[4];
       memcpy(u, t, 16);
-      st.put64(box, i, u[0], u[1], u[2], u[3]);
+      st.put64(i, u[0], u[1], u[2], u[3]);
     }
     if (q.y_tma && n + (b + 1) * C <= q.p.N) {
-      st.end(map, n + b * C, m0, box);
+      st.end(map, n + b * C, m0);
     } else {
       using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
-      store_box_rows(box, static_cast<U*>(q.p.e.y), q.p.e.y_ld, m0, n + b * C, q.p.M, q.p.N, st.lane);
+      store_box_rows(st.box, static_cast<U*>(q.p.e.y), q.p.e.y_ld, m0, n + b * C, q.p.M, q.p.N, st.lane);
     }
   }
 }
@@ -265,6 +258,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
+  if (warp == 3 && elect_one()) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_w);
+    if (q.y_tma) prefetch_map(&map_y);
+  }
+  __syncwarp();
   tc_fence_before();
   cluster_sync_all();
   tc_fence_after();
@@ -396,17 +395,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
     }
   } else {
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    Fp8Staging st{smem_u32(staging) + (uint32_t)(warp - 4) * 4096u, 0u, lane};
+    const Fp8Staging st{smem_u32(staging) + (uint32_t)(warp - 4) * 2048u, lane};
+    float4* bias4 = reinterpret_cast<float4*>(staging + L::STAGING + (warp - 4) * 512);
     const uint32_t shared_leader = cluster_addr(shared_cols, 0);
     uint32_t tc = 0;
     for (int t = pair; t < ntiles; t += npairs, ++tc) {
       const uint32_t b = tc & 1u;
-      if (!pair_wait_warp(&accf[b], (tc >> 1) & 1u, abort_flag, peer_abort, p.err, 21)) break;
-      tc_fence_after();
       int m0, n0;
       tiles.at(t, m0, n0);
       m0 += (int)rank * 128 + quarter * 32;
       n0 += half * 128;
+      if (p.e.bias) {  // this tile's, while its products run
+        const int n = n0 + 4 * lane;
+        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (q.bias_vec && n + 4 <= p.N) {
+          f = __ldg(reinterpret_cast<const float4*>(p.e.bias + n));
+        } else {
+          if (n < p.N) f.x = __ldg(p.e.bias + n);
+          if (n + 1 < p.N) f.y = __ldg(p.e.bias + n + 1);
+          if (n + 2 < p.N) f.z = __ldg(p.e.bias + n + 2);
+          if (n + 3 < p.N) f.w = __ldg(p.e.bias + n + 3);
+        }
+        __syncwarp();
+        bias4[lane] = f;
+        __syncwarp();
+      }
+      if (!pair_wait_warp(&accf[b], (tc >> 1) & 1u, abort_flag, peer_abort, p.err, 21)) break;
+      tc_fence_after();
       const int64_t m = (int64_t)m0 + lane;
       const uint32_t acc = tmem + b * kAcc1 + (uint32_t)half * 128 + ((uint32_t)(quarter * 32) << 16);
       const uint32_t acce_leader = cluster_addr(&acce[b], 0);
@@ -434,7 +449,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
           if (j == 3) release(acce_leader);
           const int n = n0 + 32 * chunk(j);
           if (n >= p.N || m0 >= p.M) continue;
-          fp8_epilogue32(q, m, n, v);
+          fp8_epilogue32(q, m, n, bias4 + 8 * chunk(j), v);
           if (p.e.y_type == FTB_F32) store_plain32<float>(q, &map_y, st, m0, n, v);
           else if (p.e.y_type == FTB_F16) store_plain32<__half>(q, &map_y, st, m0, n, v);
           else store_plain32<__nv_bfloat16>(q, &map_y, st, m0, n, v);
@@ -445,7 +460,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
         uint32_t amax = 0;
         auto finish = [&](int j, float (&v)[32]) {
           const int n = n0 + 32 * chunk(j);
-          if (inside && n < p.N) fp8_epilogue32(q, m, n, v);
+          if (inside && n < p.N) fp8_epilogue32(q, m, n, bias4 + 8 * chunk(j), v);
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (n + i >= p.N) v[i] = 0.0f;
@@ -484,11 +499,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
           for (int i = 0; i < 8; ++i)
             w[i] = fp8_pack4(nan_unless_finite(v[4 * i]), nan_unless_finite(v[4 * i + 1]),
                              nan_unless_finite(v[4 * i + 2]), nan_unless_finite(v[4 * i + 3]), inv);
-          const uint32_t box = st.begin();
-          st_shared4(box + lane * 32, w[0], w[1], w[2], w[3]);
-          st_shared4(box + lane * 32 + 16, w[4], w[5], w[6], w[7]);
-          if (n + 32 <= p.N) st.end(&map_y, n, m0, box);
-          else store_box_rows(box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, m0, n, p.M, p.N, lane);
+          st.begin();
+          st_shared4(st.box + lane * 32, w[0], w[1], w[2], w[3]);
+          st_shared4(st.box + lane * 32 + 16, w[4], w[5], w[6], w[7]);
+          if (n + 32 <= p.N) st.end(&map_y, n, m0);
+          else store_box_rows(st.box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, m0, n, p.M, p.N, lane);
         }
       }
     }
