@@ -26,7 +26,6 @@ struct Fp8Device {
   std::string err;
   int sm_count = 0;
   int pairs = 0;  // SM pairs resident at once
-  int tile_slots[4] = {0, 0, 0, 0};  // CTAs of the tile kernel resident at once, in clusters of 1, 2, 4 and 8
   // set by a kernel whose bounded wait gave up: mapped host memory, so the
   // next call reads it without a copy
   volatile int* fault = nullptr;
@@ -59,7 +58,6 @@ static void fp8_setup(int dev, Fp8Device* d) {
   if (e == cudaSuccess) e = fp8_tile_attributes<32>();
   if (e == cudaSuccess) e = fp8_tile_attributes<64>();
   if (e == cudaSuccess) e = fp8_tile_attributes<128>();
-  if (e == cudaSuccess) e = fp8_tile_slots(d->tile_slots);
   if (e == cudaSuccess) e = fp8_pair_prepare(&d->pairs);
   if (e != cudaSuccess) {
     d->rc = ST_DEVICE;
@@ -131,39 +129,42 @@ struct Fp8Choice {
   int nt, split;
 };
 
-// Picks by an estimate of the time in microseconds.  A CTA of the tile kernel
-// takes 0.40 per k-block when it waits for its loads, and an SM at least
-// 0.0097 per KB that its CTAs load; finishing costs 0.016 per token of a tile,
-// 0.008 more per token that is not shared out over the cluster; a cluster
-// costs 0.5.  A pair takes 0.28 per k-block and 1.2 per tile, and 6 more than
-// a tile before and after.  The constants are a fit to 72 shapes (m 1..4096, k and
-// n 64..8192) timed with every choice on a B200; over those shapes the pick
-// is 1.5 % slower than the best choice in the mean (geometric), 14 % at most
-// but for one.  Examples, best and next kinds: 1 x 4096 x 4096 (m, k, n): 16
-// tokens, split 4: 5.4 us, split 1: 12.2 us; 512 x 512 x 512: 16 tokens: 3.5,
-// 128 tokens: 6.8 us; 512 x 4096 x 4096: 128 tokens, split 2: 16.2, pair:
-// 17.8 us; 1024 x 4096 x 4096: pair 18.6, 128 tokens 22.6 us.
+// Picks by an estimate of the time in microseconds.  A round of the tile
+// kernel's CTAs takes 0.31 per k-block when they wait for their loads, at least
+// 0.0097 per KB that an SM's CTAs load, and 0.017 per token of a tile plus
+// 0.013 per token of the SM for its epilogue; each CTA of an SM costs 0.23, a
+// later round 1.3, a cluster 0.4.  (A round is the CTAs resident at once: two
+// per SM, fewer in clusters of 4 and 8, which do not fill the SMs' groups.)  A
+// round of pairs takes 0.29 per k-block and 0.8, and a launch 3.5 more than
+// the tile kernel's.  The constants are a fit to 525 shapes (m 1..4096, n and
+// k 64..8192) that were timed with every choice on a B200; over 263 others the
+// pick is 0.6 % slower than the best choice in the mean, 18 % at most.  For
+// example (m x k x n): 1 x 4096 x 4096 takes 5.2 us with 16 tokens per tile
+// and split 4, 12.2 unsplit; 512 x 512 x 512 takes 3.5 with 16 tokens, 6.8 with
+// 128; 256 x 4096 x 4096 11.8 with 128 tokens and split 2, 16.9 on pairs;
+// 1024 x 4096 x 4096 17.4 on pairs, 22.6 with 128 tokens.
 static Fp8Choice choose_fp8(int64_t m, int64_t n, int64_t k, const Fp8Device& d) {
-  const double sms = d.sm_count;
-  const int64_t nk = (k + 127) / 128, nt128 = (n + 127) / 128;
-  const int64_t pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
+  static const double kResident[4] = {2.0, 2.0, 1.78, 1.73};  // CTAs per SM in clusters of 1, 2, 4 and 8
+  const int64_t nk = fp8_blocks(k), tiles_n = fp8_blocks(n);
+  const double pair_tiles = (double)((m + 255) / 256) * (double)((n + 255) / 256);
   Fp8Choice best{0, 1};
-  double best_us = 7.9 + std::ceil((double)pair_tiles / d.pairs) * ((double)nk * 0.28 + 1.2);
+  double best_us = 5.19 + std::ceil(pair_tiles / d.pairs) * ((double)nk * 0.293 + 0.77);
   for (int nt = 16; nt <= 128; nt *= 2) {
-    const int64_t tiles = nt128 * ((m + nt - 1) / nt);
+    const double tiles = (double)tiles_n * (double)((m + nt - 1) / nt);
     for (int i = 0, split = 1; i < 4; ++i, split *= 2) {
-      if (split > 1 && nk < split * 2) break;  // a CTA without a k-block of its own
-      const double ctas = (double)tiles * split;
+      if (split > 1 && nk < split * 2) break;  // CTAs without a k-block
+      const double ctas = tiles * split;
       const double kb = (double)std::min<int64_t>(nk, ((nk + 3) / 4 + split - 1) / split * 4);
-      const double rounds = std::ceil(ctas / d.tile_slots[i]), per_sm = std::ceil(ctas / sms);
-      const double load = std::max(rounds * kb * 0.40, per_sm * kb * (16 + nt / 8) * 0.0097);
-      const double us = 2.0 + load + per_sm * nt * (0.016 + 0.008 / split) + (split > 1 ? 0.5 : 0.0);
+      const double rounds = std::ceil(ctas / (kResident[i] * d.sm_count)), per_sm = std::ceil(ctas / d.sm_count);
+      const double load = std::max(rounds * kb * 0.308, per_sm * kb * (16 + nt / 8) * 0.0097);
+      const double us = 1.71 + load + nt * (rounds * 0.0168 + per_sm * 0.0126) + per_sm * 0.23 +
+                        (rounds - 1) * 1.26 + (split > 1 ? 0.39 : 0.0);
       if (us < best_us) {
         best_us = us;
         best = Fp8Choice{nt, split};
       }
     }
-    if (nt >= m) break;
+    if (nt >= m) break;  // wider tiles would have empty columns only
   }
   return best;
 }

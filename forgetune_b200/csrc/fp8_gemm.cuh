@@ -509,33 +509,4 @@ inline cudaError_t fp8_tile_attributes() {
   return e;
 }
 
-// CTAs of the tile kernel resident at once in clusters of 1, 2, 4 and 8 (the
-// widest tile; the narrower ones have the same two CTAs per SM).
-template <int SPLIT>
-inline cudaError_t fp8_tile_slots1(int* slots) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(SPLIT);
-  cfg.blockDim = dim3(kFp8Threads);
-  cfg.dynamicSmemBytes = Fp8TileSmem<128>::TOTAL;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = SPLIT;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int clusters = 0;
-  const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, fp8_tile_kernel<128, SPLIT>, &cfg);
-  if (e != cudaSuccess) return e;
-  *slots = clusters * SPLIT;
-  return clusters > 0 ? cudaSuccess : cudaErrorInvalidConfiguration;
-}
-inline cudaError_t fp8_tile_slots(int (&slots)[4]) {
-  cudaError_t e = fp8_tile_slots1<1>(&slots[0]);
-  if (e == cudaSuccess) e = fp8_tile_slots1<2>(&slots[1]);
-  if (e == cudaSuccess) e = fp8_tile_slots1<4>(&slots[2]);
-  if (e == cudaSuccess) e = fp8_tile_slots1<8>(&slots[3]);
-  return e;
-}
-
 }  // namespace ftb
