@@ -20,11 +20,16 @@
 //   warp 1     tensor memory; in the leader CTA the MMAs of the pair;
 //   warp 2     scale factors of this CTA, four k-blocks at a time;
 //   warp 3     passes this CTA's landed stages on to the leader;
-//   warps 4-11 epilogue: a lane quarter and one half of the columns each,
-//              32 columns at a time through a staging box and a TMA store
-//              (plain row stores where the output's rows are not 16-byte
-//              aligned).  A quantised output needs the largest of its 128
-//              columns first: they are read from tensor memory twice.
+//   warps 4-11 epilogue: a lane quarter and one half (128) of the columns
+//              each, a lane a token, 32 columns at a time.  Outputs leave
+//              through staging boxes and TMA stores (row stores where rows are
+//              not 16-byte aligned, and for a box that ends outside); the
+//              residual arrives by TMA two boxes ahead; bias is staged while
+//              the products run.  A quantised output keeps its 128 columns,
+//              one block, in registers until their largest is known.
+// Short depths are bound by the epilogue: 8192 x 8192 outputs of depth 64 take
+// 48 us in bf16, 56 quantised, 79 with a bf16 residual (floors by bytes 21, 10
+// and 41 us).
 #pragma once
 
 #include "fp8_gemm.cuh"
@@ -32,18 +37,19 @@
 namespace ftb {
 
 constexpr int kFp8PairThreads = 384;
-constexpr int kFp8PairStages = 6;
+constexpr int kFp8PairStages = 5;
+constexpr int kFp8Boxes = 3;  // 2 KB boxes per epilogue warp: staging, or one of staging and two of residual
 constexpr int kFp8Band = 16;
 
 struct Fp8PairSmem {
   static constexpr int OPERAND_BYTES = 128 * 128;
   static constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
   static constexpr int SF_BYTES = 512 + 1024;
-  static constexpr int STAGING = 8 * 2048;  // a box per epilogue warp
-  static constexpr int BIAS = 8 * 512;      // its columns' bias
-  static constexpr int SF_OFF = kFp8PairStages * STAGE_BYTES + STAGING + BIAS;
+  static constexpr int BOXES = 8 * kFp8Boxes * 2048;
+  static constexpr int BIAS = 8 * 512;  // bias of a warp's columns
+  static constexpr int SF_OFF = kFp8PairStages * STAGE_BYTES + BOXES + BIAS;
   static constexpr int BAR_OFF = SF_OFF + 2 * SF_BYTES;
-  static constexpr int NBAR = 3 * kFp8PairStages + 4 + 4 + 2;
+  static constexpr int NBAR = 3 * kFp8PairStages + 4 + 4 + 2 + 16;
   static constexpr int TOTAL = 1024 + BAR_OFF + 8 * NBAR + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
 };
@@ -51,6 +57,7 @@ struct Fp8PairSmem {
 struct Fp8PairParams {
   Fp8Params p;
   int y_tma;     // the output has a TMA map
+  int res_tma;   // the residual has one
   int bias_vec;  // bias is 16-byte aligned
   int stall_test;
 };
@@ -68,6 +75,13 @@ __device__ __forceinline__ void umma2_fp8(uint32_t d, uint64_t a, uint64_t b, ui
 // In both CTAs: 512 bytes of this CTA's scale factors into its tensor memory.
 __device__ __forceinline__ void tmem2_copy_scales(uint32_t tmem, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d_at(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+      : "memory");
 }
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t smem) {
@@ -88,7 +102,7 @@ struct Fp8Tiles {
   }
 };
 
-// 32 consecutive columns of `row` from n as fp32 (zeros past N).
+// v += 32 consecutive columns of `row` from n.
 template <typename T>
 __device__ __forceinline__ void add_residual32(const T* row, int n, int N, bool vec, float (&v)[32]) {
   if (vec && n + 32 <= N) {
@@ -108,50 +122,176 @@ __device__ __forceinline__ void add_residual32(const T* row, int n, int N, bool 
   }
 }
 
-// The epilogue's arithmetic on 32 columns of one token; their bias is at bias4.
-__device__ __forceinline__ void fp8_epilogue32(const Fp8PairParams& q, int64_t m, int n, const float4* bias4,
-                                               float (&v)[32]) {
-  const Fp8Epilogue& e = q.p.e;
-  const int N = q.p.N;
-  if (e.bias) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 b = bias4[i];
-      v[4 * i] = __fadd_rn(v[4 * i], b.x);
-      v[4 * i + 1] = __fadd_rn(v[4 * i + 1], b.y);
-      v[4 * i + 2] = __fadd_rn(v[4 * i + 2], b.z);
-      v[4 * i + 3] = __fadd_rn(v[4 * i + 3], b.w);
-    }
-  }
-  if (e.relu) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = (v[i] != v[i] || v[i] > 0.0f) ? v[i] : 0.0f;
-  }
-  if (e.residual && m < q.p.M) {
-    if (e.res_type == FTB_F32) add_residual32(static_cast<const float*>(e.residual) + m * e.res_ld, n, N, e.res_vec, v);
-    else if (e.res_type == FTB_F16)
-      add_residual32(static_cast<const __half*>(e.residual) + m * e.res_ld, n, N, e.res_vec, v);
-    else add_residual32(static_cast<const __nv_bfloat16*>(e.residual) + m * e.res_ld, n, N, e.res_vec, v);
-  }
+__device__ __forceinline__ uint4 ld_shared4(uint32_t addr) {
+  uint4 u;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(addr));
+  return u;
 }
 
-// One epilogue warp's staging box: 32 rows x 64 bytes (64-byte swizzle; a
-// quantised output's rows are 32 bytes, unswizzled).
-struct Fp8Staging {
-  uint32_t box;
+// Max that keeps NaN: ReLU in one instruction.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 16-byte piece `i` of this lane's row in a box of 32 rows x 64 bytes, 64-byte
+// swizzle.
+__device__ __forceinline__ uint32_t box_at(uint32_t box, int lane, int i) {
+  return box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
+}
+
+// One epilogue warp: its boxes, bias and residual loads.
+struct Fp8EpilogueWarp {
+  const Fp8PairParams& q;
+  const CUtensorMap *map_y, *map_r;
+  uint32_t boxes;       // shared address of its kFp8Boxes boxes
+  const float4* bias4;  // its 128 columns
+  uint64_t* res_bar;    // [2] residual box landed
   int lane;
-  __device__ __forceinline__ void begin() const {  // the last store has read it
-    if (lane == 0) bulk_wait_read();
+  int m0, n0, half;     // its tokens and columns of this tile
+  uint32_t next;        // staging box in turn
+  uint32_t res_phase;   // bit s: parity of residual slot s
+  uint32_t res_open;    // bit s: a load into slot s has not been waited for
+  volatile int* abort_flag;
+  uint32_t peer_abort;
+
+  // the chunk that holds the columns that the accumulators share comes first:
+  // the last of accumulator 0's upper half, the first of accumulator 1's lower
+  __device__ __forceinline__ int chunk(int j) const { return half ? 3 - j : j; }
+  __device__ __forceinline__ bool inside(int n) const { return n < q.p.N && m0 < q.p.M; }
+  __device__ __forceinline__ int res_cols() const { return q.p.e.res_type == FTB_F32 ? 16 : 32; }
+
+  // Residual box x of the tile (4 of 32 columns or 8 of 16, in chunk order)
+  // goes to slot x & 1.
+  __device__ __forceinline__ int res_n(int x) const {
+    const int cols = res_cols(), per = 32 / cols;
+    return n0 + 32 * chunk(x / per) + x % per * cols;
+  }
+  __device__ __forceinline__ void res_load(int x) {
+    const int n = res_n(x);
+    if (x >= 128 / res_cols() || !inside(n)) return;
+    const int s = x & 1;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&res_bar[s], 2048);
+      tma_load_2d_at(boxes + (1 + s) * 2048, map_r, n, m0, &res_bar[s]);
+    }
+    res_open |= 1u << s;
+  }
+  __device__ __forceinline__ bool res_wait(int s, bool ignore_abort = false) {
+    const bool ok = pair_wait_warp(&res_bar[s], (res_phase >> s) & 1u, abort_flag, peer_abort, q.p.err, 22,
+                                   ignore_abort);
+    res_phase ^= 1u << s;
+    res_open &= ~(1u << s);
+    return ok;
+  }
+
+  __device__ __forceinline__ void begin_tile() {
+    if (q.p.e.bias) {
+      const int n = n0 + 4 * lane, N = q.p.N;
+      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (q.bias_vec && n + 4 <= N) {
+        f = __ldg(reinterpret_cast<const float4*>(q.p.e.bias + n));
+      } else {
+        if (n < N) f.x = __ldg(q.p.e.bias + n);
+        if (n + 1 < N) f.y = __ldg(q.p.e.bias + n + 1);
+        if (n + 2 < N) f.z = __ldg(q.p.e.bias + n + 2);
+        if (n + 3 < N) f.w = __ldg(q.p.e.bias + n + 3);
+      }
+      __syncwarp();
+      const_cast<float4*>(bias4)[lane] = f;
+      __syncwarp();
+    }
+    if (q.res_tma) {
+      res_load(0);
+      res_load(1);
+    }
+  }
+
+  // bias, ReLU and residual on chunk j of this lane's token; false on a timeout
+  __device__ __forceinline__ bool finish(int j, float (&v)[32]) {
+    const Fp8Epilogue& e = q.p.e;
+    const int n = n0 + 32 * chunk(j);
+    if (!inside(n)) {
+      if (q.res_tma) {  // its residual boxes' turn passes
+        const int per = 32 / res_cols();
+        for (int b = 0; b < per; ++b) res_load(j * per + b + 2);
+      }
+      return true;
+    }
+    if (e.bias) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 b = bias4[8 * chunk(j) + i];
+        v[4 * i] = __fadd_rn(v[4 * i], b.x);
+        v[4 * i + 1] = __fadd_rn(v[4 * i + 1], b.y);
+        v[4 * i + 2] = __fadd_rn(v[4 * i + 2], b.z);
+        v[4 * i + 3] = __fadd_rn(v[4 * i + 3], b.w);
+      }
+    }
+    if (e.relu) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = max_nan(v[i], 0.0f);
+    }
+    if (!e.residual) return true;
+    if (q.res_tma) {
+      if (e.res_type == FTB_F32) return add_boxes<float>(j, v);
+      if (e.res_type == FTB_F16) return add_boxes<__half>(j, v);
+      return add_boxes<__nv_bfloat16>(j, v);
+    }
+    const int64_t m = (int64_t)m0 + lane;
+    if (m < q.p.M) {
+      const int64_t at = m * e.res_ld;
+      if (e.res_type == FTB_F32) add_residual32(static_cast<const float*>(e.residual) + at, n, q.p.N, e.res_vec, v);
+      else if (e.res_type == FTB_F16)
+        add_residual32(static_cast<const __half*>(e.residual) + at, n, q.p.N, e.res_vec, v);
+      else add_residual32(static_cast<const __nv_bfloat16*>(e.residual) + at, n, q.p.N, e.res_vec, v);
+    }
+    return true;
+  }
+  template <typename T>
+  __device__ __forceinline__ bool add_boxes(int j, float (&v)[32]) {
+    constexpr int C = 64 / (int)sizeof(T), E = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int b = 0; b < 32 / C; ++b) {
+      const int x = j * (32 / C) + b, s = x & 1;
+      if (!inside(res_n(x))) {
+        res_load(x + 2);
+        continue;
+      }
+      if (!res_wait(s)) return false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 u = ld_shared4(box_at(boxes + (1 + s) * 2048, lane, i));
+        T t[E];
+        memcpy(t, &u, 16);
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[b * C + i * E + k] = __fadd_rn(v[b * C + i * E + k], to_f32(t[k]));
+      }
+      __syncwarp();
+      res_load(x + 2);
+    }
+    return true;
+  }
+
+  // A staging box that the stores before have been read from.
+  __device__ __forceinline__ uint32_t box_begin() {
+    if (q.res_tma) {
+      if (lane == 0) bulk_wait_read();
+      __syncwarp();
+      return boxes;
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kFp8Boxes - 1) : "memory");
     __syncwarp();
+    const uint32_t box = boxes + next * 2048u;
+    next = next + 1 == kFp8Boxes ? 0 : next + 1;
+    return box;
   }
-  __device__ __forceinline__ void put64(int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
-    st_shared4(box + lane * 64 + ((chunk ^ ((lane >> 1) & 3)) << 4), a, b, c, d);
-  }
-  __device__ __forceinline__ void end(const CUtensorMap* map, int n, int m) const {
+  __device__ __forceinline__ void box_store(uint32_t box, int n) {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      tma_store_2d(map, n, m, box);
+      tma_store_2d(map_y, n, m0, box);
       bulk_commit();
     }
   }
@@ -159,15 +299,14 @@ struct Fp8Staging {
 
 // Rows of a staged box into an output without TMA: its rows are not 16-byte
 // aligned, or the box reaches past the last column (a TMA store clips columns
-// in units of 16 bytes only).  C columns from n, R rows at a time.
+// in units of 16 bytes only).
 template <typename U>
 __device__ __forceinline__ void store_box_rows(uint32_t box, U* y, int64_t ld, int m0, int n, int M, int N, int lane) {
-  constexpr int E = (int)sizeof(U), W = E == 1 ? 32 : 64, C = W / E, R = 32 / C;
+  constexpr int E = (int)sizeof(U), C = 64 / E;
   __syncwarp();
-  for (int r0 = 0; r0 < 32; r0 += R) {
-    const int r = r0 + lane / C, c = lane % C;
-    const uint32_t swz = E == 1 ? 0u : (uint32_t)((r >> 1) & 3);
-    const uint32_t at = box + r * W + ((((uint32_t)(c * E) >> 4) ^ swz) << 4) + ((c * E) & 15);
+  for (int x = lane; x < 32 * C; x += 32) {
+    const int r = x / C, c = x % C;
+    const uint32_t at = box_at(box, r, (c * E) >> 4) + ((c * E) & 15);
     uint32_t u;
     if constexpr (E == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(at));
     else if constexpr (E == 2) asm volatile("{ .reg .u16 t; ld.shared.u16 t, [%1]; cvt.u32.u16 %0, t; }" : "=r"(u) : "r"(at));
@@ -177,15 +316,15 @@ __device__ __forceinline__ void store_box_rows(uint32_t box, U* y, int64_t ld, i
   __syncwarp();
 }
 
-// 32 finished columns of 32 tokens (lane = token) into a plain output.
+// 32 finished columns (from n) of a warp's tokens into a plain output.
 template <typename T>
-__device__ __forceinline__ void store_plain32(const Fp8PairParams& q, const CUtensorMap* map, const Fp8Staging& st, int m0,
-                                              int n, const float (&v)[32]) {
+__device__ __forceinline__ void store_plain32(Fp8EpilogueWarp& w, int n, const float (&v)[32]) {
   constexpr int C = 64 / (int)sizeof(T);  // columns per box
+  const Fp8Params& p = w.q.p;
 #pragma unroll
   for (int b = 0; b < 32 / C; ++b) {
-    if (n + b * C >= q.p.N) break;
-    st.begin();
+    if (n + b * C >= p.N) break;
+    const uint32_t box = w.box_begin();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       T t[C / 4];
@@ -193,26 +332,71 @@ __device__ __forceinline__ void store_plain32(const Fp8PairParams& q, const CUte
       for (int j = 0; j < C / 4; ++j) t[j] = from_f32<T>(v[b * C + i * (C / 4) + j]);
       uint32_t u[4];
       memcpy(u, t, 16);
-      st.put64(i, u[0], u[1], u[2], u[3]);
+      st_shared4(box_at(box, w.lane, i), u[0], u[1], u[2], u[3]);
     }
-    if (q.y_tma && n + (b + 1) * C <= q.p.N) {
-      st.end(map, n + b * C, m0);
+    if (w.q.y_tma && n + (b + 1) * C <= p.N) {
+      w.box_store(box, n + b * C);
     } else {
       using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
-      store_box_rows(st.box, static_cast<U*>(q.p.e.y), q.p.e.y_ld, m0, n + b * C, q.p.M, q.p.N, st.lane);
+      store_box_rows(box, static_cast<U*>(p.e.y), p.e.y_ld, w.m0, n + b * C, p.M, p.N, w.lane);
     }
   }
 }
 
+// One block (this lane's 128 columns, in chunk order) into a quantised output.
+__device__ __forceinline__ void store_quantized(Fp8EpilogueWarp& w, float (&v)[4][32]) {
+  const Fp8Params& p = w.q.p;
+  float top = 0.0f;  // NaN is passed over
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[j][i]));
+  uint32_t amax = __float_as_uint(top);
+  if (amax >= 0x7F800000u) {  // an infinity: the scale comes from the finite values
+    amax = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        amax = max(amax, finite_abs_bits(v[j][i]));
+        v[j][i] = nan_unless_finite(v[j][i]);
+      }
+  }
+  const uint32_t byte = fp8_scale_byte(amax);
+  const float inv = fp8_inv_scale(byte);
+  const int64_t m = (int64_t)w.m0 + w.lane;
+  if (m < p.M) p.e.ys[m * p.e.ys_ld + w.n0 / kFp8Block] = (uint8_t)byte;
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {  // boxes of 64 columns: chunks 2 b and 2 b + 1 in order
+    const int n = w.n0 + 64 * (w.half ? 1 - b : b);
+    if (n >= p.N) continue;
+    const uint32_t box = w.box_begin();
+#pragma unroll
+    for (int j = 2 * b; j < 2 * b + 2; ++j) {
+      const int first = 2 * (w.chunk(j) & 1);
+      uint32_t u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        u[i] = fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
+      st_shared4(box_at(box, w.lane, first), u[0], u[1], u[2], u[3]);
+      st_shared4(box_at(box, w.lane, first + 1), u[4], u[5], u[6], u[7]);
+    }
+    if (n + 64 <= p.N) w.box_store(box, n);
+    else store_box_rows(box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, w.m0, n, p.M, p.N, w.lane);
+  }
+}
+
+template <bool QUANT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
-                    const __grid_constant__ CUtensorMap map_y, const Fp8PairParams q) {
+                    const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_r,
+                    const Fp8PairParams q) {
   using L = Fp8PairSmem;
   constexpr int STAGES = kFp8PairStages;
   constexpr uint32_t kAcc1 = 224, kSf = 480;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* staging = smem + STAGES * L::STAGE_BYTES;
+  uint8_t* boxes = smem + STAGES * L::STAGE_BYTES;
   uint8_t* sf = smem + L::SF_OFF;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);  // this CTA's loads landed
   uint64_t* ready = full + STAGES;      // leader: both CTAs' loads landed
@@ -223,8 +407,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
   uint64_t* acce = accf + 2;            // [2] leader: accumulator read (16 warps)
   uint64_t* shared_cols = acce + 2;     // leader: the shared columns read (16 warps), once per tile
   uint64_t* drain = shared_cols + 1;    // leader: MMAs retired after an abort
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(drain + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 1) + 1;
+  uint64_t* res_bar = drain + 1;        // [8][2] an epilogue warp's residual boxes
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(res_bar + 16);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(res_bar + 16) + 1;
 
   const Fp8Params& p = q.p;
   const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
@@ -248,6 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
     }
     mbar_init(shared_cols, 16);
     mbar_init(drain, 1);
+    for (int s = 0; s < 16; ++s) mbar_init(&res_bar[s], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -262,6 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
     prefetch_map(&map_a);
     prefetch_map(&map_w);
     if (q.y_tma) prefetch_map(&map_y);
+    if (q.res_tma) prefetch_map(&map_r);
   }
   __syncwarp();
   tc_fence_before();
@@ -395,118 +582,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
     }
   } else {
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const Fp8Staging st{smem_u32(staging) + (uint32_t)(warp - 4) * 2048u, lane};
-    float4* bias4 = reinterpret_cast<float4*>(staging + L::STAGING + (warp - 4) * 512);
+    Fp8EpilogueWarp w{q, &map_y, &map_r, smem_u32(boxes) + (uint32_t)(warp - 4) * (kFp8Boxes * 2048u),
+                      reinterpret_cast<const float4*>(boxes + L::BOXES + (warp - 4) * 512), res_bar + 2 * (warp - 4),
+                      lane, 0, 0, half, 0u, 0u, 0u, abort_flag, peer_abort};
     const uint32_t shared_leader = cluster_addr(shared_cols, 0);
     uint32_t tc = 0;
-    for (int t = pair; t < ntiles; t += npairs, ++tc) {
+    bool ok = true;
+    for (int t = pair; t < ntiles && ok; t += npairs, ++tc) {
       const uint32_t b = tc & 1u;
-      int m0, n0;
-      tiles.at(t, m0, n0);
-      m0 += (int)rank * 128 + quarter * 32;
-      n0 += half * 128;
-      if (p.e.bias) {  // this tile's, while its products run
-        const int n = n0 + 4 * lane;
-        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (q.bias_vec && n + 4 <= p.N) {
-          f = __ldg(reinterpret_cast<const float4*>(p.e.bias + n));
-        } else {
-          if (n < p.N) f.x = __ldg(p.e.bias + n);
-          if (n + 1 < p.N) f.y = __ldg(p.e.bias + n + 1);
-          if (n + 2 < p.N) f.z = __ldg(p.e.bias + n + 2);
-          if (n + 3 < p.N) f.w = __ldg(p.e.bias + n + 3);
-        }
-        __syncwarp();
-        bias4[lane] = f;
-        __syncwarp();
-      }
-      if (!pair_wait_warp(&accf[b], (tc >> 1) & 1u, abort_flag, peer_abort, p.err, 21)) break;
+      tiles.at(t, w.m0, w.n0);
+      w.m0 += (int)rank * 128 + quarter * 32;
+      w.n0 += half * 128;
+      w.begin_tile();
+      if (!(ok = pair_wait_warp(&accf[b], (tc >> 1) & 1u, abort_flag, peer_abort, p.err, 21))) break;
       tc_fence_after();
-      const int64_t m = (int64_t)m0 + lane;
       const uint32_t acc = tmem + b * kAcc1 + (uint32_t)half * 128 + ((uint32_t)(quarter * 32) << 16);
       const uint32_t acce_leader = cluster_addr(&acce[b], 0);
-      // the chunk that holds the shared columns comes first: the last of
-      // accumulator 0's upper half, the first of accumulator 1's lower half
-      auto chunk = [&](int j) { return half ? 3 - j : j; };
       auto load = [&](int j, float (&v)[32]) {
         uint32_t r[32];
-        FTB_TMEM_LD32(acc + 32 * chunk(j), r);
+        FTB_TMEM_LD32(acc + 32 * w.chunk(j), r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        if (j == 0 || j == 3) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(j == 0 ? shared_leader : acce_leader);
+        }
       };
-      auto release = [&](uint32_t leader_bar) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(leader_bar);
-      };
-      if (p.e.y_type != kFp8Type) {
+      if constexpr (!QUANT) {
 #pragma unroll 1
         for (int j = 0; j < 4; ++j) {
           float v[32];
           load(j, v);
-          if (j == 0) release(shared_leader);
-          if (j == 3) release(acce_leader);
-          const int n = n0 + 32 * chunk(j);
-          if (n >= p.N || m0 >= p.M) continue;
-          fp8_epilogue32(q, m, n, bias4 + 8 * chunk(j), v);
-          if (p.e.y_type == FTB_F32) store_plain32<float>(q, &map_y, st, m0, n, v);
-          else if (p.e.y_type == FTB_F16) store_plain32<__half>(q, &map_y, st, m0, n, v);
-          else store_plain32<__nv_bfloat16>(q, &map_y, st, m0, n, v);
+          const int n = w.n0 + 32 * w.chunk(j);
+          if (ok) ok = w.finish(j, v);
+          if (!ok || !w.inside(n)) continue;
+          if (p.e.y_type == FTB_F32) store_plain32<float>(w, n, v);
+          else if (p.e.y_type == FTB_F16) store_plain32<__half>(w, n, v);
+          else store_plain32<__nv_bfloat16>(w, n, v);
         }
       } else {
-        const bool inside = n0 < p.N && m0 < p.M;
-        float first[32];
-        uint32_t amax = 0;
-        auto finish = [&](int j, float (&v)[32]) {
-          const int n = n0 + 32 * chunk(j);
-          if (inside && n < p.N) fp8_epilogue32(q, m, n, bias4 + 8 * chunk(j), v);
+        float v[4][32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (n + i >= p.N) v[i] = 0.0f;
-        };
-        load(0, first);
-        release(shared_leader);
-        finish(0, first);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) amax = max(amax, finite_abs_bits(first[i]));
-#pragma unroll 1
-        for (int j = 1; j < 4; ++j) {
-          float v[32];
-          load(j, v);
-          finish(j, v);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) amax = max(amax, finite_abs_bits(v[i]));
-        }
-        const uint32_t byte = fp8_scale_byte(amax);
-        const float inv = fp8_inv_scale(byte);
-        if (inside && m < p.M) p.e.ys[m * p.e.ys_ld + n0 / kFp8Block] = (uint8_t)byte;
-#pragma unroll 1
         for (int j = 0; j < 4; ++j) {
-          float v[32];
-          if (j == 0) {
+          load(j, v[j]);
+          if (ok) ok = w.finish(j, v[j]);
+          const int n = w.n0 + 32 * w.chunk(j);
+          if (n + 32 > p.N) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = first[i];
-          } else {
-            load(j, v);
-            if (j == 3) release(acce_leader);
-            finish(j, v);
+            for (int i = 0; i < 32; ++i)
+              if (n + i >= p.N) v[j][i] = 0.0f;
           }
-          const int n = n0 + 32 * chunk(j);
-          if (!inside || n >= p.N) continue;
-          uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = fp8_pack4(nan_unless_finite(v[4 * i]), nan_unless_finite(v[4 * i + 1]),
-                             nan_unless_finite(v[4 * i + 2]), nan_unless_finite(v[4 * i + 3]), inv);
-          st.begin();
-          st_shared4(st.box + lane * 32, w[0], w[1], w[2], w[3]);
-          st_shared4(st.box + lane * 32 + 16, w[4], w[5], w[6], w[7]);
-          if (n + 32 <= p.N) st.end(&map_y, n, m0);
-          else store_box_rows(st.box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, m0, n, p.M, p.N, lane);
         }
+        if (ok && w.inside(w.n0)) store_quantized(w, v);
       }
     }
+    for (int s = 0; s < 2; ++s)  // residual loads in flight land before the CTA leaves
+      if (w.res_open >> s & 1u) w.res_wait(s, /*ignore_abort=*/true);
     if (lane == 0) bulk_wait_all();  // this warp's stores are complete before the CTA leaves
   }
   tc_fence_before();
@@ -524,55 +657,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
 
 // Shared-memory attribute and the number of pairs that are resident at once.
 inline cudaError_t fp8_pair_prepare(int* pairs) {
-  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8PairSmem::TOTAL);
+  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Fp8PairSmem::TOTAL);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(fp8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8PairSmem::TOTAL);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2, 1, 1);
   cfg.blockDim = dim3(kFp8PairThreads, 1, 1);
   cfg.dynamicSmemBytes = Fp8PairSmem::TOTAL;
-  e = cudaOccupancyMaxActiveClusters(pairs, fp8_pair_kernel, &cfg);
+  e = cudaOccupancyMaxActiveClusters(pairs, fp8_pair_kernel<false>, &cfg);
   if (e == cudaSuccess && *pairs <= 0) e = cudaErrorInvalidConfiguration;
   return e;
 }
 
-// The output as TMA stores it: boxes of 32 rows x 64 bytes (64-byte swizzle),
-// of 32 x 32 bytes for a quantised one.  False where its rows are not 16-byte
-// aligned.
-inline bool make_map_fp8_out(CUtensorMap* map, const Fp8Epilogue& e, int64_t m, int64_t n) {
-  const int size = e.y_type == FTB_F32 ? 4 : e.y_type == kFp8Type ? 1 : 2;
-  if ((reinterpret_cast<uintptr_t>(e.y) & 15) || (e.y_ld * size) % 16) return false;
+// An output or residual as the epilogue moves it: boxes of 32 rows x 64 bytes,
+// 64-byte swizzle.  False where its rows are not 16-byte aligned.
+inline bool make_map_fp8_box(CUtensorMap* map, void* base, int type, int64_t ld, int64_t m, int64_t n) {
+  const int size = type == FTB_F32 ? 4 : type == kFp8Type ? 1 : 2;
+  if (!base || (reinterpret_cast<uintptr_t>(base) & 15) || (ld * size) % 16) return false;
   PFN_encodeTiled enc = tma_encoder();
   if (!enc) return false;
-  const int bytes = e.y_type == kFp8Type ? 32 : 64;
   cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)m};
-  cuuint64_t strides[1] = {(cuuint64_t)(e.y_ld * size)};
-  cuuint32_t box[2] = {(cuuint32_t)(bytes / size), 32};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
+  cuuint32_t box[2] = {(cuuint32_t)(64 / size), 32};
   cuuint32_t estr[2] = {1, 1};
-  const CUtensorMapDataType type = size == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                   : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
-                                               : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  return enc(map, type, 2, e.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
+  const CUtensorMapDataType dtype = size == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                    : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  return enc(map, dtype, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 inline cudaError_t launch_fp8_pair(const Fp8Operands& o, const Fp8Params& p, int max_pairs, int stall_test,
                                    cudaStream_t s) {
-  CUtensorMap map_a, map_w, map_y;
+  CUtensorMap map_a, map_w, map_y, map_r;
   if (!make_map_fp8(&map_a, o.a, p.M, p.K, o.a_ld, 128) || !make_map_fp8(&map_w, o.w, p.N, p.K, o.w_ld, 128))
     return cudaErrorInvalidValue;
   Fp8PairParams q{};
   q.p = p;
   memset(&map_y, 0, sizeof(map_y));
-  q.y_tma = make_map_fp8_out(&map_y, p.e, p.M, p.N) ? 1 : 0;
+  memset(&map_r, 0, sizeof(map_r));
+  q.y_tma = make_map_fp8_box(&map_y, p.e.y, p.e.y_type, p.e.y_ld, p.M, p.N);
   if (!q.y_tma && p.e.y_type == kFp8Type) return cudaErrorInvalidValue;
+  q.res_tma = make_map_fp8_box(&map_r, const_cast<void*>(p.e.residual), p.e.res_type, p.e.res_ld, p.M, p.N);
   q.bias_vec = (reinterpret_cast<uintptr_t>(p.e.bias) & 15) == 0;
   q.stall_test = stall_test;
   const int64_t tiles = (((int64_t)p.M + 255) / 256) * (((int64_t)p.N + 255) / 256);
   if (tiles > 0x3fffffff) return cudaErrorInvalidConfiguration;
   const unsigned pairs = (unsigned)std::min<int64_t>(tiles, max_pairs);
-  return pdl_launch(fp8_pair_kernel, dim3(2 * pairs), dim3(kFp8PairThreads), Fp8PairSmem::TOTAL, s, map_a, map_w,
-                    map_y, q);
+  return pdl_launch(p.e.y_type == kFp8Type ? fp8_pair_kernel<true> : fp8_pair_kernel<false>, dim3(2 * pairs),
+                    dim3(kFp8PairThreads), Fp8PairSmem::TOTAL, s, map_a, map_w, map_y, map_r, q);
 }
 
 }  // namespace ftb

@@ -43,7 +43,8 @@ def check_quantized(got, x, rows):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,k", [(1, 1), (1, 127), (2, 128), (3, 129), (5, 1000), (33, 784), (7, 4096), (300, 515)])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 127), (2, 128), (3, 129), (5, 1000), (33, 784), (7, 4096), (300, 515),
+                                 (1000, 128), (777, 384), (900, 64), (50, 8192), (3, 20000)])
 def test_quantize_rows(m, k, dtype):
     x = randn(m, k, seed=m * 7 + k, dtype=dtype) * 3
     check_quantized(quantize_rows(x), x, 1)
@@ -155,7 +156,8 @@ def check_block(got, want, err, rows=1):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("quantize", [False, True])
-@pytest.mark.parametrize("m,k", [(1, 1), (3, 127), (2, 1111), (300, 512), (4, 4096), (2, 8192), (3, 8200), (2, 20001)])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 127), (2, 1111), (300, 512), (4, 4096), (2, 8192), (3, 8200), (2, 20001),
+                                 (700, 64), (1001, 200), (900, 4096), (400, 1000), (2, 33000)])
 def test_rms_norm(m, k, quantize, residual, dtype):
     x = randn(m, k, seed=k, dtype=dtype) * 2
     r = randn(m, k, seed=k + 1, dtype=dtype) if residual else None
@@ -226,7 +228,8 @@ SHAPES = [(1, 1, 1), (1, 128, 128), (1, 250, 784), (2, 10, 31), (3, 129, 129), (
           (16, 128, 8192), (17, 127, 512), (31, 256, 513), (33, 300, 640), (64, 136, 96), (65, 512, 2048),
           (100, 1000, 1536), (128, 128, 128), (129, 260, 257), (200, 512, 4096), (255, 1, 384), (256, 256, 1024),
           (257, 384, 200), (300, 250, 784), (512, 768, 512), (700, 1100, 130), (1024, 520, 2000), (1, 4096, 4096),
-          (2050, 1024, 320), (1, 40000, 64), (5000, 96, 100), (640, 2304, 1152)]
+          (2050, 1024, 320), (1, 40000, 64), (5000, 96, 100), (640, 2304, 1152), (1290, 2051, 200), (2100, 2304, 130),
+          (1500, 4000, 2100), (4133, 1153, 900), (3000, 5000, 64)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -243,7 +246,8 @@ def test_linear_of_integers_is_exact(m, n, k):
 
 @pytest.mark.parametrize("out_dtype", TYPES)
 @pytest.mark.parametrize("res_dtype", [None] + TYPES)
-@pytest.mark.parametrize("m,n,k", [(1, 250, 784), (20, 384, 512), (140, 513, 300), (600, 640, 384)])
+@pytest.mark.parametrize("m,n,k", [(1, 250, 784), (20, 384, 512), (140, 513, 300), (600, 640, 384), (1290, 2051, 200),
+                                   (2100, 2304, 130)])
 def test_linear_epilogue_and_types(m, n, k, res_dtype, out_dtype):
     """Integer sums, an integer bias and residual: exact in fp32, one rounding to the output's type."""
     a, av = integers(m, k, 1, seed=1)
@@ -263,7 +267,7 @@ def test_linear_epilogue_and_types(m, n, k, res_dtype, out_dtype):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 250, 784), (16, 512, 4096), (20, 384, 512), (140, 513, 300), (600, 1000, 384),
-                                   (1030, 256, 128)])
+                                   (1030, 256, 128), (1290, 2051, 200), (2100, 2304, 130), (3000, 1984, 512)])
 def test_linear_quantized_output(m, n, k):
     a, av = integers(m, k, 1, seed=3)
     w, wv = integers(n, k, 128, seed=4)
@@ -280,6 +284,30 @@ def test_linear_quantized_output(m, n, k):
     check_block(got, want, (np.abs(want) + np.abs(f64(res))) * EPS32)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (40, 1000, 300), (300, 512, 512), (2100, 2304, 130), (1290, 2051, 200)])
+def test_linear_adds_to_its_output_in_place(m, n, k, dtype):
+    a, av = integers(m, k, 1, seed=5)
+    w, wv = integers(n, k, 128, seed=6)
+    x = (torch.arange(m * n).reshape(m, n) % 19 - 9).to(dtype).cuda()
+    want, _ = ref.linear(av, wv, None, False, f64(x))
+    y = fp8_linear(a, w, residual=x, out_dtype=dtype, out=x)
+    assert y is x and torch.equal(y.cpu(), torch.from_numpy(want).float().to(dtype))
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 300, 200), (300, 512, 512), (2100, 2304, 130)])
+def test_linear_infinities_in_a_quantized_output(m, n, k):
+    """An infinite sum is stored as NaN and leaves its block's scale to the finite ones."""
+    a, av = integers(m, k, 1, seed=7)
+    w, wv = integers(n, k, 128, seed=8)
+    bias = torch.zeros(n, device="cuda")
+    bias[5], bias[n - 1] = float("inf"), float("-inf")
+    want, _ = ref.linear(av, wv, f64(bias))
+    v, s = ref.quantize(want)
+    got = fp8_linear(a, w, bias=bias, quantize=True)
+    assert same(f64(got.scales), s) and same(f64(got.data), v)
+
+
 def linear_bound(k, mass):
     """fp32 accumulation of k exact products in any order, each step off by at
     most a whole unit (the tensor cores' alignment truncates): k 2^-23 of
@@ -287,7 +315,8 @@ def linear_bound(k, mass):
     return k * 2.0 ** -23 * mass
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 512, 4096), (16, 300, 8192), (40, 512, 1000), (333, 250, 784), (600, 1024, 2048)])
+@pytest.mark.parametrize("m,n,k", [(1, 512, 4096), (16, 300, 8192), (40, 512, 1000), (333, 250, 784), (600, 1024, 2048),
+                                   (1500, 2304, 4096)])
 def test_linear_of_quantized_normals(m, n, k):
     x, wt = randn(m, k, seed=5) * 3, randn(n, k, seed=6) / k ** 0.5
     a, w = quantize_rows(x), quantize_weight(wt)
@@ -312,7 +341,7 @@ def test_linear_extreme_scales():
         assert bool((y == 256).all())
 
 
-@pytest.mark.parametrize("m", [3, 40, 200, 600])
+@pytest.mark.parametrize("m", [3, 40, 200, 600, 20000])
 def test_linear_nan_stays_in_its_row(m):
     x, wt = randn(m, 300), randn(140, 300, seed=1)
     w = quantize_weight(wt)
@@ -327,7 +356,7 @@ def test_linear_nan_stays_in_its_row(m):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 512, 2048), (7, 512, 2048), (40, 512, 2048), (130, 512, 2048), (300, 512, 2048),
-                                   (900, 512, 2048)])
+                                   (900, 512, 2048), (1900, 2304, 512)])
 def test_linear_ignores_what_lies_around_its_operands(m, n, k):
     """Columns past k, scales past the last block and rows past the last hold NaN; k ends inside a block."""
     k -= 100
@@ -364,7 +393,7 @@ def layers():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m", [1, 5, 16, 70, 400])
+@pytest.mark.parametrize("m", [1, 5, 16, 70, 400, 3000])
 def test_block_of_operators(m, dtype, layers):
     """Each operator against float64 on the values its predecessor returned, then the chain's own error: three
     roundings to e4m3 (2^-4 each, of values whose errors average out) stay below a tenth of the result."""
@@ -383,7 +412,7 @@ def test_block_of_operators(m, dtype, layers):
     assert np.linalg.norm(f64(y) - e) < 0.1 * np.linalg.norm(e)
 
 
-@pytest.mark.parametrize("m", [1, 70, 600])
+@pytest.mark.parametrize("m", [1, 70, 600, 3000])
 def test_block_in_a_graph_and_on_two_streams(m, layers):
     x, res = randn(m, 500, seed=1), randn(m, 500, seed=2)
     x2, res2 = randn(m, 500, seed=3), randn(m, 500, seed=4)
