@@ -7,16 +7,18 @@ point raises :class:`ForgeTuneRuntimeError`.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import json
 import os
 import threading
 from typing import Optional
 
-from .build_native import LIB_PATH
+from .build_native import LIB_PATH, TORCH_OPS_PATH
 from .errors import ForgeTuneRuntimeError
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
+_ops = None
 
 c_void_p, c_size_t, c_int, c_int64, c_double, c_char_p, c_uint64 = (
     ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64, ctypes.c_double, ctypes.c_char_p,
@@ -50,11 +52,11 @@ _SIGS = {
     "ftb_philox_normal": ([c_void_p, c_uint64, c_uint64, c_uint64, c_void_p], c_int),
     "ftb_small_gemm_noalloc": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                 ctypes.c_uint32, c_void_p], c_int),
-    # the arguments' structs, packed by fp8.py
-    "ftb_quantize_rows": ([c_char_p, c_void_p], c_int),
-    "ftb_quantize_weight": ([c_char_p, c_void_p], c_int),
-    "ftb_rms_norm": ([c_char_p, c_void_p], c_int),
-    "ftb_fp8_linear": ([c_char_p, c_void_p], c_int),
+    # pointers to the argument structs (csrc/torch_ops.cpp fills them)
+    "ftb_quantize_rows": ([c_void_p, c_void_p], c_int),
+    "ftb_quantize_weight": ([c_void_p, c_void_p], c_int),
+    "ftb_rms_norm": ([c_void_p, c_void_p], c_int),
+    "ftb_fp8_linear": ([c_void_p, c_void_p], c_int),
 }
 
 EXPORTED = sorted(_SIGS)
@@ -80,6 +82,29 @@ def lib() -> ctypes.CDLL:
                 fn.restype = rest
             _lib = L
     return _lib
+
+
+def torch_ops():
+    """The extension module behind fp8.py (csrc/torch_ops.cpp), loaded once."""
+    global _ops
+    if _ops is None:
+        lib()  # the extension links the engine library
+        with _lock:
+            if _ops is None:
+                import torch  # noqa: F401  (its libraries, which the extension links)
+                if not os.path.isfile(TORCH_OPS_PATH):
+                    raise ForgeTuneRuntimeError(
+                        "_torch_ops.so is not built (%s); run `python -m forgetune_b200.build_native`"
+                        % TORCH_OPS_PATH)
+                try:
+                    spec = importlib.util.spec_from_file_location("_torch_ops", TORCH_OPS_PATH)
+                    module = importlib.util.module_from_spec(spec)
+                    spec.loader.exec_module(module)
+                except (ImportError, OSError) as e:
+                    raise ForgeTuneRuntimeError("cannot load %s (built against another torch?): %s"
+                                                % (TORCH_OPS_PATH, e)) from e
+                _ops = module
+    return _ops
 
 
 def last_error() -> str:

@@ -4,17 +4,20 @@
 
 The library holds the engine (graph blob, fusion, arena planner), every CUDA
 kernel and the C ABI declared in include/forgetune_b200.h.  It is written to
-forgetune_b200/lib/ and linked (with an rpath) by every per-model shim.
+forgetune_b200/lib/ and linked (with an rpath) by every per-model shim and by
+_torch_ops.so, the extension behind the operators on torch tensors.
 """
 
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 import time
 from concurrent.futures import ThreadPoolExecutor
 
@@ -24,6 +27,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libforgetune_b200.so")
+TORCH_OPS_PATH = os.path.join(LIB_DIR, "_torch_ops.so")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 
 SOURCES = ["runtime.cu", "fp8.cu", "engine.cpp"]
@@ -62,7 +66,7 @@ def _newer(target, files) -> bool:
 
 
 def up_to_date() -> bool:
-    return _newer(LIB_PATH, _inputs())
+    return _newer(LIB_PATH, _inputs()) and _newer(TORCH_OPS_PATH, _inputs("torch_ops.cpp"))
 
 
 def _run(cmd, target, verbose) -> None:
@@ -75,7 +79,7 @@ def _run(cmd, target, verbose) -> None:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("nvcc failed (%d):\n%s\n%s" % (r.returncode, r.stdout[-4000:], r.stderr[-8000:]))
+        raise RuntimeError("%s failed (%d):\n%s\n%s" % (os.path.basename(cmd[0]), r.returncode, r.stdout[-4000:], r.stderr[-8000:]))
     os.utime(tmp, (began, began))
     os.replace(tmp, target)
 
@@ -89,14 +93,30 @@ def _compile(source, force, verbose) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile what changed (the sources side by side) and link the library."""
+    """Compile what changed (the sources side by side), link the library and build the torch extension."""
     if not force and up_to_date():
         return LIB_PATH
     os.makedirs(OBJ_DIR, exist_ok=True)
     with ThreadPoolExecutor(len(SOURCES)) as pool:
         objs = list(pool.map(lambda s: _compile(s, force, verbose), SOURCES))
-    _run([nvcc()] + ARCH_FLAGS + ["-shared"] + objs, LIB_PATH, verbose)
+    if force or not _newer(LIB_PATH, objs):
+        _run([nvcc()] + ARCH_FLAGS + ["-shared"] + objs, LIB_PATH, verbose)
+    if force or not _newer(TORCH_OPS_PATH, _inputs("torch_ops.cpp")):
+        _build_torch_ops(verbose)
     return LIB_PATH
+
+
+def _build_torch_ops(verbose) -> None:
+    """The CPython extension behind fp8.py, against the installed torch and the engine library."""
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    torch_lib = os.path.join(torch_dir, "lib")
+    _run(["g++", "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-shared", "-I", INCLUDE]
+         + [a for d in include for a in ("-isystem", d)] + [os.path.join(CSRC, "torch_ops.cpp"), "-L", torch_lib]
+         + ["-l" + n for n in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python")]
+         + ["-L", LIB_DIR, "-l:" + os.path.basename(LIB_PATH), "-Wl,-rpath,$ORIGIN"], TORCH_OPS_PATH, verbose)
 
 
 def main() -> int:
