@@ -15,41 +15,43 @@
 // Persistent pairs walk the tiles in bands of 16 row blocks (74 pairs at work
 // then share 16 + 5 operand blocks of 256 rows through L2, not 2 + 37;
 // 8192^3: 385 us, with bands of 8 390, of 4 401).
-// Twelve warps per CTA:
+// Warps per CTA:
 //   warp 0     TMA producer of this CTA's rows (its own barriers);
 //   warp 1     tensor memory; in the leader CTA the MMAs of the pair;
 //   warp 2     scale factors of this CTA, four k-blocks at a time;
 //   warp 3     passes this CTA's landed stages on to the leader;
-//   warps 4-11 epilogue: a lane quarter and one half (128) of the columns
-//              each, a lane a token, 32 columns at a time.  Outputs leave
-//              through staging boxes and TMA stores (row stores where rows are
-//              not 16-byte aligned, and for a box that ends outside); the
-//              residual arrives by TMA two boxes ahead; bias is staged while
-//              the products run.  A quantised output keeps its 128 columns,
-//              one block, in registers until their largest is known.
-// Short depths are bound by the epilogue: 8192 x 8192 outputs of depth 64 take
-// 48 us in bf16, 56 quantised, 79 with a bf16 residual (floors by bytes 21, 10
-// and 41 us).
+//   from 4 on  the epilogue: 16 warps with 64 columns each, or 8 with 128 for a
+//              quantised output, which keeps its block of 128 columns in
+//              registers until their largest is known.  A lane is a token; 32
+//              columns at a time go out through the warp's box in shared
+//              memory and a TMA store (row stores where the output's rows are
+//              not 16-byte aligned, and for a box that ends outside).  The
+//              residual comes in by TMA through the same box; bias is staged
+//              while the products run.
+// Short depths are bound by the epilogue (TODO).
 #pragma once
 
 #include "fp8_gemm.cuh"
 
 namespace ftb {
 
-constexpr int kFp8PairThreads = 384;
-constexpr int kFp8PairStages = 5;
-constexpr int kFp8Boxes = 3;  // 2 KB boxes per epilogue warp: staging, or one of staging and two of residual
 constexpr int kFp8Band = 16;
 
-struct Fp8PairSmem {
+template <bool QUANT>
+struct Fp8PairShape {
+  static constexpr int WARPS = QUANT ? 8 : 16;       // of the epilogue
+  static constexpr int COLUMNS = 1024 / WARPS;       // of each, for one quarter of the lanes
+  static constexpr int CHUNKS = COLUMNS / 32;
+  static constexpr int THREADS = 128 + 32 * WARPS;
+  static constexpr int STAGES = QUANT ? 6 : 5;
   static constexpr int OPERAND_BYTES = 128 * 128;
   static constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
   static constexpr int SF_BYTES = 512 + 1024;
-  static constexpr int BOXES = 8 * kFp8Boxes * 2048;
-  static constexpr int BIAS = 8 * 512;  // bias of a warp's columns
-  static constexpr int SF_OFF = kFp8PairStages * STAGE_BYTES + BOXES + BIAS;
+  static constexpr int BOXES = WARPS * 2048;
+  static constexpr int BIAS = WARPS * COLUMNS * 4;
+  static constexpr int SF_OFF = STAGES * STAGE_BYTES + BOXES + BIAS;
   static constexpr int BAR_OFF = SF_OFF + 2 * SF_BYTES;
-  static constexpr int NBAR = 3 * kFp8PairStages + 4 + 4 + 2 + 16;
+  static constexpr int NBAR = 3 * STAGES + 4 + 4 + 2 + WARPS;
   static constexpr int TOTAL = 1024 + BAR_OFF + 8 * NBAR + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
 };
@@ -141,54 +143,58 @@ __device__ __forceinline__ uint32_t box_at(uint32_t box, int lane, int i) {
   return box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
 }
 
-// One epilogue warp: its boxes, bias and residual loads.
+// One epilogue warp: its box, bias and residual loads.
+template <bool QUANT>
 struct Fp8EpilogueWarp {
+  using L = Fp8PairShape<QUANT>;
   const Fp8PairParams& q;
   const CUtensorMap *map_y, *map_r;
-  uint32_t boxes;       // shared address of its kFp8Boxes boxes
-  const float4* bias4;  // its 128 columns
-  uint64_t* res_bar;    // [2] residual box landed
+  uint32_t box;         // shared address of its 2 KB
+  const float4* bias4;  // its columns
+  uint64_t* res_bar;    // residual box landed
   int lane;
-  int m0, n0, half;     // its tokens and columns of this tile
-  uint32_t next;        // staging box in turn
-  uint32_t res_phase;   // bit s: parity of residual slot s
-  uint32_t res_open;    // bit s: a load into slot s has not been waited for
+  int group;            // its columns begin at COLUMNS group
+  int m0, n0;           // its tokens and columns of this tile
+  uint32_t res_phase;   // parity of res_bar
+  bool res_open;        // a load has not been waited for
   volatile int* abort_flag;
   uint32_t peer_abort;
 
   // the chunk that holds the columns that the accumulators share comes first:
-  // the last of accumulator 0's upper half, the first of accumulator 1's lower
-  __device__ __forceinline__ int chunk(int j) const { return half ? 3 - j : j; }
+  // the last of accumulator 0, the first of accumulator 1
+  __device__ __forceinline__ int chunk(int j) const { return 2 * group >= L::WARPS / 4 ? L::CHUNKS - 1 - j : j; }
+  __device__ __forceinline__ int column(int j) const { return n0 + 32 * chunk(j); }
   __device__ __forceinline__ bool inside(int n) const { return n < q.p.N && m0 < q.p.M; }
   __device__ __forceinline__ int res_cols() const { return q.p.e.res_type == FTB_F32 ? 16 : 32; }
 
-  // Residual box x of the tile (4 of 32 columns or 8 of 16, in chunk order)
-  // goes to slot x & 1.
-  __device__ __forceinline__ int res_n(int x) const {
-    const int cols = res_cols(), per = 32 / cols;
-    return n0 + 32 * chunk(x / per) + x % per * cols;
-  }
-  __device__ __forceinline__ void res_load(int x) {
-    const int n = res_n(x);
-    if (x >= 128 / res_cols() || !inside(n)) return;
-    const int s = x & 1;
+  // Residual columns from n into the box, once the stores from it have read it.
+  __device__ __forceinline__ void res_load(int n) {
     if (lane == 0) {
-      mbar_arrive_expect_tx(&res_bar[s], 2048);
-      tma_load_2d_at(boxes + (1 + s) * 2048, map_r, n, m0, &res_bar[s]);
+      bulk_wait_read();
+      mbar_arrive_expect_tx(res_bar, 2048);
+      tma_load_2d_at(box, map_r, n, m0, res_bar);
     }
-    res_open |= 1u << s;
+    res_open = true;
   }
-  __device__ __forceinline__ bool res_wait(int s, bool ignore_abort = false) {
-    const bool ok = pair_wait_warp(&res_bar[s], (res_phase >> s) & 1u, abort_flag, peer_abort, q.p.err, 22,
-                                   ignore_abort);
-    res_phase ^= 1u << s;
-    res_open &= ~(1u << s);
+  __device__ __forceinline__ bool res_wait(bool ignore_abort = false) {
+    const bool ok = pair_wait_warp(res_bar, res_phase, abort_flag, peer_abort, q.p.err, 22, ignore_abort);
+    res_phase ^= 1u;
+    res_open = false;
     return ok;
+  }
+  // The first residual box of the first chunk from j on that is inside.
+  __device__ __forceinline__ void res_next(int j) {
+    for (; j < L::CHUNKS; ++j)
+      if (inside(column(j))) {
+        __syncwarp();
+        res_load(column(j));
+        return;
+      }
   }
 
   __device__ __forceinline__ void begin_tile() {
     if (q.p.e.bias) {
-      const int n = n0 + 4 * lane, N = q.p.N;
+      const int n = n0 + 4 * lane, N = 4 * lane < L::COLUMNS ? q.p.N : 0;
       float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (q.bias_vec && n + 4 <= N) {
         f = __ldg(reinterpret_cast<const float4*>(q.p.e.bias + n));
@@ -199,26 +205,17 @@ struct Fp8EpilogueWarp {
         if (n + 3 < N) f.w = __ldg(q.p.e.bias + n + 3);
       }
       __syncwarp();
-      const_cast<float4*>(bias4)[lane] = f;
+      if (4 * lane < L::COLUMNS) const_cast<float4*>(bias4)[lane] = f;
       __syncwarp();
     }
-    if (q.res_tma) {
-      res_load(0);
-      res_load(1);
-    }
+    if (q.res_tma) res_next(0);
   }
 
   // bias, ReLU and residual on chunk j of this lane's token; false on a timeout
   __device__ __forceinline__ bool finish(int j, float (&v)[32]) {
     const Fp8Epilogue& e = q.p.e;
-    const int n = n0 + 32 * chunk(j);
-    if (!inside(n)) {
-      if (q.res_tma) {  // its residual boxes' turn passes
-        const int per = 32 / res_cols();
-        for (int b = 0; b < per; ++b) res_load(j * per + b + 2);
-      }
-      return true;
-    }
+    const int n = column(j);
+    if (!inside(n)) return true;
     if (e.bias) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -254,40 +251,30 @@ struct Fp8EpilogueWarp {
     constexpr int C = 64 / (int)sizeof(T), E = 16 / (int)sizeof(T);
 #pragma unroll
     for (int b = 0; b < 32 / C; ++b) {
-      const int x = j * (32 / C) + b, s = x & 1;
-      if (!inside(res_n(x))) {
-        res_load(x + 2);
-        continue;
+      if (b > 0) {
+        if (!inside(column(j) + b * C)) break;
+        __syncwarp();
+        res_load(column(j) + b * C);
       }
-      if (!res_wait(s)) return false;
+      if (!res_wait()) return false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint4 u = ld_shared4(box_at(boxes + (1 + s) * 2048, lane, i));
+        const uint4 u = ld_shared4(box_at(box, lane, i));
         T t[E];
         memcpy(t, &u, 16);
 #pragma unroll
         for (int k = 0; k < E; ++k) v[b * C + i * E + k] = __fadd_rn(v[b * C + i * E + k], to_f32(t[k]));
       }
-      __syncwarp();
-      res_load(x + 2);
     }
     return true;
   }
 
-  // A staging box that the stores before have been read from.
-  __device__ __forceinline__ uint32_t box_begin() {
-    if (q.res_tma) {
-      if (lane == 0) bulk_wait_read();
-      __syncwarp();
-      return boxes;
-    }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kFp8Boxes - 1) : "memory");
+  // The box, once the store before has read it and every lane its residual.
+  __device__ __forceinline__ void box_begin() const {
+    if (lane == 0) bulk_wait_read();
     __syncwarp();
-    const uint32_t box = boxes + next * 2048u;
-    next = next + 1 == kFp8Boxes ? 0 : next + 1;
-    return box;
   }
-  __device__ __forceinline__ void box_store(uint32_t box, int n) {
+  __device__ __forceinline__ void box_store(int n) const {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
@@ -318,13 +305,13 @@ __device__ __forceinline__ void store_box_rows(uint32_t box, U* y, int64_t ld, i
 
 // 32 finished columns (from n) of a warp's tokens into a plain output.
 template <typename T>
-__device__ __forceinline__ void store_plain32(Fp8EpilogueWarp& w, int n, const float (&v)[32]) {
+__device__ __forceinline__ void store_plain32(const Fp8EpilogueWarp<false>& w, int n, const float (&v)[32]) {
   constexpr int C = 64 / (int)sizeof(T);  // columns per box
   const Fp8Params& p = w.q.p;
 #pragma unroll
   for (int b = 0; b < 32 / C; ++b) {
     if (n + b * C >= p.N) break;
-    const uint32_t box = w.box_begin();
+    w.box_begin();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       T t[C / 4];
@@ -332,19 +319,19 @@ __device__ __forceinline__ void store_plain32(Fp8EpilogueWarp& w, int n, const f
       for (int j = 0; j < C / 4; ++j) t[j] = from_f32<T>(v[b * C + i * (C / 4) + j]);
       uint32_t u[4];
       memcpy(u, t, 16);
-      st_shared4(box_at(box, w.lane, i), u[0], u[1], u[2], u[3]);
+      st_shared4(box_at(w.box, w.lane, i), u[0], u[1], u[2], u[3]);
     }
     if (w.q.y_tma && n + (b + 1) * C <= p.N) {
-      w.box_store(box, n + b * C);
+      w.box_store(n + b * C);
     } else {
       using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
-      store_box_rows(box, static_cast<U*>(p.e.y), p.e.y_ld, w.m0, n + b * C, p.M, p.N, w.lane);
+      store_box_rows(w.box, static_cast<U*>(p.e.y), p.e.y_ld, w.m0, n + b * C, p.M, p.N, w.lane);
     }
   }
 }
 
 // One block (this lane's 128 columns, in chunk order) into a quantised output.
-__device__ __forceinline__ void store_quantized(Fp8EpilogueWarp& w, float (&v)[4][32]) {
+__device__ __forceinline__ void store_quantized(const Fp8EpilogueWarp<true>& w, float (&v)[4][32]) {
   const Fp8Params& p = w.q.p;
   float top = 0.0f;  // NaN is passed over
 #pragma unroll
@@ -368,9 +355,9 @@ __device__ __forceinline__ void store_quantized(Fp8EpilogueWarp& w, float (&v)[4
   if (m < p.M) p.e.ys[m * p.e.ys_ld + w.n0 / kFp8Block] = (uint8_t)byte;
 #pragma unroll
   for (int b = 0; b < 2; ++b) {  // boxes of 64 columns: chunks 2 b and 2 b + 1 in order
-    const int n = w.n0 + 64 * (w.half ? 1 - b : b);
+    const int n = w.n0 + 64 * (w.chunk(2 * b) / 2);
     if (n >= p.N) continue;
-    const uint32_t box = w.box_begin();
+    w.box_begin();
 #pragma unroll
     for (int j = 2 * b; j < 2 * b + 2; ++j) {
       const int first = 2 * (w.chunk(j) & 1);
@@ -378,21 +365,21 @@ __device__ __forceinline__ void store_quantized(Fp8EpilogueWarp& w, float (&v)[4
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         u[i] = fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
-      st_shared4(box_at(box, w.lane, first), u[0], u[1], u[2], u[3]);
-      st_shared4(box_at(box, w.lane, first + 1), u[4], u[5], u[6], u[7]);
+      st_shared4(box_at(w.box, w.lane, first), u[0], u[1], u[2], u[3]);
+      st_shared4(box_at(w.box, w.lane, first + 1), u[4], u[5], u[6], u[7]);
     }
-    if (n + 64 <= p.N) w.box_store(box, n);
-    else store_box_rows(box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, w.m0, n, p.M, p.N, w.lane);
+    if (n + 64 <= p.N) w.box_store(n);
+    else store_box_rows(w.box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, w.m0, n, p.M, p.N, w.lane);
   }
 }
 
 template <bool QUANT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>::THREADS, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_r,
                     const Fp8PairParams q) {
-  using L = Fp8PairSmem;
-  constexpr int STAGES = kFp8PairStages;
+  using L = Fp8PairShape<QUANT>;
+  constexpr int STAGES = L::STAGES;
   constexpr uint32_t kAcc1 = 224, kSf = 480;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -404,12 +391,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
   uint64_t* sf_full = empty + STAGES;   // [2] leader: both CTAs' scale factors staged
   uint64_t* sf_empty = sf_full + 2;     // [2] the pair's MMAs done with them
   uint64_t* accf = sf_empty + 2;        // [2] accumulator complete
-  uint64_t* acce = accf + 2;            // [2] leader: accumulator read (16 warps)
-  uint64_t* shared_cols = acce + 2;     // leader: the shared columns read (16 warps), once per tile
+  uint64_t* acce = accf + 2;            // [2] leader: accumulator read (both CTAs' epilogue warps)
+  uint64_t* shared_cols = acce + 2;     // leader: the shared columns read (the same), once per tile
   uint64_t* drain = shared_cols + 1;    // leader: MMAs retired after an abort
-  uint64_t* res_bar = drain + 1;        // [8][2] an epilogue warp's residual boxes
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(res_bar + 16);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(res_bar + 16) + 1;
+  uint64_t* res_bar = drain + 1;        // [WARPS] an epilogue warp's residual box landed
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(res_bar + L::WARPS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(res_bar + L::WARPS) + 1;
 
   const Fp8Params& p = q.p;
   const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
@@ -429,11 +416,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
       mbar_init(&sf_full[s], 2);
       mbar_init(&sf_empty[s], 1);
       mbar_init(&accf[s], 1);
-      mbar_init(&acce[s], 16);
+      mbar_init(&acce[s], 2 * L::WARPS);
     }
-    mbar_init(shared_cols, 16);
+    mbar_init(shared_cols, 2 * L::WARPS);
     mbar_init(drain, 1);
-    for (int s = 0; s < 16; ++s) mbar_init(&res_bar[s], 1);
+    for (int s = 0; s < L::WARPS; ++s) mbar_init(&res_bar[s], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -581,10 +568,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
       }
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    Fp8EpilogueWarp w{q, &map_y, &map_r, smem_u32(boxes) + (uint32_t)(warp - 4) * (kFp8Boxes * 2048u),
-                      reinterpret_cast<const float4*>(boxes + L::BOXES + (warp - 4) * 512), res_bar + 2 * (warp - 4),
-                      lane, 0, 0, half, 0u, 0u, 0u, abort_flag, peer_abort};
+    const int quarter = warp & 3, e = warp - 4;
+    Fp8EpilogueWarp<QUANT> w{q, &map_y, &map_r, smem_u32(boxes) + (uint32_t)e * 2048u,
+                             reinterpret_cast<const float4*>(boxes + L::BOXES + e * L::COLUMNS * 4), res_bar + e, lane,
+                             e >> 2, 0, 0, 0u, false, abort_flag, peer_abort};
     const uint32_t shared_leader = cluster_addr(shared_cols, 0);
     uint32_t tc = 0;
     bool ok = true;
@@ -592,11 +579,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
       const uint32_t b = tc & 1u;
       tiles.at(t, w.m0, w.n0);
       w.m0 += (int)rank * 128 + quarter * 32;
-      w.n0 += half * 128;
+      w.n0 += w.group * L::COLUMNS;
       w.begin_tile();
       if (!(ok = pair_wait_warp(&accf[b], (tc >> 1) & 1u, abort_flag, peer_abort, p.err, 21))) break;
       tc_fence_after();
-      const uint32_t acc = tmem + b * kAcc1 + (uint32_t)half * 128 + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t acc = tmem + b * kAcc1 + (uint32_t)(w.group * L::COLUMNS) + ((uint32_t)(quarter * 32) << 16);
       const uint32_t acce_leader = cluster_addr(&acce[b], 0);
       auto load = [&](int j, float (&v)[32]) {
         uint32_t r[32];
@@ -604,7 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (j == 0 || j == 3) {
+        if (j == 0 || j + 1 == L::CHUNKS) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(j == 0 ? shared_leader : acce_leader);
@@ -612,23 +599,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
       };
       if constexpr (!QUANT) {
 #pragma unroll 1
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < L::CHUNKS; ++j) {
           float v[32];
           load(j, v);
-          const int n = w.n0 + 32 * w.chunk(j);
-          if (ok) ok = w.finish(j, v);
+          const int n = w.column(j);
           if (!ok || !w.inside(n)) continue;
+          if (!(ok = w.finish(j, v))) continue;
           if (p.e.y_type == FTB_F32) store_plain32<float>(w, n, v);
           else if (p.e.y_type == FTB_F16) store_plain32<__half>(w, n, v);
           else store_plain32<__nv_bfloat16>(w, n, v);
+          if (q.res_tma) w.res_next(j + 1);
         }
       } else {
-        float v[4][32];
+        float v[L::CHUNKS][32];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < L::CHUNKS; ++j) {
           load(j, v[j]);
-          if (ok) ok = w.finish(j, v[j]);
-          const int n = w.n0 + 32 * w.chunk(j);
+          const int n = w.column(j);
+          if (ok && w.inside(n)) {
+            ok = w.finish(j, v[j]);
+            if (ok && q.res_tma) w.res_next(j + 1);
+          }
           if (n + 32 > p.N) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -638,8 +629,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
         if (ok && w.inside(w.n0)) store_quantized(w, v);
       }
     }
-    for (int s = 0; s < 2; ++s)  // residual loads in flight land before the CTA leaves
-      if (w.res_open >> s & 1u) w.res_wait(s, /*ignore_abort=*/true);
+    if (w.res_open) w.res_wait(/*ignore_abort=*/true);  // a load in flight lands before the CTA leaves
     if (lane == 0) bulk_wait_all();  // this warp's stores are complete before the CTA leaves
   }
   tc_fence_before();
@@ -655,18 +645,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8PairThreads, 1)
 // host side
 // ---------------------------------------------------------------------------
 
-// Shared-memory attribute and the number of pairs that are resident at once.
+// Shared-memory attributes and the number of pairs that are resident at once.
+template <bool QUANT>
 inline cudaError_t fp8_pair_prepare(int* pairs) {
-  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Fp8PairSmem::TOTAL);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(fp8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8PairSmem::TOTAL);
+  using L = Fp8PairShape<QUANT>;
+  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel<QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2, 1, 1);
-  cfg.blockDim = dim3(kFp8PairThreads, 1, 1);
-  cfg.dynamicSmemBytes = Fp8PairSmem::TOTAL;
-  e = cudaOccupancyMaxActiveClusters(pairs, fp8_pair_kernel<false>, &cfg);
+  cfg.blockDim = dim3(L::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = L::TOTAL;
+  e = cudaOccupancyMaxActiveClusters(pairs, fp8_pair_kernel<QUANT>, &cfg);
   if (e == cudaSuccess && *pairs <= 0) e = cudaErrorInvalidConfiguration;
   return e;
 }
@@ -706,8 +695,11 @@ inline cudaError_t launch_fp8_pair(const Fp8Operands& o, const Fp8Params& p, int
   const int64_t tiles = (((int64_t)p.M + 255) / 256) * (((int64_t)p.N + 255) / 256);
   if (tiles > 0x3fffffff) return cudaErrorInvalidConfiguration;
   const unsigned pairs = (unsigned)std::min<int64_t>(tiles, max_pairs);
-  return pdl_launch(p.e.y_type == kFp8Type ? fp8_pair_kernel<true> : fp8_pair_kernel<false>, dim3(2 * pairs),
-                    dim3(kFp8PairThreads), Fp8PairSmem::TOTAL, s, map_a, map_w, map_y, map_r, q);
+  if (p.e.y_type == kFp8Type)
+    return pdl_launch(fp8_pair_kernel<true>, dim3(2 * pairs), dim3(Fp8PairShape<true>::THREADS),
+                      Fp8PairShape<true>::TOTAL, s, map_a, map_w, map_y, map_r, q);
+  return pdl_launch(fp8_pair_kernel<false>, dim3(2 * pairs), dim3(Fp8PairShape<false>::THREADS),
+                    Fp8PairShape<false>::TOTAL, s, map_a, map_w, map_y, map_r, q);
 }
 
 }  // namespace ftb
