@@ -58,8 +58,7 @@ static void fp8_setup(int dev, Fp8Device* d) {
   if (e == cudaSuccess) e = fp8_tile_attributes<32>();
   if (e == cudaSuccess) e = fp8_tile_attributes<64>();
   if (e == cudaSuccess) e = fp8_tile_attributes<128>();
-  if (e == cudaSuccess) e = fp8_pair_prepare<true>(&d->pairs);
-  if (e == cudaSuccess) e = fp8_pair_prepare<false>(&d->pairs);
+  if (e == cudaSuccess) e = fp8_pair_prepare(&d->pairs);
   if (e != cudaSuccess) {
     d->rc = ST_DEVICE;
     d->err = std::string("set-up failed: ") + cudaGetErrorString(e);

@@ -20,15 +20,20 @@
 //   warp 1     tensor memory; in the leader CTA the MMAs of the pair;
 //   warp 2     scale factors of this CTA, four k-blocks at a time;
 //   warp 3     passes this CTA's landed stages on to the leader;
-//   from 4 on  the epilogue: 16 warps with 64 columns each, or 8 with 128 for a
-//              quantised output, which keeps its block of 128 columns in
-//              registers until their largest is known.  A lane is a token; 32
-//              columns at a time go out through the warp's box in shared
-//              memory and a TMA store (row stores where the output's rows are
-//              not 16-byte aligned, and for a box that ends outside).  The
-//              residual comes in by TMA through the same box; bias is staged
-//              while the products run.
-// Short depths are bound by the epilogue (TODO).
+//   warps 4-19 epilogue: a lane quarter and 64 columns each; a lane is a token.
+//              32 columns at a time go out through the warp's box in shared
+//              memory and a TMA store, or by rows where the output's rows are
+//              not 16-byte aligned or the box ends outside; the residual comes
+//              in through the same box.  Bias is staged while the products
+//              run.  For a quantised output the two warps of a block of 128
+//              columns exchange each token's largest value.
+// Short depths are bound by the epilogue, its instructions and its turns
+// through the box: 8192 x 8192 outputs of depth 64 take 36 us in bf16, 50 in
+// f32, 43 quantised, 61 with a bf16 residual (floors by bytes 21, 41, 10 and
+// 41 us; with 8 warps of 128 columns 48, 64, 57 and 79).  Long depths are bound
+// by the operands' way through L2 and by power: 8192^3 takes 388 us in a burst,
+// 454 when repeated for seconds at the 1 kW limit (314 in a burst without
+// loads and stores).
 #pragma once
 
 #include "fp8_gemm.cuh"
@@ -37,21 +42,21 @@ namespace ftb {
 
 constexpr int kFp8Band = 16;
 
-template <bool QUANT>
+constexpr int kFp8EpiWarps = 16;
+constexpr int kFp8EpiColumns = 64;  // of an epilogue warp
+
 struct Fp8PairShape {
-  static constexpr int WARPS = QUANT ? 8 : 16;       // of the epilogue
-  static constexpr int COLUMNS = 1024 / WARPS;       // of each, for one quarter of the lanes
-  static constexpr int CHUNKS = COLUMNS / 32;
-  static constexpr int THREADS = 128 + 32 * WARPS;
-  static constexpr int STAGES = QUANT ? 6 : 5;
+  static constexpr int THREADS = 128 + 32 * kFp8EpiWarps;
+  static constexpr int STAGES = 5;
   static constexpr int OPERAND_BYTES = 128 * 128;
   static constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
   static constexpr int SF_BYTES = 512 + 1024;
-  static constexpr int BOXES = WARPS * 2048;
-  static constexpr int BIAS = WARPS * COLUMNS * 4;
-  static constexpr int SF_OFF = STAGES * STAGE_BYTES + BOXES + BIAS;
+  static constexpr int BOXES = kFp8EpiWarps * 2048;
+  static constexpr int BIAS_OFF = STAGES * STAGE_BYTES + BOXES;
+  static constexpr int AMAX_OFF = BIAS_OFF + kFp8EpiWarps * kFp8EpiColumns * 4;
+  static constexpr int SF_OFF = AMAX_OFF + 2 * kFp8EpiWarps * 32 * 4;  // of two tiles
   static constexpr int BAR_OFF = SF_OFF + 2 * SF_BYTES;
-  static constexpr int NBAR = 3 * STAGES + 4 + 4 + 2 + WARPS;
+  static constexpr int NBAR = 3 * STAGES + 4 + 4 + 2 + 2 * kFp8EpiWarps;
   static constexpr int TOTAL = 1024 + BAR_OFF + 8 * NBAR + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
 };
@@ -104,26 +109,6 @@ struct Fp8Tiles {
   }
 };
 
-// v += 32 consecutive columns of `row` from n.
-template <typename T>
-__device__ __forceinline__ void add_residual32(const T* row, int n, int N, bool vec, float (&v)[32]) {
-  if (vec && n + 32 <= N) {
-    constexpr int E = 16 / (int)sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 32 / E; ++i) {
-      const uint4 u = reinterpret_cast<const uint4*>(row + n)[i];
-      T t[E];
-      memcpy(t, &u, 16);
-#pragma unroll
-      for (int j = 0; j < E; ++j) v[i * E + j] = __fadd_rn(v[i * E + j], to_f32(t[j]));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (n + i < N) v[i] = __fadd_rn(v[i], to_f32(row[n + i]));
-  }
-}
-
 __device__ __forceinline__ uint4 ld_shared4(uint32_t addr) {
   uint4 u;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(addr));
@@ -143,17 +128,72 @@ __device__ __forceinline__ uint32_t box_at(uint32_t box, int lane, int i) {
   return box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
 }
 
+// A box from or to a matrix without TMA: its rows are not 16-byte aligned, or
+// the box reaches past the last column (a TMA store clips columns in units of
+// 16 bytes only).  Lanes take consecutive columns of a row.
+template <typename U>
+__device__ __noinline__ void load_box_rows(uint32_t box, const U* x, int64_t ld, int m0, int n, int M, int N,
+                                              int lane) {
+  constexpr int E = (int)sizeof(U), C = 64 / E, R = 32 / C, B = 8;  // R rows at a time, B times in flight
+  const int c = lane % C;
+  const U* src = x + (int64_t)(m0 + lane / C) * ld + n + c;
+  for (int r0 = lane / C; r0 < 32; r0 += R * B) {
+    U u[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      u[i] = m0 + r0 + i * R < M && n + c < N ? *src : (U)0;
+      src += R * ld;
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const uint32_t at = box_at(box, r0 + i * R, (c * E) >> 4) + ((c * E) & 15);
+      if constexpr (E == 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(u[i]) : "memory");
+      else asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(u[i]) : "memory");
+    }
+  }
+  __syncwarp();
+}
+
+template <typename U>
+__device__ __noinline__ void store_box_rows(uint32_t box, U* y, int64_t ld, int m0, int n, int M, int N, int lane) {
+  constexpr int E = (int)sizeof(U), C = E == 1 ? 32 : 64 / E, R = 32 / C, B = 8;
+  __syncwarp();
+#pragma unroll
+  for (int c0 = 0; c0 < 64 / E; c0 += C) {
+    const int c = c0 + lane % C;
+    U* dst = y + (int64_t)(m0 + lane / C) * ld + n + c;
+    for (int r0 = lane / C; r0 < 32; r0 += R * B) {
+      uint32_t u[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const uint32_t at = box_at(box, r0 + i * R, (c * E) >> 4) + ((c * E) & 15);
+        if constexpr (E == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u[i]) : "r"(at));
+        else if constexpr (E == 2)
+          asm volatile("{ .reg .u16 t; ld.shared.u16 t, [%1]; cvt.u32.u16 %0, t; }" : "=r"(u[i]) : "r"(at));
+        else asm volatile("ld.shared.u8 %0, [%1];" : "=r"(u[i]) : "r"(at));
+      }
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        if (m0 + r0 + i * R < M && n + c < N) *dst = (U)u[i];
+        dst += R * ld;
+      }
+    }
+  }
+  __syncwarp();
+}
+
 // One epilogue warp: its box, bias and residual loads.
-template <bool QUANT>
 struct Fp8EpilogueWarp {
-  using L = Fp8PairShape<QUANT>;
+  static constexpr int CHUNKS = kFp8EpiColumns / 32;
   const Fp8PairParams& q;
   const CUtensorMap *map_y, *map_r;
   uint32_t box;         // shared address of its 2 KB
   const float4* bias4;  // its columns
   uint64_t* res_bar;    // residual box landed
+  uint64_t* amax_bar;   // both warps of a block have its largest values (quantised output)
+  uint32_t* amax;       // [2][warps][32] largest |value| of 64 columns, this warp's
   int lane;
-  int group;            // its columns begin at COLUMNS group
+  int group;            // its columns begin at 64 group
   int m0, n0;           // its tokens and columns of this tile
   uint32_t res_phase;   // parity of res_bar
   bool res_open;        // a load has not been waited for
@@ -162,7 +202,7 @@ struct Fp8EpilogueWarp {
 
   // the chunk that holds the columns that the accumulators share comes first:
   // the last of accumulator 0, the first of accumulator 1
-  __device__ __forceinline__ int chunk(int j) const { return 2 * group >= L::WARPS / 4 ? L::CHUNKS - 1 - j : j; }
+  __device__ __forceinline__ int chunk(int j) const { return group >= 2 ? CHUNKS - 1 - j : j; }
   __device__ __forceinline__ int column(int j) const { return n0 + 32 * chunk(j); }
   __device__ __forceinline__ bool inside(int n) const { return n < q.p.N && m0 < q.p.M; }
   __device__ __forceinline__ int res_cols() const { return q.p.e.res_type == FTB_F32 ? 16 : 32; }
@@ -184,7 +224,7 @@ struct Fp8EpilogueWarp {
   }
   // The first residual box of the first chunk from j on that is inside.
   __device__ __forceinline__ void res_next(int j) {
-    for (; j < L::CHUNKS; ++j)
+    for (; j < CHUNKS; ++j)
       if (inside(column(j))) {
         __syncwarp();
         res_load(column(j));
@@ -194,7 +234,7 @@ struct Fp8EpilogueWarp {
 
   __device__ __forceinline__ void begin_tile() {
     if (q.p.e.bias) {
-      const int n = n0 + 4 * lane, N = 4 * lane < L::COLUMNS ? q.p.N : 0;
+      const int n = n0 + 4 * lane, N = 4 * lane < kFp8EpiColumns ? q.p.N : 0;
       float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (q.bias_vec && n + 4 <= N) {
         f = __ldg(reinterpret_cast<const float4*>(q.p.e.bias + n));
@@ -205,7 +245,7 @@ struct Fp8EpilogueWarp {
         if (n + 3 < N) f.w = __ldg(q.p.e.bias + n + 3);
       }
       __syncwarp();
-      if (4 * lane < L::COLUMNS) const_cast<float4*>(bias4)[lane] = f;
+      if (4 * lane < kFp8EpiColumns) const_cast<float4*>(bias4)[lane] = f;
       __syncwarp();
     }
     if (q.res_tma) res_next(0);
@@ -231,32 +271,28 @@ struct Fp8EpilogueWarp {
       for (int i = 0; i < 32; ++i) v[i] = max_nan(v[i], 0.0f);
     }
     if (!e.residual) return true;
-    if (q.res_tma) {
-      if (e.res_type == FTB_F32) return add_boxes<float>(j, v);
-      if (e.res_type == FTB_F16) return add_boxes<__half>(j, v);
-      return add_boxes<__nv_bfloat16>(j, v);
-    }
-    const int64_t m = (int64_t)m0 + lane;
-    if (m < q.p.M) {
-      const int64_t at = m * e.res_ld;
-      if (e.res_type == FTB_F32) add_residual32(static_cast<const float*>(e.residual) + at, n, q.p.N, e.res_vec, v);
-      else if (e.res_type == FTB_F16)
-        add_residual32(static_cast<const __half*>(e.residual) + at, n, q.p.N, e.res_vec, v);
-      else add_residual32(static_cast<const __nv_bfloat16*>(e.residual) + at, n, q.p.N, e.res_vec, v);
-    }
-    return true;
+    if (e.res_type == FTB_F32) return add_boxes<float>(j, v);
+    if (e.res_type == FTB_F16) return add_boxes<__half>(j, v);
+    return add_boxes<__nv_bfloat16>(j, v);
   }
   template <typename T>
   __device__ __forceinline__ bool add_boxes(int j, float (&v)[32]) {
     constexpr int C = 64 / (int)sizeof(T), E = 16 / (int)sizeof(T);
 #pragma unroll
     for (int b = 0; b < 32 / C; ++b) {
-      if (b > 0) {
-        if (!inside(column(j) + b * C)) break;
-        __syncwarp();
-        res_load(column(j) + b * C);
+      const int n = column(j) + b * C;
+      if (!inside(n)) break;
+      if (q.res_tma) {
+        if (b > 0) {
+          __syncwarp();
+          res_load(n);
+        }
+        if (!res_wait()) return false;
+      } else {
+        box_begin();
+        using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+        load_box_rows(box, static_cast<const U*>(q.p.e.residual), q.p.e.res_ld, m0, n, q.p.M, q.p.N, lane);
       }
-      if (!res_wait()) return false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint4 u = ld_shared4(box_at(box, lane, i));
@@ -284,28 +320,9 @@ struct Fp8EpilogueWarp {
   }
 };
 
-// Rows of a staged box into an output without TMA: its rows are not 16-byte
-// aligned, or the box reaches past the last column (a TMA store clips columns
-// in units of 16 bytes only).
-template <typename U>
-__device__ __forceinline__ void store_box_rows(uint32_t box, U* y, int64_t ld, int m0, int n, int M, int N, int lane) {
-  constexpr int E = (int)sizeof(U), C = 64 / E;
-  __syncwarp();
-  for (int x = lane; x < 32 * C; x += 32) {
-    const int r = x / C, c = x % C;
-    const uint32_t at = box_at(box, r, (c * E) >> 4) + ((c * E) & 15);
-    uint32_t u;
-    if constexpr (E == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(at));
-    else if constexpr (E == 2) asm volatile("{ .reg .u16 t; ld.shared.u16 t, [%1]; cvt.u32.u16 %0, t; }" : "=r"(u) : "r"(at));
-    else asm volatile("ld.shared.u8 %0, [%1];" : "=r"(u) : "r"(at));
-    if (m0 + r < M && n + c < N) y[(int64_t)(m0 + r) * ld + n + c] = (U)u;
-  }
-  __syncwarp();
-}
-
 // 32 finished columns (from n) of a warp's tokens into a plain output.
 template <typename T>
-__device__ __forceinline__ void store_plain32(const Fp8EpilogueWarp<false>& w, int n, const float (&v)[32]) {
+__device__ __forceinline__ void store_plain32(const Fp8EpilogueWarp& w, int n, const float (&v)[32]) {
   constexpr int C = 64 / (int)sizeof(T);  // columns per box
   const Fp8Params& p = w.q.p;
 #pragma unroll
@@ -330,55 +347,61 @@ __device__ __forceinline__ void store_plain32(const Fp8EpilogueWarp<false>& w, i
   }
 }
 
-// One block (this lane's 128 columns, in chunk order) into a quantised output.
-__device__ __forceinline__ void store_quantized(const Fp8EpilogueWarp<true>& w, float (&v)[4][32]) {
+// A lane's 64 columns, half of a block, in chunk order, into a quantised
+// output; `buf` alternates between tiles.  False on a timeout.
+__device__ __forceinline__ bool store_quantized(const Fp8EpilogueWarp& w, uint32_t buf, uint32_t phase,
+                                                float (&v)[2][32]) {
   const Fp8Params& p = w.q.p;
   float top = 0.0f;  // NaN is passed over
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[j][i]));
   uint32_t amax = __float_as_uint(top);
   if (amax >= 0x7F800000u) {  // an infinity: the scale comes from the finite values
     amax = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         amax = max(amax, finite_abs_bits(v[j][i]));
         v[j][i] = nan_unless_finite(v[j][i]);
       }
   }
+  // the other half of the block is four warps on (or back): columns 64 apart
+  uint32_t* mine = w.amax + buf * (kFp8EpiWarps * 32) + w.lane;
+  *mine = amax;
+  __syncwarp();
+  if (w.lane == 0) mbar_arrive(w.amax_bar);
+  if (!pair_wait_warp(w.amax_bar, phase, w.abort_flag, w.peer_abort, p.err, 23)) return false;
+  amax = max(amax, *(volatile uint32_t*)(w.group & 1 ? mine - 4 * 32 : mine + 4 * 32));
+  if (!w.inside(w.n0)) return true;
   const uint32_t byte = fp8_scale_byte(amax);
   const float inv = fp8_inv_scale(byte);
   const int64_t m = (int64_t)w.m0 + w.lane;
-  if (m < p.M) p.e.ys[m * p.e.ys_ld + w.n0 / kFp8Block] = (uint8_t)byte;
+  if (!(w.group & 1) && m < p.M) p.e.ys[m * p.e.ys_ld + w.n0 / kFp8Block] = (uint8_t)byte;
+  w.box_begin();
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {  // boxes of 64 columns: chunks 2 b and 2 b + 1 in order
-    const int n = w.n0 + 64 * (w.chunk(2 * b) / 2);
-    if (n >= p.N) continue;
-    w.box_begin();
+  for (int j = 0; j < 2; ++j) {
+    const int first = 2 * w.chunk(j);
+    uint32_t u[8];
 #pragma unroll
-    for (int j = 2 * b; j < 2 * b + 2; ++j) {
-      const int first = 2 * (w.chunk(j) & 1);
-      uint32_t u[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        u[i] = fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
-      st_shared4(box_at(w.box, w.lane, first), u[0], u[1], u[2], u[3]);
-      st_shared4(box_at(w.box, w.lane, first + 1), u[4], u[5], u[6], u[7]);
-    }
-    if (n + 64 <= p.N) w.box_store(n);
-    else store_box_rows(w.box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, w.m0, n, p.M, p.N, w.lane);
+    for (int i = 0; i < 8; ++i)
+      u[i] = fp8_pack4(v[j][4 * i], v[j][4 * i + 1], v[j][4 * i + 2], v[j][4 * i + 3], inv);
+    st_shared4(box_at(w.box, w.lane, first), u[0], u[1], u[2], u[3]);
+    st_shared4(box_at(w.box, w.lane, first + 1), u[4], u[5], u[6], u[7]);
   }
+  if (w.n0 + 64 <= p.N) w.box_store(w.n0);
+  else store_box_rows(w.box, static_cast<uint8_t*>(p.e.y), p.e.y_ld, w.m0, w.n0, p.M, p.N, w.lane);
+  return true;
 }
 
 template <bool QUANT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>::THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape::THREADS, 1)
     fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_r,
                     const Fp8PairParams q) {
-  using L = Fp8PairShape<QUANT>;
+  using L = Fp8PairShape;
   constexpr int STAGES = L::STAGES;
   constexpr uint32_t kAcc1 = 224, kSf = 480;
   extern __shared__ uint8_t smem_raw[];
@@ -394,9 +417,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
   uint64_t* acce = accf + 2;            // [2] leader: accumulator read (both CTAs' epilogue warps)
   uint64_t* shared_cols = acce + 2;     // leader: the shared columns read (the same), once per tile
   uint64_t* drain = shared_cols + 1;    // leader: MMAs retired after an abort
-  uint64_t* res_bar = drain + 1;        // [WARPS] an epilogue warp's residual box landed
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(res_bar + L::WARPS);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(res_bar + L::WARPS) + 1;
+  uint64_t* res_bar = drain + 1;        // [warps] an epilogue warp's residual box landed
+  uint64_t* amax_bar = res_bar + kFp8EpiWarps;  // [warps] the two warps of a block share its first one's
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(amax_bar + kFp8EpiWarps);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(amax_bar + kFp8EpiWarps) + 1;
 
   const Fp8Params& p = q.p;
   const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
@@ -416,11 +440,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
       mbar_init(&sf_full[s], 2);
       mbar_init(&sf_empty[s], 1);
       mbar_init(&accf[s], 1);
-      mbar_init(&acce[s], 2 * L::WARPS);
+      mbar_init(&acce[s], 2 * kFp8EpiWarps);
     }
-    mbar_init(shared_cols, 2 * L::WARPS);
+    mbar_init(shared_cols, 2 * kFp8EpiWarps);
     mbar_init(drain, 1);
-    for (int s = 0; s < L::WARPS; ++s) mbar_init(&res_bar[s], 1);
+    for (int s = 0; s < kFp8EpiWarps; ++s) {
+      mbar_init(&res_bar[s], 1);
+      mbar_init(&amax_bar[s], 2);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -569,9 +596,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
     }
   } else {
     const int quarter = warp & 3, e = warp - 4;
-    Fp8EpilogueWarp<QUANT> w{q, &map_y, &map_r, smem_u32(boxes) + (uint32_t)e * 2048u,
-                             reinterpret_cast<const float4*>(boxes + L::BOXES + e * L::COLUMNS * 4), res_bar + e, lane,
-                             e >> 2, 0, 0, 0u, false, abort_flag, peer_abort};
+    Fp8EpilogueWarp w{q, &map_y, &map_r, smem_u32(boxes) + (uint32_t)e * 2048u,
+                      reinterpret_cast<const float4*>(smem + L::BIAS_OFF + e * kFp8EpiColumns * 4), res_bar + e,
+                      amax_bar + (e & ~4), reinterpret_cast<uint32_t*>(smem + L::AMAX_OFF) + e * 32, lane, e >> 2, 0,
+                      0, 0u, false, abort_flag, peer_abort};
     const uint32_t shared_leader = cluster_addr(shared_cols, 0);
     uint32_t tc = 0;
     bool ok = true;
@@ -579,11 +607,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
       const uint32_t b = tc & 1u;
       tiles.at(t, w.m0, w.n0);
       w.m0 += (int)rank * 128 + quarter * 32;
-      w.n0 += w.group * L::COLUMNS;
+      w.n0 += w.group * kFp8EpiColumns;
       w.begin_tile();
       if (!(ok = pair_wait_warp(&accf[b], (tc >> 1) & 1u, abort_flag, peer_abort, p.err, 21))) break;
       tc_fence_after();
-      const uint32_t acc = tmem + b * kAcc1 + (uint32_t)(w.group * L::COLUMNS) + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t acc = tmem + b * kAcc1 + (uint32_t)(w.group * kFp8EpiColumns) + ((uint32_t)(quarter * 32) << 16);
       const uint32_t acce_leader = cluster_addr(&acce[b], 0);
       auto load = [&](int j, float (&v)[32]) {
         uint32_t r[32];
@@ -591,7 +619,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (j == 0 || j + 1 == L::CHUNKS) {
+        if (j == 0 || j + 1 == Fp8EpilogueWarp::CHUNKS) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(j == 0 ? shared_leader : acce_leader);
@@ -599,7 +627,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
       };
       if constexpr (!QUANT) {
 #pragma unroll 1
-        for (int j = 0; j < L::CHUNKS; ++j) {
+        for (int j = 0; j < Fp8EpilogueWarp::CHUNKS; ++j) {
           float v[32];
           load(j, v);
           const int n = w.column(j);
@@ -611,9 +639,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
           if (q.res_tma) w.res_next(j + 1);
         }
       } else {
-        float v[L::CHUNKS][32];
+        float v[2][32];
 #pragma unroll
-        for (int j = 0; j < L::CHUNKS; ++j) {
+        for (int j = 0; j < 2; ++j) {
           load(j, v[j]);
           const int n = w.column(j);
           if (ok && w.inside(n)) {
@@ -626,7 +654,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
               if (n + i >= p.N) v[j][i] = 0.0f;
           }
         }
-        if (ok && w.inside(w.n0)) store_quantized(w, v);
+        if (ok) ok = store_quantized(w, b, (tc & 1u), v);
       }
     }
     if (w.res_open) w.res_wait(/*ignore_abort=*/true);  // a load in flight lands before the CTA leaves
@@ -646,16 +674,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape<QUANT>:
 // ---------------------------------------------------------------------------
 
 // Shared-memory attributes and the number of pairs that are resident at once.
-template <bool QUANT>
 inline cudaError_t fp8_pair_prepare(int* pairs) {
-  using L = Fp8PairShape<QUANT>;
-  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel<QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+  using L = Fp8PairShape;
+  cudaError_t e = cudaFuncSetAttribute(fp8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(fp8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2, 1, 1);
   cfg.blockDim = dim3(L::THREADS, 1, 1);
   cfg.dynamicSmemBytes = L::TOTAL;
-  e = cudaOccupancyMaxActiveClusters(pairs, fp8_pair_kernel<QUANT>, &cfg);
+  e = cudaOccupancyMaxActiveClusters(pairs, fp8_pair_kernel<false>, &cfg);
   if (e == cudaSuccess && *pairs <= 0) e = cudaErrorInvalidConfiguration;
   return e;
 }
@@ -695,11 +724,8 @@ inline cudaError_t launch_fp8_pair(const Fp8Operands& o, const Fp8Params& p, int
   const int64_t tiles = (((int64_t)p.M + 255) / 256) * (((int64_t)p.N + 255) / 256);
   if (tiles > 0x3fffffff) return cudaErrorInvalidConfiguration;
   const unsigned pairs = (unsigned)std::min<int64_t>(tiles, max_pairs);
-  if (p.e.y_type == kFp8Type)
-    return pdl_launch(fp8_pair_kernel<true>, dim3(2 * pairs), dim3(Fp8PairShape<true>::THREADS),
-                      Fp8PairShape<true>::TOTAL, s, map_a, map_w, map_y, map_r, q);
-  return pdl_launch(fp8_pair_kernel<false>, dim3(2 * pairs), dim3(Fp8PairShape<false>::THREADS),
-                    Fp8PairShape<false>::TOTAL, s, map_a, map_w, map_y, map_r, q);
+  return pdl_launch(p.e.y_type == kFp8Type ? fp8_pair_kernel<true> : fp8_pair_kernel<false>, dim3(2 * pairs),
+                    dim3(Fp8PairShape::THREADS), Fp8PairShape::TOTAL, s, map_a, map_w, map_y, map_r, q);
 }
 
 }  // namespace ftb
