@@ -57,6 +57,7 @@ _SIGS = {
     "ftb_quantize_weight": ([c_void_p, c_void_p], c_int),
     "ftb_rms_norm": ([c_void_p, c_void_p], c_int),
     "ftb_fp8_linear": ([c_void_p, c_void_p], c_int),
+    "ftb_fp8_set_fault_injection": ([c_int], c_int),
 }
 
 EXPORTED = sorted(_SIGS)

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <exception>
 #include <mutex>
@@ -18,12 +19,11 @@
 namespace ftb {
 
 constexpr int kFp8MaxDevices = 64;
-constexpr int64_t kFp8MaxDim = int64_t(1) << 28;
+constexpr int64_t kFp8MaxDim = int64_t(1) << 27;
 
 struct Fp8Device {
-  std::once_flag once;
-  int rc = ST_OK;
-  std::string err;
+  std::mutex mu;
+  std::atomic<bool> ready{false};
   int sm_count = 0;
   int pairs = 0;  // SM pairs resident at once
   // set by a kernel whose bounded wait gave up: mapped host memory, so the
@@ -32,60 +32,74 @@ struct Fp8Device {
   int* fault_dev = nullptr;
 };
 static Fp8Device g_fp8_devices[kFp8MaxDevices];
+static std::atomic<int> g_fp8_stall{0};  // failure-detection hook
 
 static int refuse(const char* fn, const std::string& why, int status = ST_INPUT) {
   set_error(std::string(fn) + ": " + why);
   return status;
 }
 
-static void fp8_setup(int dev, Fp8Device* d) {
-  cudaError_t e = cudaDeviceGetAttribute(&d->sm_count, cudaDevAttrMultiProcessorCount, dev);
+// Once per device; "" when done.  Allocates a word and sets kernel attributes,
+// in relaxed capture mode, so that a stream under capture does not matter.
+static std::string fp8_setup(int dev, Fp8Device* d) {
   int major = 0;
+  cudaError_t e = cudaDeviceGetAttribute(&d->sm_count, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-  if (e == cudaSuccess && major != 10) {
-    d->rc = ST_DEVICE;
-    d->err = "needs a GPU of compute capability 10.0 (sm_100a)";
-    return;
-  }
-  void* h = nullptr;
-  if (e == cudaSuccess) e = cudaHostAlloc(&h, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
-  void* hd = nullptr;
+  if (e == cudaSuccess && major != 10) return "needs a GPU of compute capability 10.0 (sm_100a)";
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (e == cudaSuccess) e = cudaThreadExchangeStreamCaptureMode(&mode);
   if (e == cudaSuccess) {
-    *static_cast<int*>(h) = 0;
-    e = cudaHostGetDevicePointer(&hd, h, 0);
+    if (!d->fault) {
+      void *h = nullptr, *hd = nullptr;
+      e = cudaHostAlloc(&h, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+      if (e == cudaSuccess) {
+        *static_cast<int*>(h) = 0;
+        e = cudaHostGetDevicePointer(&hd, h, 0);
+        if (e == cudaSuccess) {
+          d->fault = static_cast<volatile int*>(h);
+          d->fault_dev = static_cast<int*>(hd);
+        } else {
+          cudaFreeHost(h);
+        }
+      }
+    }
+    if (e == cudaSuccess) e = fp8_tile_attributes<16>();
+    if (e == cudaSuccess) e = fp8_tile_attributes<32>();
+    if (e == cudaSuccess) e = fp8_tile_attributes<64>();
+    if (e == cudaSuccess) e = fp8_tile_attributes<128>();
+    if (e == cudaSuccess) e = fp8_pair_prepare(&d->pairs);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) e = back;
   }
-  if (e == cudaSuccess) e = fp8_tile_attributes<16>();
-  if (e == cudaSuccess) e = fp8_tile_attributes<32>();
-  if (e == cudaSuccess) e = fp8_tile_attributes<64>();
-  if (e == cudaSuccess) e = fp8_tile_attributes<128>();
-  if (e == cudaSuccess) e = fp8_pair_prepare(&d->pairs);
-  if (e != cudaSuccess) {
-    d->rc = ST_DEVICE;
-    d->err = std::string("set-up failed: ") + cudaGetErrorString(e);
-    cudaGetLastError();
-    return;
-  }
-  d->fault = static_cast<volatile int*>(h);
-  d->fault_dev = static_cast<int*>(hd);
+  if (e == cudaSuccess) return "";
+  cudaGetLastError();
+  return std::string("set-up failed: ") + cudaGetErrorString(e);
 }
 
-// The current device's state, set up by the first call on it.
+// The current device's state, set up by the first call on it (a set-up that
+// fails is tried again by the next).
 static int fp8_device(const char* fn, Fp8Device** out) {
   int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return refuse(fn, cudaGetErrorString(e), ST_DEVICE);
   }
   if (dev < 0 || dev >= kFp8MaxDevices) return refuse(fn, "device ordinal beyond the supported range", ST_CONFIG);
   Fp8Device& d = g_fp8_devices[dev];
-  std::call_once(d.once, [&]() { fp8_setup(dev, &d); });
-  if (d.rc != ST_OK) return refuse(fn, d.err, d.rc);
+  if (!d.ready.load(std::memory_order_acquire)) {
+    std::lock_guard<std::mutex> lock(d.mu);
+    if (!d.ready.load(std::memory_order_relaxed)) {
+      const std::string why = fp8_setup(dev, &d);
+      if (!why.empty()) return refuse(fn, why, ST_DEVICE);
+      d.ready.store(true, std::memory_order_release);
+    }
+  }
   const int code = *d.fault;
   if (code != 0) {
     *d.fault = 0;
-    return refuse(fn, "an earlier call on this device gave up a wait (code " + std::to_string(code) +
-                          "); its output is not valid", ST_DEVICE);
+    return refuse(fn, "an earlier call's kernel on this device gave up: a wait exceeded its limit (code " +
+                          std::to_string(code) + "); that call's output is not valid", ST_DEVICE);
   }
   *out = &d;
   return ST_OK;
@@ -113,6 +127,41 @@ static std::string check(const char* what, const ftb_fp8_matrix& q, int64_t cols
 static bool rows_aligned(const ftb_matrix& x) {
   return aligned(x.data, 16) && (x.ld * (x.type == FTB_F32 ? 4 : 2)) % 16 == 0;
 }
+// Bytes of a matrix in memory: rows `ld` bytes apart.
+struct Span {
+  const char* p;
+  int64_t rows, bytes, ld;
+  int64_t end() const { return (rows - 1) * ld + bytes; }
+};
+static Span span(const ftb_matrix& x, int64_t m, int64_t n) {
+  const int64_t size = x.type == FTB_F32 ? 4 : 2;
+  return {static_cast<const char*>(x.data), m, n * size, x.ld * size};
+}
+static Span span(const void* p, int64_t rows, int64_t bytes, int64_t ld) {
+  return {static_cast<const char*>(p), rows, bytes, ld};
+}
+static bool overlap(const Span& a, const Span& b) {
+  if (!a.p || !b.p || a.rows < 1 || b.rows < 1 || a.p + a.end() <= b.p || b.p + b.end() <= a.p) return false;
+  const int64_t ld = a.rows > 1 ? a.ld : b.ld;
+  if ((a.rows > 1 && a.ld != ld) || (b.rows > 1 && b.ld != ld)) return true;  // not worth telling apart
+  const int64_t d = ((b.p - a.p) % ld + ld) % ld;  // b's columns in a's rows
+  return !(d >= a.bytes && d + b.bytes <= ld);
+}
+static bool same(const Span& a, const Span& b) {
+  return a.p == b.p && a.rows == b.rows && a.bytes == b.bytes && (a.rows <= 1 || a.ld == b.ld);
+}
+// An output that shares memory with an operand, unless it is that operand in
+// place: "" or why not.
+template <size_t N>
+static std::string clashes(const char* what, const Span& out, const Span (&in)[N], const Span* in_place = nullptr,
+                           const Span* in_place2 = nullptr) {
+  for (const Span& x : in)
+    if (overlap(out, x) && !(in_place && same(out, x) && same(*in_place, x)) &&
+        !(in_place2 && same(out, x) && same(*in_place2, x)))
+      return std::string(what) + " overlaps an operand";
+  return "";
+}
+
 static bool sizes_ok(int64_t m, int64_t n, int64_t k) {
   return m >= 0 && m <= kFp8MaxDim && n >= 1 && n <= kFp8MaxDim && k >= 1 && k <= kFp8MaxDim;
 }
@@ -137,8 +186,8 @@ struct Fp8Choice {
 // per SM, fewer in clusters of 4 and 8, which do not fill the SMs' groups.)  A
 // round of pairs takes 0.29 per k-block and 0.8, and a launch 3.5 more than
 // the tile kernel's.  The constants are a fit to 525 shapes (m 1..4096, n and
-// k 64..8192) that were timed with every choice on a B200; over 263 others the
-// pick is 0.6 % slower than the best choice in the mean, 18 % at most.  For
+// k 64..8192) that were timed with every choice on a B200; over 696 others the
+// pick is 1.0 % slower than the best choice in the mean, 30 % at most.  For
 // example (m x k x n): 1 x 4096 x 4096 takes 5.2 us with 16 tokens per tile
 // and split 4, 12.2 unsplit; 512 x 512 x 512 takes 3.5 with 16 tokens, 6.8 with
 // 128; 256 x 4096 x 4096 11.8 with 128 tokens and split 2, 16.9 on pairs;
@@ -176,7 +225,7 @@ static cudaError_t launch_fp8_linear(const Fp8Operands& o, const Fp8Params& p, c
     case 32: return launch_fp8_tile<32>(o, p, c.split, s);
     case 64: return launch_fp8_tile<64>(o, p, c.split, s);
     case 128: return launch_fp8_tile<128>(o, p, c.split, s);
-    default: return launch_fp8_pair(o, p, d.pairs, 0, s);
+    default: return launch_fp8_pair(o, p, d.pairs, s);
   }
 }
 
@@ -190,6 +239,8 @@ static int guarded(const char* fn, F&& body) noexcept {
     } catch (...) {
       return ST_ALLOC;
     }
+  } catch (...) {
+    return ST_ALLOC;
   }
 }
 
@@ -204,9 +255,12 @@ FTB_API int ftb_quantize_rows(const ftb_quantize_args* args, void* stream) {
     const ftb_quantize_args& a = *args;
     if (a.m == 0) return ST_OK;
     if (!a.x.data || !a.q.data || !a.q.scales) return refuse(fn, "null pointer", ST_NULL);
-    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^28");
+    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^27");
     std::string why = check("x", a.x, a.k);
     if (why.empty()) why = check("q", a.q, a.k);
+    const Span in[1] = {span(a.x, a.m, a.k)};
+    if (why.empty()) why = clashes("q", span(a.q.data, a.m, a.k, a.q.ld), in);
+    if (why.empty()) why = clashes("q", span(a.q.scales, a.m, fp8_blocks(a.k), a.q.scales_ld), in);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
@@ -231,9 +285,12 @@ FTB_API int ftb_quantize_weight(const ftb_quantize_args* args, void* stream) {
     if (a.m == 0) return ST_OK;
     if (!a.x.data || !a.q.data || !a.q.scales) return refuse(fn, "null pointer", ST_NULL);
     if (!sizes_ok(a.m, 1, a.k) || fp8_blocks(a.m) > 65535)
-      return refuse(fn, "needs 0 <= m <= 128 * 65535 and 1 <= k <= 2^28");
+      return refuse(fn, "needs 0 <= m <= 128 * 65535 and 1 <= k <= 2^27");
     std::string why = check("x", a.x, a.k);
     if (why.empty()) why = check("q", a.q, a.k);
+    const Span in[1] = {span(a.x, a.m, a.k)};
+    if (why.empty()) why = clashes("q", span(a.q.data, a.m, a.k, a.q.ld), in);
+    if (why.empty()) why = clashes("q", span(a.q.scales, fp8_blocks(a.m), fp8_blocks(a.k), a.q.scales_ld), in);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
@@ -259,7 +316,7 @@ FTB_API int ftb_rms_norm(const ftb_rms_norm_args* args, void* stream) {
     if (!a.x.data || (!a.y.data && !a.q.data) || (a.q.data && !a.q.scales)) return refuse(fn, "null pointer", ST_NULL);
     if (a.y.data && a.q.data) return refuse(fn, "y and q are both set");
     if (a.h.data && !a.residual.data) return refuse(fn, "h is the sum with a residual: pass one");
-    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^28");
+    if (!sizes_ok(a.m, 1, a.k)) return refuse(fn, "needs 0 <= m and 1 <= k, at most 2^27");
     if (!(a.eps >= 0.0)) return refuse(fn, "eps must not be negative");
     std::string why = check("x", a.x, a.k);
     const ftb_matrix* others[3] = {&a.residual, &a.h, &a.y};
@@ -271,6 +328,15 @@ FTB_API int ftb_rms_norm(const ftb_rms_norm_args* args, void* stream) {
     }
     if (why.empty() && a.weight && !aligned(a.weight, 4)) why = "weight is not aligned to its type";
     if (why.empty() && a.q.data) why = check("q", a.q, a.k);
+    const Span x = span(a.x, a.m, a.k), r = span(a.residual, a.m, a.k), h = span(a.h, a.m, a.k);
+    const Span in[3] = {x, r, span(a.weight, 1, 4 * a.k, 0)};
+    const Span more[4] = {x, r, in[2], h};
+    if (why.empty()) why = clashes("h", h, in, &x, &r);
+    if (why.empty() && a.y.data) why = clashes("y", span(a.y, a.m, a.k), in, &x, &r);
+    if (why.empty() && a.y.data && overlap(span(a.y, a.m, a.k), h)) why = "y overlaps h";
+    if (why.empty() && a.q.data) why = clashes("q", span(a.q.data, a.m, a.k, a.q.ld), more);
+    if (why.empty() && a.q.data)
+      why = clashes("q", span(a.q.scales, a.m, fp8_blocks(a.k), a.q.scales_ld), more);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
@@ -305,7 +371,7 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
         (a.q.data && !a.q.scales))
       return refuse(fn, "null pointer", ST_NULL);
     if (a.y.data && a.q.data) return refuse(fn, "y and q are both set");
-    if (!sizes_ok(a.m, a.n, a.k)) return refuse(fn, "needs 0 <= m, 1 <= n and 1 <= k, at most 2^28");
+    if (!sizes_ok(a.m, a.n, a.k)) return refuse(fn, "needs 0 <= m, 1 <= n and 1 <= k, at most 2^27");
     if (a.flags & ~(int64_t)FTB_FP8_RELU) return refuse(fn, "unknown flags");
     std::string why = check("a", a.a, a.k);
     if (why.empty()) why = check("w", a.w, a.k);
@@ -313,6 +379,18 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
     if (why.empty() && a.residual.data) why = check("residual", a.residual, a.n);
     if (why.empty() && a.y.data) why = check("y", a.y, a.n);
     if (why.empty() && a.q.data) why = check("q", a.q, a.n);
+    const Span r = span(a.residual, a.m, a.n);
+    const Span in[6] = {span(a.a.data, a.m, a.k, a.a.ld),
+                        span(a.a.scales, a.m, fp8_blocks(a.k), a.a.scales_ld),
+                        span(a.w.data, a.n, a.k, a.w.ld),
+                        span(a.w.scales, fp8_blocks(a.n), fp8_blocks(a.k), a.w.scales_ld),
+                        span(a.bias, 1, 4 * a.n, 0),
+                        r};
+    if (why.empty() && a.y.data)
+      why = clashes("y", span(a.y, a.m, a.n), in, a.residual.type == a.y.type ? &r : nullptr);
+    if (why.empty() && a.q.data) why = clashes("q", span(a.q.data, a.m, a.n, a.q.ld), in);
+    if (why.empty() && a.q.data)
+      why = clashes("q", span(a.q.scales, a.m, fp8_blocks(a.n), a.q.scales_ld), in);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
@@ -338,6 +416,12 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
     p.e.res_vec = rows_aligned(a.residual);
     p.e.y_vec = rows_aligned(a.y);
     p.err = d->fault_dev;
+    p.stall_test = g_fp8_stall.load();
     return launched(fn, launch_fp8_linear(o, p, *d, static_cast<cudaStream_t>(stream)));
   });
+}
+
+FTB_API int ftb_fp8_set_fault_injection(int stall) {
+  g_fp8_stall.store(stall ? 1 : 0);
+  return ST_OK;
 }

@@ -57,7 +57,8 @@ struct Fp8Params {
   const uint8_t* sw;      // [N / 128, K / 128]
   int64_t sw_ld;
   Fp8Epilogue e;
-  int* err;
+  int* err;        // set when a bounded wait gives up
+  int stall_test;  // failure-detection tests: the MMA warp first waits for what nothing completes
 };
 
 // The four scale bytes of k-blocks 4 g .. 4 g + 3 as one word; bytes past the
@@ -316,6 +317,7 @@ __global__ void __launch_bounds__(kFp8Threads) fp8_tile_kernel(const __grid_cons
   } else if (warp == 1) {
     bool ok = true;
     int it = 0;
+    if (p.stall_test) ok = mbar_wait_warp(done, 0, abort_flag, p.err, 8);
     for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
       const int g = (kb - kb0) >> 2, slot = g % SLOTS, byte = kb & 3;
       const uint32_t sfa = tmem_sf + slot * 8, sfb = sfa + 4;

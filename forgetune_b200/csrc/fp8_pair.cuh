@@ -66,7 +66,6 @@ struct Fp8PairParams {
   int y_tma;     // the output has a TMA map
   int res_tma;   // the residual has one
   int bias_vec;  // bias is 16-byte aligned
-  int stall_test;
 };
 
 __device__ __forceinline__ void umma2_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
@@ -499,7 +498,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape::THREAD
     if (rank == 0) {
       bool ok = true;
       uint32_t it = 0, sg = 0, tc = 0;
-      if (q.stall_test) ok = pair_wait_warp(drain, 0, abort_flag, peer_abort, p.err, 13);
+      if (p.stall_test) ok = pair_wait_warp(drain, 0, abort_flag, peer_abort, p.err, 13);
       for (int t = pair; t < ntiles && ok; t += npairs, ++tc) {
         const uint32_t b = tc & 1u;
         if (!(ok = pair_wait_warp(&acce[b], ((tc >> 1) & 1u) ^ 1u, abort_flag, peer_abort, p.err, 14))) break;
@@ -707,8 +706,7 @@ inline bool make_map_fp8_box(CUtensorMap* map, void* base, int type, int64_t ld,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-inline cudaError_t launch_fp8_pair(const Fp8Operands& o, const Fp8Params& p, int max_pairs, int stall_test,
-                                   cudaStream_t s) {
+inline cudaError_t launch_fp8_pair(const Fp8Operands& o, const Fp8Params& p, int max_pairs, cudaStream_t s) {
   CUtensorMap map_a, map_w, map_y, map_r;
   if (!make_map_fp8(&map_a, o.a, p.M, p.K, o.a_ld, 128) || !make_map_fp8(&map_w, o.w, p.N, p.K, o.w_ld, 128))
     return cudaErrorInvalidValue;
@@ -720,7 +718,6 @@ inline cudaError_t launch_fp8_pair(const Fp8Operands& o, const Fp8Params& p, int
   if (!q.y_tma && p.e.y_type == kFp8Type) return cudaErrorInvalidValue;
   q.res_tma = make_map_fp8_box(&map_r, const_cast<void*>(p.e.residual), p.e.res_type, p.e.res_ld, p.M, p.N);
   q.bias_vec = (reinterpret_cast<uintptr_t>(p.e.bias) & 15) == 0;
-  q.stall_test = stall_test;
   const int64_t tiles = (((int64_t)p.M + 255) / 256) * (((int64_t)p.N + 255) / 256);
   if (tiles > 0x3fffffff) return cudaErrorInvalidConfiguration;
   const unsigned pairs = (unsigned)std::min<int64_t>(tiles, max_pairs);

@@ -19,9 +19,9 @@ are stored as NaN.  Products are accumulated in fp32.
 
 Inputs are 2-D; a plain input whose rows are not contiguous is copied first,
 as ``CompiledModel.run_device`` does.  The operators are for inference: they
-return tensors without gradients.  The first call on a device sets it up, so
-make it before capturing a CUDA graph.  The reference has no counterpart (its
-models are float32 only).
+return tensors without gradients.  They need no workspace, so calls may run
+on several streams at once and be captured into CUDA graphs.  The reference
+has no counterpart (its models are float32 only).
 """
 
 from __future__ import annotations

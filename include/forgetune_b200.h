@@ -239,12 +239,13 @@ FORGETUNE_EXPORT int ftb_small_gemm_noalloc(const float* d_x, const float* d_w, 
  * read or written.  Everything is enqueued on `stream` (NULL = the legacy
  * default stream) without synchronising or allocating; there is no workspace,
  * so calls may overlap, and calls may be captured into CUDA graphs.  The
- * first call on each device sets it up (and loads the library's device code):
- * make it outside stream capture.  m = 0 returns 0 without a launch.
+ * first call on each device sets it up and loads the library's device code.
+ * m = 0 returns 0 without a launch.  Sizes are at most 2^27.  An output must
+ * not share memory with an operand except in place, where said so.
  *
- * Status codes as above: -1 null pointer, -2 sizes, strides, alignment or
- * types, -5 launch error, or an earlier call's kernel on this device gave up
- * a wait (reported once, by the next call). */
+ * Status codes as above: -1 null pointer, -2 sizes, strides, alignment,
+ * types or overlaps, -5 launch error, or an earlier call's kernel on this
+ * device gave up a wait (reported once, by the next call). */
 #define FTB_F32 0
 #define FTB_F16 1
 #define FTB_BF16 2
@@ -300,6 +301,10 @@ typedef struct {
   int64_t flags;
 } ftb_fp8_linear_args;
 FORGETUNE_EXPORT int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream);
+
+/* Failure-detection hook (tests): while stall != 0 every ftb_fp8_linear launch makes one pipeline wait that
+ * nothing completes run out (about 2 s); the kernel leaves cleanly and the next call returns -5. */
+FORGETUNE_EXPORT int ftb_fp8_set_fault_injection(int stall);
 
 #ifdef __cplusplus
 }

@@ -76,6 +76,41 @@ def test_linear_refusals():
         assert call(**bad) == -2, bad
 
 
+def test_outputs_over_operands_are_refused():
+    """Overlaps other than in place; side by side in one buffer's rows is none."""
+    B = 1 << 24  # far from P
+
+    def quantize(x, q, s):
+        return rc("ftb_quantize_rows", QUANTIZE_ARGS, x, 512, 0, q, 2048, s, 2048, 4, 200)
+    assert quantize(P, P, B) == -2 and "overlaps" in _native.last_error()
+    assert quantize(P, P + 784, B) == -2  # x's rows have 800 bytes each 2048
+    assert quantize(P, B, P + 2048) == -2
+
+    def norm(**over):
+        a = dict(x=P, r=2 * B, w=3 * B, h=4 * B, y=5 * B, q=0, s=0, ld=256)
+        a.update(over)
+        ld = a["ld"]
+        return rc("ftb_rms_norm", RMS_NORM_ARGS, a["x"], ld, 0, a["r"], ld, 0, a["w"], 1e-6, a["h"], ld, 0, a["y"], ld,
+                  0, a["q"], 256, a["s"], 4, 4, 200)
+    for bad in (dict(h=P + 4), dict(y=P + 16), dict(h=5 * B), dict(h=P, y=P), dict(y=3 * B), dict(h=3 * B + 400),
+                dict(y=0, q=P, s=B), dict(y=0, q=B, s=P + 800 - 4), dict(y=0, q=4 * B + 16, s=B)):
+        assert norm(**bad) == -2 and "overlaps" in _native.last_error(), bad
+
+    def linear(**over):
+        a = dict(y=B, res=2 * B, bias=3 * B, a=4 * B, sa=5 * B, w=6 * B, sw=7 * B, q=0, s=0, yt=0, rt=0)
+        a.update(over)
+        return rc("ftb_fp8_linear", LINEAR_ARGS, a["a"], 256, a["sa"], 4, a["w"], 256, a["sw"], 4, a["bias"], a["res"],
+                  130, a["rt"], a["y"], 130, a["yt"], a["q"], 144, a["s"], 4, 3, 130, 200, 0)
+    for bad in (dict(y=2 * B + 4), dict(y=2 * B, yt=1), dict(y=3 * B), dict(y=4 * B), dict(y=5 * B), dict(y=6 * B),
+                dict(y=7 * B), dict(y=0, q=4 * B, s=B), dict(y=0, q=B, s=5 * B), dict(y=0, q=2 * B, s=B)):
+        assert linear(**bad) == -2 and "overlaps" in _native.last_error(), bad
+    # allowed as far as the checks go: without a GPU the next step is the device
+    if _native.device_count() == 0:
+        for good in (norm(), norm(h=P), norm(y=P), norm(h=2 * B), norm(h=P, y=2 * B), norm(ld=512, h=P + 800),
+                     linear(), linear(y=2 * B), quantize(P, P + 800, B)):
+            assert good == -5, _native.last_error()
+
+
 def fp8(*shape):
     return torch.zeros(*shape).to(torch.float8_e4m3fn)
 

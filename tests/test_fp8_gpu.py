@@ -4,12 +4,14 @@ Quantisation is compared bit for bit: x / scale is exact, so only the one
 rounding to e4m3 remains.  The products of small integers are compared bit
 for bit too: every partial sum is then exact in fp32, whatever the order."""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
 
 import forgetune_b200 as ft
-from forgetune_b200 import InvalidShapeError, Fp8Rows, Fp8Weight, fp8_linear, quantize_rows, quantize_weight, rms_norm
+from forgetune_b200 import _native, InvalidShapeError, Fp8Rows, Fp8Weight, fp8_linear, quantize_rows, quantize_weight, rms_norm
 
 from . import fp8_reference as ref
 
@@ -439,6 +441,84 @@ def test_block_in_a_graph_and_on_two_streams(m, layers):
         assert torch.equal(y1, want) and torch.equal(y2, want2)
 
 
+def test_calls_from_several_threads(layers):
+    """Four threads, a stream each, one and many tokens at once."""
+    sizes = (1, 33, 700, 3000)
+    want = [block(randn(m, 500, seed=m), randn(m, 500, seed=m + 1), *layers)[0] for m in sizes]
+    torch.cuda.synchronize()
+    got = [None] * len(sizes)
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = block(randn(sizes[i], 500, seed=sizes[i]), randn(sizes[i], 500, seed=sizes[i] + 1), *layers)[0]
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_graphs_replayed_at_once(layers):
+    """There is no workspace for them to share."""
+    graphs = []
+    for seed in (1, 2):
+        x, res = randn(200, 500, seed=seed), randn(200, 500, seed=seed + 5)
+        want = block(x, res, *layers)[0]
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            y = block(x, res, *layers)[0]
+        graphs.append((graph, torch.cuda.Stream(), y, want, x, res))
+    for _ in range(20):
+        for graph, stream, *_rest in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for _, _, y, want, _, _ in graphs)
+
+
+def test_offsets_past_32_bits():
+    """Rows that begin beyond 2^31 elements (and bytes) of their matrix."""
+    m, k = 270000, 8192
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = randn(3, k, dtype=torch.bfloat16)
+    check_quantized(Fp8Rows((q := quantize_rows(x)).data[-3:], q.scales[-3:]), x[-3:], 1)
+    del q
+    y, h = rms_norm(x, residual=x)
+    want, _ = ref.rms_norm(f64(x[-3:]) * 2, None, 1e-6)
+    check_plain(y[-3:], want, torch.bfloat16, norm_bound(k))
+    del x, y, h
+    m, n, k = 70000, 32768, 128
+    a, av = integers(m, k, 1, seed=1)
+    w, wv = integers(n, k, 128, seed=2)
+    y = fp8_linear(a, w)
+    want, _ = ref.linear(av[-2:], wv)
+    assert same(f64(y[-2:]), want)
+    want, _ = ref.linear(av[:2], wv)
+    assert same(f64(y[:2]), want)
+
+
+@pytest.mark.parametrize("m", [3, 3000])
+def test_a_wait_that_runs_out_is_reported_and_recoverable(m, layers):
+    """The hook makes the MMA warp wait for what nothing completes; the kernel leaves after its limit, the next
+    call reports it, and the one after works."""
+    x, res = randn(m, 500, seed=1), randn(m, 500, seed=2)
+    want = block(x, res, *layers)[0]
+    q = quantize_rows(x)
+    _native.lib().ftb_fp8_set_fault_injection(1)
+    try:
+        fp8_linear(q, layers[1])
+        torch.cuda.synchronize()
+    finally:
+        _native.lib().ftb_fp8_set_fault_injection(0)
+    with pytest.raises(ft.ForgeTuneRuntimeError, match="exceeded its limit"):
+        fp8_linear(q, layers[1])
+    assert torch.equal(block(x, res, *layers)[0], want)
+
+
 def test_empty_batch():
     w = quantize_weight(randn(130, 200))
     x = torch.empty(0, 200, device="cuda")
@@ -482,3 +562,9 @@ def test_refusals_on_device_tensors():
         fp8_linear(Fp8Rows(odd, q.scales), w)
     with pytest.raises(ft.ForgeTuneRuntimeError, match="eps"):
         rms_norm(x, eps=-1.0)
+    with pytest.raises(ft.ForgeTuneRuntimeError, match="overlaps"):
+        rms_norm(x, residual=x, out=x, residual_out=x)
+    with pytest.raises(ft.ForgeTuneRuntimeError, match="overlaps"):
+        fp8_linear(q, quantize_weight(randn(256, 256)), quantize=True, out=q)
+    with pytest.raises(ValueError):
+        fp8_linear(q, w, quantize=True, out_dtype=torch.float32)
