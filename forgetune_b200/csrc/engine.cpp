@@ -27,6 +27,7 @@ const char* op_name(int32_t op) {
     case OP_CONV2D: return "CONV2D";
     case OP_FLATTEN: return "FLATTEN";
     case OP_FUSED_CONV2D_RELU: return "FUSED_CONV2D_RELU";
+    case OP_RMSNORM: return "RMSNORM";
     case OP_GEMM: return "GEMM";
     case OP_CONV: return "CONV";
     default: return "UNKNOWN";
@@ -138,6 +139,7 @@ Graph parse_blob(const void* data, size_t bytes) {
         throw std::runtime_error("graph blob: non-positive dimension");
     n.conv.sh = r[12]; n.conv.sw = r[13]; n.conv.ph = r[14];
     n.conv.pw = r[15]; n.conv.dh = r[16]; n.conv.dw = r[17];
+    if (n.op == OP_RMSNORM) std::memcpy(&n.eps, &r[12], sizeof(n.eps));
     n.const_offset = static_cast<uint64_t>(r[18]);
     n.const_count = static_cast<uint64_t>(r[19]);
     if (n.op == OP_CONST) {
@@ -555,6 +557,23 @@ Program build_program(const void* blob, size_t bytes) {
         s.kind = n.op == OP_RELU ? ST_RELU : n.op == OP_SIGMOID ? ST_SIGMOID : n.op == OP_TANH ? ST_TANH : ST_COPY;
         s.a = operand_of(g, prog.plan, n.inputs[0]);
         s.elems_per_sample = n.shape.static_elems();
+        break;
+      }
+      case OP_RMSNORM: {
+        require(n.inputs.size() == 1 || n.inputs.size() == 2, "RMSNORM: needs one or two inputs");
+        const Node& x = g.node(n.inputs[0]);
+        require(x.shape.rank == 2 && same_shape(x.shape, n.shape), "RMSNORM: input and output must be [B, N]");
+        require(std::isfinite(n.eps) && n.eps >= 0.0, "RMSNORM: eps must not be negative");
+        s.kind = ST_RMSNORM;
+        s.N = x.shape.dims[1];
+        s.eps = static_cast<float>(n.eps);
+        s.a = operand_of(g, prog.plan, n.inputs[0]);
+        s.elems_per_sample = n.shape.static_elems();
+        if (n.inputs.size() == 2) {
+          const Node& w = g.node(n.inputs[1]);
+          require(w.op == OP_CONST && w.shape.rank == 1 && w.shape.dims[0] == s.N, "RMSNORM: weight must be a constant [N]");
+          s.b = operand_of(g, prog.plan, n.inputs[1]);
+        }
         break;
       }
       default:

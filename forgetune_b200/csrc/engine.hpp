@@ -4,7 +4,8 @@
 // forgetune_b200/graph_blob.py (the compile step).  It carries the
 // reference IR after export -- INPUT / CONST / MATMUL / ADD / RELU / MUL /
 // SIGMOID / TANH / CONV2D / FLATTEN nodes in topological order
-// (include/forgetune/ir.hpp:162-177 of the reference) -- plus the weights.
+// (include/forgetune/ir.hpp:162-177 of the reference), and RMSNORM, which the
+// reference does not have -- plus the weights.
 // The engine then
 //   1. fuses, following src/fusion.cpp:6-131 of the reference
 //      (MATMUL->ADD->RELU, CONV2D->RELU), and additionally folds the bias
@@ -39,6 +40,8 @@ enum OpKind : int32_t {
   OP_CONV2D = 10,
   OP_FLATTEN = 11,
   OP_FUSED_CONV2D_RELU = 12,
+  // no counterpart in the reference
+  OP_RMSNORM = 13,  // x [, weight], over the last dimension of [B, N]
   // engine-internal, produced by fusion only
   OP_GEMM = 100,  // x.W with an epilogue (bias / relu / residual / relu)
   OP_CONV = 101,  // implicit-GEMM conv with an epilogue
@@ -68,6 +71,7 @@ struct Node {
   std::vector<int32_t> inputs;
   Shape shape;
   ConvAttrs conv;
+  double eps = 0.0;  // OP_RMSNORM
   uint64_t const_offset = 0;  // floats into the weight section
   uint64_t const_count = 0;
   bool deleted = false;
@@ -177,6 +181,7 @@ enum StepKind : int32_t {
   ST_TANH = 10,
   ST_COPY = 11,
   ST_FILL_CONST = 12,  // graph output that is a constant
+  ST_RMSNORM = 13,     // width in N, weight in b (or none)
 };
 
 struct Step {
@@ -194,6 +199,7 @@ struct Step {
   int64_t elems_per_sample = 0;
   int64_t row_len = 0;   // ADD_ROW / MUL_ROW width
   int64_t channels = 0;  // ADD_CHANNEL: C, HW in row_len
+  float eps = 0.0f;      // RMSNORM
   bool static_rows = false;  // operand is not batch-dependent
   // device weight-layout slots, filled at upload: W[K,N] for SIMT,
   // W^T split into tf32 hi / lo [N,Kp] for the tensor-core path

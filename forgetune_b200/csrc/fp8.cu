@@ -14,6 +14,7 @@
 #include "fp8_gemm.cuh"
 #include "fp8_pair.cuh"
 #include "fp8_rows.cuh"
+#include "rms_norm.hpp"
 #include "status.hpp"
 
 namespace ftb {
@@ -242,6 +243,20 @@ static int guarded(const char* fn, F&& body) noexcept {
   } catch (...) {
     return ST_ALLOC;
   }
+}
+
+cudaError_t rms_norm_f32(const float* x, const float* weight, float eps, float* y, int64_t m, int64_t k, int sm_count,
+                         cudaStream_t s) {
+  RowsParams p{};
+  p.x = x;
+  p.x_ld = k;
+  p.weight = weight;
+  p.eps = eps;
+  p.y = y;
+  p.y_ld = k;
+  p.m = m;
+  p.k = k;
+  return launch_rms_norm(p, FTB_F32, sm_count, s);
 }
 
 }  // namespace ftb

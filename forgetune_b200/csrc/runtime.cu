@@ -28,6 +28,7 @@
 #include "engine.hpp"
 #include "forgetune_b200.h"
 #include "philox.cuh"
+#include "rms_norm.hpp"
 #include "simt_gemm.cuh"
 #include "splitk_gemv.cuh"
 #include "status.hpp"
@@ -916,6 +917,17 @@ static int enqueue(const Model* m, const Replica* rep, ExecCtx* c, const float* 
           ew_unary_kernel<EW_SIGMOID><<<g, 256, 0, s>>>(ptr(st.a), ptr(st.out), n);
         else
           ew_unary_kernel<EW_TANH><<<g, 256, 0, s>>>(ptr(st.a), ptr(st.out), n);
+        break;
+      }
+      case ST_RMSNORM: {
+        const int64_t m = rows * st.elems_per_sample / st.N;
+        if (m <= 0) break;
+        const float* w = st.b.space == SP_NONE ? nullptr : ptr(st.b);
+        const cudaError_t e = rms_norm_f32(ptr(st.a), w, st.eps, ptr(st.out), m, st.N, sm, s);
+        if (e != cudaSuccess) {
+          set_error(std::string("RMSNORM launch failed: ") + cudaGetErrorString(e));
+          return ST_DEVICE;
+        }
         break;
       }
       case ST_COPY:

@@ -9,6 +9,7 @@ vocabulary, with the reference's conventions
 * ``aten.conv2d`` / ``aten.convolution`` (groups 1, not transposed) -> CONV2D (:622-698)
 * ``aten.add`` / ``aten.mul`` -> ADD / MUL with the larger operand first (:18-46, :386-417)
 * ``aten.relu`` / ``sigmoid`` / ``tanh`` -> RELU / SIGMOID / TANH
+* ``aten.rms_norm`` over the features of [B, N] -> RMSNORM (no counterpart in the reference)
 * ``aten.flatten(x, 1, -1)`` and ``view``/``reshape`` to [B, -1] -> FLATTEN (:486-620)
 
 Only one float32 input and one output are supported, as in the reference;
@@ -28,7 +29,7 @@ from .errors import InvalidGraphError, InvalidShapeError, UnsupportedOpError
 # op codes shared with the native engine (csrc/engine.hpp: OpKind)
 OPS = {
     "INPUT": 0, "CONST": 1, "MATMUL": 2, "ADD": 3, "RELU": 4, "OUTPUT": 5,
-    "MUL": 7, "SIGMOID": 8, "TANH": 9, "CONV2D": 10, "FLATTEN": 11,
+    "MUL": 7, "SIGMOID": 8, "TANH": 9, "CONV2D": 10, "FLATTEN": 11, "RMSNORM": 13,
 }
 
 
@@ -41,6 +42,7 @@ class IRNode:
     name: str = ""
     const: Optional[np.ndarray] = None
     conv: Optional[Dict[str, int]] = None
+    eps: Optional[float] = None  # RMSNORM
 
 
 @dataclass
@@ -243,6 +245,20 @@ def export_to_ir(model: torch.nn.Module, example_inputs, dynamic_batch: bool = F
                 env[node.name] = xi
             else:
                 env[node.name] = g.add("FLATTEN", [xi], out, node.name)
+        elif "aten.rms_norm" in target:
+            xi = env[args[0].name]
+            xs = g.shape(xi)
+            weight = args[2] if len(args) > 2 else None
+            eps = args[3] if len(args) > 3 else None
+            if len(xs) != 2 or list(args[1]) != [xs[1]]:
+                raise UnsupportedOpError(target, "only normalising the features of [B, features] is supported")
+            ins = [xi]
+            if weight is not None:
+                if g.nodes[env[weight.name]].const is None:
+                    raise UnsupportedOpError(target, "weight must be a parameter")
+                ins.append(env[weight.name])
+            nid = env[node.name] = g.add("RMSNORM", ins, xs, node.name)
+            g.nodes[nid].eps = float(torch.finfo(torch.float32).eps if eps is None else eps)
         elif "aten.dropout" in target or "aten.clone" in target or "aten.contiguous" in target \
                 or "aten.alias" in target or "aten.detach" in target:
             env[node.name] = env[args[0].name]

@@ -6,7 +6,8 @@ Layout (all little-endian int64 unless noted; parsed by csrc/engine.cpp):
                      max_batch, flags, kernel_policy, static_batch,
                      n_weight_floats, nodes_offset, weights_offset
   nodes (20 words each): id, op, n_inputs, inputs[4], rank, dims[4],
-                     stride_h, stride_w, pad_h, pad_w, dil_h, dil_w,
+                     stride_h, stride_w, pad_h, pad_w, dil_h, dil_w
+                     (RMSNORM: eps as the bits of a float64, then five unused),
                      const_offset (floats), const_count
   weights: float32, each constant starting on a 64-byte boundary
 
@@ -115,8 +116,9 @@ def serialize(g: IRGraph, *, enable_fusion: bool, bias_first_fused: bool, kernel
             off, cnt = w_floats, arr.size
             weights.append(arr)
             w_floats += arr.size
+        first = struct.unpack("<q", struct.pack("<d", n.eps))[0] if n.op == "RMSNORM" else c.get("sh", 1)
         records.append([remap[old], OPS[n.op], len(n.inputs)] + ins + [len(n.shape)] + dims
-                       + [c.get("sh", 1), c.get("sw", 1), c.get("ph", 0), c.get("pw", 0),
+                       + [first, c.get("sw", 1), c.get("ph", 0), c.get("pw", 0),
                           c.get("dh", 1), c.get("dw", 1), off, cnt])
     nodes_off = HEADER_WORDS * 8
     w_off = nodes_off + len(records) * NODE_WORDS * 8

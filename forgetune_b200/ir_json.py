@@ -226,9 +226,11 @@ def load_graph_json(src: Union[str, bytes, Dict[str, Any]]) -> IRGraph:
 
 
 def to_graph_json(g: IRGraph, indent: int = 2) -> str:
-    """The IR in the reference's schema 2.0 (src/json_io.cpp:121-200)."""
+    """The IR in the reference's schema 2.0 (src/json_io.cpp:121-200), which has no RMSNORM."""
     nodes = []
     for n in g.nodes:
+        if n.op == "RMSNORM":
+            raise UnsupportedOpError("RMSNORM", "the reference's graph.json has no such node")
         nd: Dict[str, Any] = {"id": n.id, "op": n.op, "name": n.name, "inputs": list(n.inputs),
                               "shape": list(n.shape), "dtype": "f32",
                               "const_data": [float(v) for v in np.asarray(n.const, np.float32).ravel()]
@@ -284,6 +286,9 @@ def evaluate(g: IRGraph, x: np.ndarray) -> np.ndarray:
             v = 1.0 / (1.0 + np.exp(-a[0]))
         elif n.op == "TANH":
             v = np.tanh(a[0])
+        elif n.op == "RMSNORM":
+            v = a[0] / np.sqrt((a[0] * a[0]).mean(axis=-1, keepdims=True) + n.eps)
+            v = v * a[1] if len(a) > 1 else v
         elif n.op == "FLATTEN":
             v = a[0].reshape(a[0].shape[0], -1)
         elif n.op == "CONV2D":
