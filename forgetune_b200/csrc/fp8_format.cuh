@@ -67,12 +67,32 @@ __device__ __forceinline__ float fp8_inv_scale(uint32_t byte) { return __uint_as
 // which the saturating conversion would make 448.
 __device__ __forceinline__ float nan_unless_finite(float v) { return __fmaf_rn(v, 0.0f, v); }
 
+// Two fp32 operations in one instruction, each rounded as usual.  The kernels
+// over rows are short of issue slots when the power limit lowers the clock.
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\t"
+      "mul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\t"
+      "add.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+// (s, t) += (a a, b b)
+__device__ __forceinline__ void add_squares2(float& s, float& t, float a, float b) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\t"
+      "fma.rn.f32x2 p, q, q, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(s), "+f"(t)
+      : "f"(a), "f"(b));
+}
+
 // Four values (finite or NaN) over the scale as e4m3, the first in the lowest byte.
 __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inv) {
-  a *= inv;
-  b *= inv;
-  c *= inv;
-  d *= inv;
+  mul2(a, b, inv, inv);
+  mul2(c, d, inv, inv);
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));

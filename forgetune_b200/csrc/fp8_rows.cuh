@@ -201,12 +201,13 @@ __device__ __forceinline__ void quantize_vecs(float (&v)[N][VEC], const uint32_t
   }
 }
 
+// Bits of the largest |v|; NaN is passed over (it converts to NaN by itself).
 template <int VEC>
 __device__ __forceinline__ uint32_t abs_max_bits(const float (&v)[VEC]) {
-  uint32_t a = 0;
+  float a = 0.0f;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  return a;
+  for (int i = 0; i < VEC; ++i) a = fmaxf(a, fabsf(v[i]));
+  return __float_as_uint(a);
 }
 
 // The same from 16 bytes of T: 16-bit types compare two at a time as integers.
@@ -327,17 +328,24 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(RowsParams p) {
   if (threadIdx.x == 0) p.s[blockIdx.y * p.s_ld + blockIdx.x] = (uint8_t)byte;
 }
 
-// Sum of the squares, pairwise.
+// Sum of squares in four partial sums.
+struct SquareSum {
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  template <int VEC>
+  __device__ __forceinline__ void add(const float (&v)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      add_squares2(s[0], s[1], v[i], v[i + 1]);
+      add_squares2(s[2], s[3], v[i + 2], v[i + 3]);
+    }
+  }
+  __device__ __forceinline__ float total() const { return (s[0] + s[1]) + (s[2] + s[3]); }
+};
+
 template <int VEC>
-__device__ __forceinline__ float square_sum(const float (&v)[VEC]) {
-  float t[VEC / 2];
+__device__ __forceinline__ void add_vec(float (&v)[VEC], const float (&t)[VEC]) {
 #pragma unroll
-  for (int i = 0; i < VEC / 2; ++i) t[i] = v[2 * i] * v[2 * i] + v[2 * i + 1] * v[2 * i + 1];
-#pragma unroll
-  for (int n = VEC / 4; n; n >>= 1)
-#pragma unroll
-    for (int i = 0; i < n; ++i) t[i] += t[i + n];
-  return t[0];
+  for (int i = 0; i < VEC; i += 2) add2(v[i], v[i + 1], t[i], t[i + 1]);
 }
 
 // What follows once a row's h and scale are known: N vectors of it, vector n
@@ -355,15 +363,15 @@ __device__ __forceinline__ void norm_finish(const RowsParams& p, int64_t row, in
     const int at = c + n * step;
     if (!p.weight) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[n][i] *= scale;
+      for (int i = 0; i < VEC; i += 2) mul2(v[n][i], v[n][i + 1], scale, scale);
     } else if (MODE == ROW_WHOLE || (MODE == ROW_VECTORS && at < k)) {
 #pragma unroll
       for (int i = 0; i < VEC; i += 4) {
         const float4 w = *reinterpret_cast<const float4*>(p.weight + at + i);
-        v[n][i] = v[n][i] * scale * w.x;
-        v[n][i + 1] = v[n][i + 1] * scale * w.y;
-        v[n][i + 2] = v[n][i + 2] * scale * w.z;
-        v[n][i + 3] = v[n][i + 3] * scale * w.w;
+        mul2(v[n][i], v[n][i + 1], scale, scale);
+        mul2(v[n][i + 2], v[n][i + 3], scale, scale);
+        mul2(v[n][i], v[n][i + 1], w.x, w.y);
+        mul2(v[n][i + 2], v[n][i + 3], w.z, w.w);
       }
     } else {
 #pragma unroll
@@ -397,7 +405,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const RowsParams p, cons
   grid_dep_wait();
   grid_dep_trigger();
   float v[NV][VEC];
-  float ss = 0.0f;
+  SquareSum sum;
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* r = static_cast<const T*>(p.residual) + row * p.r_ld;
   uint4 xu[NV], ru[NV];
@@ -413,11 +421,11 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const RowsParams p, cons
     if (p.residual) {
       float t[VEC];
       unpack_vec<T>(ru[j], t);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] += t[i];
+      add_vec(v[j], t);
     }
-    ss += square_sum(v[j]);
+    sum.add(v[j]);
   }
+  float ss = sum.total();
   for (int o = min(lanes, 32) / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (lanes > 32) {
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = lanes >> 5, first = w & ~(warps - 1);
@@ -449,16 +457,16 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p)
     if (r) {
       float t[VEC];
       unpack_vec<T>(load_vec<T, MODE>(r, c, k), t);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] += t[i];
+      add_vec(v, t);
     }
   };
-  float ss = 0.0f;
+  SquareSum sum;
   for (int64_t c = (int64_t)threadIdx.x * VEC; c < p.k; c += step) {
     float v[VEC];
     load((int)c, v);
-    ss += square_sum(v);
+    sum.add(v);
   }
+  float ss = sum.total();
 #pragma unroll
   for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (lane == 0) part[w] = ss;
