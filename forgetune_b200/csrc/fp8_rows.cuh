@@ -127,24 +127,24 @@ __device__ __forceinline__ uint32_t scale_code(uint32_t a) {
   return a == 0u ? 0u : a >= 0x7F800000u ? 0x1FFu : c;
 }
 
-// The largest code of each block: 128 / VEC neighbouring lanes.  For VEC 8 two
-// vectors' codes share a word, which halves the shuffles.
+// The largest of each block's 128 / VEC neighbouring lanes, of values below
+// 2^16.  For VEC 8 two vectors share a word, which halves the shuffles.
 template <int VEC, int N>
-__device__ __forceinline__ void block_codes(uint32_t (&code)[N]) {
+__device__ __forceinline__ void block_max16(uint32_t (&x)[N]) {
   if constexpr (VEC == 4) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) code[n] = __reduce_max_sync(0xffffffffu, code[n]);
+    for (int n = 0; n < N; ++n) x[n] = __reduce_max_sync(0xffffffffu, x[n]);
   } else {
     constexpr int W = (N + 1) / 2;
     uint32_t w[W];
 #pragma unroll
-    for (int i = 0; i < W; ++i) w[i] = code[2 * i] | (2 * i + 1 < N ? code[(2 * i + 1) % N] << 16 : 0u);
+    for (int i = 0; i < W; ++i) w[i] = x[2 * i] | (2 * i + 1 < N ? x[(2 * i + 1) % N] << 16 : 0u);
 #pragma unroll
     for (int o = 8; o; o >>= 1)
 #pragma unroll
       for (int i = 0; i < W; ++i) w[i] = __vmaxu2(w[i], __shfl_xor_sync(0xffffffffu, w[i], o));
 #pragma unroll
-    for (int n = 0; n < N; ++n) code[n] = (n & 1) ? w[n / 2] >> 16 : w[n / 2] & 0xFFFFu;
+    for (int n = 0; n < N; ++n) x[n] = (n & 1) ? w[n / 2] >> 16 : w[n / 2] & 0xFFFFu;
   }
 }
 
@@ -154,6 +154,24 @@ struct VecPlace {
   uint8_t *q, *s;
   int left;
 };
+
+// One vector and, from the block's first lane, its scale.
+template <bool WHOLE, int VEC>
+__device__ __forceinline__ void store_quantized(const float (&v)[VEC], uint32_t byte, const VecPlace& o) {
+  const float inv = fp8_inv_scale(byte);
+  uint32_t w[VEC / 4];
+#pragma unroll
+  for (int i = 0; i < VEC / 4; ++i) w[i] = fp8_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
+  if (WHOLE || o.left >= VEC) {
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(o.q) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(o.q) = w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i < o.left) o.q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+  }
+  if ((threadIdx.x & (kFp8Block / VEC - 1)) == 0 && (WHOLE || o.left > 0)) *o.s = (uint8_t)byte;
+}
 
 // A warp quantises N vectors per lane at once (a vector's 32 lanes are two
 // blocks for VEC 8, one for VEC 4) and stores values and scales where at(n)
@@ -178,27 +196,9 @@ __device__ __forceinline__ void quantize_vecs(float (&v)[N][VEC], const uint32_t
       code[n] = scale_code(f);
     }
   }
-  block_codes<VEC>(code);
-  const bool lead = (threadIdx.x & (kFp8Block / VEC - 1)) == 0;
+  block_max16<VEC>(code);
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const uint32_t byte = code[n] ? code[n] - 1u : 127u;
-    const float inv = fp8_inv_scale(byte);
-    const VecPlace o = at(n);
-    uint32_t w[VEC / 4];
-#pragma unroll
-    for (int i = 0; i < VEC / 4; ++i)
-      w[i] = fp8_pack4(v[n][4 * i], v[n][4 * i + 1], v[n][4 * i + 2], v[n][4 * i + 3], inv);
-    if (WHOLE || o.left >= VEC) {
-      if constexpr (VEC == 8) *reinterpret_cast<uint2*>(o.q) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t*>(o.q) = w[0];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i < o.left) o.q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
-    }
-    if (lead && (WHOLE || o.left > 0)) *o.s = (uint8_t)byte;
-  }
+  for (int n = 0; n < N; ++n) store_quantized<WHOLE>(v[n], code[n] ? code[n] - 1u : 127u, at(n));
 }
 
 // Bits of the largest |v|; NaN is passed over (it converts to NaN by itself).
@@ -210,18 +210,45 @@ __device__ __forceinline__ uint32_t abs_max_bits(const float (&v)[VEC]) {
   return __float_as_uint(a);
 }
 
-// The same from 16 bytes of T: 16-bit types compare two at a time as integers.
+// The same from 16 bytes of a 16-bit type, which compare two at a time as
+// integers; the result is the 16 bits.
+__device__ __forceinline__ uint32_t abs_max_bits16(const uint4& u) {
+  const uint32_t m = 0x7FFF7FFFu;
+  const uint32_t w = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+  return max(w >> 16, w & 0xFFFFu);
+}
+// ... as the bits of fp32.
 template <typename T>
-__device__ __forceinline__ uint32_t abs_max_bits(const uint4& u) {
-  if constexpr (sizeof(T) == 4) {
-    return max(max(u.x & 0x7FFFFFFFu, u.y & 0x7FFFFFFFu), max(u.z & 0x7FFFFFFFu, u.w & 0x7FFFFFFFu));
-  } else {
-    const uint32_t m = 0x7FFF7FFFu;
-    const uint32_t w = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
-    const uint32_t h = max(w >> 16, w & 0xFFFFu);
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
-    else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+__device__ __forceinline__ uint32_t widen_bits(uint32_t h) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return h << 16;
+  else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+}
+
+// A warp's N vectors as loaded, into values and scales.  A 16-bit type's
+// largest values go through the shuffles as they are, two to a word.
+template <typename T, bool WHOLE, int N, typename At>
+__device__ __forceinline__ void quantize_loaded(const uint4 (&u)[N], At&& at) {
+  constexpr int VEC = kRowVec<T>;
+  float v[N][VEC];
+#pragma unroll
+  for (int n = 0; n < N; ++n) unpack_vec<T>(u[n], v[n]);
+  if constexpr (VEC == 8) {
+    constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+    uint32_t h[N], most = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) h[n] = abs_max_bits16(u[n]), most = max(most, h[n]);
+    if (!__any_sync(0xffffffffu, most >= kInf)) {
+      block_max16<VEC>(h);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        store_quantized<WHOLE>(v[n], fp8_scale_byte(widen_bits<T>(h[n])), at(n));
+      return;
+    }
   }
+  uint32_t a[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) a[n] = abs_max_bits(v[n]);
+  quantize_vecs<WHOLE>(v, a, at);
 }
 
 // A row is cut into units of 32 vectors.  Long rows: grid (rows, CTAs per row),
@@ -241,17 +268,10 @@ __global__ void __launch_bounds__(256, MODE != ROW_ELEMENTS ? 4 : 1) quantize_ro
   uint4 u[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) u[n] = load_vec<T, MODE>(x, c + n * STEP, k);
-  float v[N][VEC];
-  uint32_t a[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    a[n] = abs_max_bits<T>(u[n]);
-    unpack_vec<T>(u[n], v[n]);
-  }
   uint8_t *q = p.q + row * p.q_ld + c, *s = p.s + row * p.s_ld + c / kFp8Block;
   auto at = [&](int n) { return VecPlace{q + n * STEP, s + n * (STEP / kFp8Block), k - c - n * STEP}; };
-  if (chunk + N * STEP <= k) quantize_vecs<true>(v, a, at);
-  else quantize_vecs<false>(v, a, at);
+  if (chunk + N * STEP <= k) quantize_loaded<T, true>(u, at);
+  else quantize_loaded<T, false>(u, at);
 }
 
 // Short rows, of `blocks` blocks: the lanes of a block take N blocks in turn,
@@ -269,8 +289,6 @@ __global__ void __launch_bounds__(256) quantize_short_kernel(const RowsParams p,
     row = row0 + r;
     c = row < p.m ? (int)((b - r * blocks) * kFp8Block + lane % L * VEC) : k;
   };
-  float v[N][VEC];
-  uint32_t a[N];
   uint4 u[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -279,12 +297,7 @@ __global__ void __launch_bounds__(256) quantize_short_kernel(const RowsParams p,
     place(n, row, c);
     u[n] = load_vec<T, MODE>(static_cast<const T*>(p.x) + row * p.x_ld, c, k);
   }
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    a[n] = abs_max_bits<T>(u[n]);
-    unpack_vec<T>(u[n], v[n]);
-  }
-  quantize_vecs<false>(v, a, [&](int n) {
+  quantize_loaded<T, false>(u, [&](int n) {
     int64_t row;
     int c;
     place(n, row, c);
