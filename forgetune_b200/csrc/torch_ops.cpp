@@ -84,12 +84,11 @@ Matrix input(PyObject* o, const char* what) {
   Matrix r;
   r.m = t->size(0);
   r.k = t->size(1);
-  int64_t ld = row_stride(*t);
+  r.t = t->is_neg() ? t->resolve_neg() : *t;  // a view that stands for the negated values
+  int64_t ld = row_stride(r.t);
   if (ld < 0) {
-    r.t = t->contiguous();
+    r.t = r.t.contiguous();
     ld = r.k;
-  } else {
-    r.t = *t;
   }
   r.a = as_matrix(r.t, ld);
   return r;
@@ -113,7 +112,7 @@ Matrix output(PyObject* o, const char* what, int64_t m, int64_t n, at::ScalarTyp
     return r;
   }
   const at::Tensor* t = tensor(o);
-  if (!t || t->scalar_type() != type || t->layout() != at::kStrided)
+  if (!t || t->scalar_type() != type || t->layout() != at::kStrided || t->is_neg())
     type_error(std::string(what) + " must be a " + c10::toString(type) + " tensor");
   check_place(*t, what, m, n, dev);
   const int64_t ld = row_stride(*t);
@@ -191,7 +190,8 @@ at::Tensor vector(PyObject* o, const char* what, int64_t n, at::Device dev) {
     shape_error(std::string(what) + " must be [" + std::to_string(n) + "], got " + show(t->sizes()));
   if (t->device() != dev)
     value_error(std::string(what) + " is on " + t->device().str() + ", the input on " + dev.str());
-  return n == 1 || t->stride(0) == 1 ? *t : t->contiguous();
+  const at::Tensor v = t->is_neg() ? t->resolve_neg() : *t;
+  return n == 1 || v.stride(0) == 1 ? v : v.contiguous();
 }
 
 // One C call on the current stream of `dev`.

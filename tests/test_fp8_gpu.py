@@ -4,6 +4,8 @@ Quantisation is compared bit for bit: x / scale is exact, so only the one
 rounding to e4m3 remains.  The products of small integers are compared bit
 for bit too: every partial sum is then exact in fp32, whatever the order."""
 
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -478,6 +480,68 @@ def test_two_graphs_replayed_at_once(layers):
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(y, want) for _, _, y, want, _, _ in graphs)
+
+
+def test_graph_with_branches(layers):
+    """Captured on two streams that fork and join: operators with more than one predecessor."""
+    xs = [randn(m, 500, seed=m) for m in (3, 900)]
+    rs = [randn(m, 500, seed=m + 1) for m in (3, 900)]
+    want = [block(x, r, *layers)[0] for x, r in zip(xs, rs)]
+    want.append(rms_norm(want[0], residual=want[1][:3])[0])
+    torch.cuda.synchronize()
+    main, side, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        side.wait_stream(main)
+        y0 = block(xs[0], rs[0], *layers)[0]
+        with torch.cuda.stream(side):
+            y1 = block(xs[1], rs[1], *layers)[0]
+        main.wait_stream(side)
+        y2 = rms_norm(y0, residual=y1[:3])[0]
+    for _ in range(5):
+        for y in (y0, y1, y2):
+            y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((y0, y1, y2), want))
+
+
+def test_first_call_inside_a_capture():
+    """In a process of its own: set-up and code loading happen while a stream is being captured."""
+    code = """
+import torch
+from forgetune_b200 import quantize_rows, quantize_weight, rms_norm, fp8_linear
+x = torch.randn(700, 512, device="cuda")
+w = torch.randn(2000, 512, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    h, r = rms_norm(x, residual=x, quantize=True)
+    y = fp8_linear(h, quantize_weight(w))
+    z = fp8_linear(quantize_rows(x[:2]), quantize_weight(w))
+g.replay()
+h, r = rms_norm(x, residual=x, quantize=True)
+assert torch.equal(y, fp8_linear(h, quantize_weight(w)))
+assert torch.equal(z, fp8_linear(quantize_rows(x[:2]), quantize_weight(w)))
+print("captured")
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
+def test_views_that_stand_for_other_values():
+    """Negated views, requires_grad leaves, bias and weight as strided vectors."""
+    z = torch.randn(4, 300, dtype=torch.complex64, device="cuda")
+    x = z.conj().imag  # a view with the negative bit
+    assert x.is_neg()
+    check_quantized(quantize_rows(x), x.clone(), 1)
+    assert torch.equal(rms_norm(x), rms_norm(x.clone()))
+    w = torch.nn.Parameter(randn(140, 300))
+    wq = quantize_weight(w)
+    assert not wq.data.requires_grad
+    b = randn(140, 2)[:, 0]
+    got = fp8_linear(x, wq, bias=b)
+    assert torch.equal(got, fp8_linear(x.clone(), wq, bias=b.contiguous())) and not got.requires_grad
+    g = randn(1).expand(300)
+    assert torch.equal(rms_norm(x, g), rms_norm(x, g.contiguous()))
 
 
 def test_offsets_past_32_bits():
