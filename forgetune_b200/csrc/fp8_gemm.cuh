@@ -33,7 +33,6 @@
 namespace ftb {
 
 constexpr int kFp8Threads = 256;
-constexpr int kFp8MaxSplit = 8;  // CTAs that share a tile's depth: the portable cluster size
 
 // What an epilogue reads and writes.
 struct Fp8Epilogue {
@@ -291,11 +290,13 @@ __global__ void __launch_bounds__(kFp8Threads) fp8_tile_kernel(const __grid_cons
   grid_dep_trigger();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_sf = tmem + L::D_COLS;
-  float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of this lane's outputs
+  // of this lane's outputs; plain loads: a kernel before this one may have
+  // written them after this one began (see grid_dep_wait)
+  float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (p.e.bias) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (n0 + 4 * lane + i < p.N) bias[i] = __ldg(p.e.bias + n0 + 4 * lane + i);
+      if (n0 + 4 * lane + i < p.N) bias[i] = p.e.bias[n0 + 4 * lane + i];
   }
 
   if (warp == 0) {

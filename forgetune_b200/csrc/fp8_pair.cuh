@@ -236,12 +236,12 @@ struct Fp8EpilogueWarp {
       const int n = n0 + 4 * lane, N = 4 * lane < kFp8EpiColumns ? q.p.N : 0;
       float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (q.bias_vec && n + 4 <= N) {
-        f = __ldg(reinterpret_cast<const float4*>(q.p.e.bias + n));
+        f = *reinterpret_cast<const float4*>(q.p.e.bias + n);
       } else {
-        if (n < N) f.x = __ldg(q.p.e.bias + n);
-        if (n + 1 < N) f.y = __ldg(q.p.e.bias + n + 1);
-        if (n + 2 < N) f.z = __ldg(q.p.e.bias + n + 2);
-        if (n + 3 < N) f.w = __ldg(q.p.e.bias + n + 3);
+        if (n < N) f.x = q.p.e.bias[n];
+        if (n + 1 < N) f.y = q.p.e.bias[n + 1];
+        if (n + 2 < N) f.z = q.p.e.bias[n + 2];
+        if (n + 3 < N) f.w = q.p.e.bias[n + 3];
       }
       __syncwarp();
       if (4 * lane < kFp8EpiColumns) const_cast<float4*>(bias4)[lane] = f;
