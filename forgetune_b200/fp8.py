@@ -15,7 +15,9 @@ The format is e4m3 values with one power-of-two scale (ue8m0, the format the
 tensor cores take) for each block of 128 along a row of activations and for
 each 128 x 128 block of a weight: the smallest power of two with
 ``max|x| / scale <= 448``, 1 for a block of zeros.  Values that are not finite
-are stored as NaN.  Products are accumulated in fp32.
+are stored as NaN.  Products are accumulated in fp32 by the tensor cores, which
+truncate where they add: relative error 5e-7 at depth 8192 for values of both
+signs, 4e-6 for sums of one sign.
 
 Inputs are 2-D; a plain input whose rows are not contiguous is copied first,
 as ``CompiledModel.run_device`` does.  The operators are for inference: they
