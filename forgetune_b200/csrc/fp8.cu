@@ -188,7 +188,7 @@ struct Fp8Choice {
 // round of pairs takes 0.29 per k-block and 0.8, and a launch 3.5 more than
 // the tile kernel's.  The constants are a fit to 525 shapes (m 1..4096, n and
 // k 64..8192) that were timed with every choice on a B200; over 696 others the
-// pick is 1.0 % slower than the best choice in the mean, 30 % at most.  For
+// pick is 1.1 % slower than the best choice in the mean, 28 % at most.  For
 // example (m x k x n): 1 x 4096 x 4096 takes 5.2 us with 16 tokens per tile
 // and split 4, 12.2 unsplit; 512 x 512 x 512 takes 3.5 with 16 tokens, 6.8 with
 // 128; 256 x 4096 x 4096 11.8 with 128 tokens and split 2, 16.9 on pairs;
