@@ -452,6 +452,97 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const RowsParams p, cons
   norm_finish<T, MODE>(p, row, c0, step, k, scale, v);
 }
 
+// The same where rows are not on 16-byte boundaries: element by element, lanes
+// on consecutive elements, so that a warp's access is 64 or 128 bytes in a
+// row.  A warp has NU quantisation blocks, four elements of each per lane, 32
+// apart.  Bound by the number of accesses and by the loads in flight: 16384 x
+// 7001 without residual 154 us in bf16 (45 % of the memory rate), 184 in fp32
+// (76 %).  With eight or four consecutive elements per lane, as in the
+// quantise kernels above, a warp's accesses spread over four times the lines
+// (373 and 302 us).
+template <typename T, int NU>
+__global__ void __launch_bounds__(1024) rms_norm_elements_kernel(const RowsParams p, const int warps) {
+  __shared__ float part[32];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int in_row = w % warps, first = w - in_row;
+  const int64_t row = (int64_t)blockIdx.x * ((int)(blockDim.x >> 5) / warps) + w / warps;
+  const int k = row < p.m ? (int)p.k : 0;
+  auto column = [&](int n, int i) { return (in_row * NU + n) * kFp8Block + 32 * i + lane; };
+  grid_dep_wait();
+  grid_dep_trigger();
+  const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
+  const T* r = static_cast<const T*>(p.residual) + row * p.r_ld;
+  float v[NU][4];
+  {
+    T a[NU][4], b[NU][4];
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[n][i] = column(n, i) < k ? x[column(n, i)] : from_f32<T>(0.0f);
+    if (p.residual) {
+#pragma unroll
+      for (int n = 0; n < NU; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[n][i] = column(n, i) < k ? r[column(n, i)] : from_f32<T>(0.0f);
+    }
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[n][i] = p.residual ? to_f32(a[n][i]) + to_f32(b[n][i]) : to_f32(a[n][i]);
+  }
+  SquareSum sum;
+#pragma unroll
+  for (int n = 0; n < NU; ++n) sum.add(v[n]);
+  float ss = sum.total();
+#pragma unroll
+  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (warps > 1) {
+    if (lane == 0) part[w] = ss;
+    __syncthreads();
+    ss = lane < warps ? part[first + lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  }
+  const float scale = rsqrtf(ss / (float)p.k + p.eps);
+  if (p.h) {
+    T* h = static_cast<T*>(p.h) + row * p.h_ld;
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (column(n, i) < k) h[column(n, i)] = from_f32<T>(v[n][i]);
+  }
+#pragma unroll
+  for (int n = 0; n < NU; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[n][i] = v[n][i] * scale * (p.weight && column(n, i) < k ? p.weight[column(n, i)] : 1.0f);
+  if (!p.q) {
+    T* y = static_cast<T*>(p.y) + row * p.y_ld;
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (column(n, i) < k) y[column(n, i)] = from_f32<T>(v[n][i]);
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (column(n, i) < k) a = max(a, finite_abs_bits(v[n][i]));
+      v[n][i] = nan_unless_finite(v[n][i]);
+    }
+    const uint32_t byte = fp8_scale_byte(__reduce_max_sync(0xffffffffu, a));
+    const uint32_t q = fp8_pack4(v[n][0], v[n][1], v[n][2], v[n][3], fp8_inv_scale(byte));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (column(n, i) < k) (p.q + row * p.q_ld)[column(n, i)] = (uint8_t)(q >> (8 * i));
+    if (lane == 0 && column(n, 0) < k) (p.s + row * p.s_ld)[column(n, 0) / kFp8Block] = (uint8_t)byte;
+  }
+}
+
 // Rows too long for registers: one CTA per row, which reads it twice.
 template <typename T, RowMode MODE>
 __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p) {
@@ -548,9 +639,23 @@ inline cudaError_t launch_rms_norm_t(const RowsParams& p, int sm_count, cudaStre
                    rows_vector<T>(p.residual, p.r_ld, p.m) && rows_vector<T>(p.h, p.h_ld, p.m) &&
                    rows_vector<T>(p.y, p.y_ld, p.m) && (reinterpret_cast<uintptr_t>(p.weight) & 15) == 0;
   const int64_t vectors = (p.k + kRowVec<T> - 1) / kRowVec<T>;
+  if (!vec) {
+    const int64_t units = fp8_blocks(p.k);
+    if (units > 32 * 4)
+      return pdl_launch(rms_norm_long_kernel<T, ROW_ELEMENTS>, dim3((unsigned)p.m), dim3(1024), 0, s, p);
+    // Blocks per warp as the vectors below; four at most, since eight do not
+    // fit the registers of 1024 threads (4096 x 20001 fp32: 273 us against 189
+    // in two passes; bf16 291 against 354, quantised with a residual 527
+    // against 426).
+    const int nu = units <= 32 && (p.m < 2 * sm_count || units == 1) ? 1 : units == 2 ? 2 : 4;
+    const int warps = ((int)units + nu - 1) / nu, rows = std::max(1, 8 / warps);
+    return pdl_launch(nu == 1   ? rms_norm_elements_kernel<T, 1>
+                      : nu == 2 ? rms_norm_elements_kernel<T, 2>
+                                : rms_norm_elements_kernel<T, 4>,
+                      dim3((unsigned)((p.m + rows - 1) / rows)), dim3(32 * warps * rows), 0, s, p, warps);
+  }
   if (vectors > 1024 * 4)  // more than the registers of 1024 threads hold
-    return pdl_launch(vec ? rms_norm_long_kernel<T, ROW_VECTORS> : rms_norm_long_kernel<T, ROW_ELEMENTS>,
-                      dim3((unsigned)p.m), dim3(1024), 0, s, p);
+    return pdl_launch(rms_norm_long_kernel<T, ROW_VECTORS>, dim3((unsigned)p.m), dim3(1024), 0, s, p);
   // Many rows: up to four vectors per lane, so that few warps share a row and
   // many loads are in flight (16384 x 8192 bf16, residual, quantised: 149 us
   // with four, 200 with two, 241 with one).  Few rows: one per lane, the
@@ -561,7 +666,6 @@ inline cudaError_t launch_rms_norm_t(const RowsParams& p, int sm_count, cudaStre
   int lanes = p.q ? kFp8Block / kRowVec<T> : 8;
   while ((int64_t)lanes * nv < vectors) lanes *= 2;
   const int rows = std::max(256, lanes) / lanes;
-  if (!vec) return launch_rms_norm_m<T, ROW_ELEMENTS>(p, nv, lanes, s);
   if ((int64_t)lanes * nv == vectors && p.m % rows == 0) return launch_rms_norm_m<T, ROW_WHOLE>(p, nv, lanes, s);
   return launch_rms_norm_m<T, ROW_VECTORS>(p, nv, lanes, s);
 }

@@ -182,6 +182,32 @@ def test_rms_norm(m, k, quantize, residual, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(1, 129), (2, 255), (700, 129), (301, 257), (300, 385), (299, 1111), (300, 4097),
+                                 (2, 4097), (2, 7001), (400, 512), (300, 16384), (2, 16384), (2, 16385), (1, 32769)])
+def test_rms_norm_rows_off_16_byte_boundaries(m, k, dtype):
+    """Rows that begin one element off a boundary, with columns before and behind that stay as they are; the
+    same values in rows on boundaries give the reference."""
+    bx, br = randn(m, k + 9, seed=k, dtype=dtype) * 2, randn(m, k + 9, seed=k + 1, dtype=dtype)
+    bx[:, 0] = br[:, 0] = float("nan")
+    bx[:, k + 1:] = br[:, k + 1:] = float("nan")
+    x, r = bx[:, 1:k + 1], br[:, 1:k + 1]
+    w = (randn(k + 1, seed=k + 2) + 1)[1:]
+    want, h = ref.rms_norm(f64(x), f64(w), 1e-5, f64(r))
+    absolute = (np.abs(f64(x)) + np.abs(f64(r))) * EPS32 * np.abs(want) / np.maximum(np.abs(h), 1e-30)
+    by, bh = torch.full_like(bx, 7), torch.full_like(bx, 7)
+    y, hg = rms_norm(x, w, eps=1e-5, residual=r, out=by[:, 1:k + 1], residual_out=bh[:, 1:k + 1])
+    check_plain(y, want, dtype, norm_bound(k), absolute)
+    check_plain(hg, h, dtype, EPS32)
+    for b in (by, bh):
+        assert bool((b[:, 0] == 7).all()) and bool((b[:, k + 1:] == 7).all())
+    q, hq = rms_norm(x, w, eps=1e-5, residual=r, quantize=True)
+    assert torch.equal(hq, hg)
+    check_block(q, want, np.abs(want) * norm_bound(k) + absolute)
+    plain, _ = ref.rms_norm(f64(x), None, 1e-5)
+    check_plain(rms_norm(x, eps=1e-5), plain, dtype, norm_bound(k))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_rms_norm_in_place_strided_and_without_weight(dtype):
     base = randn(10, 900, dtype=dtype)
     x, r = base[:, 3:803], randn(10, 800, seed=1, dtype=dtype)
