@@ -207,6 +207,35 @@ def test_rms_norm_rows_off_16_byte_boundaries(m, k, dtype):
     check_plain(rms_norm(x, eps=1e-5), plain, dtype, norm_bound(k))
 
 
+@pytest.mark.parametrize("k", [129, 1111])
+def test_rms_norm_rows_off_16_byte_boundaries_and_what_is_not_finite(k):
+    x = randn(5, k)
+    x[1] = 0
+    x[2, 7] = float("nan")
+    x[3, 9] = float("inf")
+    y, q = f64(rms_norm(x)), rms_norm(x, quantize=True)
+    d, s = f64(q.data), f64(q.scales)
+    rest = np.arange(k) != 9
+    for v in (y, d):
+        assert np.all(v[1] == 0) and np.all(np.isnan(v[2]))
+        assert np.isnan(v[3, 9]) and np.all(v[3, rest] == 0)  # x / inf
+    assert np.all(s[[1, 2, 3]] == 1)
+    want, _ = ref.rms_norm(f64(x[[0, 4]]), None, 1e-6)
+    check_plain(torch.from_numpy(y[[0, 4]]), want, torch.float32, norm_bound(k))
+    # one value that is not finite after the norm: its block's scale comes from the others
+    w = torch.ones(k, device="cuda")
+    w[3] = float("inf")
+    q = rms_norm(x[:1], w, quantize=True)
+    full, _ = ref.rms_norm(f64(x[:1]), None, 1e-6)
+    d, s = f64(q.data), f64(q.scales)
+    assert np.isnan(d[0, 3])
+    full[0, 3] = d[0, 3] = 0
+    top = np.abs(full[0, :128]).max()
+    assert 224 * s[0, 0] * (1 - 1e-4) < top <= 448 * s[0, 0] * (1 + 1e-4)
+    assert np.all(np.abs(d * ref.spread(s, 1, full.shape) - full)
+                  <= np.abs(full) * (2.0 ** -4 + 1e-4) + ref.spread(s, 1, full.shape) * 2.0 ** -10)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rms_norm_in_place_strided_and_without_weight(dtype):
     base = randn(10, 900, dtype=dtype)
