@@ -163,6 +163,18 @@ static std::string clashes(const char* what, const Span& out, const Span (&in)[N
   return "";
 }
 
+// A quantised output of m rows and `scale_rows` rows of scales: over an operand,
+// or the one over the other.
+template <size_t N>
+static std::string clashes(const char* what, const ftb_fp8_matrix& q, int64_t m, int64_t scale_rows, int64_t k,
+                           const Span (&in)[N]) {
+  const Span values = span(q.data, m, k, q.ld), scales = span(q.scales, scale_rows, fp8_blocks(k), q.scales_ld);
+  std::string why = clashes(what, values, in);
+  if (why.empty()) why = clashes(what, scales, in);
+  if (why.empty() && overlap(values, scales)) why = std::string(what) + " scales overlap its values";
+  return why;
+}
+
 static bool sizes_ok(int64_t m, int64_t n, int64_t k) {
   return m >= 0 && m <= kFp8MaxDim && n >= 1 && n <= kFp8MaxDim && k >= 1 && k <= kFp8MaxDim;
 }
@@ -274,8 +286,7 @@ FTB_API int ftb_quantize_rows(const ftb_quantize_args* args, void* stream) {
     std::string why = check("x", a.x, a.k);
     if (why.empty()) why = check("q", a.q, a.k);
     const Span in[1] = {span(a.x, a.m, a.k)};
-    if (why.empty()) why = clashes("q", span(a.q.data, a.m, a.k, a.q.ld), in);
-    if (why.empty()) why = clashes("q", span(a.q.scales, a.m, fp8_blocks(a.k), a.q.scales_ld), in);
+    if (why.empty()) why = clashes("q", a.q, a.m, a.m, a.k, in);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
@@ -304,8 +315,7 @@ FTB_API int ftb_quantize_weight(const ftb_quantize_args* args, void* stream) {
     std::string why = check("x", a.x, a.k);
     if (why.empty()) why = check("q", a.q, a.k);
     const Span in[1] = {span(a.x, a.m, a.k)};
-    if (why.empty()) why = clashes("q", span(a.q.data, a.m, a.k, a.q.ld), in);
-    if (why.empty()) why = clashes("q", span(a.q.scales, fp8_blocks(a.m), fp8_blocks(a.k), a.q.scales_ld), in);
+    if (why.empty()) why = clashes("q", a.q, a.m, fp8_blocks(a.m), a.k, in);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
@@ -349,9 +359,7 @@ FTB_API int ftb_rms_norm(const ftb_rms_norm_args* args, void* stream) {
     if (why.empty()) why = clashes("h", h, in, &x, &r);
     if (why.empty() && a.y.data) why = clashes("y", span(a.y, a.m, a.k), in, &x, &r);
     if (why.empty() && a.y.data && overlap(span(a.y, a.m, a.k), h)) why = "y overlaps h";
-    if (why.empty() && a.q.data) why = clashes("q", span(a.q.data, a.m, a.k, a.q.ld), more);
-    if (why.empty() && a.q.data)
-      why = clashes("q", span(a.q.scales, a.m, fp8_blocks(a.k), a.q.scales_ld), more);
+    if (why.empty() && a.q.data) why = clashes("q", a.q, a.m, a.m, a.k, more);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;
@@ -403,9 +411,7 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
                         r};
     if (why.empty() && a.y.data)
       why = clashes("y", span(a.y, a.m, a.n), in, a.residual.type == a.y.type ? &r : nullptr);
-    if (why.empty() && a.q.data) why = clashes("q", span(a.q.data, a.m, a.n, a.q.ld), in);
-    if (why.empty() && a.q.data)
-      why = clashes("q", span(a.q.scales, a.m, fp8_blocks(a.n), a.q.scales_ld), in);
+    if (why.empty() && a.q.data) why = clashes("q", a.q, a.m, a.m, a.n, in);
     if (!why.empty()) return refuse(fn, why);
     Fp8Device* d = nullptr;
     if (const int rc = fp8_device(fn, &d)) return rc;

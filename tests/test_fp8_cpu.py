@@ -76,6 +76,24 @@ def test_linear_refusals():
         assert call(**bad) == -2, bad
 
 
+def test_scales_over_their_own_values_are_refused():
+    B = 1 << 24  # far from P
+
+    def calls(s, s_ld=512):
+        yield rc("ftb_quantize_rows", QUANTIZE_ARGS, P, 512, 0, B, 512, s, s_ld, 4, 200)
+        yield rc("ftb_quantize_weight", QUANTIZE_ARGS, P, 512, 0, B, 512, s, s_ld, 4, 200)
+        yield rc("ftb_rms_norm", RMS_NORM_ARGS, P, 512, 0, 0, 0, 0, 0, 1e-6, 0, 0, 0, 0, 0, 0, B, 512, s, s_ld, 4, 200)
+        yield rc("ftb_fp8_linear", LINEAR_ARGS, P, 512, 2 * B, 4, 3 * B, 512, 4 * B, 4, 0, 0, 0, 0, 0, 0, 0, B, 512, s,
+                 s_ld, 4, 200, 200, 0)
+    for s, s_ld in ((B, 512), (B + 196, 512), (B + 512, 4), (B + 3 * 512 + 8, 4)):
+        for got in calls(s, s_ld):
+            assert got == -2 and "overlap" in _native.last_error(), (s - B, s_ld)
+    if _native.device_count() == 0:  # the scales behind each row's values, or behind them all
+        for s, s_ld in ((B + 208, 512), (B + 4 * 512, 4)):
+            for got in calls(s, s_ld):
+                assert got == -5, _native.last_error()
+
+
 def test_outputs_over_operands_are_refused():
     """Overlaps other than in place; side by side in one buffer's rows is none."""
     B = 1 << 24  # far from P
