@@ -109,13 +109,7 @@ __device__ __forceinline__ uint4 load_vec(const T* row, int c, int k) {
 
 template <typename T, RowMode MODE>
 __device__ __forceinline__ void store_vec(T* row, int c, int k, const float (&v)[kRowVec<T>]) {
-  if constexpr (MODE != ROW_ELEMENTS) {
-    if (MODE == ROW_WHOLE || c < k) *reinterpret_cast<uint4*>(row + c) = pack_vec<T>(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kRowVec<T>; ++i)
-      if (c + i < k) row[c + i] = from_f32<T>(v[i]);
-  }
+  if (MODE == ROW_WHOLE || c < k) *reinterpret_cast<uint4*>(row + c) = pack_vec<T>(v);
 }
 
 // The scale byte plus one of a lane's largest |x| (as bits), 0 where all are
@@ -377,7 +371,7 @@ __device__ __forceinline__ void norm_finish(const RowsParams& p, int64_t row, in
     if (!p.weight) {
 #pragma unroll
       for (int i = 0; i < VEC; i += 2) mul2(v[n][i], v[n][i + 1], scale, scale);
-    } else if (MODE == ROW_WHOLE || (MODE == ROW_VECTORS && at < k)) {
+    } else if (MODE == ROW_WHOLE || at < k) {
 #pragma unroll
       for (int i = 0; i < VEC; i += 4) {
         const float4 w = *reinterpret_cast<const float4*>(p.weight + at + i);
@@ -386,9 +380,6 @@ __device__ __forceinline__ void norm_finish(const RowsParams& p, int64_t row, in
         mul2(v[n][i], v[n][i + 1], w.x, w.y);
         mul2(v[n][i + 2], v[n][i + 3], w.z, w.w);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[n][i] = at + i < k ? v[n][i] * scale * p.weight[at + i] : 0.0f;
     }
   }
   if (p.q) {
@@ -488,6 +479,55 @@ __device__ __forceinline__ void quantize_elements(float (&v)[4], uint8_t* q, uin
   if (c % kFp8Block == 0 && c < k) s[c / kFp8Block] = (uint8_t)byte;
 }
 
+// h of NU blocks, held as above: c is the lane's first column.
+template <typename T, int NU>
+__device__ __forceinline__ void load_elements(const RowsParams& p, int64_t row, int c, int k, float (&v)[NU][4]) {
+  const T* x = static_cast<const T*>(p.x) + row * p.x_ld + c;
+  const T* r = static_cast<const T*>(p.residual) + row * p.r_ld + c;
+  T a[NU][4], b[NU][4];
+  auto at = [](int n, int i) { return n * kFp8Block + 32 * i; };
+#pragma unroll
+  for (int n = 0; n < NU; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[n][i] = c + at(n, i) < k ? x[at(n, i)] : from_f32<T>(0.0f);
+  if (p.residual) {
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[n][i] = c + at(n, i) < k ? r[at(n, i)] : from_f32<T>(0.0f);
+  }
+#pragma unroll
+  for (int n = 0; n < NU; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[n][i] = p.residual ? to_f32(a[n][i]) + to_f32(b[n][i]) : to_f32(a[n][i]);
+}
+
+// ... and its outputs.
+template <typename T, int NU>
+__device__ __forceinline__ void finish_elements(const RowsParams& p, int64_t row, int c, int k, float scale,
+                                                float (&v)[NU][4]) {
+  auto column = [&](int n, int i) { return c + n * kFp8Block + 32 * i; };
+  auto store = [&](T* t) {
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (column(n, i) < k) t[column(n, i)] = from_f32<T>(v[n][i]);
+  };
+  if (p.h) store(static_cast<T*>(p.h) + row * p.h_ld);
+#pragma unroll
+  for (int n = 0; n < NU; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[n][i] = v[n][i] * scale * (p.weight && column(n, i) < k ? p.weight[column(n, i)] : 1.0f);
+  if (p.q) {
+#pragma unroll
+    for (int n = 0; n < NU; ++n) quantize_elements(v[n], p.q + row * p.q_ld, p.s + row * p.s_ld, column(n, 0), k);
+  } else {
+    store(static_cast<T*>(p.y) + row * p.y_ld);
+  }
+}
+
 // The same where rows are not on 16-byte boundaries: element by element, lanes
 // on consecutive elements, so that a warp's access is 64 or 128 bytes in a
 // row.  A warp has NU quantisation blocks, four elements of each per lane, 32
@@ -504,30 +544,11 @@ __global__ void __launch_bounds__(1024) rms_norm_elements_kernel(const RowsParam
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int in_row = w % warps, first = w - in_row;
   const int64_t row = (int64_t)blockIdx.x * ((int)(blockDim.x >> 5) / warps) + w / warps;
-  const int k = row < p.m ? (int)p.k : 0;
-  auto column = [&](int n, int i) { return (in_row * NU + n) * kFp8Block + 32 * i + lane; };
+  const int k = row < p.m ? (int)p.k : 0, c = in_row * NU * kFp8Block + lane;
   grid_dep_wait();
   grid_dep_trigger();
-  const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
-  const T* r = static_cast<const T*>(p.residual) + row * p.r_ld;
   float v[NU][4];
-  {
-    T a[NU][4], b[NU][4];
-#pragma unroll
-    for (int n = 0; n < NU; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[n][i] = column(n, i) < k ? x[column(n, i)] : from_f32<T>(0.0f);
-    if (p.residual) {
-#pragma unroll
-      for (int n = 0; n < NU; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[n][i] = column(n, i) < k ? r[column(n, i)] : from_f32<T>(0.0f);
-    }
-#pragma unroll
-    for (int n = 0; n < NU; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[n][i] = p.residual ? to_f32(a[n][i]) + to_f32(b[n][i]) : to_f32(a[n][i]);
-  }
+  load_elements<T>(p, row, c, k, v);
   SquareSum sum;
 #pragma unroll
   for (int n = 0; n < NU; ++n) sum.add(v[n]);
@@ -541,37 +562,13 @@ __global__ void __launch_bounds__(1024) rms_norm_elements_kernel(const RowsParam
 #pragma unroll
     for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   }
-  const float scale = rsqrtf(ss / (float)p.k + p.eps);
-  if (p.h) {
-    T* h = static_cast<T*>(p.h) + row * p.h_ld;
-#pragma unroll
-    for (int n = 0; n < NU; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (column(n, i) < k) h[column(n, i)] = from_f32<T>(v[n][i]);
-  }
-#pragma unroll
-  for (int n = 0; n < NU; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[n][i] = v[n][i] * scale * (p.weight && column(n, i) < k ? p.weight[column(n, i)] : 1.0f);
-  if (!p.q) {
-    T* y = static_cast<T*>(p.y) + row * p.y_ld;
-#pragma unroll
-    for (int n = 0; n < NU; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (column(n, i) < k) y[column(n, i)] = from_f32<T>(v[n][i]);
-    return;
-  }
-#pragma unroll
-  for (int n = 0; n < NU; ++n) quantize_elements(v[n], p.q + row * p.q_ld, p.s + row * p.s_ld, column(n, 0), k);
+  finish_elements<T>(p, row, c, k, rsqrtf(ss / (float)p.k + p.eps), v);
 }
 
 // Rows too long for registers: one CTA per row, which reads it twice.
-template <typename T, RowMode MODE>
+template <typename T, bool VECTORS>
 __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p) {
-  constexpr int VEC = kRowVec<T>;
+  constexpr int VEC = kRowVec<T>, NU = 2;
   __shared__ float part[32];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dep_wait();
@@ -579,21 +576,29 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p)
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.r_ld : nullptr;
-  const int64_t step = 1024 * VEC;
+  const int64_t step = VECTORS ? 1024 * VEC : 32 * NU * kFp8Block;
   const int k = (int)p.k;
-  auto load = [&](int c, float (&v)[VEC]) {
-    unpack_vec<T>(load_vec<T, MODE>(x, c, k), v);
-    if (r) {
-      float t[VEC];
-      unpack_vec<T>(load_vec<T, MODE>(r, c, k), t);
-      add_vec(v, t);
+  using Values = float[VECTORS ? 1 : NU][VECTORS ? VEC : 4];  // a lane's part of a step
+  auto load = [&](int c, Values& v) {
+    if constexpr (VECTORS) {
+      unpack_vec<T>(load_vec<T, ROW_VECTORS>(x, c, k), v[0]);
+      if (r) {
+        float t[VEC];
+        unpack_vec<T>(load_vec<T, ROW_VECTORS>(r, c, k), t);
+        add_vec(v[0], t);
+      }
+    } else {
+      load_elements<T>(p, row, c, k, v);
     }
   };
+  const int64_t c0 = w * (step / 32);  // a warp's first column; whole warps stay together to quantise
+  const int in_warp = VECTORS ? lane * VEC : lane;
   SquareSum sum;
-  for (int64_t c = (int64_t)threadIdx.x * VEC; c < p.k; c += step) {
-    float v[VEC];
-    load((int)c, v);
-    sum.add(v);
+  for (int64_t c = c0; c < p.k; c += step) {
+    Values v;
+    load((int)c + in_warp, v);
+#pragma unroll
+    for (auto& u : v) sum.add(u);
   }
   float ss = sum.total();
 #pragma unroll
@@ -604,11 +609,11 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const RowsParams p)
 #pragma unroll
   for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   const float scale = rsqrtf(ss / (float)p.k + p.eps);
-  for (int64_t c0 = (int64_t)w * 32 * VEC; c0 < p.k; c0 += step) {  // whole warps: they quantise together
-    const int c = (int)c0 + lane * VEC;
-    float v[1][VEC];
-    load(c, v[0]);
-    norm_finish<T, MODE>(p, row, c, 0, k, scale, v);
+  for (int64_t c = c0; c < p.k; c += step) {
+    Values v;
+    load((int)c + in_warp, v);
+    if constexpr (VECTORS) norm_finish<T, ROW_VECTORS>(p, row, (int)c + in_warp, 0, k, scale, v);
+    else finish_elements<T>(p, row, (int)c + in_warp, k, scale, v);
   }
 }
 
@@ -667,7 +672,7 @@ inline cudaError_t launch_rms_norm_t(const RowsParams& p, int sm_count, cudaStre
   if (!vec) {
     const int64_t units = fp8_blocks(p.k);
     if (units > 32 * 4)
-      return pdl_launch(rms_norm_long_kernel<T, ROW_ELEMENTS>, dim3((unsigned)p.m), dim3(1024), 0, s, p);
+      return pdl_launch(rms_norm_long_kernel<T, false>, dim3((unsigned)p.m), dim3(1024), 0, s, p);
     // Blocks per warp as the vectors below; four at most, since eight do not
     // fit the registers of 1024 threads (4096 x 20001 fp32: 273 us against 189
     // in two passes; bf16 291 against 354, quantised with a residual 527
@@ -680,7 +685,7 @@ inline cudaError_t launch_rms_norm_t(const RowsParams& p, int sm_count, cudaStre
                       dim3((unsigned)((p.m + rows - 1) / rows)), dim3(32 * warps * rows), 0, s, p, warps);
   }
   if (vectors > 1024 * 4)  // more than the registers of 1024 threads hold
-    return pdl_launch(rms_norm_long_kernel<T, ROW_VECTORS>, dim3((unsigned)p.m), dim3(1024), 0, s, p);
+    return pdl_launch(rms_norm_long_kernel<T, true>, dim3((unsigned)p.m), dim3(1024), 0, s, p);
   // Many rows: up to four vectors per lane, so that few warps share a row and
   // many loads are in flight (16384 x 8192 bf16, residual, quantised: 149 us
   // with four, 200 with two, 241 with one).  Few rows: one per lane, the
