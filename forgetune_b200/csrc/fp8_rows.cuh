@@ -397,14 +397,14 @@ __device__ __forceinline__ void norm_finish(const RowsParams& p, int64_t row, in
 
 //   h = x + residual (fp32),  y = h / sqrt(mean(h^2) + eps) weight
 // `lanes` threads per row, which keep it in registers: NV vectors per lane.  A
-// row has 8 or 16 lanes of a warp (rows that short), a warp or several; a CTA
-// has one row or several.
+// row has 8 or 16 lanes of a warp (rows that short), or whole warps; a CTA has
+// one row or several.
 template <typename T, RowMode MODE, int NV>
 __global__ void __launch_bounds__(1024) rms_norm_kernel(const RowsParams p, const int lanes) {
   constexpr int VEC = kRowVec<T>;
   __shared__ float part[32];
-  const int in_row = threadIdx.x & (lanes - 1);  // lanes is a power of two
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+  const int row_in_cta = (int)threadIdx.x / lanes, in_row = (int)threadIdx.x - row_in_cta * lanes;
+  const int64_t row = (int64_t)blockIdx.x * ((int)blockDim.x / lanes) + row_in_cta;
   const int c0 = in_row * VEC, step = lanes * VEC, k = row < p.m ? (int)p.k : 0;
   grid_dep_wait();
   grid_dep_trigger();
@@ -432,10 +432,10 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const RowsParams p, cons
   float ss = sum.total();
   for (int o = min(lanes, 32) / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if (lanes > 32) {
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = lanes >> 5, first = w & ~(warps - 1);
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = lanes >> 5;
     if (lane == 0) part[w] = ss;
     __syncthreads();
-    ss = lane < warps ? part[first + lane] : 0.0f;
+    ss = lane < warps ? part[row_in_cta * warps + lane] : 0.0f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   }
@@ -532,7 +532,7 @@ __device__ __forceinline__ void finish_elements(const RowsParams& p, int64_t row
 // on consecutive elements, so that a warp's access is 64 or 128 bytes in a
 // row.  A warp has NU quantisation blocks, four elements of each per lane, 32
 // apart.  Bound by the number of accesses and by the loads in flight: 16384 x
-// 7001 without residual 154 us in bf16 (45 % of the memory rate), 184 in fp32
+// 7001 without residual 152 us in bf16 (46 % of the memory rate), 184 in fp32
 // (76 %).  With eight or four consecutive elements per lane, a warp's accesses
 // spread over four times the lines (373 and 302 us).  The quantise kernels
 // above keep that order all the same: they store a lane's values as one word,
@@ -656,12 +656,12 @@ inline cudaError_t launch_quantize_weight(const RowsParams& p, int type, cudaStr
 
 template <typename T, RowMode MODE>
 inline cudaError_t launch_rms_norm_m(const RowsParams& p, int nv, int lanes, cudaStream_t s) {
-  const int threads = std::max(256, lanes), rows = threads / lanes;
+  const int rows = std::max(1, 256 / lanes);
   const unsigned grid = (unsigned)((p.m + rows - 1) / rows);
   return pdl_launch(nv == 4   ? rms_norm_kernel<T, MODE, 4>
                     : nv == 2 ? rms_norm_kernel<T, MODE, 2>
                               : rms_norm_kernel<T, MODE, 1>,
-                    dim3(grid), dim3(threads), 0, s, p, lanes);
+                    dim3(grid), dim3(rows * lanes), 0, s, p, lanes);
 }
 template <typename T>
 inline cudaError_t launch_rms_norm_t(const RowsParams& p, int sm_count, cudaStream_t s) {
@@ -671,12 +671,13 @@ inline cudaError_t launch_rms_norm_t(const RowsParams& p, int sm_count, cudaStre
   const int64_t vectors = (p.k + kRowVec<T> - 1) / kRowVec<T>;
   if (!vec) {
     const int64_t units = fp8_blocks(p.k);
-    if (units > 32 * 4)
+    // Two passes above 128 blocks, which is what the registers of 1024 threads
+    // hold, and in 16 bits, where the second pass finds more of the row in the
+    // caches, above 64: 4096 x 12001 bf16 75 us in two passes, 92 in registers;
+    // 16384 x 7001 bf16 191 and 152; 4096 x 16001 fp32 139 and 121.
+    if (units > (sizeof(T) == 4 ? 128 : 64))
       return pdl_launch(rms_norm_long_kernel<T, false>, dim3((unsigned)p.m), dim3(1024), 0, s, p);
-    // Blocks per warp as the vectors below; four at most, since eight do not
-    // fit the registers of 1024 threads (4096 x 20001 fp32: 273 us against 189
-    // in two passes; bf16 291 against 354, quantised with a residual 527
-    // against 426).
+    // blocks per warp as the vectors below
     const int nu = units <= 32 && (p.m < 2 * sm_count || units == 1) ? 1 : units == 2 ? 2 : 4;
     const int warps = ((int)units + nu - 1) / nu, rows = std::max(1, 8 / warps);
     return pdl_launch(nu == 1   ? rms_norm_elements_kernel<T, 1>
@@ -692,10 +693,14 @@ inline cudaError_t launch_rms_norm_t(const RowsParams& p, int sm_count, cudaStre
   // shortest time (1 x 4096: 2.5 us against 3.4 with four).
   int nv = 1;
   if (p.m >= 2 * sm_count || vectors > 1024) nv = vectors <= 32 ? 1 : vectors <= 64 ? 2 : 4;
-  // a quantisation block's lanes stay together
+  // Whole warps, as many as the row needs (16384 x 5120 bf16, residual,
+  // quantised: 87 us with five warps, 111 with eight), or the lanes of several
+  // rows side by side in a warp.  A quantisation block's lanes stay together.
+  const int need = (int)((vectors + nv - 1) / nv);
   int lanes = p.q ? kFp8Block / kRowVec<T> : 8;
-  while ((int64_t)lanes * nv < vectors) lanes *= 2;
-  const int rows = std::max(256, lanes) / lanes;
+  while (lanes < 32 && lanes < need) lanes *= 2;
+  if (lanes < need) lanes = (need + 31) / 32 * 32;
+  const int rows = std::max(1, 256 / lanes);
   if ((int64_t)lanes * nv == vectors && p.m % rows == 0) return launch_rms_norm_m<T, ROW_WHOLE>(p, nv, lanes, s);
   return launch_rms_norm_m<T, ROW_VECTORS>(p, nv, lanes, s);
 }

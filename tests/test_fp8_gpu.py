@@ -182,8 +182,26 @@ def test_rms_norm(m, k, quantize, residual, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(1, 384), (2, 1536), (300, 384), (301, 768), (299, 1280), (300, 1288), (333, 2560),
+                                 (300, 4104), (297, 5120), (300, 7168), (300, 11008), (2, 8320), (300, 16384),
+                                 (300, 136), (299, 264), (5, 640)])
+def test_rms_norm_rows_of_any_number_of_warps(m, k, dtype):
+    x, r, w = randn(m, k, seed=k, dtype=dtype) * 2, randn(m, k, seed=k + 1, dtype=dtype), randn(k, seed=k + 2) + 1
+    want, h = ref.rms_norm(f64(x), f64(w), 1e-5, f64(r))
+    absolute = (np.abs(f64(x)) + np.abs(f64(r))) * EPS32 * np.abs(want) / np.maximum(np.abs(h), 1e-30)
+    y, hg = rms_norm(x, w, eps=1e-5, residual=r)
+    check_plain(y, want, dtype, norm_bound(k), absolute)
+    check_plain(hg, h, dtype, EPS32)
+    check_block(rms_norm(x, w, eps=1e-5, residual=r, quantize=True)[0], want,
+                np.abs(want) * norm_bound(k) + absolute)
+    plain, _ = ref.rms_norm(f64(x), None, 1e-5)
+    check_plain(rms_norm(x, eps=1e-5), plain, dtype, norm_bound(k))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,k", [(1, 129), (2, 255), (700, 129), (301, 257), (300, 385), (299, 1111), (300, 4097),
-                                 (2, 4097), (2, 7001), (400, 512), (300, 16384), (2, 16384), (2, 16385), (1, 32769)])
+                                 (2, 4097), (2, 7001), (400, 512), (300, 8192), (299, 8193), (300, 16384), (2, 16384), (2, 16385),
+                                 (1, 32769)])
 def test_rms_norm_rows_off_16_byte_boundaries(m, k, dtype):
     """Rows that begin one element off a boundary, with columns before and behind that stay as they are; the
     same values in rows on boundaries give the reference."""
