@@ -143,6 +143,7 @@ static Span span(const void* p, int64_t rows, int64_t bytes, int64_t ld) {
 }
 static bool overlap(const Span& a, const Span& b) {
   if (!a.p || !b.p || a.rows < 1 || b.rows < 1 || a.p + a.end() <= b.p || b.p + b.end() <= a.p) return false;
+  if (a.rows == 1 && b.rows == 1) return true;  // their ranges meet (a vector's span has no stride)
   const int64_t ld = a.rows > 1 ? a.ld : b.ld;
   if ((a.rows > 1 && a.ld != ld) || (b.rows > 1 && b.ld != ld)) return true;  // not worth telling apart
   const int64_t d = ((b.p - a.p) % ld + ld) % ld;  // b's columns in a's rows

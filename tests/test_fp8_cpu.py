@@ -129,6 +129,45 @@ def test_outputs_over_operands_are_refused():
             assert good == -5, _native.last_error()
 
 
+def test_one_row_outputs_over_operands_are_refused():
+    """The same for one row, where both spans may be without a stride (a norm weight, a bias)."""
+    B = 1 << 24  # far from P
+
+    def quantize(name, x, q, s):
+        return rc(name, QUANTIZE_ARGS, x, 256, 0, q, 256, s, 4, 1, 200)
+    for name in ("ftb_quantize_rows", "ftb_quantize_weight"):
+        for x, q, s in ((P, P, B), (P, P + 784, B), (P, B, P + 400), (P, B, B), (P, B, B + 196)):
+            assert quantize(name, x, q, s) == -2 and "overlap" in _native.last_error(), (name, x - P, q - P, s - P)
+
+    def norm(**over):
+        a = dict(x=P, r=2 * B, w=3 * B, h=4 * B, y=5 * B, q=0, s=0)
+        a.update(over)
+        return rc("ftb_rms_norm", RMS_NORM_ARGS, a["x"], 256, 0, a["r"], 256, 0, a["w"], 1e-6, a["h"], 256, 0, a["y"],
+                  256, 0, a["q"], 256, a["s"], 4, 1, 200)
+    for bad in (dict(h=P + 4), dict(y=P + 16), dict(h=5 * B), dict(h=P, y=P), dict(y=3 * B), dict(y=3 * B + 796),
+                dict(y=3 * B - 796), dict(h=3 * B), dict(h=3 * B + 400), dict(y=0, q=P, s=B), dict(y=0, q=B, s=P + 796),
+                dict(y=0, q=4 * B + 16, s=B), dict(y=0, q=3 * B, s=B), dict(y=0, q=3 * B + 784, s=B),
+                dict(y=0, q=B, s=3 * B), dict(y=0, q=B, s=3 * B + 796)):
+        assert norm(**bad) == -2 and "overlaps" in _native.last_error(), bad
+
+    def linear(**over):
+        a = dict(y=B, res=2 * B, bias=3 * B, a=4 * B, sa=5 * B, w=6 * B, sw=7 * B, q=0, s=0, yt=0, rt=0)
+        a.update(over)
+        return rc("ftb_fp8_linear", LINEAR_ARGS, a["a"], 256, a["sa"], 4, a["w"], 256, a["sw"], 4, a["bias"], a["res"],
+                  130, a["rt"], a["y"], 130, a["yt"], a["q"], 144, a["s"], 4, 1, 130, 200, 0)
+    for bad in (dict(y=2 * B + 4), dict(y=2 * B, yt=1), dict(y=3 * B), dict(y=3 * B + 516), dict(y=3 * B - 516),
+                dict(y=4 * B), dict(y=5 * B), dict(y=6 * B), dict(y=7 * B), dict(y=0, q=4 * B, s=B),
+                dict(y=0, q=B, s=5 * B), dict(y=0, q=2 * B, s=B), dict(y=0, q=3 * B, s=B), dict(y=0, q=3 * B + 512, s=B),
+                dict(y=0, q=B, s=3 * B), dict(y=0, q=B, s=3 * B + 516)):
+        assert linear(**bad) == -2 and "overlaps" in _native.last_error(), bad
+    # allowed as far as the checks go: in place, or right behind the operand
+    if _native.device_count() == 0:
+        for good in (norm(), norm(h=P), norm(y=P), norm(h=2 * B), norm(h=P, y=2 * B), norm(y=3 * B + 800),
+                     norm(y=3 * B - 800), norm(y=0, q=3 * B + 800, s=3 * B + 1008), linear(), linear(y=2 * B),
+                     linear(y=3 * B + 520), linear(y=3 * B - 520), quantize("ftb_quantize_rows", P, P + 800, P + 1008)):
+            assert good == -5, _native.last_error()
+
+
 def fp8(*shape):
     return torch.zeros(*shape).to(torch.float8_e4m3fn)
 
