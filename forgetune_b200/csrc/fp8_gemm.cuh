@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(kFp8Threads) fp8_tile_kernel(const __grid_cons
 #pragma unroll 1
       for (int c0 = 0; c0 < tokens; c0 += 32) {
         uint32_t r[32];
+        __syncwarp();  // warp-collective
         FTB_TMEM_LD32(tmem + c0 + ((uint32_t)(q * 32) << 16), r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll

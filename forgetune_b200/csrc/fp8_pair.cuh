@@ -614,6 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8PairShape::THREAD
       const uint32_t acce_leader = cluster_addr(&acce[b], 0);
       auto load = [&](int j, float (&v)[32]) {
         uint32_t r[32];
+        __syncwarp();  // warp-collective, and one lane has sent a box or arrived since
         FTB_TMEM_LD32(acc + 32 * w.chunk(j), r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll

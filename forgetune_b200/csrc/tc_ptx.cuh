@@ -214,7 +214,11 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t caddr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(caddr), "r"(v) : "memory");
 }
 
+// All threads of the cluster.  The barrier's instructions want whole converged
+// warps, and lanes may have gone apart before (one that arrived on a barrier,
+// columns past a ragged edge).
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
