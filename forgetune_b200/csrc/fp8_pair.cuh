@@ -178,6 +178,8 @@ __device__ __noinline__ void store_box_rows(uint32_t box, U* y, int64_t ld, int 
       }
     }
   }
+  // the box next receives a residual by TMA: after these ordinary accesses
+  fence_proxy_async_smem();
   __syncwarp();
 }
 

@@ -32,3 +32,10 @@ def test_cluster_barriers_begin_with_a_warp_barrier():
     assert len(re.findall(r"barrier\.cluster\.arrive", text["tc_ptx.cuh"])) == 1
     assert re.search(r"cluster_sync_all\(\)\s*\{\s*__syncwarp\(\);\s*asm volatile\(\"barrier\.cluster\.arrive",
                      text["tc_ptx.cuh"])
+
+
+def test_a_box_stored_by_rows_is_fenced_before_the_copy_engine_writes_it():
+    """Ordinary accesses to shared memory and a TMA load into the same bytes are ordered by a proxy fence of the
+    lanes that made them, then the warp barrier before the lane that sends the load."""
+    body = re.search(r"void store_box_rows\(.*?\n\}", code("fp8_pair.cuh"), re.S).group(0)
+    assert re.search(r"fence_proxy_async_smem\(\);\s*__syncwarp\(\);\s*\}$", body)
