@@ -58,6 +58,7 @@ _SIGS = {
     "ftb_rms_norm": ([c_void_p, c_void_p], c_int),
     "ftb_fp8_linear": ([c_void_p, c_void_p], c_int),
     "ftb_fp8_set_fault_injection": ([c_int], c_int),
+    "ftb_fp8_set_kernel": ([c_int, c_int], c_int),
 }
 
 EXPORTED = sorted(_SIGS)

@@ -34,6 +34,7 @@ struct Fp8Device {
 };
 static Fp8Device g_fp8_devices[kFp8MaxDevices];
 static std::atomic<int> g_fp8_stall{0};  // failure-detection hook
+static std::atomic<int> g_fp8_kernel{-1};  // kernel hook: 16 nt + split, or -1 for the estimate's choice
 
 static int refuse(const char* fn, const std::string& why, int status = ST_INPUT) {
   set_error(std::string(fn) + ": " + why);
@@ -233,7 +234,8 @@ static Fp8Choice choose_fp8(int64_t m, int64_t n, int64_t k, const Fp8Device& d)
 }
 
 static cudaError_t launch_fp8_linear(const Fp8Operands& o, const Fp8Params& p, const Fp8Device& d, cudaStream_t s) {
-  const Fp8Choice c = choose_fp8(p.M, p.N, p.K, d);
+  const int set = g_fp8_kernel.load(std::memory_order_relaxed);
+  const Fp8Choice c = set < 0 ? choose_fp8(p.M, p.N, p.K, d) : Fp8Choice{set / 16, set % 16};
   switch (c.nt) {
     case 16: return launch_fp8_tile<16>(o, p, c.split, s);
     case 32: return launch_fp8_tile<32>(o, p, c.split, s);
@@ -445,5 +447,18 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
 
 FTB_API int ftb_fp8_set_fault_injection(int stall) {
   g_fp8_stall.store(stall ? 1 : 0);
+  return ST_OK;
+}
+
+FTB_API int ftb_fp8_set_kernel(int nt, int split) {
+  if (nt == -1) {
+    g_fp8_kernel.store(-1);
+    return ST_OK;
+  }
+  const bool tile = (nt == 16 || nt == 32 || nt == 64 || nt == 128) &&
+                    (split == 1 || split == 2 || split == 4 || split == 8);
+  if (!tile && !(nt == 0 && split == 1))
+    return refuse("ftb_fp8_set_kernel", "needs nt 16, 32, 64 or 128 with split 1, 2, 4 or 8, nt 0 with split 1, or nt -1");
+  g_fp8_kernel.store(16 * nt + split);
   return ST_OK;
 }

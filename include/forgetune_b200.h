@@ -306,6 +306,11 @@ FORGETUNE_EXPORT int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* strea
  * nothing completes run out (about 2 s); the kernel leaves cleanly and the next call returns -5. */
 FORGETUNE_EXPORT int ftb_fp8_set_fault_injection(int stall);
 
+/* Kernel hook (tests): ftb_fp8_linear takes this kernel for every shape from now on, in place of the one whose
+ * estimated time is shortest: nt = 16, 32, 64 or 128 tokens per tile with the depth split over 1, 2, 4 or 8 CTAs,
+ * nt = 0 with split 1 for SM pairs, nt = -1 for the estimate again.  -2 for any other combination. */
+FORGETUNE_EXPORT int ftb_fp8_set_kernel(int nt, int split);
+
 #ifdef __cplusplus
 }
 #endif

@@ -168,6 +168,19 @@ def test_one_row_outputs_over_operands_are_refused():
             assert good == -5, _native.last_error()
 
 
+def test_kernel_hook_refuses_kernels_that_do_not_exist():
+    hook = _native.lib().ftb_fp8_set_kernel
+    try:
+        for nt in (16, 32, 64, 128):
+            for split in (1, 2, 4, 8):
+                assert hook(nt, split) == 0
+        assert hook(0, 1) == 0 and hook(-1, 0) == 0
+        for nt, split in ((48, 1), (256, 1), (16, 0), (16, 3), (16, 16), (0, 0), (0, 2), (-2, 1), (128, -1), (1 << 30, 1)):
+            assert hook(nt, split) == -2 and "ftb_fp8_set_kernel" in _native.last_error(), (nt, split)
+    finally:
+        assert hook(-1, 0) == 0
+
+
 def fp8(*shape):
     return torch.zeros(*shape).to(torch.float8_e4m3fn)
 
