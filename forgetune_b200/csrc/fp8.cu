@@ -97,12 +97,11 @@ static int fp8_device(const char* fn, Fp8Device** out) {
       d.ready.store(true, std::memory_order_release);
     }
   }
-  const int code = *d.fault;
-  if (code != 0) {
-    *d.fault = 0;
+  // taken by one caller: of threads that find it at once, the others go on
+  const int code = *d.fault != 0 ? __atomic_exchange_n(const_cast<int*>(d.fault), 0, __ATOMIC_RELAXED) : 0;
+  if (code != 0)
     return refuse(fn, "an earlier call's kernel on this device gave up: a wait exceeded its limit (code " +
                           std::to_string(code) + "); that call's output is not valid", ST_DEVICE);
-  }
   *out = &d;
   return ST_OK;
 }

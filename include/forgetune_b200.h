@@ -244,8 +244,11 @@ FORGETUNE_EXPORT int ftb_small_gemm_noalloc(const float* d_x, const float* d_w, 
  * not share memory with an operand except in place, where said so.
  *
  * Status codes as above: -1 null pointer, -2 sizes, strides, alignment,
- * types or overlaps, -5 launch error, or an earlier call's kernel on this
- * device gave up a wait (reported once, by the next call). */
+ * types or overlaps, -5 launch error, or an earlier kernel on this device gave
+ * up a wait.  That is reported once, by the next call with m > 0 on the device
+ * after it happened, of whatever operator, thread or stream, which then launches
+ * nothing; a replayed graph makes no call, so a caller that only replays makes
+ * one to find out. */
 #define FTB_F32 0
 #define FTB_F16 1
 #define FTB_BF16 2

@@ -2,12 +2,13 @@
 output path against float64, exact by integers (see integers)."""
 
 import contextlib
+import threading
 
 import numpy as np
 import pytest
 import torch
 
-from forgetune_b200 import _native, fp8_linear
+from forgetune_b200 import ForgeTuneRuntimeError, _native, fp8_linear, quantize_rows
 
 from . import fp8_reference as ref
 from .test_fp8_gpu import TYPES, f64, guarded, integers, same
@@ -137,3 +138,35 @@ def test_every_kernel_on_inputs_written_right_before(nt, split):
         got = [call(i % 3) for i in range(12)]
     for i, g in enumerate(got):
         assert all(torch.equal(x, y) for x, y in zip(g, want[i % 3])), i
+
+
+def test_a_wait_that_ran_out_is_reported_to_one_of_many_threads():
+    """Eight threads call at once after it: one is told, the others' calls run."""
+    a, w = integers(5, 256, 1, seed=1)[0], integers(130, 256, 128, seed=2)[0]
+    x = torch.randn(5, 256, device="cuda")
+    want = quantize_rows(x)
+    fp8_linear(a, w)
+    torch.cuda.synchronize()
+    _native.lib().ftb_fp8_set_fault_injection(1)
+    try:
+        fp8_linear(a, w)
+        torch.cuda.synchronize()
+    finally:
+        _native.lib().ftb_fp8_set_fault_injection(0)
+    told, right, start = [], [], threading.Barrier(8)
+
+    def work():
+        start.wait()
+        try:
+            q = quantize_rows(x)
+            torch.cuda.current_stream().synchronize()
+            right.append(torch.equal(q.data.view(torch.uint8), want.data.view(torch.uint8)))
+        except ForgeTuneRuntimeError as e:
+            told.append(str(e))
+    threads = [threading.Thread(target=work) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(told) == 1 and "exceeded its limit" in told[0]
+    assert len(right) == 7 and all(right)
