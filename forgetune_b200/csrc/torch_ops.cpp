@@ -7,6 +7,7 @@
 // rms_norm with residual and quantised output 6.1 (13.5), fp8_linear 4.4
 // (8.3); about 1.3 us of it is each output's allocation, 2.7 the launch.
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty_strided.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -94,6 +95,20 @@ Matrix input(PyObject* o, const char* what) {
   return r;
 }
 
+// A caller's output is written past autograd: refused where autograd would
+// have to know, as torch's own out= forms do (a leaf in no_grad is fine).
+void check_written(const at::Tensor& t, const char* what) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    value_error(std::string(what) + " requires grad: the operators have no backward pass (call them in torch.no_grad())");
+}
+
+// ... and counted as a change in place, so that a backward pass that saved the
+// old values refuses to run on the new ones.  Tensors made in inference mode
+// have no count.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void check_place(const at::Tensor& t, const char* what, int64_t m, int64_t n, at::Device dev) {
   if (t.dim() != 2 || t.size(0) != m || t.size(1) != n)
     shape_error(std::string(what) + " must be " + show(m, n) + ", got " + show(t.sizes()));
@@ -117,6 +132,7 @@ Matrix output(PyObject* o, const char* what, int64_t m, int64_t n, at::ScalarTyp
   check_place(*t, what, m, n, dev);
   const int64_t ld = row_stride(*t);
   if (ld < 0) shape_error(std::string(what) + ": rows must be contiguous and must not overlap");
+  check_written(*t, what);
   r.t = *t;
   r.a = as_matrix(r.t, ld);
   return r;
@@ -176,6 +192,8 @@ Fp8 fp8_output(PyObject* data, PyObject* scales, const char* what, int64_t m, in
   if (data == Py_None) return new_fp8(m, k, 1, dev);
   Fp8 r = fp8(data, scales, 1, what);
   check_place(r.data, what, m, k, dev);
+  check_written(r.data, what);
+  check_written(r.scales, what);
   lay_out(r, what);
   return r;
 }
@@ -206,6 +224,16 @@ void call(const char* name, int (*fn)(const Args*, void*), const Args& args, at:
   Py_END_ALLOW_THREADS
   if (rc != 0)
     throw Refused{g_runtime_error, std::string(name) + " failed (" + std::to_string(rc) + "): " + ftb_last_error()};
+}
+
+// The caller's outputs among these (`given`: what the caller passed, None for a new tensor).
+void written(PyObject* given, const Matrix& y) {
+  if (given != Py_None) written(y.t);
+}
+void written(PyObject* given, const Fp8& q) {
+  if (given == Py_None) return;
+  written(q.data);
+  written(q.scales);
 }
 
 void run_quantize_rows(const Matrix& x, const Fp8& q) {
@@ -265,6 +293,7 @@ PyObject* op_quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Matrix x = input(a[0], "quantize_rows: x");
     const Fp8 q = fp8_output(a[1], a[2], "quantize_rows: out", x.m, x.k, x.t.device());
     run_quantize_rows(x, q);
+    written(a[1], q);
     return pair(wrap(q.data), wrap(q.scales));
   });
 }
@@ -320,6 +349,9 @@ PyObject* op_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       args.y = y.a;
     }
     call("ftb_rms_norm", ftb_rms_norm, args, dev);
+    if (quantize) written(a[5], q);
+    else written(a[5], y);
+    if (h.t.defined()) written(a[7], h);
     PyObject* r = PyTuple_New(3);
     if (!r) return nullptr;
     PyTuple_SET_ITEM(r, 0, wrap(quantize ? q.data : y.t));
@@ -391,6 +423,8 @@ PyObject* op_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     args.a = x.a;
     args.w = w.a;
     call("ftb_fp8_linear", ftb_fp8_linear, args, dev);
+    if (quantize) written(a[9], q);
+    else written(a[9], y);
     return pair(wrap(quantize ? q.data : y.t), quantize ? wrap(q.scales) : none());
   });
 }

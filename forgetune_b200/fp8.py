@@ -21,7 +21,10 @@ signs, 4e-6 for sums of one sign.
 
 Inputs are 2-D; a plain input whose rows are not contiguous is copied first,
 as ``CompiledModel.run_device`` does.  The operators are for inference: they
-return tensors without gradients.  They need no workspace, so calls may run
+return tensors without gradients.  An
+output that requires grad is refused outside ``torch.no_grad()``; writing into
+a caller's tensor counts as a change in place, which a backward pass that
+saved it reports.  They need no workspace, so calls may run
 on several streams at once and be captured into CUDA graphs.  The reference
 has no counterpart (its models are float32 only).
 """
