@@ -75,6 +75,12 @@ struct Matrix {
 
 ftb_matrix as_matrix(const at::Tensor& t, int64_t ld) { return {t.data_ptr(), ld, plain_type(t.scalar_type())}; }
 
+// A forward-mode tangent would be dropped, which reads as a derivative of zero.
+void check_tangent(const at::Tensor& t, const char* what) {
+  if (t._fw_grad(0).defined())
+    value_error(std::string(what) + " has a forward-mode tangent: the operators have no derivatives (unpack it first)");
+}
+
 // A plain 2-D CUDA input, copied where its rows are not contiguous.
 Matrix input(PyObject* o, const char* what) {
   const at::Tensor* t = tensor(o);
@@ -82,6 +88,7 @@ Matrix input(PyObject* o, const char* what) {
     type_error(std::string(what) + " must be a float32, float16 or bfloat16 CUDA tensor");
   if (t->dim() != 2 || t->size(1) < 1)
     shape_error(std::string(what) + " must be 2-D with at least one column, got " + show(t->sizes()));
+  check_tangent(*t, what);
   Matrix r;
   r.m = t->size(0);
   r.k = t->size(1);
@@ -98,6 +105,7 @@ Matrix input(PyObject* o, const char* what) {
 // A caller's output is written past autograd: refused where autograd would
 // have to know, as torch's own out= forms do (a leaf in no_grad is fine).
 void check_written(const at::Tensor& t, const char* what) {
+  check_tangent(t, what);
   if (t.requires_grad() && at::GradMode::is_enabled())
     value_error(std::string(what) + " requires grad: the operators have no backward pass (call them in torch.no_grad())");
 }
@@ -208,6 +216,7 @@ at::Tensor vector(PyObject* o, const char* what, int64_t n, at::Device dev) {
     shape_error(std::string(what) + " must be [" + std::to_string(n) + "], got " + show(t->sizes()));
   if (t->device() != dev)
     value_error(std::string(what) + " is on " + t->device().str() + ", the input on " + dev.str());
+  check_tangent(*t, what);
   const at::Tensor v = t->is_neg() ? t->resolve_neg() : *t;
   return n == 1 || v.stride(0) == 1 ? v : v.contiguous();
 }

@@ -60,3 +60,21 @@ def test_tensors_made_in_inference_mode_are_outputs_anywhere():
             call()
     for call, _ in made:
         call()
+
+
+def test_forward_mode_tangents_are_refused():
+    x, r, b = torch.randn(4, 256, device="cuda"), torch.randn(4, 128, device="cuda"), torch.randn(128, device="cuda")
+    g = torch.randn(256, device="cuda")
+    w = quantize_weight(torch.randn(128, 256, device="cuda"))
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: quantize_rows(dual(x)), lambda: quantize_weight(dual(x)), lambda: rms_norm(dual(x)),
+                     lambda: rms_norm(x, dual(g)), lambda: rms_norm(x, residual=dual(x)),
+                     lambda: rms_norm(x, out=dual(x)), lambda: fp8_linear(dual(x), w),
+                     lambda: fp8_linear(x, w, bias=dual(b)), lambda: fp8_linear(x, w, residual=dual(r)),
+                     lambda: fp8_linear(x, w, out=dual(r))):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        fp8_linear(torch.autograd.forward_ad.unpack_dual(dual(x)).primal, w)
+    fp8_linear(x, w, bias=b, residual=r)
