@@ -159,6 +159,7 @@ Fp8 fp8(PyObject* data, PyObject* scales, int64_t row_block, const char* what) {
     type_error(std::string(what) + ": data must be a torch.float8_e4m3fn tensor");
   if (!s || s->scalar_type() != at::kFloat8_e8m0fnu || s->layout() != at::kStrided)
     type_error(std::string(what) + ": scales must be a torch.float8_e8m0fnu tensor");
+  if (d->is_neg() || s->is_neg()) type_error(std::string(what) + ": data and scales must not be negated views");
   if (d->dim() != 2 || d->size(1) < 1)
     shape_error(std::string(what) + ": data must be [rows, k] with k >= 1, got " + show(d->sizes()));
   Fp8 r;

@@ -246,3 +246,13 @@ def test_argument_structs_match_the_header(tmp_path):
     subprocess.run(["gcc", "-I", include, str(src), "-o", str(tmp_path / "t")], check=True)
     got = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()
     assert [int(v) for v in got] == [QUANTIZE_ARGS.size, RMS_NORM_ARGS.size, LINEAR_ARGS.size, 0, 1, 2, 1]
+
+
+def test_containers_refuse_negated_views():
+    """A view that stands for the negated values has the values' own bytes."""
+    d, s = fp8(3, 200), scale(3, 2)
+    for cls, dd, ss in ((Fp8Rows, torch._neg_view(d), s), (Fp8Rows, d, torch._neg_view(s)),
+                        (Fp8Weight, torch._neg_view(d), scale(1, 2))):
+        for make in (cls, cls.pack):
+            with pytest.raises(TypeError, match="negat"):
+                make(dd, ss)
