@@ -13,7 +13,8 @@ import os
 import threading
 from typing import Optional
 
-from .build_native import LIB_PATH, TORCH_OPS_PATH
+from . import build_native
+from .build_native import LIB_PATH
 from .errors import ForgeTuneRuntimeError
 
 _lock = threading.Lock()
@@ -94,17 +95,22 @@ def torch_ops():
         with _lock:
             if _ops is None:
                 import torch  # noqa: F401  (its libraries, which the extension links)
-                if not os.path.isfile(TORCH_OPS_PATH):
+                path = build_native.TORCH_OPS_PATH
+                if not os.path.isfile(path):
                     raise ForgeTuneRuntimeError(
-                        "_torch_ops.so is not built (%s); run `python -m forgetune_b200.build_native`"
-                        % TORCH_OPS_PATH)
+                        "_torch_ops.so is not built (%s); run `python -m forgetune_b200.build_native`" % path)
+                built_for, target = build_native.torch_ops_built_for(path), build_native.torch_ops_target()
+                if built_for != target:
+                    raise ForgeTuneRuntimeError(
+                        "%s is built for %s, this is %s; run `python -m forgetune_b200.build_native`"
+                        % (path, built_for, target))
                 try:
-                    spec = importlib.util.spec_from_file_location("_torch_ops", TORCH_OPS_PATH)
+                    spec = importlib.util.spec_from_file_location("_torch_ops", path)
                     module = importlib.util.module_from_spec(spec)
                     spec.loader.exec_module(module)
                 except (ImportError, OSError) as e:
-                    raise ForgeTuneRuntimeError("cannot load %s (built against another torch?): %s"
-                                                % (TORCH_OPS_PATH, e)) from e
+                    raise ForgeTuneRuntimeError("cannot load %s (to build it again: `python -m "
+                                                "forgetune_b200.build_native --force`): %s" % (path, e)) from e
                 _ops = module
     return _ops
 

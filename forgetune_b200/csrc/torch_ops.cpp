@@ -21,6 +21,12 @@
 
 #include "forgetune_b200.h"
 
+#ifndef FTB_TORCH_OPS_TARGET
+#define FTB_TORCH_OPS_TARGET "unknown"
+#endif
+// Read from the file, before it is loaded: the layouts above are compiled in.
+extern "C" __attribute__((used)) const char ftb_torch_ops_built_for[] = "_torch_ops built for: " FTB_TORCH_OPS_TARGET;
+
 namespace {
 
 PyObject* g_shape_error = nullptr;    // forgetune_b200.errors.InvalidShapeError

@@ -12,9 +12,9 @@ host compiler runs per model; the kernels are built once, in-tree.
 from __future__ import annotations
 
 import os
-import shutil
 import subprocess
 
+from . import build_native
 from .build_native import INCLUDE, LIB_DIR, LIB_PATH
 from .errors import CompilationError
 
@@ -206,9 +206,9 @@ def emit_source(blob_path: str, blob_bytes: int, blob_sha: str, dynamic: bool, m
 
 
 def host_compiler() -> str:
-    for c in (os.environ.get("CXX"), shutil.which("g++"), shutil.which("c++"), shutil.which("clang++")):
-        if c:
-            return c
+    c = build_native.host_compiler()
+    if c:
+        return c
     raise CompilationError("no host C++ compiler found (g++, c++ or clang++)")
 
 
