@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from forgetune_b200 import ForgeTuneRuntimeError, _native, fp8_linear, quantize_rows
+from forgetune_b200 import ForgeTuneRuntimeError, _native, fp8_linear, quantize_rows, quantize_weight
 
 from . import fp8_reference as ref
 from .test_fp8_gpu import TYPES, f64, guarded, integers, same
@@ -170,3 +170,29 @@ def test_a_wait_that_ran_out_is_reported_to_one_of_many_threads():
         t.join()
     assert len(told) == 1 and "exceeded its limit" in told[0]
     assert len(right) == 7 and all(right)
+
+
+@pytest.mark.parametrize("nt,split", KERNELS)
+def test_every_kernel_right_behind_what_writes_its_operands(nt, split):
+    """Weights and activations quantised into memory of the ones before, the product launched early behind them
+    (its first weights are sent for before they are written)."""
+    m, n, k = (nt or 256) + 40, 900, 1500
+    xs = [torch.randn(m, k, device="cuda") for _ in range(3)]
+    ws = [torch.randn(n, k, device="cuda") for _ in range(3)]
+    with kernel(nt, split):
+        want = []
+        for x, w in zip(xs, ws):
+            a, b = quantize_rows(x), quantize_weight(w)
+            torch.cuda.synchronize()
+            want.append(fp8_linear(a, b))
+            torch.cuda.synchronize()
+        del a, b
+        places, got = set(), []
+        for i in range(12):
+            a, b = quantize_rows(xs[i % 3]), quantize_weight(ws[i % 3])
+            places.add(b.data.data_ptr())
+            got.append(fp8_linear(a, b))
+            del a, b
+    assert len(places) < 12  # memory is taken again
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 3]), i
