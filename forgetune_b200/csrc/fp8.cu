@@ -193,12 +193,15 @@ struct Fp8Choice {
 };
 
 // Picks by an estimate of the time in microseconds.  A round of the tile
-// kernel's CTAs takes 0.31 per k-block when they wait for their loads, at least
+// kernel's CTAs takes 0.31 per k-block (paid in series: the same with one CTA on
+// the GPU as with many, and with rings of three, four and five stages), at least
 // 0.0097 per KB that an SM's CTAs load, and 0.017 per token of a tile plus
 // 0.013 per token of the SM for its epilogue; each CTA of an SM costs 0.23, a
-// later round 1.3, a cluster 0.4.  (A round is the CTAs resident at once: two
-// per SM, fewer in clusters of 4 and 8, which do not fill the SMs' groups.)  A
-// round of pairs takes 0.29 per k-block and 0.8, and a launch 3.5 more than
+// later round 1.3, a cluster 0.4.  A round is counted as two CTAs per SM, fewer
+// in clusters of 4 and 8, which do not fill the SMs' groups: what registers and
+// shared memory leave room for, but for 16 and 32 tokens unsplit, of which three
+// fit.  There it counts rounds that do not happen: most of the worst picks below
+// take 64 or 128 tokens where 32 unsplit is best.  A round of pairs takes 0.29 per k-block and 0.8, and a launch 3.5 more than
 // the tile kernel's.  The constants are a fit to 525 shapes (m 1..4096, n and
 // k 64..8192) that were timed with every choice on a B200; over 696 others the
 // pick is 1.1 % slower than the best choice in the mean, 28 % at most.  For

@@ -226,10 +226,13 @@ struct Fp8TileSmem {
   static constexpr int W_BYTES = 128 * 128;
   static constexpr int A_BYTES = NT * 128;
   static constexpr int STAGE_BYTES = W_BYTES + A_BYTES;
-  // Three stages of few tokens (two to four CTAs fit on an SM) let the next
-  // launch's CTAs settle in beside the running ones: a chain of norm and two
-  // layers of 4096 x 8192 at 16 tokens takes 20.3 us a layer, with five stages
-  // and no prefetch of weights 22.6.
+  // Three stages of few tokens, and the first weights sent for ahead of the
+  // launch's turn: a chain of norm and two layers of 4096 x 8192 at 16 tokens
+  // takes 20.5 us a layer; with five stages 21.5, without those weights 21.2,
+  // with neither change 22.6.  One product of 16 x 8192 x 4096 with its weights
+  // in HBM: 8.9, 9.4, 9.2 and 9.9.  Registers (118 to 128) hold the split forms
+  // to two CTAs per SM with either ring, so it is not room for a third that the
+  // shorter one gains by; what it is has not been found.
   static constexpr int STAGES = NT == 64 ? 4 : 3;
   static constexpr int SF_SLOTS = 2;
   static constexpr int SF_BYTES = 1024;  // 512 of each operand

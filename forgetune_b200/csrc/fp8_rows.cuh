@@ -6,8 +6,9 @@
 // A lane has a vector of VEC consecutive elements, 16 bytes of input: 8 of a
 // 16-bit type, 4 of fp32.  A quantisation block of 128 is then 16 or 32
 // neighbouring lanes, so its largest value is a few shuffles away.  Rows whose
-// base, stride or length keep them off 16-byte boundaries take the same
-// kernels with element-wise loads and stores.
+// base, stride or length keep them off 16-byte boundaries are quantised by the
+// same kernels with element-wise loads; the norm has kernels of its own for them
+// (rms_norm_elements_kernel and a form of rms_norm_long_kernel).
 #pragma once
 
 #include <algorithm>
@@ -246,7 +247,8 @@ __device__ __forceinline__ void quantize_loaded(const uint4 (&u)[N], At&& at) {
 }
 
 // A row is cut into units of 32 vectors.  Long rows: grid (rows, CTAs per row),
-// a warp takes N units of a row, all in flight together.
+// a warp takes N units of a row, all in flight together.  (The bf16 form in
+// vectors spills 12 bytes at its 64 registers, the bound that four CTAs set.)
 constexpr int kQuantUnits = 4;
 
 template <typename T, RowMode MODE>
@@ -398,7 +400,8 @@ __device__ __forceinline__ void norm_finish(const RowsParams& p, int64_t row, in
 //   h = x + residual (fp32),  y = h / sqrt(mean(h^2) + eps) weight
 // `lanes` threads per row, which keep it in registers: NV vectors per lane.  A
 // row has 8 or 16 lanes of a warp (rows that short), or whole warps; a CTA has
-// one row or several.
+// one row or several.  (The 16-bit forms of four vectors that may end past the
+// row spill 20 bytes at their 64 registers, which 1024 threads allow.)
 template <typename T, RowMode MODE, int NV>
 __global__ void __launch_bounds__(1024) rms_norm_kernel(const RowsParams p, const int lanes) {
   constexpr int VEC = kRowVec<T>;
