@@ -16,6 +16,7 @@ import argparse
 import importlib.util
 import os
 import re
+import shlex
 import shutil
 import subprocess
 import sys
@@ -115,6 +116,10 @@ def torch_ops_lacks() -> Optional[str]:
         return "Python.h"
     if not host_compiler():
         return "a host C++ compiler (g++, c++, clang++ or $CXX)"
+    try:
+        nvcc()
+    except RuntimeError:
+        return "nvcc, beside CUDA's headers"
     return None
 
 
@@ -131,7 +136,10 @@ def _run(cmd, target, verbose) -> None:
     cmd = cmd + ["-o", tmp]
     if verbose:
         print(" ".join(cmd), flush=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError("cannot run %s: %s" % (cmd[0], e)) from e
     if r.returncode != 0:
         raise RuntimeError("%s failed (%d):\n%s\n%s" % (os.path.basename(cmd[0]), r.returncode, r.stdout[-4000:], r.stderr[-8000:]))
     os.utime(tmp, (began, began))
@@ -171,7 +179,9 @@ def _build_torch_ops(verbose) -> None:
     include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     torch_lib = os.path.join(torch_dir, "lib")
-    _run([host_compiler(), "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-shared", "-I", INCLUDE,
+    cxx = host_compiler()
+    cxx = [cxx] if os.path.isfile(cxx) else shlex.split(cxx)  # $CXX may be a command with arguments
+    _run(cxx + ["-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-shared", "-I", INCLUDE,
           '-DFTB_TORCH_OPS_TARGET="%s"' % torch_ops_target()]
          + [a for d in include for a in ("-isystem", d)] + [os.path.join(CSRC, "torch_ops.cpp"), "-L", torch_lib]
          + ["-l" + n for n in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python")]

@@ -31,7 +31,7 @@ def fake_compiler(tmp_path, text):
 
 def test_the_library_alone_where_the_extension_cannot_be_built(elsewhere, monkeypatch, tmp_path):
     real = build_native.sysconfig.get_paths
-    monkeypatch.setattr(build_native.sysconfig, "get_paths", lambda: dict(real(), include=str(tmp_path)))
+    monkeypatch.setattr(build_native.sysconfig, "get_paths", lambda *a, **k: dict(real(*a, **k), include=str(tmp_path)))
     with pytest.warns(UserWarning, match="Python.h"):
         assert build_native.build() == build_native.LIB_PATH
     assert not os.path.exists(elsewhere) and build_native.up_to_date()
@@ -70,3 +70,21 @@ def test_the_extension_in_the_tree_is_for_this_torch():
     assert built_for == build_native.torch_ops_target()
     for part in (str(torch.__version__), torch.version.git_version, sysconfig.get_config_var("SOABI")):
         assert part in built_for
+
+
+def test_a_compiler_with_arguments_and_one_that_is_not_there(elsewhere, monkeypatch, tmp_path):
+    target = build_native.torch_ops_target()
+    cxx = fake_compiler(tmp_path, "_torch_ops built for: %s\0" % target)
+    monkeypatch.setenv("CXX", cxx + " -march=native")
+    build_native.build()
+    assert (tmp_path / "ran").read_text().startswith("-march=native ") and build_native.up_to_date()
+    monkeypatch.setenv("CXX", str(tmp_path / "nowhere"))
+    with pytest.raises(RuntimeError, match="nowhere"):
+        build_native._build_torch_ops(False)
+
+
+def test_no_nvcc_and_the_library_in_place(elsewhere, monkeypatch):
+    monkeypatch.delenv("NVCC", raising=False)
+    monkeypatch.setattr(build_native, "nvcc", lambda: (_ for _ in ()).throw(RuntimeError("nvcc not found")))
+    with pytest.warns(UserWarning, match="nvcc"):
+        assert build_native.build() == build_native.LIB_PATH
