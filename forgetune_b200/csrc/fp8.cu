@@ -206,10 +206,10 @@ struct Fp8Choice {
 // constants are a fit to 525 shapes (m 1..4096, n and k 64..8192) that were
 // timed with every choice on a B200; over 696 others the pick is 1.1 % slower
 // than the best choice in the mean, 28 % at most.  For example (m x k x n): 1 x
-// 4096 x 4096 takes 5.2 us with 16 tokens per tile and split 4, 12.2 unsplit;
-// 512 x 512 x 512 takes 3.5 with 16 tokens, 6.8 with 128; 256 x 4096 x 4096
-// 11.8 with 128 tokens and split 2, 16.9 on pairs; 1024 x 4096 x 4096 17.4 on
-// pairs, 22.6 with 128 tokens.
+// 4096 x 4096 takes 5.0 us with 16 tokens per tile and split 4, 11.8 unsplit;
+// 512 x 512 x 512 takes 3.3 with 16 tokens, 6.9 with 128; 256 x 4096 x 4096
+// 11.9 with 128 tokens and split 2, 15.2 on pairs; 1024 x 4096 x 4096 16.6 on
+// pairs, 22.3 with 128 tokens.
 static Fp8Choice choose_fp8(int64_t m, int64_t n, int64_t k, const Fp8Device& d) {
   static const double kResident[4] = {2.0, 2.0, 1.78, 1.73};  // CTAs per SM in clusters of 1, 2, 4 and 8
   const int64_t nk = fp8_blocks(k), tiles_n = fp8_blocks(n);
