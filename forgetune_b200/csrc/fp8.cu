@@ -6,7 +6,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <exception>
 #include <mutex>
 #include <string>
 
@@ -14,36 +13,21 @@
 #include "fp8_gemm.cuh"
 #include "fp8_pair.cuh"
 #include "fp8_rows.cuh"
+#include "op_common.hpp"
 #include "rms_norm.hpp"
-#include "status.hpp"
 
 namespace ftb {
 
 constexpr int kFp8MaxDevices = 64;
 constexpr int64_t kFp8MaxDim = int64_t(1) << 27;
 
-struct Fp8Device {
-  std::mutex mu;
-  std::atomic<bool> ready{false};
-  int sm_count = 0;
-  int pairs = 0;  // SM pairs resident at once
-  // set by a kernel whose bounded wait gave up: mapped host memory, so the
-  // next call reads it without a copy
-  volatile int* fault = nullptr;
-  int* fault_dev = nullptr;
-};
-static Fp8Device g_fp8_devices[kFp8MaxDevices];
+static OpDevice g_fp8_devices[kFp8MaxDevices];
 static std::atomic<int> g_fp8_stall{0};  // failure-detection hook
 static std::atomic<int> g_fp8_kernel{-1};  // kernel hook: 16 nt + split, or -1 for the estimate's choice
 
-static int refuse(const char* fn, const std::string& why, int status = ST_INPUT) {
-  set_error(std::string(fn) + ": " + why);
-  return status;
-}
-
 // Once per device; "" when done.  Allocates a word and sets kernel attributes,
 // in relaxed capture mode, so that a stream under capture does not matter.
-static std::string fp8_setup(int dev, Fp8Device* d) {
+static std::string fp8_setup(int dev, OpDevice* d) {
   int major = 0;
   cudaError_t e = cudaDeviceGetAttribute(&d->sm_count, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
@@ -78,9 +62,7 @@ static std::string fp8_setup(int dev, Fp8Device* d) {
   return std::string("set-up failed: ") + cudaGetErrorString(e);
 }
 
-// The current device's state, set up by the first call on it (a set-up that
-// fails is tried again by the next).
-static int fp8_device(const char* fn, Fp8Device** out) {
+int op_device(const char* fn, OpDevice** out) {
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) {
@@ -88,7 +70,7 @@ static int fp8_device(const char* fn, Fp8Device** out) {
     return refuse(fn, cudaGetErrorString(e), ST_DEVICE);
   }
   if (dev < 0 || dev >= kFp8MaxDevices) return refuse(fn, "device ordinal beyond the supported range", ST_CONFIG);
-  Fp8Device& d = g_fp8_devices[dev];
+  OpDevice& d = g_fp8_devices[dev];
   if (!d.ready.load(std::memory_order_acquire)) {
     std::lock_guard<std::mutex> lock(d.mu);
     if (!d.ready.load(std::memory_order_relaxed)) {
@@ -106,61 +88,11 @@ static int fp8_device(const char* fn, Fp8Device** out) {
   return ST_OK;
 }
 
-static bool is_plain(int64_t type) { return type == FTB_F32 || type == FTB_F16 || type == FTB_BF16; }
-static bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
-// Rows of `cols` elements `ld` apart: enough room, and the alignment of the
-// element type (plain) or of the copy engine (quantised).  "" when fine.
-static std::string check(const char* what, const ftb_matrix& x, int64_t cols) {
-  if (!is_plain(x.type)) return std::string(what) + " must be float32, float16 or bfloat16";
-  if (!aligned(x.data, x.type == FTB_F32 ? 4 : 2)) return std::string(what) + " is not aligned to its type";
-  if (x.ld < cols) return std::string(what) + " rows overlap (stride below the row length)";
-  return "";
-}
 static std::string check(const char* what, const ftb_fp8_matrix& q, int64_t cols) {
   if (!aligned(q.data, 16) || q.ld % 16 || q.ld < cols)
     return std::string(what) + " values need 16-byte aligned rows (base and stride) of at least their length";
   if (!aligned(q.scales, 4) || q.scales_ld % 4 || q.scales_ld < fp8_blocks(cols))
     return std::string(what) + " scales need 4-byte aligned rows (base and stride) of at least their length";
-  return "";
-}
-// Base and rows on 16-byte boundaries.
-static bool rows_aligned(const ftb_matrix& x) {
-  return aligned(x.data, 16) && (x.ld * (x.type == FTB_F32 ? 4 : 2)) % 16 == 0;
-}
-// Bytes of a matrix in memory: rows `ld` bytes apart.
-struct Span {
-  const char* p;
-  int64_t rows, bytes, ld;
-  int64_t end() const { return (rows - 1) * ld + bytes; }
-};
-static Span span(const ftb_matrix& x, int64_t m, int64_t n) {
-  const int64_t size = x.type == FTB_F32 ? 4 : 2;
-  return {static_cast<const char*>(x.data), m, n * size, x.ld * size};
-}
-static Span span(const void* p, int64_t rows, int64_t bytes, int64_t ld) {
-  return {static_cast<const char*>(p), rows, bytes, ld};
-}
-static bool overlap(const Span& a, const Span& b) {
-  if (!a.p || !b.p || a.rows < 1 || b.rows < 1 || a.p + a.end() <= b.p || b.p + b.end() <= a.p) return false;
-  if (a.rows == 1 && b.rows == 1) return true;  // their ranges meet (a vector's span has no stride)
-  const int64_t ld = a.rows > 1 ? a.ld : b.ld;
-  if ((a.rows > 1 && a.ld != ld) || (b.rows > 1 && b.ld != ld)) return true;  // not worth telling apart
-  const int64_t d = ((b.p - a.p) % ld + ld) % ld;  // b's columns in a's rows
-  return !(d >= a.bytes && d + b.bytes <= ld);
-}
-static bool same(const Span& a, const Span& b) {
-  return a.p == b.p && a.rows == b.rows && a.bytes == b.bytes && (a.rows <= 1 || a.ld == b.ld);
-}
-// An output that shares memory with an operand, unless it is that operand in
-// place: "" or why not.
-template <size_t N>
-static std::string clashes(const char* what, const Span& out, const Span (&in)[N], const Span* in_place = nullptr,
-                           const Span* in_place2 = nullptr) {
-  for (const Span& x : in)
-    if (overlap(out, x) && !(in_place && same(out, x) && same(*in_place, x)) &&
-        !(in_place2 && same(out, x) && same(*in_place2, x)))
-      return std::string(what) + " overlaps an operand";
   return "";
 }
 
@@ -178,12 +110,6 @@ static std::string clashes(const char* what, const ftb_fp8_matrix& q, int64_t m,
 
 static bool sizes_ok(int64_t m, int64_t n, int64_t k) {
   return m >= 0 && m <= kFp8MaxDim && n >= 1 && n <= kFp8MaxDim && k >= 1 && k <= kFp8MaxDim;
-}
-
-static int launched(const char* fn, cudaError_t e) {
-  if (e == cudaSuccess) return ST_OK;
-  cudaGetLastError();
-  return refuse(fn, std::string("launch failed: ") + cudaGetErrorString(e), ST_DEVICE);
 }
 
 // The kernel for a product: the tile kernel with NT tokens per tile and a
@@ -210,7 +136,7 @@ struct Fp8Choice {
 // 512 x 512 x 512 takes 3.3 with 16 tokens, 6.9 with 128; 256 x 4096 x 4096
 // 11.9 with 128 tokens and split 2, 15.2 on pairs; 1024 x 4096 x 4096 16.6 on
 // pairs, 22.3 with 128 tokens.
-static Fp8Choice choose_fp8(int64_t m, int64_t n, int64_t k, const Fp8Device& d) {
+static Fp8Choice choose_fp8(int64_t m, int64_t n, int64_t k, const OpDevice& d) {
   static const double kResident[4] = {2.0, 2.0, 1.78, 1.73};  // CTAs per SM in clusters of 1, 2, 4 and 8
   const int64_t nk = fp8_blocks(k), tiles_n = fp8_blocks(n);
   const double pair_tiles = (double)((m + 255) / 256) * (double)((n + 255) / 256);
@@ -236,7 +162,7 @@ static Fp8Choice choose_fp8(int64_t m, int64_t n, int64_t k, const Fp8Device& d)
   return best;
 }
 
-static cudaError_t launch_fp8_linear(const Fp8Operands& o, const Fp8Params& p, const Fp8Device& d, cudaStream_t s) {
+static cudaError_t launch_fp8_linear(const Fp8Operands& o, const Fp8Params& p, const OpDevice& d, cudaStream_t s) {
   const int set = g_fp8_kernel.load(std::memory_order_relaxed);
   const Fp8Choice c = set < 0 ? choose_fp8(p.M, p.N, p.K, d) : Fp8Choice{set / 16, set % 16};
   switch (c.nt) {
@@ -245,21 +171,6 @@ static cudaError_t launch_fp8_linear(const Fp8Operands& o, const Fp8Params& p, c
     case 64: return launch_fp8_tile<64>(o, p, c.split, s);
     case 128: return launch_fp8_tile<128>(o, p, c.split, s);
     default: return launch_fp8_pair(o, p, d.pairs, s);
-  }
-}
-
-template <typename F>
-static int guarded(const char* fn, F&& body) noexcept {
-  try {
-    return body();
-  } catch (const std::exception& e) {
-    try {
-      return refuse(fn, e.what(), ST_ALLOC);
-    } catch (...) {
-      return ST_ALLOC;
-    }
-  } catch (...) {
-    return ST_ALLOC;
   }
 }
 
@@ -294,8 +205,8 @@ FTB_API int ftb_quantize_rows(const ftb_quantize_args* args, void* stream) {
     const Span in[1] = {span(a.x, a.m, a.k)};
     if (why.empty()) why = clashes("q", a.q, a.m, a.m, a.k, in);
     if (!why.empty()) return refuse(fn, why);
-    Fp8Device* d = nullptr;
-    if (const int rc = fp8_device(fn, &d)) return rc;
+    OpDevice* d = nullptr;
+    if (const int rc = op_device(fn, &d)) return rc;
     RowsParams p{};
     p.x = a.x.data;
     p.x_ld = a.x.ld;
@@ -323,8 +234,8 @@ FTB_API int ftb_quantize_weight(const ftb_quantize_args* args, void* stream) {
     const Span in[1] = {span(a.x, a.m, a.k)};
     if (why.empty()) why = clashes("q", a.q, a.m, fp8_blocks(a.m), a.k, in);
     if (!why.empty()) return refuse(fn, why);
-    Fp8Device* d = nullptr;
-    if (const int rc = fp8_device(fn, &d)) return rc;
+    OpDevice* d = nullptr;
+    if (const int rc = op_device(fn, &d)) return rc;
     RowsParams p{};
     p.x = a.x.data;
     p.x_ld = a.x.ld;
@@ -367,8 +278,8 @@ FTB_API int ftb_rms_norm(const ftb_rms_norm_args* args, void* stream) {
     if (why.empty() && a.y.data && overlap(span(a.y, a.m, a.k), h)) why = "y overlaps h";
     if (why.empty() && a.q.data) why = clashes("q", a.q, a.m, a.m, a.k, more);
     if (!why.empty()) return refuse(fn, why);
-    Fp8Device* d = nullptr;
-    if (const int rc = fp8_device(fn, &d)) return rc;
+    OpDevice* d = nullptr;
+    if (const int rc = op_device(fn, &d)) return rc;
     RowsParams p{};
     p.x = a.x.data;
     p.x_ld = a.x.ld;
@@ -419,8 +330,8 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
       why = clashes("y", span(a.y, a.m, a.n), in, a.residual.type == a.y.type ? &r : nullptr);
     if (why.empty() && a.q.data) why = clashes("q", a.q, a.m, a.m, a.n, in);
     if (!why.empty()) return refuse(fn, why);
-    Fp8Device* d = nullptr;
-    if (const int rc = fp8_device(fn, &d)) return rc;
+    OpDevice* d = nullptr;
+    if (const int rc = op_device(fn, &d)) return rc;
     Fp8Operands o{a.a.data, a.a.ld, a.w.data, a.w.ld};
     Fp8Params p{};
     p.M = (int)a.m;
