@@ -60,6 +60,11 @@ _SIGS = {
     "ftb_fp8_linear": ([c_void_p, c_void_p], c_int),
     "ftb_fp8_set_fault_injection": ([c_int], c_int),
     "ftb_fp8_set_kernel": ([c_int, c_int], c_int),
+    "ftb_rotate_heads": ([c_void_p, c_void_p], c_int),
+    "ftb_append_heads": ([c_void_p, c_void_p], c_int),
+    "ftb_paged_attention": ([c_void_p, c_void_p], c_int),
+    "ftb_paged_attention_workspace": ([c_void_p], c_int64),
+    "ftb_token_logprobs": ([c_void_p, c_void_p], c_int),
 }
 
 EXPORTED = sorted(_SIGS)
@@ -88,7 +93,7 @@ def lib() -> ctypes.CDLL:
 
 
 def torch_ops():
-    """The extension module behind fp8.py (csrc/torch_ops.cpp), loaded once."""
+    """The extension module behind fp8.py and decoder.py (csrc/torch_ops.cpp), loaded once."""
     global _ops
     if _ops is None:
         lib()  # the extension links the engine library

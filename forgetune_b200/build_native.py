@@ -35,7 +35,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libforgetune_b200.so")
 TORCH_OPS_PATH = os.path.join(LIB_DIR, "_torch_ops.so")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 
-SOURCES = ["runtime.cu", "fp8.cu", "engine.cpp"]
+SOURCES = ["runtime.cu", "fp8.cu", "decoder.cu", "engine.cpp"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -173,7 +173,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 def _build_torch_ops(verbose) -> None:
-    """The CPython extension behind fp8.py, against the installed torch and the engine library."""
+    """The CPython extension behind fp8.py and decoder.py, against the installed torch and the engine library."""
     torch_dir = _torch_dir()
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),

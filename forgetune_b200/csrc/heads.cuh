@@ -1,0 +1,298 @@
+// Heads of queries and keys turned by their tokens' positions, normalised
+// first where asked, and keys and values stored into a paged cache.
+//
+//   n = x / sqrt(mean(x^2) + eps) w          over the head (or n = x)
+//   a_i = position f_i,  c_i = A cos a_i,  s_i = A sin a_i
+//   y_i = n_i c_i - n_j s_i,  y_j = n_j c_i + n_i s_i
+//
+// with pairs (i, j) = (i, i + r/2), or (2 i, 2 i + 1) where interleaved, over
+// the first r elements of the head; the rest of it is n.  Angles are formed in
+// 64 bits, reduced to a fraction of a turn there and passed on in 32: an angle
+// of a million radians is then as exact as one of one radian.  The sum of
+// squares, the norm and the rotation are fp32, and a value is rounded once.
+//
+// Bound by the bytes of x and y.  A lane holds V pairs of a head (two pieces
+// of V elements: either side of the half, or side by side where interleaved),
+// so no value crosses lanes but the sum of squares; LPH lanes share a head.  A
+// block takes HB heads per group of LPH lanes, loads them all, finds its
+// tokens' sequences and makes their cosines meanwhile, once per token for all
+// of its heads.
+#pragma once
+
+#include <algorithm>
+#include <cstring>
+
+#include "fp8_format.cuh"
+#include "tc_ptx.cuh"
+
+namespace ftb {
+
+constexpr int kHeadsThreads = 256;
+constexpr int kHeadsMaxDim = 512;
+
+// New tokens of several sequences and the pages that hold them.
+struct PagedBatchParams {
+  const int* page_table;  // [seqs, most_pages], rows table_ld apart
+  int64_t table_ld;
+  const int* starts;      // [seqs + 1] first row of each sequence
+  const int* lengths;     // [seqs] tokens with the new ones
+  int seqs, most_pages, page_size, pages;
+};
+
+// Number of entries <= t among starts[0 .. n), by a whole warp (32 blocks a step).
+__device__ __forceinline__ int count_not_above(const int* starts, int n, int t, int lane) {
+  int lo = 0;
+  while (n > 0) {
+    const int step = (n + 31) >> 5, i = lo + (lane + 1) * step - 1;
+    const int c = __popc(__ballot_sync(0xffffffffu, (lane + 1) * (int64_t)step <= n && starts[i] <= t));
+    lo += c * step;
+    n = min(step, n - c * step);
+    if (step == 1) break;
+  }
+  return lo;
+}
+
+// Sequence and position of row t; false where it belongs to none.
+__device__ __forceinline__ bool place_of(const PagedBatchParams& b, int t, int lane, int* seq, int64_t* position) {
+  const int s = count_not_above(b.starts, b.seqs + 1, t, lane) - 1;
+  *seq = s;
+  if (s < 0 || s >= b.seqs) return false;
+  *position = (int64_t)b.lengths[s] - b.starts[s + 1] + t;
+  return true;
+}
+
+struct HeadsParams {
+  const void* x[3];  // q, k, v [tokens, heads, dim]
+  int64_t x_token[3], x_head[3];
+  int heads[3];
+  void* y[3];        // q's output; the pool of keys, of values
+  int64_t y_token[3], y_head[3], y_page[3];
+  const float* weight[2];
+  float eps;
+  int norm;
+  const double* frequencies;
+  int pairs;         // r / 2
+  double amplitude;
+  int interleaved;
+  int tokens, dim;
+  const void* positions;  // of each token, or null: from the batch
+  int positions64;
+  PagedBatchParams batch;
+  int units, lanes;       // units of V pairs in a head, lanes that share them
+  int per_block;          // heads of a token that a block takes
+  int tokens_per_block, blocks_per_token;
+};
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Piece {
+  T v[V];
+};
+
+// One of the two pieces of unit u: its first element.
+template <int V>
+__device__ __forceinline__ void unit_at(const HeadsParams& p, int u, int* a, int* b) {
+  const int turned = p.pairs / V;
+  if (u >= turned) {
+    *a = 2 * p.pairs + (u - turned) * 2 * V;
+    *b = *a + V;
+  } else if (p.interleaved) {
+    *a = 2 * u * V;
+    *b = *a + V;
+  } else {
+    *a = u * V;
+    *b = *a + p.pairs;
+  }
+}
+
+template <typename T, typename O, int V, int UPL, int HB>
+__global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const HeadsParams p) {
+  extern __shared__ float2 turn[];  // [tokens of the block][pairs]
+  __shared__ int64_t where[64];     // position of a token
+  __shared__ int page_of[64];       // its page; -1: no place in the pool, -2: no sequence
+  grid_dep_wait();
+  grid_dep_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = (int)(blockIdx.x / p.blocks_per_token) * p.tokens_per_block;
+  const int h0 = (int)(blockIdx.x % p.blocks_per_token) * p.per_block;
+  const int all = p.heads[0] + p.heads[1] + p.heads[2];
+  const int group = threadIdx.x / p.lanes, groups = kHeadsThreads / p.lanes, l = threadIdx.x % p.lanes;
+
+  Piece<T, V> in[HB][UPL][2];
+  int tok[HB], kind[HB], head[HB];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    const int flat = i * groups + group;
+    tok[i] = flat / p.per_block;
+    int h = h0 + flat % p.per_block;
+    kind[i] = tok[i] < p.tokens_per_block && t0 + tok[i] < p.tokens && h < all ? 0 : -1;
+    if (kind[i] == 0 && h >= p.heads[0]) {
+      h -= p.heads[0];
+      kind[i] = 1;
+      if (h >= p.heads[1]) {
+        h -= p.heads[1];
+        kind[i] = 2;
+      }
+    }
+    head[i] = h;
+    const int k = max(kind[i], 0);
+    const T* x = static_cast<const T*>(p.x[k]) + (int64_t)(t0 + tok[i]) * p.x_token[k] + h * p.x_head[k];
+#pragma unroll
+    for (int j = 0; j < UPL; ++j) {
+      const int u = l + j * p.lanes;
+      int a, b;
+      unit_at<V>(p, u, &a, &b);
+      memset(&in[i][j], 0, sizeof(in[i][j]));
+      if (kind[i] >= 0 && u < p.units) {
+        in[i][j][0] = *reinterpret_cast<const Piece<T, V>*>(x + a);
+        if (b < p.dim) in[i][j][1] = *reinterpret_cast<const Piece<T, V>*>(x + b);
+      }
+    }
+  }
+
+  for (int i = warp; i < p.tokens_per_block; i += kHeadsThreads / 32) {
+    const int t = t0 + i;
+    int64_t position = 0;
+    int page = -2;
+    if (t < p.tokens) {
+      if (p.positions) {
+        position = p.positions64 ? static_cast<const int64_t*>(p.positions)[t] : static_cast<const int*>(p.positions)[t];
+        page = -1;
+      } else {
+        int seq;
+        if (place_of(p.batch, t, lane, &seq, &position)) {
+          const int64_t n = position >= 0 ? position / p.batch.page_size : p.batch.most_pages;
+          page = n < p.batch.most_pages ? p.batch.page_table[seq * p.batch.table_ld + n] : -1;
+          if (page < 0 || page >= p.batch.pages) page = -1;
+        }
+      }
+    }
+    if (lane == 0) {
+      where[i] = position;
+      page_of[i] = page;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.tokens_per_block * p.pairs; i += kHeadsThreads) {
+    // a / 2 pi in turns; what is left of whole turns is at most half a turn
+    double a = (double)where[i / p.pairs] * p.frequencies[i % p.pairs] * 0.15915494309189535;
+    a -= rint(a);
+    float s, c;
+    sincospif((float)(2.0 * a), &s, &c);
+    turn[i] = make_float2((float)(p.amplitude * c), (float)(p.amplitude * s));
+  }
+  __syncthreads();
+
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    float v[UPL][2][V];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < UPL; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          v[j][s][e] = to_f32(in[i][j][s].v[e]);
+          sum = __fmaf_rn(v[j][s][e], v[j][s][e], sum);
+        }
+    if (p.norm) {  // whole warps: lanes of other kinds take part
+      for (int d = p.lanes >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    }
+    const int k = kind[i];
+    if (k < 0) continue;
+    const int page = page_of[tok[i]];
+    if (page == -2 || (k > 0 && page < 0)) continue;
+    const float r = p.norm ? 1.0f / sqrtf(sum / (float)p.dim + p.eps) : 1.0f;
+    const float* w = k < 2 ? p.weight[k] : nullptr;
+    O* y = static_cast<O*>(p.y[k]) + head[i] * p.y_head[k];
+    y += k == 0 ? (int64_t)(t0 + tok[i]) * p.y_token[0]
+                : (int64_t)page * p.y_page[k] + where[tok[i]] % p.batch.page_size * p.y_token[k];
+    const float2* cs = turn + tok[i] * p.pairs;
+#pragma unroll
+    for (int j = 0; j < UPL; ++j) {
+      const int u = l + j * p.lanes;
+      if (u >= p.units) continue;
+      int a, b;
+      unit_at<V>(p, u, &a, &b);
+      if (k < 2 && p.norm) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          v[j][0][e] *= r;
+          v[j][1][e] *= r;
+          if (w) {
+            v[j][0][e] *= w[a + e];
+            if (b + e < p.dim) v[j][1][e] *= w[b + e];
+          }
+        }
+      }
+      if (k < 2 && u < p.pairs / V) {
+        if (p.interleaved && V > 1) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {  // pair e of the unit: elements 2 e and 2 e + 1 of the two pieces
+            float& m = v[j][2 * e / V][2 * e % V];
+            float& n = v[j][2 * e / V][2 * e % V + 1 < V ? 2 * e % V + 1 : 0];
+            const float2 q = cs[u * V + e];
+            const float z = __fmaf_rn(m, q.x, -__fmul_rn(n, q.y));
+            n = __fmaf_rn(n, q.x, __fmul_rn(m, q.y));
+            m = z;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float2 q = cs[u * V + e];
+            const float m = v[j][0][e], n = v[j][1][e];
+            v[j][0][e] = __fmaf_rn(m, q.x, -__fmul_rn(n, q.y));
+            v[j][1][e] = __fmaf_rn(n, q.x, __fmul_rn(m, q.y));
+          }
+        }
+      }
+      Piece<O, V> out[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[s].v[e] = from_f32<O>(v[j][s][e]);
+      *reinterpret_cast<Piece<O, V>*>(y + a) = out[0];
+      if (b < p.dim) *reinterpret_cast<Piece<O, V>*>(y + b) = out[1];
+    }
+  }
+}
+
+template <typename T, typename O, int V, int UPL, int HB>
+cudaError_t launch_heads_as(HeadsParams p, cudaStream_t s) {
+  p.units = p.pairs / V + (p.dim - 2 * p.pairs + 2 * V - 1) / (2 * V);
+  p.lanes = 1;
+  while (p.lanes < 32 && p.lanes < p.units) p.lanes *= 2;
+  const int slots = kHeadsThreads / p.lanes * HB, all = p.heads[0] + p.heads[1] + p.heads[2];
+  p.per_block = std::min(all, slots);
+  p.blocks_per_token = (all + slots - 1) / slots;
+  // tokens that share a block, their cosines in at most 16 KB
+  p.tokens_per_block = std::max(1, std::min({slots / p.per_block, 64, p.pairs ? 2048 / p.pairs : 64, p.tokens}));
+  const int64_t blocks = ((int64_t)p.tokens + p.tokens_per_block - 1) / p.tokens_per_block * p.blocks_per_token;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  return pdl_launch(heads_kernel<T, O, V, UPL, HB>, dim3((unsigned)blocks), dim3(kHeadsThreads),
+                    (size_t)p.tokens_per_block * p.pairs * sizeof(float2), s, p);
+}
+
+// `vec`: every base and stride is a multiple of four elements.  Vectors also
+// need dim and r in multiples of eight; four heads per lane group are loaded at
+// once where that leaves blocks for all SMs.
+template <typename T, typename O>
+cudaError_t launch_heads_types(const HeadsParams& p, bool vec, int sm_count, cudaStream_t s) {
+  if (!vec || p.dim % 8 || p.pairs % 4) return launch_heads_as<T, O, 1, 8, 1>(p, s);
+  if (p.dim > 256) return launch_heads_as<T, O, 4, 2, 1>(p, s);
+  const int64_t all = (int64_t)p.tokens * (p.heads[0] + p.heads[1] + p.heads[2]);
+  if (all * p.dim < (int64_t)sm_count * kHeadsThreads * 8 * 4) return launch_heads_as<T, O, 4, 1, 1>(p, s);
+  return launch_heads_as<T, O, 4, 1, 4>(p, s);
+}
+
+inline cudaError_t launch_heads(const HeadsParams& p, int in, int out, bool vec, int sm_count, cudaStream_t s) {
+  if (in == FTB_F32) {
+    if (out == FTB_F32) return launch_heads_types<float, float>(p, vec, sm_count, s);
+    if (out == FTB_F16) return launch_heads_types<float, __half>(p, vec, sm_count, s);
+    return launch_heads_types<float, __nv_bfloat16>(p, vec, sm_count, s);
+  }
+  if (in == FTB_F16) return launch_heads_types<__half, __half>(p, vec, sm_count, s);
+  return launch_heads_types<__nv_bfloat16, __nv_bfloat16>(p, vec, sm_count, s);
+}
+
+}  // namespace ftb

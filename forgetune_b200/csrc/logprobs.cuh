@@ -1,0 +1,380 @@
+// Log probabilities of given tokens, the entropy of the distribution and its
+// top alternatives, from rows of logits.
+//
+//   L = log sum_i exp(x_i),  logprob = x_token - L,  H = -sum_i p_i log p_i = L - sum_i p_i x_i
+//
+// in one pass over the row: with the running maximum m, s = sum exp(x - m) and
+// t = sum exp(x - m) (x - m); when m grows by d, s and t become s e^-d and
+// (t - s d) e^-d.  Then L = m + log s and H = log s - t / s.
+//
+// The alternatives come from the same pass.  The maxima of 256 disjoint parts
+// of the row are values of the row, so the k-th largest of them is at most the
+// k-th largest value: only threads whose own maximum reaches it can hold one
+// of the top k, and only their vectors are read again (from L2), by whole
+// warps.  What reaches the bound is ordered by value and, where equal, by
+// index, as one 64-bit number, and ranked by counting.  Where too many values
+// reach it (many equal ones), a bisection over the values finds the k-th.
+//
+// Bound by the logits' bytes, read once.  A block takes a row; of few rows a
+// cluster of up to eight blocks takes one, and the first joins their sums and
+// lists over distributed shared memory.
+#pragma once
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <cstring>
+
+#include "fp8_format.cuh"
+#include "tc_ptx.cuh"
+
+namespace ftb {
+
+constexpr int kLogprobsThreads = 512;
+constexpr int kLogprobsParts = kLogprobsThreads / 2;
+constexpr int kLogprobsMaxTop = 64;
+constexpr int kLogprobsCandidates = 1024;
+
+struct LogprobsParams {
+  const void* x;  // [m, n], rows ld apart
+  int64_t ld;
+  int m, n, top;
+  const void* tokens;
+  int tokens64;
+  int64_t token_stride;
+  float *logprobs, *entropy;
+  float* top_values;     // [m, top]
+  int64_t* top_tokens;
+};
+
+// Values in their order as whole numbers: zeros alike, NaN below all others.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0u;
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0u) return __uint_as_float(0x7FC00000u);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Running sums of a part of a row; m stays finite from below.
+struct RowSums {
+  float m, s, t;
+  __device__ __forceinline__ void raise(float top) {
+    const float d = m - top;  // <= 0
+    const float f = ex2(d * 1.4426950408889634f);
+    t = __fmaf_rn(s, fmaxf(d, -1e4f), t) * f;
+    s *= f;
+    m = top;
+  }
+  __device__ __forceinline__ void add(const RowSums& o) {
+    RowSums b = o;
+    const float top = fmaxf(m, b.m);
+    raise(top);
+    b.raise(top);
+    s += b.s;
+    t += b.t;
+  }
+};
+
+template <typename T>
+struct RowVectors {
+  static constexpr int W = 16 / (int)sizeof(T);
+  const T* row;
+  int n, off, count;  // the row starts `off` elements into its first vector
+  __device__ __forceinline__ RowVectors(const T* r, int size) : row(r), n(size) {
+    off = (int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
+    count = (n + off + W - 1) / W;
+  }
+  __device__ __forceinline__ int first(int v) const { return v * W - off; }
+  __device__ __forceinline__ bool whole(int v) const { return first(v) >= 0 && first(v) + W <= n; }
+  // Vector v; what lies outside of the row reads as -inf.
+  __device__ __forceinline__ uint4 load(int v) const {
+    const int e = first(v);
+    if (whole(v)) return __ldg(reinterpret_cast<const uint4*>(row + e));
+    T t[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) t[i] = e + i >= 0 && e + i < n ? row[e + i] : from_f32<T>(-INFINITY);
+    uint4 u;
+    memcpy(&u, t, 16);
+    return u;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& u, float* f) {
+  constexpr int W = 16 / (int)sizeof(T);
+  T t[W];
+  memcpy(t, &u, 16);
+#pragma unroll
+  for (int i = 0; i < W; ++i) f[i] = to_f32(t[i]);
+}
+
+struct LogprobsSmem {
+  unsigned long long found[kLogprobsCandidates];
+  unsigned long long best[kLogprobsMaxTop];  // in order
+  uint32_t part[kLogprobsParts];
+  RowSums sums[kLogprobsThreads / 32];
+  RowSums total;
+  int count, best_count;
+  uint32_t bound;
+};
+
+// The k-th largest key of vectors [v0, v1) by bisection, then what is above it
+// and, in order of index, of what equals it as much as is wanted.  All threads.
+template <typename T>
+__device__ __noinline__ void find_by_bisection(const RowVectors<T>& r, int v0, int v1, int k, LogprobsSmem& sm) {
+  constexpr int W = RowVectors<T>::W;
+  uint32_t lo = 0;  // at least k keys are >= lo
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t mid = lo | (1u << bit);
+    __syncthreads();
+    if (threadIdx.x == 0) sm.count = 0;
+    __syncthreads();
+    int c = 0;
+    for (int v = v0 + threadIdx.x; v < v1; v += kLogprobsThreads) {
+      float f[W];
+      unpack<T>(r.load(v), f);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const int e = r.first(v) + i;
+        c += e >= 0 && e < r.n && order_key(f[i]) >= mid;
+      }
+    }
+    c = __reduce_add_sync(0xffffffffu, c);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&sm.count, c);
+    __syncthreads();
+    if (sm.count >= k) lo = mid;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sm.count = 0;
+  __syncthreads();
+  for (int v = v0 + threadIdx.x; v < v1; v += kLogprobsThreads) {
+    float f[W];
+    unpack<T>(r.load(v), f);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int e = r.first(v) + i;
+      const uint32_t key = order_key(f[i]);
+      if (e >= 0 && e < r.n && key > lo)
+        sm.found[atomicAdd(&sm.count, 1)] = (unsigned long long)key << 32 | (0xFFFFFFFFu - (uint32_t)e);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int have = sm.count;
+    const int e0 = max(0, r.first(v0)), e1 = min(r.n, r.first(v1));
+    for (int e = e0; e < e1 && have < k; e += 32) {
+      const int i = e + (int)threadIdx.x;
+      const bool hit = i < e1 && order_key(to_f32(r.row[i])) == lo;
+      const uint32_t mask = __ballot_sync(0xffffffffu, hit);
+      const int at = have + __popc(mask & ((1u << threadIdx.x) - 1u));
+      if (hit && at < k) sm.found[at] = (unsigned long long)lo << 32 | (0xFFFFFFFFu - (uint32_t)i);
+      have = min(k, have + __popc(mask));
+    }
+    __syncwarp();
+    if (threadIdx.x == 0) sm.count = have;
+  }
+  __syncthreads();
+}
+
+// The k largest of found[0 .. count) into best, in order.  All threads.
+__device__ __forceinline__ void rank_found(LogprobsSmem& sm, int k) {
+  const int count = sm.count;
+  for (int i = threadIdx.x; i < count; i += kLogprobsThreads) {
+    const unsigned long long mine = sm.found[i];
+    int rank = 0;
+    for (int j = 0; j < count; ++j) rank += sm.found[j] > mine;
+    if (rank < k) sm.best[rank] = mine;
+  }
+  if (threadIdx.x == 0) sm.best_count = min(k, count);
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLogprobsThreads, 2) logprobs_kernel(const LogprobsParams p, const int split) {
+  constexpr int W = RowVectors<T>::W, U = 4;
+  __shared__ LogprobsSmem sm;
+  grid_dep_wait();
+  grid_dep_trigger();
+  const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = (int)(blockIdx.x / split), rank = (int)(blockIdx.x % split);
+  const RowVectors<T> r(static_cast<const T*>(p.x) + row * p.ld, p.n);
+  const int v0 = (int)((int64_t)r.count * rank / split), v1 = (int)((int64_t)r.count * (rank + 1) / split);
+
+  RowSums a{-FLT_MAX, 0.0f, 0.0f};
+  float top = -INFINITY;
+  for (int v = v0 + tid; v < v1; v += U * kLogprobsThreads) {
+    uint4 u[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float none = -INFINITY;
+      T t[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) t[k] = from_f32<T>(none);
+      memcpy(&u[i], t, 16);
+      if (v + i * kLogprobsThreads < v1) u[i] = r.load(v + i * kLogprobsThreads);
+    }
+    float f[U][W], high = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      unpack<T>(u[i], f[i]);
+#pragma unroll
+      for (int k = 0; k < W; ++k) high = fmaxf(high, f[i][k]);
+    }
+    top = fmaxf(top, high);
+    if (high > a.m) a.raise(high);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const float d = f[i][k] - a.m, e = ex2(d * 1.4426950408889634f);
+        a.s += e;
+        a.t = __fmaf_rn(e, fmaxf(d, -1e4f), a.t);  // 0 for -inf
+      }
+  }
+  const uint32_t mine = v0 + tid < v1 ? order_key(top) : 0u;
+
+  for (int d = 16; d > 0; d >>= 1) {
+    RowSums b{__shfl_xor_sync(0xffffffffu, a.m, d), __shfl_xor_sync(0xffffffffu, a.s, d),
+              __shfl_xor_sync(0xffffffffu, a.t, d)};
+    a.add(b);
+  }
+  if (lane == 0) sm.sums[warp] = a;
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+  if (!(tid & 1)) sm.part[tid >> 1] = max(mine, other);
+  if (tid == 0) sm.count = 0;
+  __syncthreads();
+  if (tid == 0) {
+    RowSums all = sm.sums[0];
+    for (int w = 1; w < kLogprobsThreads / 32; ++w) all.add(sm.sums[w]);
+    sm.total = all;
+  }
+  const int e0 = max(0, r.first(v0)), e1 = min(p.n, r.first(v1)), k = min(p.top, e1 - e0);
+  if (p.top > 0) {
+    if (k > 0) {
+      if (tid < kLogprobsParts) {
+        const uint32_t key = sm.part[tid];
+        int above = 0;
+        for (int j = 0; j < kLogprobsParts; ++j) above += sm.part[j] > key || (sm.part[j] == key && j < tid);
+        if (above == k - 1) sm.bound = key;
+      }
+      __syncthreads();
+      const uint32_t bound = sm.bound;
+      uint32_t todo = __ballot_sync(0xffffffffu, v0 + tid < v1 && mine >= bound);
+      while (todo) {
+        const int t = (warp << 5) + __ffs(todo) - 1;
+        todo &= todo - 1;
+        for (int v = v0 + t + lane * kLogprobsThreads; v < v1; v += 32 * kLogprobsThreads) {
+          float f[W];
+          unpack<T>(r.load(v), f);
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const int e = r.first(v) + i;
+            const uint32_t key = order_key(f[i]);
+            if (key >= bound && e >= 0 && e < p.n) {
+              const int at = atomicAdd(&sm.count, 1);
+              if (at < kLogprobsCandidates)
+                sm.found[at] = (unsigned long long)key << 32 | (0xFFFFFFFFu - (uint32_t)e);
+            }
+          }
+        }
+      }
+      __syncthreads();
+      if (sm.count > kLogprobsCandidates || sm.count < k) find_by_bisection<T>(r, v0, v1, k, sm);
+      rank_found(sm, k);
+    } else if (tid == 0) {
+      sm.best_count = 0;
+    }
+  }
+  if (split > 1) {
+    cluster_sync_all();
+    if (rank == 0) {
+      if (tid == 0) {
+        RowSums all = sm.total;
+        for (int c = 1; c < split; ++c) {
+          RowSums b;
+          const uint32_t at = cluster_addr(&sm.total, c);
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.m) : "r"(at) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1 + 4];" : "=f"(b.s) : "r"(at) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1 + 8];" : "=f"(b.t) : "r"(at) : "memory");
+          all.add(b);
+        }
+        sm.total = all;
+        sm.count = 0;
+      }
+      __syncthreads();
+      if (p.top > 0) {
+        const int c = tid / kLogprobsMaxTop, i = tid % kLogprobsMaxTop;  // eight lists of 64
+        if (c < split) {
+          int have;
+          asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(have) : "r"(cluster_addr(&sm.best_count, c)) : "memory");
+          if (i < have) {
+            unsigned long long key;
+            asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(cluster_addr(&sm.best[i], c)) : "memory");
+            sm.found[atomicAdd(&sm.count, 1)] = key;
+          }
+        }
+        __syncthreads();
+        rank_found(sm, p.top);
+      }
+    }
+    cluster_sync_all();  // no block leaves while its shared memory is read
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+  const float m = sm.total.m, logs = logf(sm.total.s);
+  if (tid == 0) {
+    const int64_t at = row * p.token_stride;
+    const int64_t token = p.tokens64 ? static_cast<const int64_t*>(p.tokens)[at] : static_cast<const int*>(p.tokens)[at];
+    p.logprobs[row] = token >= 0 && token < p.n ? (to_f32(r.row[token]) - m) - logs : __uint_as_float(0x7FC00000u);
+    p.entropy[row] = logs - sm.total.t / sm.total.s;
+  }
+  for (int i = tid; i < p.top; i += kLogprobsThreads) {
+    const unsigned long long key = sm.best[i];
+    p.top_values[(int64_t)row * p.top + i] = (key_value((uint32_t)(key >> 32)) - m) - logs;
+    p.top_tokens[(int64_t)row * p.top + i] = (int64_t)(0xFFFFFFFFu - (uint32_t)key);
+  }
+}
+
+// Blocks per row: one where the rows fill the GPU (two blocks an SM), else as
+// many of up to eight as still find 8 KB each.
+inline int logprobs_split(int64_t m, int64_t bytes, int sm_count) {
+  int split = 1;
+  while (split < 8 && m * split * 2 <= 2 * sm_count && bytes / (2 * split) >= 8192) split *= 2;
+  return split;
+}
+
+template <typename T>
+cudaError_t launch_logprobs_type(const LogprobsParams& p, int sm_count, cudaStream_t s) {
+  const int split = logprobs_split(p.m, (int64_t)p.n * (int64_t)sizeof(T), sm_count);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.m * (unsigned)split);
+  cfg.blockDim = dim3(kLogprobsThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, p, split);
+}
+
+inline cudaError_t launch_logprobs(const LogprobsParams& p, int type, int sm_count, cudaStream_t s) {
+  if (type == FTB_F32) return launch_logprobs_type<float>(p, sm_count, s);
+  if (type == FTB_F16) return launch_logprobs_type<__half>(p, sm_count, s);
+  return launch_logprobs_type<__nv_bfloat16>(p, sm_count, s);
+}
+
+}  // namespace ftb

@@ -1,7 +1,7 @@
-// Python entry points of the block-scaled 8-bit operators on torch tensors.
+// Python entry points of the operators on torch tensors.
 //
 // The checks, output allocations and argument structs behind forgetune_b200/fp8.py
-// in C++, ending in the C ABI (include/forgetune_b200.h).  A one-row call costs
+// and decoder.py in C++, ending in the C ABI (include/forgetune_b200.h).  A one-row call costs
 // more on the host than on the GPU.  Host time per call on the GPU's machine,
 // against the same steps in Python through ctypes: quantize_rows 5.1 us (9.2),
 // rms_norm with residual and quantised output 6.1 (13.5), fp8_linear 4.4
@@ -16,6 +16,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <exception>
 #include <string>
 
@@ -445,6 +446,337 @@ PyObject* op_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------------------
+// a decoder layer's heads, paged cache and logits (decoder.py)
+// ---------------------------------------------------------------------------
+struct Heads {
+  at::Tensor t;
+  ftb_heads a{nullptr, 0, 0, 0};
+  int64_t tokens = 0, heads = 0, dim = 0;
+};
+
+// Strides of [tokens, heads, dim] whose heads are whole and apart; false for others.
+bool lay_heads(Heads& r) {
+  const at::Tensor& t = r.t;
+  r.tokens = t.size(0);
+  r.heads = t.size(1);
+  r.dim = t.size(2);
+  const int64_t token = r.tokens > 1 ? t.stride(0) : 0, head = r.heads > 1 ? t.stride(1) : 0;
+  r.a = {t.data_ptr(), token, head, plain_type(t.scalar_type())};
+  if (r.dim > 1 && t.stride(2) != 1) return false;
+  if (r.tokens > 1 && r.heads > 1) {
+    return token >= head ? head >= r.dim && token >= (r.heads - 1) * head + r.dim
+                         : token >= r.dim && head >= (r.tokens - 1) * token + r.dim;
+  }
+  return (r.tokens <= 1 || token >= r.dim) && (r.heads <= 1 || head >= r.dim);
+}
+
+// A CUDA input of heads, copied where they are not whole or overlap.
+Heads heads_input(PyObject* o, const char* what) {
+  const at::Tensor* t = tensor(o);
+  if (!t || !t->is_cuda() || plain_type(t->scalar_type()) < 0 || t->layout() != at::kStrided)
+    type_error(std::string(what) + " must be a float32, float16 or bfloat16 CUDA tensor");
+  if (t->dim() != 3 || t->size(1) < 1 || t->size(2) < 1)
+    shape_error(std::string(what) + " must be [tokens, heads, dim] with at least one head and element, got " +
+                show(t->sizes()));
+  check_tangent(*t, what);
+  Heads r;
+  r.t = t->is_neg() ? t->resolve_neg() : *t;
+  if (!lay_heads(r)) {
+    r.t = r.t.contiguous();
+    lay_heads(r);
+  }
+  return r;
+}
+
+void check_device(const at::Tensor& t, const char* what, at::Device dev) {
+  if (t.device() != dev)
+    value_error(std::string(what) + " is on " + t.device().str() + ", the input on " + dev.str());
+}
+
+void check_heads(const Heads& x, const char* what, int64_t tokens, int64_t dim, at::ScalarType type, at::Device dev) {
+  if (x.tokens != tokens || x.dim != dim)
+    shape_error(std::string(what) + " must be [" + std::to_string(tokens) + ", heads, " + std::to_string(dim) +
+                "], got " + show(x.t.sizes()));
+  if (x.t.scalar_type() != type) type_error(std::string(what) + " must be " + c10::toString(type));
+  check_device(x.t, what, dev);
+}
+
+// New heads, or the caller's.
+Heads heads_output(PyObject* o, const char* what, const Heads& like, at::ScalarType type) {
+  Heads r;
+  if (o == Py_None) {
+    r.t = at::empty_strided({like.tokens, like.heads, like.dim}, {like.heads * like.dim, like.dim, 1},
+                            at::TensorOptions().dtype(type).device(like.t.device()));
+    lay_heads(r);
+    return r;
+  }
+  const at::Tensor* t = tensor(o);
+  if (!t || t->scalar_type() != type || t->layout() != at::kStrided || t->is_neg())
+    type_error(std::string(what) + " must be a " + c10::toString(type) + " tensor");
+  if (t->dim() != 3 || t->size(0) != like.tokens || t->size(1) != like.heads || t->size(2) != like.dim)
+    shape_error(std::string(what) + " must be " + show(like.t.sizes()) + ", got " + show(t->sizes()));
+  check_device(*t, what, like.t.device());
+  r.t = *t;
+  if (!lay_heads(r)) shape_error(std::string(what) + ": heads must be contiguous and must not overlap");
+  check_written(*t, what);
+  return r;
+}
+
+// Whole numbers on the device, copied where they are not in rows.
+at::Tensor whole(PyObject* o, const char* what, int64_t dims, bool wide, at::Device dev) {
+  const at::Tensor* t = tensor(o);
+  if (!t || t->layout() != at::kStrided || !(t->scalar_type() == at::kInt || (wide && t->scalar_type() == at::kLong)))
+    type_error(std::string(what) + " must be an int32 " + (wide ? "or int64 " : "") + "tensor");
+  if (t->dim() != dims) shape_error(std::string(what) + " must be " + std::to_string(dims) + "-D, got " + show(t->sizes()));
+  check_device(*t, what, dev);
+  const bool rows = dims == 2 ? row_stride(*t) >= 0 : t->size(0) <= 1 || t->stride(0) == 1;
+  return rows ? *t : t->contiguous();
+}
+
+struct Paged {
+  at::Tensor keys, values, table, starts, lengths;
+  ftb_paged_cache cache{};
+  ftb_paged_batch batch{};
+};
+
+// The pools of keys and values, taken as they lie, and the batch.
+Paged paged(const char* fn, PyObject* const* a, bool written_to, at::Device dev) {
+  Paged r;
+  at::Tensor* pool[2] = {&r.keys, &r.values};
+  const char* names[2] = {": keys", ": values"};
+  for (int i = 0; i < 2; ++i) {
+    const std::string what = std::string(fn) + names[i];
+    const at::Tensor* t = tensor(a[i]);
+    if (!t || plain_type(t->scalar_type()) < 0 || t->layout() != at::kStrided || t->is_neg())
+      type_error(what + " must be a float32, float16 or bfloat16 tensor");
+    if (t->dim() != 4 || t->numel() == 0)
+      shape_error(what + " must be [pages, page_size, kv_heads, dim], none of them 0, got " + show(t->sizes()));
+    if (t->size(3) > 1 && t->stride(3) != 1) shape_error(what + ": the values of a head must be contiguous");
+    check_device(*t, what.c_str(), dev);
+    if (written_to) check_written(*t, what.c_str());
+    else check_tangent(*t, what.c_str());
+    *pool[i] = *t;
+  }
+  if (r.keys.sizes() != r.values.sizes())
+    shape_error(std::string(fn) + ": values must be " + show(r.keys.sizes()) + " as keys are, got " + show(r.values.sizes()));
+  if (r.keys.scalar_type() != r.values.scalar_type())
+    type_error(std::string(fn) + ": values must be " + c10::toString(r.keys.scalar_type()) + " as keys are");
+  auto stride = [](const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+  r.cache = {r.keys.data_ptr(), r.values.data_ptr(), stride(r.keys, 0), stride(r.keys, 1), stride(r.keys, 2),
+             stride(r.values, 0), stride(r.values, 1), stride(r.values, 2), plain_type(r.keys.scalar_type()),
+             r.keys.size(0), r.keys.size(1), r.keys.size(2), r.keys.size(3)};
+  r.table = whole(a[2], (std::string(fn) + ": page_table").c_str(), 2, false, dev);
+  r.starts = whole(a[3], (std::string(fn) + ": starts").c_str(), 1, false, dev);
+  r.lengths = whole(a[4], (std::string(fn) + ": lengths").c_str(), 1, false, dev);
+  const int64_t b = r.lengths.size(0);
+  if (b < 1 || r.table.size(0) != b || r.table.size(1) < 1 || r.starts.size(0) != b + 1)
+    shape_error(std::string(fn) + ": page_table must be [sequences, pages], starts [sequences + 1] and lengths "
+                                  "[sequences], got " + show(r.table.sizes()) + ", " + show(r.starts.sizes()) + " and " +
+                show(r.lengths.sizes()));
+  r.batch = {static_cast<const int32_t*>(r.table.data_ptr()), row_stride(r.table), r.table.size(1), b,
+             static_cast<const int32_t*>(r.starts.data_ptr()), static_cast<const int32_t*>(r.lengths.data_ptr())};
+  return r;
+}
+
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Refused{nullptr, ""};
+  return v;
+}
+int64_t integer(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw Refused{nullptr, ""};
+  return v;
+}
+
+struct Rotation {
+  at::Tensor frequencies;
+  ftb_rotation a{};
+};
+
+// frequencies (None: no rotation), eps, norm, interleaved, amplitude
+Rotation rotation(const char* fn, PyObject* f, PyObject* const* a, int64_t dim, at::Device dev) {
+  Rotation r;
+  if (f != Py_None) {
+    const std::string what = std::string(fn) + ": frequencies";
+    const at::Tensor* t = tensor(f);
+    if (!t || t->scalar_type() != at::kDouble || t->layout() != at::kStrided || t->is_neg())
+      type_error(what + " must be a float64 tensor (see rope_frequencies)");
+    if (t->dim() != 1 || t->size(0) < 1 || 2 * t->size(0) > dim)
+      shape_error(what + " must be [pairs] with at most half of dim " + std::to_string(dim) + ", got " + show(t->sizes()));
+    check_device(*t, what.c_str(), dev);
+    check_tangent(*t, what.c_str());
+    r.frequencies = t->size(0) == 1 || t->stride(0) == 1 ? *t : t->contiguous();
+    r.a.frequencies = static_cast<const double*>(r.frequencies.data_ptr());
+    r.a.pairs = t->size(0);
+  }
+  r.a.eps = number(a[0]);
+  r.a.norm = truth(a[1]);
+  r.a.interleaved = truth(a[2]);
+  r.a.amplitude = number(a[3]);
+  return r;
+}
+
+const float* head_weight(at::Tensor& keep, PyObject* o, const char* what, bool norm, int64_t dim, at::Device dev) {
+  if (o != Py_None && !norm) value_error(std::string(what) + " needs norm=True");
+  keep = vector(o, what, dim, dev);
+  return keep.defined() ? static_cast<const float*>(keep.data_ptr()) : nullptr;
+}
+
+// rotate_heads(x, positions, frequencies, weight, eps, norm, interleaved, amplitude, out) -> y
+PyObject* op_rotate_heads(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    const Heads x = heads_input(a[0], "rotate_heads: x");
+    const at::Device dev = x.t.device();
+    const at::Tensor positions = whole(a[1], "rotate_heads: positions", 1, true, dev);
+    if (positions.size(0) != x.tokens)
+      shape_error("rotate_heads: positions must be [" + std::to_string(x.tokens) + "], got " + show(positions.sizes()));
+    const Rotation rot = rotation("rotate_heads", a[2], a + 4, x.dim, dev);
+    at::Tensor weight;
+    ftb_rotate_args args{};
+    args.weight = head_weight(weight, a[3], "rotate_heads: weight", rot.a.norm, x.dim, dev);
+    const Heads y = heads_output(a[8], "rotate_heads: out", x, x.t.scalar_type());
+    args.x = x.a;
+    args.y = y.a;
+    args.tokens = x.tokens;
+    args.heads = x.heads;
+    args.dim = x.dim;
+    args.positions = positions.data_ptr();
+    args.positions64 = positions.scalar_type() == at::kLong;
+    args.rotation = rot.a;
+    if (x.tokens > 0) call("ftb_rotate_heads", ftb_rotate_heads, args, dev);
+    if (a[8] != Py_None) written(y.t);
+    return wrap(y.t);
+  });
+}
+
+// append_heads(q, k, v, keys, values, page_table, starts, lengths, frequencies, q_weight, k_weight, eps, norm,
+//              interleaved, amplitude, out) -> q
+PyObject* op_append_heads(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 16, [&]() -> PyObject* {
+    const Heads q = heads_input(a[0], "append_heads: q");
+    const at::Device dev = q.t.device();
+    const Heads k = heads_input(a[1], "append_heads: k"), v = heads_input(a[2], "append_heads: v");
+    const Paged p = paged("append_heads", a + 3, true, dev);
+    const at::ScalarType held = p.keys.scalar_type();
+    check_heads(q, "append_heads: q", q.tokens, p.cache.dim, q.t.scalar_type(), dev);
+    check_heads(k, "append_heads: k", q.tokens, p.cache.dim, q.t.scalar_type(), dev);
+    check_heads(v, "append_heads: v", q.tokens, p.cache.dim, q.t.scalar_type(), dev);
+    if (k.heads != p.cache.kv_heads || v.heads != p.cache.kv_heads)
+      shape_error("append_heads: k and v must have the cache's " + std::to_string(p.cache.kv_heads) + " heads, got " +
+                  std::to_string(k.heads) + " and " + std::to_string(v.heads));
+    if (q.t.scalar_type() != held && q.t.scalar_type() != at::kFloat)
+      type_error(std::string("append_heads: q, k and v must be float32 or the cache's ") + c10::toString(held));
+    const Rotation rot = rotation("append_heads", a[8], a + 11, q.dim, dev);
+    at::Tensor wq, wk;
+    ftb_append_args args{};
+    args.q_weight = head_weight(wq, a[9], "append_heads: q_weight", rot.a.norm, q.dim, dev);
+    args.k_weight = head_weight(wk, a[10], "append_heads: k_weight", rot.a.norm, q.dim, dev);
+    const Heads y = heads_output(a[15], "append_heads: out", q, held);
+    args.q = q.a;
+    args.k = k.a;
+    args.v = v.a;
+    args.q_out = y.a;
+    args.tokens = q.tokens;
+    args.heads = q.heads;
+    args.cache = p.cache;
+    args.batch = p.batch;
+    args.rotation = rot.a;
+    if (q.tokens > 0) call("ftb_append_heads", ftb_append_heads, args, dev);
+    written(p.keys);
+    written(p.values);
+    if (a[15] != Py_None) written(y.t);
+    return wrap(y.t);
+  });
+}
+
+// paged_attention(q, keys, values, page_table, starts, lengths, scale, window, out) -> out
+PyObject* op_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    const Heads q = heads_input(a[0], "paged_attention: q");
+    const at::Device dev = q.t.device();
+    const Paged p = paged("paged_attention", a + 1, false, dev);
+    check_heads(q, "paged_attention: q", q.tokens, p.cache.dim, p.keys.scalar_type(), dev);
+    if (q.heads % p.cache.kv_heads)
+      shape_error("paged_attention: q has " + std::to_string(q.heads) + " heads, the cache " +
+                  std::to_string(p.cache.kv_heads) + ": not a multiple");
+    ftb_attention_args args{};
+    args.scale = a[6] == Py_None ? 1.0 / std::sqrt((double)q.dim) : number(a[6]);
+    args.window = a[7] == Py_None ? 0 : integer(a[7]);
+    if (args.window < 0) value_error("paged_attention: window must not be negative");
+    const Heads y = heads_output(a[8], "paged_attention: out", q, q.t.scalar_type());
+    args.q = q.a;
+    args.out = y.a;
+    args.tokens = q.tokens;
+    args.heads = q.heads;
+    args.cache = p.cache;
+    args.batch = p.batch;
+    if (q.tokens > 0) {
+      c10::cuda::OptionalCUDAGuard guard;
+      if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
+      const int64_t bytes = ftb_paged_attention_workspace(&args);
+      if (bytes < 0)
+        throw Refused{g_runtime_error, "ftb_paged_attention_workspace failed (" + std::to_string(bytes) + "): " + ftb_last_error()};
+      at::Tensor work;  // from torch's allocator: kept from other streams' use, and a graph's own under capture
+      if (bytes > 0) {
+        work = at::empty_strided({bytes}, {1}, at::TensorOptions().dtype(at::kByte).device(dev));
+        args.workspace = work.data_ptr();
+        args.workspace_bytes = bytes;
+      }
+      call("ftb_paged_attention", ftb_paged_attention, args, dev);
+    }
+    if (a[8] != Py_None) written(y.t);
+    return wrap(y.t);
+  });
+}
+
+// token_logprobs(logits, tokens, top) -> (logprobs, entropy[, top_logprobs, top_tokens])
+PyObject* op_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 3, [&]() -> PyObject* {
+    const Matrix x = input(a[0], "token_logprobs: logits");
+    const at::Device dev = x.t.device();
+    const at::Tensor tokens = whole(a[1], "token_logprobs: tokens", 1, true, dev);
+    if (tokens.size(0) != x.m)
+      shape_error("token_logprobs: tokens must be [" + std::to_string(x.m) + "], got " + show(tokens.sizes()));
+    const int64_t top = integer(a[2]);
+    if (top < 0 || top > 64 || top > x.k)
+      value_error("token_logprobs: top must be 0 to 64 and at most the " + std::to_string(x.k) + " logits of a row");
+    auto make = [&](int64_t cols, at::ScalarType type) {
+      const auto o = at::TensorOptions().dtype(type).device(dev);
+      return cols ? at::empty_strided({x.m, cols}, {cols, 1}, o) : at::empty_strided({x.m}, {1}, o);
+    };
+    const at::Tensor logprobs = make(0, at::kFloat), entropy = make(0, at::kFloat);
+    at::Tensor values, ids;
+    ftb_logprobs_args args{};
+    args.logits = x.a;
+    args.m = x.m;
+    args.n = x.k;
+    args.tokens = tokens.data_ptr();
+    args.tokens64 = tokens.scalar_type() == at::kLong;
+    args.token_stride = 1;
+    args.logprobs = static_cast<float*>(logprobs.data_ptr());
+    args.entropy = static_cast<float*>(entropy.data_ptr());
+    args.top = top;
+    if (top) {
+      values = make(top, at::kFloat);
+      ids = make(top, at::kLong);
+      args.top_logprobs = static_cast<float*>(values.data_ptr());
+      args.top_tokens = static_cast<int64_t*>(ids.data_ptr());
+    }
+    if (x.m > 0) call("ftb_token_logprobs", ftb_token_logprobs, args, dev);
+    PyObject* r = PyTuple_New(top ? 4 : 2);
+    if (!r) return nullptr;
+    PyTuple_SET_ITEM(r, 0, wrap(logprobs));
+    PyTuple_SET_ITEM(r, 1, wrap(entropy));
+    if (top) {
+      PyTuple_SET_ITEM(r, 2, wrap(values));
+      PyTuple_SET_ITEM(r, 3, wrap(ids));
+    }
+    return r;
+  });
+}
+
 PyMethodDef kMethods[] = {
     {"check", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(op_check)), METH_FASTCALL, nullptr},
     {"quantize_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(op_quantize_rows)), METH_FASTCALL, nullptr},
@@ -452,6 +784,12 @@ PyMethodDef kMethods[] = {
      nullptr},
     {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(op_rms_norm)), METH_FASTCALL, nullptr},
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(op_linear)), METH_FASTCALL, nullptr},
+    {"rotate_heads", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(op_rotate_heads)), METH_FASTCALL, nullptr},
+    {"append_heads", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(op_append_heads)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(op_paged_attention)), METH_FASTCALL,
+     nullptr},
+    {"token_logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(op_token_logprobs)), METH_FASTCALL,
+     nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -314,6 +314,119 @@ FORGETUNE_EXPORT int ftb_fp8_set_fault_injection(int stall);
  * nt = 0 with split 1 for SM pairs, nt = -1 for the estimate again.  -2 for any other combination. */
 FORGETUNE_EXPORT int ftb_fp8_set_kernel(int nt, int split);
 
+/* Operators around a decoder layer's attention and behind its logits.  No
+ * counterpart in the reference.  The rules of the 8-bit operators above hold:
+ * device arrays on the current device, everything enqueued on `stream` without
+ * synchronising or allocating, the same status codes, outputs that share
+ * memory with an operand refused except in place where said so.
+ *
+ * Heads are [tokens, heads, dim], the values of a head consecutive, with any
+ * stride between tokens and between heads.  A paged cache is a pool of keys and
+ * one of values, [pages, page_size, kv_heads, dim] each, the values of a head
+ * consecutive, with any other strides.
+ *
+ * A batch is `sequences` sequences side by side: rows starts[b] to starts[b + 1]
+ * of the heads are the new tokens of sequence b, which has lengths[b] tokens
+ * with them, so that its i-th new token is at position lengths[b] -
+ * (starts[b + 1] - starts[b]) + i.  The token at position j lies in page
+ * page_table[b][j / page_size], at j % page_size.  starts, lengths and
+ * page_table are read on the device when the kernels run.  starts must not
+ * fall.  Rows in no sequence are left as they were. */
+typedef struct {
+  void* data;
+  int64_t token, head; /* strides in elements */
+  int64_t type;        /* FTB_F32, FTB_F16 or FTB_BF16 */
+} ftb_heads;
+
+typedef struct {
+  void *keys, *values;
+  int64_t k_page, k_token, k_head, v_page, v_token, v_head; /* strides in elements */
+  int64_t type, pages, page_size, kv_heads, dim;
+} ftb_paged_cache;
+
+typedef struct {
+  const int32_t* page_table; /* [sequences, most_pages], rows table_ld apart */
+  int64_t table_ld, most_pages, sequences;
+  const int32_t *starts, *lengths; /* [sequences + 1], [sequences] */
+} ftb_paged_batch;
+
+/* Rotary positions: pair i of a head turns by position * frequencies[i] (in 64 bits), times the amplitude.
+ * Pairs are elements (i, i + pairs), or (2 i, 2 i + 1) where interleaved is not 0; elements from 2 * pairs on
+ * stay as they are.  pairs = 0: no rotation.  norm != 0: the head is first divided by sqrt(mean(x^2) + eps) and
+ * multiplied by a weight [dim] (null: ones). */
+typedef struct {
+  const double* frequencies;
+  int64_t pairs, interleaved;
+  double amplitude;
+  int64_t norm;
+  double eps;
+} ftb_rotation;
+
+/* y = x with each head normalised and turned by its token's position; positions are int32 (positions64 = 0)
+ * or int64.  y has x's type and may be x itself (same pointer and strides).  dim is at most 512. */
+typedef struct {
+  ftb_heads x, y;
+  int64_t tokens, heads, dim;
+  const void* positions;
+  int64_t positions64;
+  ftb_rotation rotation;
+  const float* weight;
+} ftb_rotate_args;
+FORGETUNE_EXPORT int ftb_rotate_heads(const ftb_rotate_args* args, void* stream);
+
+/* The same of the queries q and keys k of a batch's new tokens by their positions: queries into q_out, keys and
+ * the values v as they are into the cache.  q, k and v have one type, the cache's or float32; q_out has the cache's
+ * type and may be q itself where the types are alike.  A token whose position has no page in the pool is not
+ * stored.  Two tokens must not have the same place. */
+typedef struct {
+  ftb_heads q, k, v, q_out;
+  int64_t tokens, heads;
+  ftb_paged_cache cache;
+  ftb_paged_batch batch;
+  ftb_rotation rotation;
+  const float *q_weight, *k_weight;
+} ftb_append_args;
+FORGETUNE_EXPORT int ftb_append_heads(const ftb_append_args* args, void* stream);
+
+/* out[t, h] = sum_j softmax_j(scale q[t, h] . key_j) value_j over the tokens j of t's sequence up to t's own
+ * position, and with window > 0 the last `window` of them only; head h reads kv head h / (heads / kv_heads).  A
+ * token at a negative position sees nothing and gets zeros.  Keys and values that a token does not see do not
+ * change its output, whatever they hold; a value that is not finite makes its element of the outputs that see it
+ * not finite.  A page number outside the pool, or a length beyond the table, makes outputs of that sequence NaN;
+ * nothing outside is read.  q, out and the cache have one type.
+ *
+ * `workspace` holds ftb_paged_attention_workspace(args) bytes on 16-byte boundaries (0: may be null), which no
+ * other call may use until this one's kernels are done; its contents do not matter. */
+typedef struct {
+  ftb_heads q, out;
+  int64_t tokens, heads;
+  ftb_paged_cache cache;
+  ftb_paged_batch batch;
+  double scale;
+  int64_t window;
+  void* workspace;
+  int64_t workspace_bytes;
+} ftb_attention_args;
+FORGETUNE_EXPORT int ftb_paged_attention(const ftb_attention_args* args, void* stream);
+/* Bytes, or a negative status. */
+FORGETUNE_EXPORT int64_t ftb_paged_attention_workspace(const ftb_attention_args* args);
+
+/* Of each row of logits [m, n]: the log probability of tokens[i] (int32, or int64 where tokens64 is not 0,
+ * token_stride apart; NaN for one outside of [0, n)), the entropy, and the `top` (0 to 64) largest log
+ * probabilities, largest first, with their tokens; equal ones go by the lower token, NaN comes last.  Rows of
+ * alternatives are `top` apart. */
+typedef struct {
+  ftb_matrix logits;
+  int64_t m, n;
+  const void* tokens;
+  int64_t tokens64, token_stride;
+  float *logprobs, *entropy;
+  int64_t top;
+  float* top_logprobs;
+  int64_t* top_tokens;
+} ftb_logprobs_args;
+FORGETUNE_EXPORT int ftb_token_logprobs(const ftb_logprobs_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
