@@ -11,9 +11,12 @@
 #include "heads.cuh"
 #include "logprobs.cuh"
 #include "op_common.hpp"
+#include "paged_attention.cuh"
 #include "paged_rows.cuh"
 
 namespace ftb {
+
+cudaError_t decoder_prepare() { return paged_attention_prepare(); }
 
 constexpr int64_t kMaxTokens = int64_t(1) << 27, kMaxHeads = 4096, kMaxStride = int64_t(1) << 40;
 
@@ -284,6 +287,33 @@ static int check_attention(const char* fn, const ftb_attention_args& a) {
   return why.empty() ? (int)ST_OK : refuse(fn, why);
 }
 
+static PagedAttentionParams params(const ftb_attention_args& a) {
+  const ftb_paged_cache& c = a.cache;
+  PagedAttentionParams p{};
+  p.q = a.q.data;
+  p.q_token = a.q.token;
+  p.q_head = a.q.head;
+  p.out = a.out.data;
+  p.o_token = a.out.token;
+  p.o_head = a.out.head;
+  p.keys = c.keys;
+  p.values = c.values;
+  p.k_page = c.k_page;
+  p.k_token = c.k_token;
+  p.k_head = c.k_head;
+  p.v_page = c.v_page;
+  p.v_token = c.v_token;
+  p.v_head = c.v_head;
+  p.batch = params(a.batch, c);
+  p.tokens = (int)a.tokens;
+  p.heads = (int)a.heads;
+  p.kv_heads = (int)c.kv_heads;
+  p.dim = (int)c.dim;
+  p.window = (int)a.window;
+  p.scale = (float)(a.scale * 1.4426950408889634);
+  return p;
+}
+
 }  // namespace ftb
 
 FTB_API int64_t ftb_paged_attention_workspace(const ftb_attention_args* args) {
@@ -291,7 +321,9 @@ FTB_API int64_t ftb_paged_attention_workspace(const ftb_attention_args* args) {
   return guarded(fn, [&]() -> int {
     if (!args) return refuse(fn, "null arguments", ST_NULL);
     if (args->tokens == 0) return 0;
-    return check_attention(fn, *args);
+    if (const int rc = check_attention(fn, *args)) return rc;
+    const PagedAttentionParams p = params(*args);
+    return paged_on_tensor_cores(p, (int)args->cache.type) ? (int)paged_workspace(p) : 0;
   });
 }
 
@@ -305,29 +337,12 @@ FTB_API int ftb_paged_attention(const ftb_attention_args* args, void* stream) {
     if (const int rc = check_attention(fn, a)) return rc;
     OpDevice* d = nullptr;
     if (const int rc = op_device(fn, &d)) return rc;
-    PagedAttentionParams p{};
-    p.q = a.q.data;
-    p.q_token = a.q.token;
-    p.q_head = a.q.head;
-    p.out = a.out.data;
-    p.o_token = a.out.token;
-    p.o_head = a.out.head;
-    p.keys = c.keys;
-    p.values = c.values;
-    p.k_page = c.k_page;
-    p.k_token = c.k_token;
-    p.k_head = c.k_head;
-    p.v_page = c.v_page;
-    p.v_token = c.v_token;
-    p.v_head = c.v_head;
-    p.batch = params(a.batch, c);
-    p.tokens = (int)a.tokens;
-    p.heads = (int)a.heads;
-    p.kv_heads = (int)c.kv_heads;
-    p.dim = (int)c.dim;
-    p.window = (int)a.window;
-    p.scale = (float)(a.scale * 1.4426950408889634);
-    return launched(fn, launch_paged_rows(p, (int)c.type, static_cast<cudaStream_t>(stream)));
+    const PagedAttentionParams p = params(a);
+    const auto st = static_cast<cudaStream_t>(stream);
+    if (!paged_on_tensor_cores(p, (int)c.type)) return launched(fn, launch_paged_rows(p, (int)c.type, st));
+    if (a.workspace_bytes < paged_workspace(p) || !a.workspace || !aligned(a.workspace, 16))
+      return refuse(fn, "needs the workspace that ftb_paged_attention_workspace tells, on 16-byte boundaries");
+    return launched(fn, launch_paged_attention(p, (int)c.type, a.workspace, d->sm_count, d->fault_dev, op_stall(), st));
   });
 }
 

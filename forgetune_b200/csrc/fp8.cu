@@ -54,6 +54,7 @@ static std::string fp8_setup(int dev, OpDevice* d) {
     if (e == cudaSuccess) e = fp8_tile_attributes<64>();
     if (e == cudaSuccess) e = fp8_tile_attributes<128>();
     if (e == cudaSuccess) e = fp8_pair_prepare(&d->pairs);
+    if (e == cudaSuccess) e = decoder_prepare();
     const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
     if (e == cudaSuccess) e = back;
   }
@@ -61,6 +62,8 @@ static std::string fp8_setup(int dev, OpDevice* d) {
   cudaGetLastError();
   return std::string("set-up failed: ") + cudaGetErrorString(e);
 }
+
+int op_stall() { return g_fp8_stall.load(); }
 
 int op_device(const char* fn, OpDevice** out) {
   int dev = 0;
@@ -354,7 +357,7 @@ FTB_API int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream) {
     p.e.res_vec = rows_aligned(a.residual);
     p.e.y_vec = rows_aligned(a.y);
     p.err = d->fault_dev;
-    p.stall_test = g_fp8_stall.load();
+    p.stall_test = op_stall();
     return launched(fn, launch_fp8_linear(o, p, *d, static_cast<cudaStream_t>(stream)));
   });
 }

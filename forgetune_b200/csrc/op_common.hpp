@@ -30,6 +30,12 @@ struct OpDevice {
 // device gave up a wait (fp8.cu).
 int op_device(const char* fn, OpDevice** out);
 
+// Kernel attributes of the operators in decoder.cu, once per device.
+cudaError_t decoder_prepare();
+
+// Failure-detection hook: whether launches stall (ftb_fp8_set_fault_injection).
+int op_stall();
+
 inline int refuse(const char* fn, const std::string& why, int status = ST_INPUT) {
   set_error(std::string(fn) + ": " + why);
   return status;

@@ -1,0 +1,945 @@
+// Attention of new tokens over a paged cache on the tensor cores.
+//
+//   S = scale Q K^T (masked),  P = exp(S - m),  O = P V / sum P
+//
+// in one pass over the keys: a row keeps its reference m and its sum, and O
+// lies in tensor memory.  m is raised (and O rescaled) only where a tile's
+// maximum is above it by more than 2^8: any reference gives the same quotient,
+// and weights up to 2^8 are as exact as weights up to 1.
+//
+// Rows.  The queries that share a kv head are the rows of one matrix, row r =
+// (token r / G, head r % G), so that one token of G heads costs one row of
+// loads, not G.  A unit of work is up to 256 rows of one sequence and kv head
+// (two tiles of 128 that share every tile of keys and values), or, where the
+// sequence has at most 128, all of its rows, with the tiles of keys going to
+// the two halves of the block in turn and the halves joined at the end.
+//
+// Work.  Every unit's cost is a formula of its sequence's numbers, so each
+// block sums them up and takes its equal share, from an offset in the middle
+// of one unit to one in the middle of another: long contexts are split over
+// blocks as finely as needed and short ones gathered, by the device's own
+// numbers, without a plan from the host.  A block has at most two parts of
+// units that others share; they go to the workspace (O, m and the sum), and
+// paged_join_kernel joins them in order.  No atomics: the same bits each time.
+//
+// Block: twelve warps.
+//   warps 0-3, 4-7  softmax of the two halves: a thread is a row.  S from
+//                   tensor memory, mask, maximum, exponentials, P back over S
+//                   as the A operand of P V; at the end O to global memory
+//   warp 8          units of the block; keys and values by TMA, boxes of as
+//                   many tokens as lie in one page, into a ring of tiles
+//   warp 9          tensor memory and the products (one elected lane): while
+//                   one half is in its softmax, the other's run
+//   warps 10-11     Q of the next unit by cp.async; tiles that some row sees
+//                   in part: values outside of the unit's keys become 0, and
+//                   so do values that are not finite (0 weights would make
+//                   them NaN); rows that do see one are marked at the end
+//
+// Shared memory: Q of two tiles, and a ring of 128-token tiles of K or V,
+// 128-byte swizzle, in columns of 64.  Tensor memory: S and P of both halves at
+// [0, 256), O at [256, 512).
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <type_traits>
+
+#include "paged_rows.cuh"
+#include "tc_ptx.cuh"
+
+namespace ftb {
+
+constexpr int kPagedThreads = 384;
+constexpr int kPagedTile = 128;      // keys of a tile, rows of a half
+constexpr int kPagedUnitOver = 160;  // a unit's own cost, in keys
+constexpr int kPagedLeast = 448;     // keys (with it) that are worth a block
+constexpr float kPagedRaise = 8.0f;  // log2
+constexpr int kPagedBlocks = 148;    // at most: B200's SMs
+
+// What the blocks leave for the join: for each block whose last unit others go on with.
+struct PagedMeta {
+  int open, last, kvh, r0, rows, tok0, pos0, pad;
+};
+
+struct PagedTensorParams {
+  PagedAttentionParams a;
+  int group;         // query heads of a kv head
+  int box;           // tokens of a TMA box: in one page
+  int negative;      // the scale is below 0 (a.scale is its absolute value)
+  int rows_bound;    // rows of a part in the workspace
+  PagedMeta* meta;   // [blocks]
+  float* parts;      // [2 blocks][rows_bound] of (m, sum), then O [DH]
+  int* err;
+  int stall_test;    // failure-detection tests: the MMA warp first waits for what nothing completes
+};
+
+struct PagedUnit {
+  int seq, kvh, r0, rows, tok0, pos0;
+  int tb, te;          // tiles of keys of this part
+  int lo, hi;          // keys that some row sees
+  int first, last;     // positions of the first and the last row
+  int alternate;       // the halves take the tiles in turn
+  int slot;            // part of the workspace, -1: the whole unit
+  int done;
+  volatile int bad;    // a page outside of the pool
+  volatile int dirty;  // a value that is not finite in a tile seen in part
+};
+
+// Cost of the first n tiles of rows of a sequence, in keys times G: tile i sees
+// about base + 256 (i + 1) / G keys, at most `cap`.
+struct PagedCost {
+  int64_t base, cap, over;
+  __device__ __forceinline__ int64_t tile(int64_t i) const { return min(cap, base + 256 * (i + 1)) + over; }
+  __device__ __forceinline__ int64_t first(int64_t n) const {
+    const int64_t k = cap <= base ? 0 : min(n, (cap - base) / 256);
+    return k * base + 128 * k * (k + 1) + (n - k) * (k < n ? cap : 0) + n * over;
+  }
+};
+
+struct PagedSequence {
+  int tok0, n, len, tiles;
+  PagedCost cost;
+  int64_t head;  // cost of a kv head
+};
+
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedTensorParams& p, int b) {
+  const PagedBatchParams& t = p.a.batch;
+  PagedSequence s;
+  s.tok0 = max(0, min(t.starts[b], p.a.tokens));
+  s.n = max(0, min(t.starts[b + 1], p.a.tokens) - s.tok0);
+  s.len = t.lengths[b];
+  const int64_t rows = (int64_t)s.n * p.group;
+  s.tiles = rows == 0 ? 0 : rows <= kPagedTile ? 1 : (int)((rows + 255) / 256);
+  const int64_t G = p.group, len = max((int64_t)0, min((int64_t)s.len, (int64_t)t.most_pages * t.page_size));
+  s.cost.base = max((int64_t)0, len - s.n) * G;
+  s.cost.cap = s.tiles == 1 ? len * G : (int64_t)1 << 50;
+  if (p.a.window) s.cost.cap = min(s.cost.cap, (int64_t)p.a.window * G + (s.tiles == 1 ? rows : 256));
+  s.cost.over = kPagedUnitOver * G;
+  s.head = s.cost.first(s.tiles);
+  return s;
+}
+
+template <int DH>
+struct PagedSmem {
+  static constexpr int HALVES = DH / 64;
+  static constexpr int TILE = kPagedTile * DH * 2;
+  static constexpr int STAGES = DH == 128 ? 5 : 10;
+  static constexpr int Q_OFF = STAGES * TILE;
+  static constexpr int ML_OFF = Q_OFF + 2 * TILE;  // [128] of (m, sum)
+  static constexpr int UNIT_OFF = ML_OFF + 128 * 8;
+  static constexpr int UNITS = 2;
+  static constexpr int BAR_OFF = (UNIT_OFF + UNITS * (int)sizeof(PagedUnit) + 15) / 16 * 16;
+  static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 4 + 4;
+  static constexpr int TOTAL = 1024 + BAR_OFF + 8 * NBAR + 16;
+  static_assert(TOTAL <= 227 * 1024, "shared memory budget");
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t paged_idesc(int n, bool b_by_rows) {
+  constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | (b_by_rows ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kPagedTile >> 4) << 24);
+}
+
+// Operand tiles of 128-byte rows in the 128-byte swizzle, 8-row groups 1024
+// bytes apart: K-major (Q, K: rows are M or N, 64 of the depth side by side) and
+// MN-major (V: rows are the depth, 64 of N side by side, the next 64 a tile of
+// 128 rows further).
+__device__ __forceinline__ uint64_t paged_desc(uint32_t saddr, uint32_t lead) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// A in tensor memory: a lane a row, eight columns 16 values of the depth
+__device__ __forceinline__ void umma_f16_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
+// Whether some row of the unit sees tile t in part.
+__device__ __forceinline__ bool paged_masked(const PagedUnit& u, int t, int window) {
+  return (t + 1) * kPagedTile > u.first + 1 || (window && t * kPagedTile <= u.last - window);
+}
+
+// End of the tiles that half w of a unit sees.
+__device__ __forceinline__ int paged_end(const PagedUnit& u, int w, int group) {
+  if (u.alternate || w == 1) return u.te;
+  const int last = u.pos0 + (u.r0 + min(u.rows, kPagedTile) - 1) / group;
+  return max(u.tb, min(u.te, last < 0 ? 0 : last / kPagedTile + 1));
+}
+
+// Tiles of keys that half w takes.
+__device__ __forceinline__ int paged_count(const PagedUnit& u, int w, int group) {
+  if (u.alternate) return (u.te - u.tb + 1 - w) >> 1;
+  return w == 1 && u.rows <= kPagedTile ? 0 : paged_end(u, w, group) - u.tb;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Halves of a word that are infinities or NaN, as all-ones halves.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+  return __vcmpeq2(w & e, e);
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(kPagedThreads, 1)
+    paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                           const PagedTensorParams p) {
+  using L = PagedSmem<DH>;
+  constexpr int STAGES = L::STAGES, HALVES = L::HALVES, UNITS = L::UNITS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
+  PagedUnit* units = reinterpret_cast<PagedUnit*>(smem + L::UNIT_OFF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);  // a tile of K or V landed
+  uint64_t* empty = full + STAGES;       // the products are done with it
+  uint64_t* u_full = empty + STAGES;     // a unit is described
+  uint64_t* u_empty = u_full + UNITS;    // every role is done with it
+  uint64_t* q_full = u_empty + UNITS;    // its Q landed
+  uint64_t* q_empty = q_full + 1;        // its last S = Q K^T is done
+  uint64_t* s_full = q_empty + 1;        // [2] S of a half
+  uint64_t* p_full = s_full + 2;         // [2] its P is in tensor memory, O rescaled
+  uint64_t* pv_done = p_full + 2;        // [2] P V is done
+  uint64_t* o_free = pv_done + 2;        // [2] O was read (in units where the half had tiles)
+  uint64_t* v_seen = o_free + 2;         // a tile of V seen in part is there
+  uint64_t* v_clean = v_seen + 1;        // ... and clean
+  uint64_t* ml_full = v_clean + 1;       // m and sum of the second half
+  uint64_t* drain = ml_full + 1;         // products retired after an abort
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 1) + 1;
+
+  const PagedAttentionParams& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.group;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < UNITS; ++s) {
+      mbar_init(&u_full[s], 1);
+      mbar_init(&u_empty[s], 11);  // eight softmax warps, the products, two of Q
+    }
+    mbar_init(q_full, 2);
+    mbar_init(q_empty, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 4);
+      mbar_init(&pv_done[w], 1);
+      mbar_init(&o_free[w], 4);
+    }
+    mbar_init(v_seen, 1);
+    mbar_init(v_clean, 2);
+    mbar_init(ml_full, 4);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(const_cast<uint32_t*>(tmem_slot))),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == 10 && elect_one()) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_v)) : "memory");
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dep_wait();
+  grid_dep_trigger();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t ring = smem_u32(smem), q_smem = smem_u32(smem + L::Q_OFF);
+
+  if (warp == 8) {
+    // ---- units, keys and values ----
+    bool ok = true;
+    uint32_t it = 0, uc = 0;
+    const PagedBatchParams& bt = a.batch;
+    int64_t total = 0;
+    for (int b = lane; b < bt.seqs; b += 32) total += paged_sequence(p, b).head * a.kv_heads;
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    const int64_t blocks = max((int64_t)1, min((int64_t)gridDim.x, total / ((int64_t)kPagedLeast * G)));
+    const int64_t share = (total + blocks - 1) / blocks;
+    const int64_t begin = min(total, (int64_t)blockIdx.x * share), end = min(total, begin + share);
+    PagedMeta meta{};
+    // the sequence that `begin` lies in
+    int64_t at = 0;
+    int seq = 0;
+    if (begin < end) {
+      for (int b0 = 0;; b0 += 32) {
+        const int64_t c = b0 + lane < bt.seqs ? paged_sequence(p, b0 + lane).head * a.kv_heads : 0;
+        int64_t sum = c;
+        for (int d = 1; d < 32; d <<= 1) {
+          const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
+          if (lane >= d) sum += o;
+        }
+        const uint32_t beyond = __ballot_sync(0xffffffffu, at + sum > begin);
+        if (beyond || b0 + 32 >= bt.seqs) {
+          const int l = beyond ? __ffs(beyond) - 1 : 31;
+          seq = b0 + l;
+          at += __shfl_sync(0xffffffffu, sum - c, l);
+          break;
+        }
+        at += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    int64_t now = begin;  // offset of the next part
+    while (ok) {
+      // the unit at `now`
+      PagedUnit u{};
+      bool open = false, head_part = false;
+      int64_t u1 = 0;
+      u.done = 1;
+      if (now < end) {
+        PagedSequence s = paged_sequence(p, seq);
+        while (s.head * a.kv_heads <= now - at) {
+          at += s.head * a.kv_heads;
+          s = paged_sequence(p, ++seq);
+        }
+        const int64_t in = now - at;
+        u.done = 0;
+        u.seq = seq;
+        u.kvh = (int)(in / s.head);
+        const int64_t rest = in - u.kvh * s.head;
+        int lo = 0, hi = s.tiles - 1;  // the tile of rows: first(i) <= rest < first(i + 1)
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (s.cost.first(mid) <= rest) lo = mid;
+          else hi = mid - 1;
+        }
+        const int64_t u0 = at + u.kvh * s.head + s.cost.first(lo), cost = s.cost.tile(lo);
+        u1 = u0 + cost;
+        const int64_t rows = (int64_t)s.n * G;
+        u.r0 = lo * 256;
+        u.rows = (int)min((int64_t)256, rows - u.r0);
+        u.alternate = rows <= kPagedTile;
+        u.tok0 = s.tok0;
+        u.pos0 = (int)max((int64_t)s.len - s.n, -((int64_t)1 << 30));
+        u.first = u.pos0 + u.r0 / G;
+        u.last = u.pos0 + (u.r0 + u.rows - 1) / G;
+        if (s.len > (int64_t)bt.most_pages * bt.page_size) {
+          u.bad = 1;
+        } else {
+          u.hi = max(0, u.last + 1);
+          u.lo = a.window ? (int)max((int64_t)0, (int64_t)u.first - a.window + 1) : 0;
+        }
+        const int tb = u.lo / kPagedTile, n = max(0, (u.hi + kPagedTile - 1) / kPagedTile - tb);
+        head_part = now > u0;
+        open = u1 > end;
+        u.tb = tb + (int)(n * (now - u0) / cost);
+        u.te = open ? tb + (int)(n * (end - u0) / cost) : tb + n;
+        u.slot = head_part ? 2 * (int)blockIdx.x : open ? 2 * (int)blockIdx.x + 1 : -1;
+        if (open && !head_part) meta = PagedMeta{1, (int)((u1 - 1) / share), u.kvh, u.r0, u.rows, u.tok0, u.pos0, 0};
+        now = min(u1, end);
+      }
+      const uint32_t us = uc % UNITS;
+      if (!(ok = mbar_wait_warp(&u_empty[us], ((uc / UNITS) & 1u) ^ 1u, abort_flag, p.err, 41))) break;
+      if (lane == 0) {
+        PagedUnit& d = units[us];
+        d.seq = u.seq, d.kvh = u.kvh, d.r0 = u.r0, d.rows = u.rows, d.tok0 = u.tok0, d.pos0 = u.pos0;
+        d.first = u.first, d.last = u.last;
+        d.tb = u.tb, d.te = u.te, d.lo = u.lo, d.hi = u.hi, d.alternate = u.alternate, d.slot = u.slot;
+        d.done = u.done, d.bad = u.bad, d.dirty = 0;
+        mbar_arrive(&u_full[us]);
+      }
+      __syncwarp();
+      ++uc;
+      if (u.done) break;
+      // K and V in the order of their products: K0 [K(i + 1)] V(i) where the
+      // halves alternate, K0 V(i) [K(i + 1)] where they share
+      const int n = u.te - u.tb;
+      const int* table = bt.page_table + u.seq * bt.table_ld;
+      for (int j = 0; j < 2 * n && ok; ++j, ++it) {
+        int t;
+        bool is_v;
+        if (j == 0) t = 0, is_v = false;
+        else if (j == 2 * n - 1) t = n - 1, is_v = true;
+        else if (u.alternate) is_v = !(j & 1), t = is_v ? j / 2 - 1 : (j + 1) / 2;
+        else is_v = j & 1, t = is_v ? j / 2 : j / 2;
+        const int key = (u.tb + t) * kPagedTile + lane * p.box;
+        int page = -1;
+        const bool wanted = lane * p.box < kPagedTile && key < u.hi && key + p.box > u.lo;
+        if (wanted) page = table[key / bt.page_size];
+        const bool real = wanted && page >= 0 && page < bt.pages;
+        if (__any_sync(0xffffffffu, wanted && !real) && lane == 0) units[us].bad = 1;
+        const uint32_t s = it % STAGES;
+        if (!(ok = mbar_wait_warp(&empty[s], ((it / STAGES) & 1u) ^ 1u, abort_flag, p.err, 42))) break;
+        const uint32_t boxes = (uint32_t)__popc(__ballot_sync(0xffffffffu, real));
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], boxes * (uint32_t)p.box * DH * 2);
+        __syncwarp();
+        if (real) {
+          const CUtensorMap* map = is_v ? &map_v : &map_k;
+          const uint32_t dst = ring + s * L::TILE + (uint32_t)(lane * p.box) * 128u;
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h)
+            tma_load_4d(dst + h * (kPagedTile * 128), map, h * 64, key % bt.page_size, u.kvh, page, &full[s]);
+        }
+        __syncwarp();
+      }
+    }
+    if (lane == 0) p.meta[blockIdx.x] = meta;
+    if (!ok)  // the copies in flight land before the block leaves
+      for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
+        mbar_wait_warp(&full[j % STAGES], (j / STAGES) & 1u, abort_flag, p.err, 43, /*ignore_abort=*/true);
+  } else if (warp == 9) {
+    // ---- products ----
+    bool ok = true;
+    uint32_t it = 0, uc = 0, pc[2] = {0, 0}, oc[2] = {0, 0}, vc = 0;
+    const uint32_t idesc_s = paged_idesc<T>(kPagedTile, false), idesc_o = paged_idesc<T>((a.dim + 15) / 16 * 16, true);
+    const int steps = (a.dim + 15) / 16;
+    if (p.stall_test) ok = mbar_wait_warp(drain, 0, abort_flag, p.err, 44);
+    auto wait_tile = [&](uint32_t i) {
+      return mbar_wait_warp(&full[i % STAGES], (i / STAGES) & 1u, abort_flag, p.err, 45);
+    };
+    // S of half w from the K tile in stage s
+    auto product_s = [&](int w, int q_tile, uint32_t s) {
+      if (elect_one()) {
+        const uint32_t q = q_smem + q_tile * L::TILE, k = ring + s * L::TILE;
+        for (int i = 0; i < steps; ++i) {
+          const uint32_t off = (i >> 2) * (kPagedTile * 128) + (i & 3) * 32;
+          umma_f16(tmem + w * 128, paged_desc(q + off, 16), paged_desc(k + off, 16), idesc_s, i > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[w]);
+      }
+      __syncwarp();
+    };
+    auto product_o = [&](int w, uint32_t s, bool add) {
+      if (elect_one()) {
+        const uint32_t v = ring + s * L::TILE;
+#pragma unroll
+        for (int i = 0; i < kPagedTile / 16; ++i)
+          umma_f16_tmem_a(tmem + 256 + w * 128, tmem + w * 128 + i * 8, paged_desc(v + i * 2048, kPagedTile * 128), idesc_o,
+                          add || i > 0 ? 1u : 0u);
+        umma_commit(&pv_done[w]);
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+      __syncwarp();
+    };
+    while (ok) {
+      const uint32_t us = uc % UNITS;
+      if (!(ok = mbar_wait_warp(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 46))) break;
+      const PagedUnit& u = units[us];
+      if (u.done) break;
+      const int n = u.te - u.tb, alternate = u.alternate, tb = u.tb;
+      const int count[2] = {paged_count(u, 0, G), paged_count(u, 1, G)};
+      if (!(ok = mbar_wait_warp(q_full, uc & 1u, abort_flag, p.err, 47))) break;
+      tc_fence_after();
+      if (n > 0) {
+        if (!(ok = wait_tile(it))) break;
+        tc_fence_after();
+        if (count[0] > 0) product_s(0, 0, it % STAGES);
+        if (!alternate && count[1] > 0) product_s(1, 1, it % STAGES);
+        commit(&empty[it % STAGES]);
+        ++it;
+        if (alternate && n > 1) {
+          if (!(ok = wait_tile(it))) break;
+          tc_fence_after();
+          product_s(1, 0, it % STAGES);
+          commit(&empty[it % STAGES]);
+          ++it;
+        }
+      }
+      if (n <= (alternate ? 2 : 1)) commit(q_empty);
+      for (int t = 0; t < n && ok; ++t) {
+        const uint32_t v = it++;
+        if (!(ok = wait_tile(v))) break;
+        if (paged_masked(u, tb + t, a.window)) {
+          if (lane == 0) mbar_arrive(v_seen);
+          __syncwarp();
+          if (!(ok = mbar_wait_warp(v_clean, vc & 1u, abort_flag, p.err, 48))) break;
+          ++vc;
+        }
+        const int ahead = t + (alternate ? 2 : 1);  // S of this tile of keys follows
+        const uint32_t k = it;
+        if (ahead < n) {
+          ++it;
+          if (!alternate && !(ok = wait_tile(k))) break;
+        }
+        for (int w = alternate ? t & 1 : 0; w < (alternate ? (t & 1) + 1 : 2); ++w) {
+          const int i = alternate ? t >> 1 : t;  // number of the tile among the half's
+          if (i >= count[w]) continue;
+          if (i == 0) {
+            if (!(ok = mbar_wait_warp(&o_free[w], (oc[w] & 1u) ^ 1u, abort_flag, p.err, 49))) break;
+            ++oc[w];
+          }
+          if (!(ok = mbar_wait_warp(&p_full[w], pc[w] & 1u, abort_flag, p.err, 50))) break;
+          ++pc[w];
+          tc_fence_after();
+          product_o(w, v % STAGES, i > 0);
+          if (alternate) commit(&empty[v % STAGES]);
+          if (i + 1 < count[w]) {
+            if (alternate) {
+              if (!(ok = wait_tile(k))) break;
+              tc_fence_after();
+            }
+            product_s(w, alternate ? 0 : w, k % STAGES);
+          }
+        }
+        if (!ok) break;
+        if (!alternate) commit(&empty[v % STAGES]);
+        if (ahead < n) {
+          commit(&empty[k % STAGES]);
+          if (ahead == n - 1) commit(q_empty);
+        }
+      }
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(&u_empty[us]);
+      __syncwarp();
+      ++uc;
+    }
+    if (!ok) {
+      commit(drain);
+      mbar_wait_warp(drain, 0, abort_flag, p.err, 52, /*ignore_abort=*/true);
+    }
+  } else if (warp >= 10) {
+    // ---- Q, and values of tiles that are seen in part ----
+    const int me = warp - 10;
+    bool ok = true;
+    uint32_t it = 0, uc = 0, vc = 0;
+    while (ok) {
+      const uint32_t us = uc % UNITS;
+      if (!(ok = mbar_wait_warp(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 53))) break;
+      PagedUnit& u = units[us];
+      if (u.done) break;
+      if (!(ok = mbar_wait_warp(q_empty, (uc & 1u) ^ 1u, abort_flag, p.err, 54))) break;
+      {
+        constexpr int CH = DH / 8;  // 16-byte pieces of a row
+        const int c = lane % CH, rows = u.rows;
+        const T* q = static_cast<const T*>(a.q) + (int64_t)u.tok0 * a.q_token + (int64_t)u.kvh * G * a.q_head + c * 8;
+        for (int r = me * (32 / CH) + lane / CH; r < rows; r += 2 * (32 / CH)) {
+          const int row = u.r0 + r, tok = row / G, g = row - tok * G;
+          const uint32_t dst = q_smem + (r >> 7) * L::TILE + (c >> 3) * (kPagedTile * 128) + (r & 127) * 128 +
+                               (((c & 7) ^ (r & 7)) << 4);
+          const bool real = c * 8 < a.dim;
+          cp_async16(dst, real ? static_cast<const void*>(q + (int64_t)tok * a.q_token + (int64_t)g * a.q_head) : a.q, real);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        __syncwarp();
+      }
+      const int n = u.te - u.tb;
+      for (int t = 0; t < n && ok; ++t) {
+        if (!paged_masked(u, u.tb + t, a.window)) continue;
+        const uint32_t v = it + (u.alternate ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1), s = v % STAGES;
+        // the products wait at this tile: it has landed, and stays until it is clean
+        if (!(ok = mbar_wait_warp(v_seen, vc & 1u, abort_flag, p.err, 51))) break;
+        ++vc;
+        if (!(ok = mbar_wait_warp(&full[s], (v / STAGES) & 1u, abort_flag, p.err, 55))) break;
+        const int key0 = (u.tb + t) * kPagedTile;
+        uint32_t found = 0;
+#pragma unroll 4
+        for (int i = me * 32 + lane; i < kPagedTile * HALVES * 8; i += 64) {
+          const int key = key0 + ((i >> 3) & 127);
+          uint4* x = reinterpret_cast<uint4*>(smem + s * L::TILE + i * 16);
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (key >= u.lo && key < u.hi) {
+            w = *x;
+            const uint32_t m0 = not_finite2<T>(w.x), m1 = not_finite2<T>(w.y), m2 = not_finite2<T>(w.z),
+                           m3 = not_finite2<T>(w.w);
+            if (!(m0 | m1 | m2 | m3)) continue;
+            found = 1;
+            w = make_uint4(w.x & ~m0, w.y & ~m1, w.z & ~m2, w.w & ~m3);
+          }
+          *x = w;
+        }
+        if (found) u.dirty = 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_clean);
+        __syncwarp();
+      }
+      it += 2 * n;
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(&u_empty[us]);
+      __syncwarp();
+      ++uc;
+    }
+  } else {
+    // ---- softmax ----
+    const int w = warp >> 2, quarter = warp & 3;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_tmem = tmem + w * 128 + lanes;
+    bool ok = true;
+    uint32_t uc = 0, cnt[2] = {0, 0}, oc = 0, mc = 0;  // oc: units of which the first half had tiles
+    while (ok) {
+      const uint32_t us = uc % UNITS;
+      if (!(ok = mbar_wait_warp(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 56))) break;
+      const PagedUnit& u = units[us];
+      if (u.done) break;
+      const int alternate = u.alternate, tb = u.tb;
+      const int count[2] = {paged_count(u, 0, G), paged_count(u, 1, G)};
+      const int r = (alternate ? 0 : w * kPagedTile) + quarter * 32 + lane;  // row of the unit
+      const bool real = r < u.rows, active = (alternate ? 0 : w * kPagedTile) + quarter * 32 < u.rows;
+      const int tok = (u.r0 + r) / G, position = u.pos0 + tok;
+      float m = -INFINITY, sum = 0.0f;
+      const uint32_t o_tmem = tmem + 256 + w * 128 + lanes;
+      for (int i = 0; i < count[w] && ok; ++i) {
+        const int t = tb + (alternate ? 2 * i + w : i);
+        if (!(ok = mbar_wait_warp(&s_full[w], (cnt[w] + i) & 1u, abort_flag, p.err, 57))) break;
+        tc_fence_after();
+        if (active) {
+          uint32_t s[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            __syncwarp();
+            FTB_TMEM_LD32(s_tmem + c * 32, s[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) FTB_TMEM_WAIT_LD32(s[c]);
+          if (p.negative) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) s[c][k] ^= 0x80000000u;
+          }
+          // columns that this row sees: low < column <= high
+          const int high = position - t * kPagedTile, low = a.window ? (int)max((int64_t)high - a.window, (int64_t)-1) : -1;
+          if (__any_sync(0xffffffffu, real && (high < kPagedTile - 1 || low >= 0))) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (c * 32 + k > high || c * 32 + k <= low) s[c][k] = 0xFF800000u;
+          }
+          float top[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+            for (int k = 1; k < 32; ++k) top[c] = fmaxf(top[c], __uint_as_float(s[c][k]));
+          }
+          const float high_s = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
+          const bool raise = real && high_s > m + kPagedRaise;
+          if (__any_sync(0xffffffffu, raise)) {
+            float keep = 1.0f;
+            if (raise) {
+              keep = ex2(m - high_s);
+              sum *= keep;
+              m = high_s;
+            }
+            if (i > 0) {
+              if (!(ok = mbar_wait_warp(&pv_done[w], (cnt[w] + i - 1) & 1u, abort_flag, p.err, 58))) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c * 32 < a.dim; ++c) {
+                uint32_t o[32];
+                __syncwarp();
+                FTB_TMEM_LD32(o_tmem + c * 32, o);
+                FTB_TMEM_WAIT_LD32(o);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                FTB_TMEM_ST32(o_tmem + c * 32, o);
+              }
+            }
+          }
+          const float base = m == -INFINITY ? 0.0f : m;
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t o[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int c = 2 * h + (k >> 4), e = 2 * k & 31;
+              const float x = ex2(__fmaf_rn(__uint_as_float(s[c][e]), a.scale, -base));
+              const float y = ex2(__fmaf_rn(__uint_as_float(s[c][e + 1]), a.scale, -base));
+              part[k & 1] += x;
+              part[2 + (k & 1)] += y;
+              o[k] = pack2<T>(x, y);
+            }
+            FTB_TMEM_ST32(s_tmem + h * 32, o);
+          }
+          sum += (part[0] + part[1]) + (part[2] + part[3]);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[w]);
+        __syncwarp();
+      }
+      if (!ok) break;
+      // ---- O ----
+      const uint32_t end[2] = {cnt[0] + count[0], cnt[1] + count[1]};
+      const bool both = alternate && count[0] > 0, mine = !alternate || w == 0;
+      float f[2] = {1.0f, 1.0f};  // factors of the halves' O
+      if (both && w == 1) {
+        // the first half has read those of the unit before
+        if (!(ok = mbar_wait_warp(&o_free[0], (oc & 1u) ^ 1u, abort_flag, p.err, 61))) break;
+        ml[quarter * 32 + lane] = make_float2(m, sum);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ml_full);
+        __syncwarp();
+      }
+      if (both && w == 0) {
+        if (!(ok = mbar_wait_warp(ml_full, mc & 1u, abort_flag, p.err, 59))) break;
+        const float2 x = ml[quarter * 32 + lane];
+        const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
+        f[0] = ex2(m - base);
+        f[1] = ex2(x.x - base);
+        sum = sum * f[0] + x.y * f[1];
+        m = top;
+      }
+      if (both) ++mc;
+      if (mine) {
+        for (int h = 0; h < 2 && ok; ++h)
+          if ((both || h == w) && count[h] > 0)
+            ok = mbar_wait_warp(&pv_done[h], (end[h] - 1) & 1u, abort_flag, p.err, 60);
+        if (!ok) break;
+        tc_fence_after();
+        const bool bad = u.bad, dirty = u.dirty;
+        const int g = u.r0 + r - tok * G;
+        float* part = p.parts + (int64_t)max(u.slot, 0) * p.rows_bound * (2 + DH);
+        if (u.slot >= 0 && real) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, bad ? NAN : sum);
+        part += 2 * p.rows_bound + (int64_t)r * DH;
+        T* out = static_cast<T*>(a.out) + (int64_t)(u.tok0 + tok) * a.o_token + (int64_t)(u.kvh * G + g) * a.o_head;
+        const float inv = 1.0f / sum;
+        if (active) {
+#pragma unroll 1
+          for (int c = 0; c * 32 < a.dim; ++c) {
+            float v[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (!((both || h == w) && count[h] > 0)) continue;
+              uint32_t o[32];
+              __syncwarp();
+              FTB_TMEM_LD32(tmem + 256 + h * 128 + lanes + c * 32, o);
+              FTB_TMEM_WAIT_LD32(o);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = both ? __fmaf_rn(__uint_as_float(o[k]), f[h], v[k]) : __uint_as_float(o[k]);
+            }
+            if (dirty && real) {  // values that are not finite and that this row sees, in tiles seen in part
+              for (int key = (int)max((int64_t)u.tb * kPagedTile, a.window ? (int64_t)position - a.window + 1 : 0);
+                   key <= position && key < u.te * kPagedTile; ++key) {
+                if (!paged_masked(u, key / kPagedTile, a.window)) continue;
+                const int page = a.batch.page_table[u.seq * a.batch.table_ld + key / a.batch.page_size];
+                if (page < 0 || page >= a.batch.pages) continue;
+                const T* x = static_cast<const T*>(a.values) + page * a.v_page + key % a.batch.page_size * a.v_token +
+                             (int64_t)u.kvh * a.v_head + c * 32;
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (c * 32 + k < a.dim && !isfinite(to_f32(x[k]))) v[k] = NAN;
+              }
+            }
+            if (u.slot >= 0) {
+              if (real) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 4)
+                  *reinterpret_cast<float4*>(part + c * 32 + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+              }
+            } else if (real) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = bad ? NAN : position < 0 ? 0.0f : v[k] * inv;
+#pragma unroll
+              for (int k = 0; k < 32; k += 8)
+                if (c * 32 + k < a.dim)
+                  *reinterpret_cast<uint4*>(out + c * 32 + k) =
+                      make_uint4(pack2<T>(v[k], v[k + 1]), pack2<T>(v[k + 2], v[k + 3]), pack2<T>(v[k + 4], v[k + 5]),
+                                 pack2<T>(v[k + 6], v[k + 7]));
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          for (int h = 0; h < 2; ++h)
+            if ((both || h == w) && count[h] > 0) mbar_arrive(&o_free[h]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&u_empty[us]);
+      __syncwarp();
+      cnt[0] = end[0];
+      cnt[1] = end[1];
+      oc += count[0] > 0;
+      ++uc;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// Units that several blocks worked on: block x of the grid joins the one that
+// block x of paged_attention_kernel began and did not finish, a warp a row.
+// O = sum_k O_k 2^(m_k - m) / sum_k sum_k 2^(m_k - m), parts in order.
+template <typename T, int DH>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedTensorParams p) {
+  grid_dep_wait();
+  grid_dep_trigger();
+  constexpr int E = DH / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const PagedMeta u = p.meta[blockIdx.x];
+  if (!u.open) return;
+  const PagedAttentionParams& a = p.a;
+  const int parts = u.last - (int)blockIdx.x + 1;
+  const int64_t stride = (int64_t)p.rows_bound * (2 + DH);
+  auto part = [&](int k) { return p.parts + (k == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + k)) * stride; };
+  for (int r = blockIdx.y * 32 + warp; r < min(u.rows, (int)blockIdx.y * 32 + 32); r += 8) {
+    float top = -INFINITY;
+    for (int k = lane; k < parts; k += 32) top = fmaxf(top, part(k)[2 * r]);
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+      const float2 x = *reinterpret_cast<const float2*>(part(k) + 2 * r);
+      const float* v = part(k) + 2 * p.rows_bound + (int64_t)r * DH + lane * E;
+      float t[E];
+      if constexpr (E == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(v);
+        t[0] = y.x, t[1] = y.y, t[2] = y.z, t[3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(v);
+        t[0] = y.x, t[1] = y.y;
+      }
+      const float f = ex2(x.x - base);
+      sum = __fmaf_rn(x.y, f, sum);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = lane * E + e < a.dim ? __fmaf_rn(t[e], f, o[e]) : 0.0f;
+    }
+    const int tok = (u.r0 + r) / p.group, g = u.r0 + r - tok * p.group;
+    T* out = static_cast<T*>(a.out) + (int64_t)(u.tok0 + tok) * a.o_token + (int64_t)(u.kvh * p.group + g) * a.o_head;
+    const bool nothing = u.pos0 + tok < 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (lane * E + e < a.dim) out[lane * E + e] = from_f32<T>(nothing ? 0.0f : o[e] / sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// A pool as the kernel reads it: boxes of 64 elements of a head by `box` tokens.
+inline bool make_map_pool(CUtensorMap* map, const void* base, int type, int64_t dim, int64_t page_size, int64_t kv_heads,
+                          int64_t pages, int64_t token, int64_t head, int64_t page, int box) {
+  PFN_encodeTiled enc = tma_encoder();
+  if (!enc) return false;
+  auto bytes = [&](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 ? stride * 2 : (dim * 2 + 15) / 16 * 16); };
+  cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)page_size, (cuuint64_t)kv_heads, (cuuint64_t)pages};
+  cuuint64_t strides[3] = {bytes(page_size, token), bytes(kv_heads, head), bytes(pages, page)};
+  cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(map, type == FTB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+             const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Whether the tensor-core kernel takes a call: 16-bit types, heads of up to 128
+// in eights, pages of whole 16 tokens, and 16-byte boundaries throughout.
+inline bool paged_on_tensor_cores(const PagedAttentionParams& p, int type) {
+  if (type == FTB_F32 || p.dim > 128 || p.dim % 8 || p.batch.page_size % 16) return false;
+  for (const void* x : {p.q, (const void*)p.out, p.keys, p.values})
+    if (reinterpret_cast<uintptr_t>(x) & 15) return false;
+  for (int64_t s : {p.q_token, p.q_head, p.o_token, p.o_head, p.k_page, p.k_token, p.k_head, p.v_page, p.v_token, p.v_head})
+    if (s % 8) return false;
+  return true;
+}
+
+inline int paged_rows_bound(const PagedAttentionParams& p) {
+  return (int)std::min<int64_t>(256, ((int64_t)p.tokens * (p.heads / p.kv_heads) + 3) / 4 * 4);
+}
+constexpr int64_t kPagedMetaBytes = (int64_t)kPagedBlocks * (int64_t)sizeof(PagedMeta);
+inline int64_t paged_workspace(const PagedAttentionParams& p) {
+  return kPagedMetaBytes + 2 * (int64_t)kPagedBlocks * paged_rows_bound(p) * (2 + (p.dim <= 64 ? 64 : 128)) * 4;
+}
+
+inline cudaError_t paged_attention_prepare() {
+  cudaError_t e = cudaSuccess;
+  auto set = [&](auto kernel, int bytes) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  };
+  set(paged_attention_kernel<__half, 64>, PagedSmem<64>::TOTAL);
+  set(paged_attention_kernel<__half, 128>, PagedSmem<128>::TOTAL);
+  set(paged_attention_kernel<__nv_bfloat16, 64>, PagedSmem<64>::TOTAL);
+  set(paged_attention_kernel<__nv_bfloat16, 128>, PagedSmem<128>::TOTAL);
+  return e;
+}
+
+template <typename T, int DH>
+cudaError_t launch_paged_as(PagedTensorParams& p, int type, int blocks, cudaStream_t s) {
+  const PagedAttentionParams& a = p.a;
+  CUtensorMap map_k, map_v;
+  if (!make_map_pool(&map_k, a.keys, type, a.dim, a.batch.page_size, a.kv_heads, a.batch.pages, a.k_token, a.k_head, a.k_page, p.box) ||
+      !make_map_pool(&map_v, a.values, type, a.dim, a.batch.page_size, a.kv_heads, a.batch.pages, a.v_token, a.v_head, a.v_page, p.box))
+    return cudaErrorInvalidValue;
+  cudaError_t e = pdl_launch(paged_attention_kernel<T, DH>, dim3((unsigned)blocks), dim3(kPagedThreads), PagedSmem<DH>::TOTAL, s,
+                             map_k, map_v, p);
+  if (e == cudaSuccess)
+    e = pdl_launch(paged_join_kernel<T, DH>, dim3((unsigned)blocks, (unsigned)(p.rows_bound + 31) / 32), dim3(256), 0, s, p);
+  return e;
+}
+
+inline cudaError_t launch_paged_attention(const PagedAttentionParams& a, int type, void* workspace, int sm_count, int* err,
+                                          int stall, cudaStream_t s) {
+  const int blocks = std::min(sm_count, kPagedBlocks);
+  PagedTensorParams p{};
+  p.a = a;
+  p.a.scale = std::fabs(a.scale);
+  if (p.a.scale == 0.0f) p.a.scale = 1e-30f;  // equal weights either way, and a masked score stays -inf
+  p.negative = a.scale < 0.0f;
+  p.group = a.heads / a.kv_heads;
+  p.box = 16;
+  while (p.box < kPagedTile && a.batch.page_size % (2 * p.box) == 0) p.box *= 2;
+  p.rows_bound = paged_rows_bound(a);
+  p.meta = static_cast<PagedMeta*>(workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kPagedMetaBytes);
+  p.err = err;
+  p.stall_test = stall;
+  if (type == FTB_F16) return a.dim <= 64 ? launch_paged_as<__half, 64>(p, type, blocks, s) : launch_paged_as<__half, 128>(p, type, blocks, s);
+  return a.dim <= 64 ? launch_paged_as<__nv_bfloat16, 64>(p, type, blocks, s) : launch_paged_as<__nv_bfloat16, 128>(p, type, blocks, s);
+}
+
+}  // namespace ftb

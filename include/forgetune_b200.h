@@ -305,7 +305,8 @@ typedef struct {
 } ftb_fp8_linear_args;
 FORGETUNE_EXPORT int ftb_fp8_linear(const ftb_fp8_linear_args* args, void* stream);
 
-/* Failure-detection hook (tests): while stall != 0 every ftb_fp8_linear launch makes one pipeline wait that
+/* Failure-detection hook (tests): while stall != 0 every ftb_fp8_linear launch, and every ftb_paged_attention
+ * launch of the tensor-core kernel, makes one pipeline wait that
  * nothing completes run out (about 2 s); the kernel leaves cleanly and the next call returns -5. */
 FORGETUNE_EXPORT int ftb_fp8_set_fault_injection(int stall);
 
