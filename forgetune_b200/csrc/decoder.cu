@@ -119,6 +119,7 @@ static PagedBatchParams params(const ftb_paged_batch& b, const ftb_paged_cache& 
   p.most_pages = (int)b.most_pages;
   p.page_size = (int)c.page_size;
   p.pages = (int)c.pages;
+  p.by_page = FastDiv((uint32_t)c.page_size);
   return p;
 }
 

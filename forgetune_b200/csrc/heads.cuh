@@ -30,6 +30,18 @@ namespace ftb {
 constexpr int kHeadsThreads = 256;
 constexpr int kHeadsMaxDim = 512;
 
+// n / d for 0 <= n < 2^31 by a product: with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1 it is
+// (floor(m n / 2^32) + n) / 2^l (Granlund and Montgomery's division by invariant integers).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t by) : d(by), mul(0), shift(0) {
+    while (((uint64_t)1 << shift) < d) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int of(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
+
 // New tokens of several sequences and the pages that hold them.
 struct PagedBatchParams {
   const int* page_table;  // [seqs, most_pages], rows table_ld apart
@@ -37,6 +49,7 @@ struct PagedBatchParams {
   const int* starts;      // [seqs + 1] first row of each sequence
   const int* lengths;     // [seqs] tokens with the new ones
   int seqs, most_pages, page_size, pages;
+  FastDiv by_page;
 };
 
 // Number of entries <= t among starts[0 .. n), by a whole warp (32 blocks a step).
@@ -160,7 +173,7 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const HeadsParams 
       } else {
         int seq;
         if (place_of(p.batch, t, lane, &seq, &position)) {
-          const int64_t n = position >= 0 ? position / p.batch.page_size : p.batch.most_pages;
+          const int n = position >= 0 ? p.batch.by_page.of((int)position) : p.batch.most_pages;
           page = n < p.batch.most_pages ? p.batch.page_table[seq * p.batch.table_ld + n] : -1;
           if (page < 0 || page >= p.batch.pages) page = -1;
         }

@@ -65,6 +65,9 @@ struct PagedMeta {
 struct PagedTensorParams {
   PagedAttentionParams a;
   int group;         // query heads of a kv head
+  FastDiv by_group;
+  int step;          // tokens in 256 rows
+  int q_tma;         // Q has a TMA map: the group divides a tile's rows
   int box;           // tokens of a TMA box: in one page
   int negative;      // the scale is below 0 (a.scale is its absolute value)
   int rows_bound;    // rows of a part in the workspace
@@ -86,39 +89,45 @@ struct PagedUnit {
   volatile int dirty;  // a value that is not finite in a tile seen in part
 };
 
-// Cost of the first n tiles of rows of a sequence, in keys times G: tile i sees
-// about base + 256 (i + 1) / G keys, at most `cap`.
+// Cost of the first n tiles of rows of a sequence, in keys: tile i sees about
+// base + step (i + 1), at most `cap`.
 struct PagedCost {
-  int64_t base, cap, over;
-  __device__ __forceinline__ int64_t tile(int64_t i) const { return min(cap, base + 256 * (i + 1)) + over; }
-  __device__ __forceinline__ int64_t first(int64_t n) const {
-    const int64_t k = cap <= base ? 0 : min(n, (cap - base) / 256);
-    return k * base + 128 * k * (k + 1) + (n - k) * (k < n ? cap : 0) + n * over;
+  int64_t base, step, cap;
+  __device__ __forceinline__ int64_t tile(int i) const { return min(cap, base + step * (i + 1)) + kPagedUnitOver; }
+  __device__ __forceinline__ int64_t first(int n) const {
+    int64_t k = n;  // tiles below the cap
+    if (cap < base + step * n) k = cap <= base ? 0 : min((int64_t)n, (int64_t)((uint32_t)(cap - base) / (uint32_t)step));
+    return k * base + step * (k * (k + 1) / 2) + (n - k) * cap + (int64_t)n * kPagedUnitOver;
   }
 };
 
 struct PagedSequence {
   int tok0, n, len, tiles;
   PagedCost cost;
-  int64_t head;  // cost of a kv head
+  int64_t head, whole;  // cost of a kv head, of all
 };
 
 __device__ __forceinline__ PagedSequence paged_sequence(const PagedTensorParams& p, int b) {
   const PagedBatchParams& t = p.a.batch;
   PagedSequence s;
-  s.tok0 = max(0, min(t.starts[b], p.a.tokens));
-  s.n = max(0, min(t.starts[b + 1], p.a.tokens) - s.tok0);
+  const int start = t.starts[b], stop = t.starts[b + 1];
   s.len = t.lengths[b];
+  s.tok0 = max(0, min(start, p.a.tokens));
+  s.n = max(0, min(stop, p.a.tokens) - s.tok0);
   const int64_t rows = (int64_t)s.n * p.group;
-  s.tiles = rows == 0 ? 0 : rows <= kPagedTile ? 1 : (int)((rows + 255) / 256);
-  const int64_t G = p.group, len = max((int64_t)0, min((int64_t)s.len, (int64_t)t.most_pages * t.page_size));
-  s.cost.base = max((int64_t)0, len - s.n) * G;
-  s.cost.cap = s.tiles == 1 ? len * G : (int64_t)1 << 50;
-  if (p.a.window) s.cost.cap = min(s.cost.cap, (int64_t)p.a.window * G + (s.tiles == 1 ? rows : 256));
-  s.cost.over = kPagedUnitOver * G;
+  s.tiles = rows == 0 ? 0 : rows <= kPagedTile ? 1 : (int)((rows + 255) >> 8);
+  const int64_t len = max((int64_t)0, min((int64_t)s.len, (int64_t)t.most_pages * t.page_size));
+  s.cost.base = max((int64_t)0, len - s.n);
+  s.cost.step = p.step;
+  s.cost.cap = len;
+  if (p.a.window) s.cost.cap = min(len, (int64_t)p.a.window + p.step);
   s.head = s.cost.first(s.tiles);
+  s.whole = s.head * p.a.kv_heads;
   return s;
 }
+
+// floor(x / y) of whole numbers below 2^53
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) { return (int64_t)((double)x / (double)y); }
 
 template <int DH>
 struct PagedSmem {
@@ -130,7 +139,7 @@ struct PagedSmem {
   static constexpr int UNIT_OFF = ML_OFF + 128 * 8;
   static constexpr int UNITS = 2;
   static constexpr int BAR_OFF = (UNIT_OFF + UNITS * (int)sizeof(PagedUnit) + 15) / 16 * 16;
-  static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 4 + 4;
+  static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 5 + 4;
   static constexpr int TOTAL = 1024 + BAR_OFF + 8 * NBAR + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
 };
@@ -188,16 +197,16 @@ __device__ __forceinline__ bool paged_masked(const PagedUnit& u, int t, int wind
 }
 
 // End of the tiles that half w of a unit sees.
-__device__ __forceinline__ int paged_end(const PagedUnit& u, int w, int group) {
+__device__ __forceinline__ int paged_end(const PagedUnit& u, int w, const FastDiv& by_group) {
   if (u.alternate || w == 1) return u.te;
-  const int last = u.pos0 + (u.r0 + min(u.rows, kPagedTile) - 1) / group;
+  const int last = u.pos0 + by_group.of(u.r0 + min(u.rows, kPagedTile) - 1);
   return max(u.tb, min(u.te, last < 0 ? 0 : last / kPagedTile + 1));
 }
 
 // Tiles of keys that half w takes.
-__device__ __forceinline__ int paged_count(const PagedUnit& u, int w, int group) {
+__device__ __forceinline__ int paged_count(const PagedUnit& u, int w, const FastDiv& by_group) {
   if (u.alternate) return (u.te - u.tb + 1 - w) >> 1;
-  return w == 1 && u.rows <= kPagedTile ? 0 : paged_end(u, w, group) - u.tb;
+  return w == 1 && u.rows <= kPagedTile ? 0 : paged_end(u, w, by_group) - u.tb;
 }
 
 template <typename T>
@@ -208,17 +217,35 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
-// Halves of a word that are infinities or NaN, as all-ones halves.
+// Top bit of each half of a word: an infinity or a NaN (the exponent's last bit
+// carries into it; the other bits mean nothing).
 template <typename T>
-__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
-  return __vcmpeq2(w & e, e);
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  return std::is_same<T, __half>::value ? (w & 0x7C007C00u) + 0x04000400u : (w & 0x7F807F80u) + 0x00800080u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+  const uint32_t m = not_finite<T>(w);
+  return w & ~((m & 0x8000u ? 0xFFFFu : 0u) | (m & 0x80000000u ? 0xFFFF0000u : 0u));
+}
+
+// (x, y) = (x, y) a + b
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %2};\n\tmov.b64 r, {%3, %3};\n\t"
+      "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 template <typename T, int DH>
 __global__ void __launch_bounds__(kPagedThreads, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                           const PagedTensorParams p) {
+                           const __grid_constant__ CUtensorMap map_q, const PagedTensorParams p) {
   using L = PagedSmem<DH>;
   constexpr int STAGES = L::STAGES, HALVES = L::HALVES, UNITS = L::UNITS;
   extern __shared__ uint8_t smem_raw[];
@@ -232,7 +259,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   uint64_t* q_full = u_empty + UNITS;    // its Q landed
   uint64_t* q_empty = q_full + 1;        // its last S = Q K^T is done
   uint64_t* s_full = q_empty + 1;        // [2] S of a half
-  uint64_t* p_full = s_full + 2;         // [2] its P is in tensor memory, O rescaled
+  uint64_t* p_half = s_full + 2;         // [2] its P of 64 keys is in tensor memory, O rescaled
+  uint64_t* p_full = p_half + 2;         // [2] all of its P
   uint64_t* pv_done = p_full + 2;        // [2] P V is done
   uint64_t* o_free = pv_done + 2;        // [2] O was read (in units where the half had tiles)
   uint64_t* v_seen = o_free + 2;         // a tile of V seen in part is there
@@ -259,6 +287,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     mbar_init(q_empty, 1);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&s_full[w], 1);
+      mbar_init(&p_half[w], 4);
       mbar_init(&p_full[w], 4);
       mbar_init(&pv_done[w], 1);
       mbar_init(&o_free[w], 4);
@@ -295,19 +324,18 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     bool ok = true;
     uint32_t it = 0, uc = 0;
     const PagedBatchParams& bt = a.batch;
-    int64_t total = 0;
-    for (int b = lane; b < bt.seqs; b += 32) total += paged_sequence(p, b).head * a.kv_heads;
+    int64_t total = 0, mine = 0;
+    for (int b = lane; b < bt.seqs; b += 32) total += mine = paged_sequence(p, b).whole;
     for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    const int64_t blocks = max((int64_t)1, min((int64_t)gridDim.x, total / ((int64_t)kPagedLeast * G)));
-    const int64_t share = (total + blocks - 1) / blocks;
+    const int blocks = (int)max((int64_t)1, min((int64_t)gridDim.x, total / kPagedLeast));
+    const int64_t share = quotient(total, blocks) + 1;
     const int64_t begin = min(total, (int64_t)blockIdx.x * share), end = min(total, begin + share);
     PagedMeta meta{};
-    // the sequence that `begin` lies in
-    int64_t at = 0;
+    int64_t at = 0;  // offset of the sequence that `begin` lies in
     int seq = 0;
     if (begin < end) {
       for (int b0 = 0;; b0 += 32) {
-        const int64_t c = b0 + lane < bt.seqs ? paged_sequence(p, b0 + lane).head * a.kv_heads : 0;
+        const int64_t c = b0 + lane >= bt.seqs ? 0 : bt.seqs <= 32 ? mine : paged_sequence(p, b0 + lane).whole;
         int64_t sum = c;
         for (int d = 1; d < 32; d <<= 1) {
           const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
@@ -323,40 +351,38 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         at += __shfl_sync(0xffffffffu, sum, 31);
       }
     }
+    PagedSequence s{};
+    if (begin < end) s = paged_sequence(p, seq);
     int64_t now = begin;  // offset of the next part
     while (ok) {
       // the unit at `now`
       PagedUnit u{};
-      bool open = false, head_part = false;
-      int64_t u1 = 0;
       u.done = 1;
       if (now < end) {
-        PagedSequence s = paged_sequence(p, seq);
-        while (s.head * a.kv_heads <= now - at) {
-          at += s.head * a.kv_heads;
+        while (s.whole <= now - at) {
+          at += s.whole;
           s = paged_sequence(p, ++seq);
         }
-        const int64_t in = now - at;
         u.done = 0;
         u.seq = seq;
-        u.kvh = (int)(in / s.head);
-        const int64_t rest = in - u.kvh * s.head;
+        int64_t rest = now - at;
+        u.kvh = (int)quotient(rest, s.head);
+        rest -= u.kvh * s.head;
         int lo = 0, hi = s.tiles - 1;  // the tile of rows: first(i) <= rest < first(i + 1)
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
           if (s.cost.first(mid) <= rest) lo = mid;
           else hi = mid - 1;
         }
-        const int64_t u0 = at + u.kvh * s.head + s.cost.first(lo), cost = s.cost.tile(lo);
-        u1 = u0 + cost;
+        const int64_t cost = s.cost.tile(lo), u0 = now - (rest - s.cost.first(lo)), u1 = u0 + cost;
         const int64_t rows = (int64_t)s.n * G;
         u.r0 = lo * 256;
         u.rows = (int)min((int64_t)256, rows - u.r0);
         u.alternate = rows <= kPagedTile;
         u.tok0 = s.tok0;
         u.pos0 = (int)max((int64_t)s.len - s.n, -((int64_t)1 << 30));
-        u.first = u.pos0 + u.r0 / G;
-        u.last = u.pos0 + (u.r0 + u.rows - 1) / G;
+        u.first = u.pos0 + p.by_group.of(u.r0);
+        u.last = u.pos0 + p.by_group.of(u.r0 + u.rows - 1);
         if (s.len > (int64_t)bt.most_pages * bt.page_size) {
           u.bad = 1;
         } else {
@@ -364,12 +390,28 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           u.lo = a.window ? (int)max((int64_t)0, (int64_t)u.first - a.window + 1) : 0;
         }
         const int tb = u.lo / kPagedTile, n = max(0, (u.hi + kPagedTile - 1) / kPagedTile - tb);
-        head_part = now > u0;
-        open = u1 > end;
-        u.tb = tb + (int)(n * (now - u0) / cost);
-        u.te = open ? tb + (int)(n * (end - u0) / cost) : tb + n;
-        u.slot = head_part ? 2 * (int)blockIdx.x : open ? 2 * (int)blockIdx.x + 1 : -1;
-        if (open && !head_part) meta = PagedMeta{1, (int)((u1 - 1) / share), u.kvh, u.r0, u.rows, u.tok0, u.pos0, 0};
+        // where a share's border cuts the unit, the same for the blocks on either side; not within two tiles of its ends
+        auto cut = [&](int64_t x) {
+          const int c = (int)((float)n * ((float)(x - u0) / (float)cost) + 0.5f);
+          return c < 2 ? 0 : n - c < 2 ? n : c;
+        };
+        const int c1 = now > u0 ? cut(now) : 0, c2 = u1 > end ? cut(end) : n;
+        if (c1 == n && n > 0) {  // the block before took all of it
+          now = min(u1, end);
+          continue;
+        }
+        if (u1 > end && c2 == 0) {  // the block behind does
+          u.done = 1;
+        } else {
+          u.tb = tb + c1;
+          u.te = tb + c2;
+          u.slot = c1 > 0 ? 2 * (int)blockIdx.x : c2 < n ? 2 * (int)blockIdx.x + 1 : -1;
+          if (c1 == 0 && c2 < n) {
+            int last = (int)quotient(u1 - 1, share);
+            while (cut((int64_t)last * share) == n) --last;
+            meta = PagedMeta{1, last, u.kvh, u.r0, u.rows, u.tok0, u.pos0, 0};
+          }
+        }
         now = min(u1, end);
       }
       const uint32_t us = uc % UNITS;
@@ -389,30 +431,37 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       // halves alternate, K0 V(i) [K(i + 1)] where they share
       const int n = u.te - u.tb;
       const int* table = bt.page_table + u.seq * bt.table_ld;
-      for (int j = 0; j < 2 * n && ok; ++j, ++it) {
-        int t;
-        bool is_v;
-        if (j == 0) t = 0, is_v = false;
-        else if (j == 2 * n - 1) t = n - 1, is_v = true;
-        else if (u.alternate) is_v = !(j & 1), t = is_v ? j / 2 - 1 : (j + 1) / 2;
-        else is_v = j & 1, t = is_v ? j / 2 : j / 2;
-        const int key = (u.tb + t) * kPagedTile + lane * p.box;
-        int page = -1;
-        const bool wanted = lane * p.box < kPagedTile && key < u.hi && key + p.box > u.lo;
-        if (wanted) page = table[key / bt.page_size];
-        const bool real = wanted && page >= 0 && page < bt.pages;
-        if (__any_sync(0xffffffffu, wanted && !real) && lane == 0) units[us].bad = 1;
+      // number j of them: its tile, and this lane's key and page (-1: none wanted, -2: none there)
+      auto tile_of = [&](int j) {
+        if (j == 0) return 0;
+        if (j == 2 * n - 1) return n - 1;
+        return u.alternate && !(j & 1) ? j / 2 - 1 : u.alternate ? (j + 1) / 2 : j / 2;
+      };
+      auto key_of = [&](int j) { return (u.tb + tile_of(j)) * kPagedTile + lane * p.box; };
+      auto page_of = [&](int j) {
+        const int key = key_of(j);
+        if (j >= 2 * n || lane * p.box >= kPagedTile || key >= u.hi || key + p.box <= u.lo) return -1;
+        const int page = table[bt.by_page.of(key)];
+        return page < 0 || page >= bt.pages ? -2 : page;
+      };
+      int ahead = page_of(0);
+      for (int j = 0; j < 2 * n; ++j, ++it) {
+        const bool is_v = j == 2 * n - 1 || (j > 0 && (u.alternate ? !(j & 1) : (j & 1)));
+        const int key = key_of(j), page = ahead;
+        ahead = page_of(j + 1);
+        if (__any_sync(0xffffffffu, page == -2) && lane == 0) units[us].bad = 1;
         const uint32_t s = it % STAGES;
         if (!(ok = mbar_wait_warp(&empty[s], ((it / STAGES) & 1u) ^ 1u, abort_flag, p.err, 42))) break;
-        const uint32_t boxes = (uint32_t)__popc(__ballot_sync(0xffffffffu, real));
+        const uint32_t boxes = (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0));
         if (lane == 0) mbar_arrive_expect_tx(&full[s], boxes * (uint32_t)p.box * DH * 2);
         __syncwarp();
-        if (real) {
+        if (page >= 0) {
           const CUtensorMap* map = is_v ? &map_v : &map_k;
           const uint32_t dst = ring + s * L::TILE + (uint32_t)(lane * p.box) * 128u;
+          const int in = key - bt.by_page.of(key) * bt.page_size;
 #pragma unroll
           for (int h = 0; h < HALVES; ++h)
-            tma_load_4d(dst + h * (kPagedTile * 128), map, h * 64, key % bt.page_size, u.kvh, page, &full[s]);
+            tma_load_4d(dst + h * (kPagedTile * 128), map, h * 64, in, u.kvh, page, &full[s]);
         }
         __syncwarp();
       }
@@ -443,14 +492,14 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       }
       __syncwarp();
     };
-    auto product_o = [&](int w, uint32_t s, bool add) {
+    auto product_o = [&](int w, uint32_t s, int half, bool add) {
       if (elect_one()) {
         const uint32_t v = ring + s * L::TILE;
 #pragma unroll
-        for (int i = 0; i < kPagedTile / 16; ++i)
+        for (int i = half * 4; i < half * 4 + 4; ++i)
           umma_f16_tmem_a(tmem + 256 + w * 128, tmem + w * 128 + i * 8, paged_desc(v + i * 2048, kPagedTile * 128), idesc_o,
                           add || i > 0 ? 1u : 0u);
-        umma_commit(&pv_done[w]);
+        if (half) umma_commit(&pv_done[w]);
       }
       __syncwarp();
     };
@@ -464,7 +513,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       const PagedUnit& u = units[us];
       if (u.done) break;
       const int n = u.te - u.tb, alternate = u.alternate, tb = u.tb;
-      const int count[2] = {paged_count(u, 0, G), paged_count(u, 1, G)};
+      const int count[2] = {paged_count(u, 0, p.by_group), paged_count(u, 1, p.by_group)};
       if (!(ok = mbar_wait_warp(q_full, uc & 1u, abort_flag, p.err, 47))) break;
       tc_fence_after();
       if (n > 0) {
@@ -505,10 +554,13 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
             if (!(ok = mbar_wait_warp(&o_free[w], (oc[w] & 1u) ^ 1u, abort_flag, p.err, 49))) break;
             ++oc[w];
           }
+          if (!(ok = mbar_wait_warp(&p_half[w], pc[w] & 1u, abort_flag, p.err, 62))) break;
+          tc_fence_after();
+          product_o(w, v % STAGES, 0, i > 0);
           if (!(ok = mbar_wait_warp(&p_full[w], pc[w] & 1u, abort_flag, p.err, 50))) break;
           ++pc[w];
           tc_fence_after();
-          product_o(w, v % STAGES, i > 0);
+          product_o(w, v % STAGES, 1, true);
           if (alternate) commit(&empty[v % STAGES]);
           if (i + 1 < count[w]) {
             if (alternate) {
@@ -545,12 +597,28 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       PagedUnit& u = units[us];
       if (u.done) break;
       if (!(ok = mbar_wait_warp(q_empty, (uc & 1u) ^ 1u, abort_flag, p.err, 54))) break;
-      {
+      if (p.q_tma) {  // G heads by 128 / G tokens: rows behind the unit's are other tokens', of which nothing is used
+        if (elect_one()) {
+          const int tiles = u.rows > kPagedTile ? 2 : 1;
+          if (me == 0) {
+            mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * L::TILE));
+            const int per = kPagedTile / G, tok = u.tok0 + p.by_group.of(u.r0);
+            for (int i = 0; i < tiles; ++i)
+#pragma unroll
+              for (int h = 0; h < HALVES; ++h)
+                tma_load_4d(q_smem + i * L::TILE + h * (kPagedTile * 128), &map_q, h * 64, 0, tok + i * per, u.kvh, q_full);
+          } else {
+            mbar_arrive(q_full);
+          }
+        }
+        __syncwarp();
+      } else {
         constexpr int CH = DH / 8;  // 16-byte pieces of a row
         const int c = lane % CH, rows = u.rows;
         const T* q = static_cast<const T*>(a.q) + (int64_t)u.tok0 * a.q_token + (int64_t)u.kvh * G * a.q_head + c * 8;
+#pragma unroll 4
         for (int r = me * (32 / CH) + lane / CH; r < rows; r += 2 * (32 / CH)) {
-          const int row = u.r0 + r, tok = row / G, g = row - tok * G;
+          const int row = u.r0 + r, tok = p.by_group.of(row), g = row - tok * G;
           const uint32_t dst = q_smem + (r >> 7) * L::TILE + (c >> 3) * (kPagedTile * 128) + (r & 127) * 128 +
                                (((c & 7) ^ (r & 7)) << 4);
           const bool real = c * 8 < a.dim;
@@ -571,22 +639,38 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         ++vc;
         if (!(ok = mbar_wait_warp(&full[s], (v / STAGES) & 1u, abort_flag, p.err, 55))) break;
         const int key0 = (u.tb + t) * kPagedTile;
+        constexpr int CH = DH / 8;
+        uint8_t* tile = smem + s * L::TILE;
+        auto piece = [&](int row, int c) { return reinterpret_cast<uint4*>(tile + (c >> 3) * (kPagedTile * 128) + row * 128 + (c & 7) * 16); };
+        const int c = lane % CH, r_first = me * (32 / CH) + lane / CH;
+        constexpr int STEP = 2 * (32 / CH);
+        // keys outside of the unit's
+        for (int row = r_first; row < min(kPagedTile, u.lo - key0); row += STEP) *piece(row, c) = make_uint4(0, 0, 0, 0);
+        for (int row = max(r_first, r_first + (u.hi - key0 - r_first + STEP - 1) / STEP * STEP); row < kPagedTile; row += STEP)
+          *piece(row, c) = make_uint4(0, 0, 0, 0);
+        // keys that some rows see and others do not: the last ones, and those before the last row's window
         uint32_t found = 0;
-#pragma unroll 4
-        for (int i = me * 32 + lane; i < kPagedTile * HALVES * 8; i += 64) {
-          const int key = key0 + ((i >> 3) & 127);
-          uint4* x = reinterpret_cast<uint4*>(smem + s * L::TILE + i * 16);
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (key >= u.lo && key < u.hi) {
-            w = *x;
-            const uint32_t m0 = not_finite2<T>(w.x), m1 = not_finite2<T>(w.y), m2 = not_finite2<T>(w.z),
-                           m3 = not_finite2<T>(w.w);
-            if (!(m0 | m1 | m2 | m3)) continue;
+        auto scan = [&](int from, int to) {
+          from = max(from, max(0, u.lo - key0)), to = min(to, min(kPagedTile, u.hi - key0));
+          for (int row0 = from + r_first; row0 < to; row0 += 4 * STEP) {
+            uint4 x[4];
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = row0 + i * STEP < to ? *piece(row0 + i * STEP, c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= not_finite<T>(x[i].x) | not_finite<T>(x[i].y) | not_finite<T>(x[i].z) | not_finite<T>(x[i].w);
+            if (!(any & 0x80008000u)) continue;
             found = 1;
-            w = make_uint4(w.x & ~m0, w.y & ~m1, w.z & ~m2, w.w & ~m3);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (row0 + i * STEP < to)
+                *piece(row0 + i * STEP, c) = make_uint4(finite_or_zero<T>(x[i].x), finite_or_zero<T>(x[i].y),
+                                                        finite_or_zero<T>(x[i].z), finite_or_zero<T>(x[i].w));
           }
-          *x = w;
-        }
+        };
+        const int late = u.first + 1 - key0;
+        scan(late, kPagedTile);
+        if (a.window) scan(0, (int)min((int64_t)late, (int64_t)u.last - a.window - key0 + 1));
         if (found) u.dirty = 1;
         fence_proxy_async_smem();
         __syncwarp();
@@ -612,10 +696,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       const PagedUnit& u = units[us];
       if (u.done) break;
       const int alternate = u.alternate, tb = u.tb;
-      const int count[2] = {paged_count(u, 0, G), paged_count(u, 1, G)};
+      const int count[2] = {paged_count(u, 0, p.by_group), paged_count(u, 1, p.by_group)};
       const int r = (alternate ? 0 : w * kPagedTile) + quarter * 32 + lane;  // row of the unit
       const bool real = r < u.rows, active = (alternate ? 0 : w * kPagedTile) + quarter * 32 < u.rows;
-      const int tok = (u.r0 + r) / G, position = u.pos0 + tok;
+      const int tok = p.by_group.of(u.r0 + r), position = u.pos0 + tok;
       float m = -INFINITY, sum = 0.0f;
       const uint32_t o_tmem = tmem + 256 + w * 128 + lanes;
       for (int i = 0; i < count[w] && ok; ++i) {
@@ -649,9 +733,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           float top[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            top[c] = __uint_as_float(s[c][0]);
+            top[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
 #pragma unroll
-            for (int k = 1; k < 32; ++k) top[c] = fmaxf(top[c], __uint_as_float(s[c][k]));
+            for (int k = 2; k < 32; k += 2) top[c] = max3(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
           }
           const float high_s = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
           const bool raise = real && high_s > m + kPagedRaise;
@@ -685,16 +769,25 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               const int c = 2 * h + (k >> 4), e = 2 * k & 31;
-              const float x = ex2(__fmaf_rn(__uint_as_float(s[c][e]), a.scale, -base));
-              const float y = ex2(__fmaf_rn(__uint_as_float(s[c][e + 1]), a.scale, -base));
-              part[k & 1] += x;
-              part[2 + (k & 1)] += y;
+              float x = __uint_as_float(s[c][e]), y = __uint_as_float(s[c][e + 1]);
+              fma2(x, y, a.scale, -base);
+              x = ex2(x);
+              y = ex2(y);
+              add2(part[2 * (k & 1)], part[2 * (k & 1) + 1], x, y);
               o[k] = pack2<T>(x, y);
             }
             FTB_TMEM_ST32(s_tmem + h * 32, o);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            if (h == 0) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[w]);
+              __syncwarp();
+            }
           }
           sum += (part[0] + part[1]) + (part[2] + part[3]);
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        } else if (lane == 0) {
+          mbar_arrive(&p_half[w]);
         }
         tc_fence_before();
         __syncwarp();
@@ -757,7 +850,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               for (int key = (int)max((int64_t)u.tb * kPagedTile, a.window ? (int64_t)position - a.window + 1 : 0);
                    key <= position && key < u.te * kPagedTile; ++key) {
                 if (!paged_masked(u, key / kPagedTile, a.window)) continue;
-                const int page = a.batch.page_table[u.seq * a.batch.table_ld + key / a.batch.page_size];
+                const int page = a.batch.page_table[u.seq * a.batch.table_ld + a.batch.by_page.of(key)];
                 if (page < 0 || page >= a.batch.pages) continue;
                 const T* x = static_cast<const T*>(a.values) + page * a.v_page + key % a.batch.page_size * a.v_token +
                              (int64_t)u.kvh * a.v_head + c * 32;
@@ -849,7 +942,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTensorParams
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = lane * E + e < a.dim ? __fmaf_rn(t[e], f, o[e]) : 0.0f;
     }
-    const int tok = (u.r0 + r) / p.group, g = u.r0 + r - tok * p.group;
+    const int tok = p.by_group.of(u.r0 + r), g = u.r0 + r - tok * p.group;
     T* out = static_cast<T*>(a.out) + (int64_t)(u.tok0 + tok) * a.o_token + (int64_t)(u.kvh * p.group + g) * a.o_head;
     const bool nothing = u.pos0 + tok < 0;
 #pragma unroll
@@ -862,15 +955,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedTensorParams
 // host side
 // ---------------------------------------------------------------------------
 
-// A pool as the kernel reads it: boxes of 64 elements of a head by `box` tokens.
-inline bool make_map_pool(CUtensorMap* map, const void* base, int type, int64_t dim, int64_t page_size, int64_t kv_heads,
-                          int64_t pages, int64_t token, int64_t head, int64_t page, int box) {
+// Heads as the kernel reads them: [n3][n2][n1][dim] with strides in elements, in boxes of 64 elements by b1 by b2.
+inline bool make_map_heads(CUtensorMap* map, const void* base, int type, int64_t dim, int64_t n1, int64_t n2, int64_t n3,
+                           int64_t s1, int64_t s2, int64_t s3, int b1, int b2) {
   PFN_encodeTiled enc = tma_encoder();
   if (!enc) return false;
   auto bytes = [&](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 ? stride * 2 : (dim * 2 + 15) / 16 * 16); };
-  cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)page_size, (cuuint64_t)kv_heads, (cuuint64_t)pages};
-  cuuint64_t strides[3] = {bytes(page_size, token), bytes(kv_heads, head), bytes(pages, page)};
-  cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+  cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)n1, (cuuint64_t)n2, (cuuint64_t)n3};
+  cuuint64_t strides[3] = {bytes(n1, s1), bytes(n2, s2), bytes(n3, s3)};
+  cuuint32_t boxes[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return enc(map, type == FTB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
              const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -911,12 +1004,20 @@ inline cudaError_t paged_attention_prepare() {
 template <typename T, int DH>
 cudaError_t launch_paged_as(PagedTensorParams& p, int type, int blocks, cudaStream_t s) {
   const PagedAttentionParams& a = p.a;
-  CUtensorMap map_k, map_v;
-  if (!make_map_pool(&map_k, a.keys, type, a.dim, a.batch.page_size, a.kv_heads, a.batch.pages, a.k_token, a.k_head, a.k_page, p.box) ||
-      !make_map_pool(&map_v, a.values, type, a.dim, a.batch.page_size, a.kv_heads, a.batch.pages, a.v_token, a.v_head, a.v_page, p.box))
+  CUtensorMap map_k, map_v, map_q;
+  // tokens of a page, kv heads, pages
+  if (!make_map_heads(&map_k, a.keys, type, a.dim, a.batch.page_size, a.kv_heads, a.batch.pages, a.k_token, a.k_head,
+                      a.k_page, p.box, 1) ||
+      !make_map_heads(&map_v, a.values, type, a.dim, a.batch.page_size, a.kv_heads, a.batch.pages, a.v_token, a.v_head,
+                      a.v_page, p.box, 1))
     return cudaErrorInvalidValue;
+  // heads of a group, tokens, groups
+  std::memset(&map_q, 0, sizeof(map_q));
+  p.q_tma = kPagedTile % p.group == 0 &&
+            make_map_heads(&map_q, a.q, type, a.dim, p.group, a.tokens, a.kv_heads, a.q_head, a.q_token, a.q_head * p.group,
+                           p.group, kPagedTile / p.group);
   cudaError_t e = pdl_launch(paged_attention_kernel<T, DH>, dim3((unsigned)blocks), dim3(kPagedThreads), PagedSmem<DH>::TOTAL, s,
-                             map_k, map_v, p);
+                             map_k, map_v, map_q, p);
   if (e == cudaSuccess)
     e = pdl_launch(paged_join_kernel<T, DH>, dim3((unsigned)blocks, (unsigned)(p.rows_bound + 31) / 32), dim3(256), 0, s, p);
   return e;
@@ -931,6 +1032,8 @@ inline cudaError_t launch_paged_attention(const PagedAttentionParams& a, int typ
   if (p.a.scale == 0.0f) p.a.scale = 1e-30f;  // equal weights either way, and a masked score stays -inf
   p.negative = a.scale < 0.0f;
   p.group = a.heads / a.kv_heads;
+  p.by_group = FastDiv((uint32_t)p.group);
+  p.step = std::max(1, 256 / p.group);
   p.box = 16;
   while (p.box < kPagedTile && a.batch.page_size % (2 * p.box) == 0) p.box *= 2;
   p.rows_bound = paged_rows_bound(a);
