@@ -22,18 +22,20 @@
 // units that others share; they go to the workspace (O, m and the sum), and
 // paged_join_kernel joins them in order.  No atomics: the same bits each time.
 //
-// Block: twelve warps.
-//   warps 0-3, 4-7  softmax of the two halves: a thread is a row.  S from
-//                   tensor memory, mask, maximum, exponentials, P back over S
-//                   as the A operand of P V; at the end O to global memory
-//   warp 8          units of the block; keys and values by TMA, boxes of as
-//                   many tokens as lie in one page, into a ring of tiles
-//   warp 9          tensor memory and the products (one elected lane): while
-//                   one half is in its softmax, the other's run
-//   warps 10-11     Q of the next unit by cp.async; tiles that some row sees
-//                   in part: values outside of the unit's keys become 0, and
-//                   so do values that are not finite (0 weights would make
-//                   them NaN); rows that do see one are marked at the end
+// Block: twenty warps.
+//   warps 0-7, 8-15  softmax of the two halves: a thread has 64 of a row's 128
+//                    scores, the other 64 are four warps on.  S from tensor
+//                    memory, mask, maximum (exchanged by the two), exponentials,
+//                    P back over S as the A operand of P V; at the end O to
+//                    global memory
+//   warp 16          units of the block; keys and values by TMA, boxes of as
+//                    many tokens as lie in one page, into a ring of tiles
+//   warp 17          tensor memory and the products (one elected lane): while
+//                    one half is in its softmax, the other's run
+//   warps 18-19      Q of the next unit; tiles that some row sees in part:
+//                    values outside of the unit's keys become 0, and so do
+//                    values that are not finite (0 weights would make them
+//                    NaN); rows that do see one are marked at the end
 //
 // Shared memory: Q of two tiles, and a ring of 128-token tiles of K or V,
 // 128-byte swizzle, in columns of 64.  Tensor memory: S and P of both halves at
@@ -50,7 +52,8 @@
 
 namespace ftb {
 
-constexpr int kPagedThreads = 384;
+constexpr int kPagedThreads = 640;
+constexpr int kPagedProducer = 16, kPagedProducts = 17, kPagedQueries = 18;  // warps
 constexpr int kPagedTile = 128;      // keys of a tile, rows of a half
 constexpr int kPagedUnitOver = 160;  // a unit's own cost, in keys
 constexpr int kPagedLeast = 448;     // keys (with it) that are worth a block
@@ -135,12 +138,12 @@ struct PagedSmem {
   static constexpr int TILE = kPagedTile * DH * 2;
   static constexpr int STAGES = DH == 128 ? 5 : 10;
   static constexpr int Q_OFF = STAGES * TILE;
-  static constexpr int ML_OFF = Q_OFF + 2 * TILE;  // [128] of (m, sum)
-  static constexpr int UNIT_OFF = ML_OFF + 128 * 8;
+  static constexpr int ROW_OFF = Q_OFF + 2 * TILE;  // [16 softmax warps][32]: a row's maximum or sum
+  static constexpr int UNIT_OFF = ROW_OFF + 16 * 32 * 4;
   static constexpr int UNITS = 2;
   static constexpr int BAR_OFF = (UNIT_OFF + UNITS * (int)sizeof(PagedUnit) + 15) / 16 * 16;
-  static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 5 + 4;
-  static constexpr int TOTAL = 1024 + BAR_OFF + 8 * NBAR + 16;
+  static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 4 + 5;
+  static constexpr int TOTAL = BAR_OFF + 8 * NBAR + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
 };
 
@@ -242,15 +245,48 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// (x, y) += (a, b) f
+__device__ __forceinline__ void fma2_to(float& x, float& y, float a, float b, float f) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %4};\n\t"
+      "fma.rn.f32x2 p, q, r, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b), "f"(f));
+}
+
+// Of 32 elements from c on of a row's output, a bit for each in which a value of
+// a tile seen in part is not finite and the row, at `position`, sees it.  Such
+// values were left out of the products.
+template <typename T>
+__device__ __forceinline__ uint32_t paged_marks(const PagedTensorParams& p, const PagedUnit& u, int position, int c) {
+  const PagedAttentionParams& a = p.a;
+  uint32_t bits = 0;
+  const int64_t from = a.window ? (int64_t)position - a.window + 1 : 0;
+#pragma unroll 1
+  for (int key = (int)max((int64_t)u.tb * kPagedTile, from); key <= position && key < u.te * kPagedTile; ++key) {
+    if (!paged_masked(u, key / kPagedTile, a.window)) continue;
+    const int page = a.batch.page_table[u.seq * a.batch.table_ld + a.batch.by_page.of(key)];
+    if (page < 0 || page >= a.batch.pages) continue;
+    const T* x = static_cast<const T*>(a.values) + page * a.v_page + key % a.batch.page_size * a.v_token +
+                 (int64_t)u.kvh * a.v_head + c;
+#pragma unroll 1
+    for (int k = 0; k < 32 && c + k < a.dim; ++k)
+      if (!isfinite(to_f32(x[k]))) bits |= 1u << k;
+  }
+  return bits;
+}
+
 template <typename T, int DH>
 __global__ void __launch_bounds__(kPagedThreads, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                            const __grid_constant__ CUtensorMap map_q, const PagedTensorParams p) {
   using L = PagedSmem<DH>;
   constexpr int STAGES = L::STAGES, HALVES = L::HALVES, UNITS = L::UNITS;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
+  extern __shared__ __align__(1024) uint8_t paged_smem[];  // the swizzle's unit
+  uint8_t* smem = paged_smem;
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(p.err, 0, 40);
+    return;
+  }
   PagedUnit* units = reinterpret_cast<PagedUnit*>(smem + L::UNIT_OFF);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);  // a tile of K or V landed
   uint64_t* empty = full + STAGES;       // the products are done with it
@@ -259,14 +295,14 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   uint64_t* q_full = u_empty + UNITS;    // its Q landed
   uint64_t* q_empty = q_full + 1;        // its last S = Q K^T is done
   uint64_t* s_full = q_empty + 1;        // [2] S of a half
-  uint64_t* p_half = s_full + 2;         // [2] its P of 64 keys is in tensor memory, O rescaled
-  uint64_t* p_full = p_half + 2;         // [2] all of its P
+  uint64_t* p_full = s_full + 2;         // [2] its P is in tensor memory, O rescaled
   uint64_t* pv_done = p_full + 2;        // [2] P V is done
   uint64_t* o_free = pv_done + 2;        // [2] O was read (in units where the half had tiles)
   uint64_t* v_seen = o_free + 2;         // a tile of V seen in part is there
   uint64_t* v_clean = v_seen + 1;        // ... and clean
   uint64_t* ml_full = v_clean + 1;       // m and sum of the second half
-  uint64_t* drain = ml_full + 1;         // products retired after an abort
+  uint64_t* ml_free = ml_full + 1;       // ... read
+  uint64_t* drain = ml_free + 1;         // products retired after an abort
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 1) + 1;
 
@@ -281,32 +317,32 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     }
     for (int s = 0; s < UNITS; ++s) {
       mbar_init(&u_full[s], 1);
-      mbar_init(&u_empty[s], 11);  // eight softmax warps, the products, two of Q
+      mbar_init(&u_empty[s], 19);  // sixteen softmax warps, the products, two of Q
     }
     mbar_init(q_full, 2);
     mbar_init(q_empty, 1);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&s_full[w], 1);
-      mbar_init(&p_half[w], 4);
-      mbar_init(&p_full[w], 4);
+      mbar_init(&p_full[w], 8);
       mbar_init(&pv_done[w], 1);
-      mbar_init(&o_free[w], 4);
+      mbar_init(&o_free[w], 8);
     }
     mbar_init(v_seen, 1);
     mbar_init(v_clean, 2);
-    mbar_init(ml_full, 4);
+    mbar_init(ml_full, 8);
+    mbar_init(ml_free, 8);
     mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == kPagedProducts) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(const_cast<uint32_t*>(tmem_slot))),
                  "r"(512u)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp == 10 && elect_one()) {
+  if (warp == kPagedQueries && elect_one()) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_v)) : "memory");
   }
@@ -319,7 +355,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const uint32_t ring = smem_u32(smem), q_smem = smem_u32(smem + L::Q_OFF);
 
-  if (warp == 8) {
+  if (warp == kPagedProducer) {
     // ---- units, keys and values ----
     bool ok = true;
     uint32_t it = 0, uc = 0;
@@ -470,7 +506,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     if (!ok)  // the copies in flight land before the block leaves
       for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
         mbar_wait_warp(&full[j % STAGES], (j / STAGES) & 1u, abort_flag, p.err, 43, /*ignore_abort=*/true);
-  } else if (warp == 9) {
+  } else if (warp == kPagedProducts) {
     // ---- products ----
     bool ok = true;
     uint32_t it = 0, uc = 0, pc[2] = {0, 0}, oc[2] = {0, 0}, vc = 0;
@@ -492,14 +528,14 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       }
       __syncwarp();
     };
-    auto product_o = [&](int w, uint32_t s, int half, bool add) {
+    auto product_o = [&](int w, uint32_t s, bool add) {
       if (elect_one()) {
         const uint32_t v = ring + s * L::TILE;
 #pragma unroll
-        for (int i = half * 4; i < half * 4 + 4; ++i)
+        for (int i = 0; i < kPagedTile / 16; ++i)
           umma_f16_tmem_a(tmem + 256 + w * 128, tmem + w * 128 + i * 8, paged_desc(v + i * 2048, kPagedTile * 128), idesc_o,
                           add || i > 0 ? 1u : 0u);
-        if (half) umma_commit(&pv_done[w]);
+        umma_commit(&pv_done[w]);
       }
       __syncwarp();
     };
@@ -547,20 +583,19 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           ++it;
           if (!alternate && !(ok = wait_tile(k))) break;
         }
-        for (int w = alternate ? t & 1 : 0; w < (alternate ? (t & 1) + 1 : 2); ++w) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (!ok || (alternate && w != (t & 1))) continue;
           const int i = alternate ? t >> 1 : t;  // number of the tile among the half's
           if (i >= count[w]) continue;
           if (i == 0) {
             if (!(ok = mbar_wait_warp(&o_free[w], (oc[w] & 1u) ^ 1u, abort_flag, p.err, 49))) break;
             ++oc[w];
           }
-          if (!(ok = mbar_wait_warp(&p_half[w], pc[w] & 1u, abort_flag, p.err, 62))) break;
-          tc_fence_after();
-          product_o(w, v % STAGES, 0, i > 0);
           if (!(ok = mbar_wait_warp(&p_full[w], pc[w] & 1u, abort_flag, p.err, 50))) break;
           ++pc[w];
           tc_fence_after();
-          product_o(w, v % STAGES, 1, true);
+          product_o(w, v % STAGES, i > 0);
           if (alternate) commit(&empty[v % STAGES]);
           if (i + 1 < count[w]) {
             if (alternate) {
@@ -586,9 +621,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       commit(drain);
       mbar_wait_warp(drain, 0, abort_flag, p.err, 52, /*ignore_abort=*/true);
     }
-  } else if (warp >= 10) {
+  } else if (warp >= kPagedQueries) {
     // ---- Q, and values of tiles that are seen in part ----
-    const int me = warp - 10;
+    const int me = warp - kPagedQueries;
     bool ok = true;
     uint32_t it = 0, uc = 0, vc = 0;
     while (ok) {
@@ -685,59 +720,78 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     }
   } else {
     // ---- softmax ----
-    const int w = warp >> 2, quarter = warp & 3;
+    const int w = warp >> 3, side = (warp >> 2) & 1, quarter = warp & 3;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tmem = tmem + w * 128 + lanes;
+    // the warp with the other scores of the same rows, and where the two leave theirs
+    float* rows = reinterpret_cast<float*>(smem + L::ROW_OFF) + lane;
+    // what the two warps of a row have, for both.  A place is written again only when its
+    // reader is known to be past this: behind a barrier of theirs or the next S.
+    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + w * 4 + quarter) : "memory"); };
+    auto exchange = [&](float x) {
+      rows[warp * 32] = x;
+      meet();
+      return rows[(warp ^ 4) * 32];
+    };
     bool ok = true;
-    uint32_t uc = 0, cnt[2] = {0, 0}, oc = 0, mc = 0;  // oc: units of which the first half had tiles
+    uint32_t uc = 0, cnt0 = 0, cnt1 = 0, mc = 0;
     while (ok) {
       const uint32_t us = uc % UNITS;
       if (!(ok = mbar_wait_warp(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 56))) break;
       const PagedUnit& u = units[us];
       if (u.done) break;
       const int alternate = u.alternate, tb = u.tb;
-      const int count[2] = {paged_count(u, 0, p.by_group), paged_count(u, 1, p.by_group)};
+      const int count0 = paged_count(u, 0, p.by_group), count1 = paged_count(u, 1, p.by_group), count = w ? count1 : count0;
+      const uint32_t done = w ? cnt1 : cnt0;  // tiles of this half so far
       const int r = (alternate ? 0 : w * kPagedTile) + quarter * 32 + lane;  // row of the unit
       const bool real = r < u.rows, active = (alternate ? 0 : w * kPagedTile) + quarter * 32 < u.rows;
       const int tok = p.by_group.of(u.r0 + r), position = u.pos0 + tok;
       float m = -INFINITY, sum = 0.0f;
-      const uint32_t o_tmem = tmem + 256 + w * 128 + lanes;
-      for (int i = 0; i < count[w] && ok; ++i) {
+      for (int i = 0; i < count && ok; ++i) {
         const int t = tb + (alternate ? 2 * i + w : i);
-        if (!(ok = mbar_wait_warp(&s_full[w], (cnt[w] + i) & 1u, abort_flag, p.err, 57))) break;
+        if (!(ok = mbar_wait_warp(&s_full[w], (done + i) & 1u, abort_flag, p.err, 57))) break;
         tc_fence_after();
         if (active) {
-          uint32_t s[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            __syncwarp();
-            FTB_TMEM_LD32(s_tmem + c * 32, s[c]);
-          }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) FTB_TMEM_WAIT_LD32(s[c]);
-          if (p.negative) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int k = 0; k < 32; ++k) s[c][k] ^= 0x80000000u;
-          }
           // columns that this row sees: low < column <= high
-          const int high = position - t * kPagedTile, low = a.window ? (int)max((int64_t)high - a.window, (int64_t)-1) : -1;
-          if (__any_sync(0xffffffffu, real && (high < kPagedTile - 1 || low >= 0))) {
+          const int high = position - t * kPagedTile - side * 64;
+          const int low = a.window ? (int)max((int64_t)high - a.window, (int64_t)-1) : -1;
+          const bool partly = __any_sync(0xffffffffu, real && (high < 63 || low >= 0));
+          // 32 scores; twice the first ones, since all 64 and what else a thread keeps do not fit its registers
+          // (spilled ones went to L2: 8700 cycles for two tiles instead of XXXX)
+          uint32_t x[32];
+          auto load = [&](int c) {
+            __syncwarp();
+            FTB_TMEM_LD32(s_tmem + side * 64 + c * 32, x);
+            FTB_TMEM_WAIT_LD32(x);
+            if (p.negative) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+              for (int k = 0; k < 32; ++k) x[k] ^= 0x80000000u;
+            }
+            if (partly) {
+              const int h = min(high - c * 32, 31), l = max(low - c * 32, -1);
+              const uint32_t seen = h < 0 || l > 30 ? 0u : (0xFFFFFFFFu >> (31 - h)) & (0xFFFFFFFFu << (l + 1));
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                if (c * 32 + k > high || c * 32 + k <= low) s[c][k] = 0xFF800000u;
-          }
-          float top[4];
+                if (!(seen & (1u << k))) x[k] = 0xFF800000u;
+            }
+          };
+          auto largest = [&]() {
+            float top[2];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            top[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+            for (int c = 0; c < 2; ++c) {
+              top[c] = fmaxf(__uint_as_float(x[16 * c]), __uint_as_float(x[16 * c + 1]));
 #pragma unroll
-            for (int k = 2; k < 32; k += 2) top[c] = max3(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-          }
-          const float high_s = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
+              for (int k = 2; k < 16; k += 2)
+                top[c] = max3(top[c], __uint_as_float(x[16 * c + k]), __uint_as_float(x[16 * c + k + 1]));
+            }
+            return fmaxf(top[0], top[1]);
+          };
+          load(0);
+          float high_s = largest();
+          load(1);
+          high_s = fmaxf(high_s, largest());
+          // after this both warps have their S, over which P goes
+          high_s = fmaxf(high_s, exchange(high_s)) * a.scale;
           const bool raise = real && high_s > m + kPagedRaise;
           if (__any_sync(0xffffffffu, raise)) {
             float keep = 1.0f;
@@ -746,48 +800,39 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               sum *= keep;
               m = high_s;
             }
-            if (i > 0) {
-              if (!(ok = mbar_wait_warp(&pv_done[w], (cnt[w] + i - 1) & 1u, abort_flag, p.err, 58))) break;
-              tc_fence_after();
+            if (i > 0) {  // this S followed the last P V, so O is complete; each warp has half of its columns
 #pragma unroll 1
-              for (int c = 0; c * 32 < a.dim; ++c) {
+              for (int c = side * (DH / 2); c < (side + 1) * (DH / 2) && c < a.dim; c += 32) {
                 uint32_t o[32];
                 __syncwarp();
-                FTB_TMEM_LD32(o_tmem + c * 32, o);
+                FTB_TMEM_LD32(tmem + 256 + w * 128 + lanes + c, o);
                 FTB_TMEM_WAIT_LD32(o);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                FTB_TMEM_ST32(o_tmem + c * 32, o);
+                FTB_TMEM_ST32(tmem + 256 + w * 128 + lanes + c, o);
               }
             }
           }
           const float base = m == -INFINITY ? 0.0f : m;
           float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          uint32_t o[32];
+          auto weights = [&](uint32_t* to) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t o[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int c = 2 * h + (k >> 4), e = 2 * k & 31;
-              float x = __uint_as_float(s[c][e]), y = __uint_as_float(s[c][e + 1]);
-              fma2(x, y, a.scale, -base);
-              x = ex2(x);
-              y = ex2(y);
-              add2(part[2 * (k & 1)], part[2 * (k & 1) + 1], x, y);
-              o[k] = pack2<T>(x, y);
+            for (int k = 0; k < 16; ++k) {
+              float u = __uint_as_float(x[2 * k]), v = __uint_as_float(x[2 * k + 1]);
+              fma2(u, v, a.scale, -base);
+              u = ex2(u);
+              v = ex2(v);
+              add2(part[2 * (k & 1)], part[2 * (k & 1) + 1], u, v);
+              to[k] = pack2<T>(u, v);
             }
-            FTB_TMEM_ST32(s_tmem + h * 32, o);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            if (h == 0) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_half[w]);
-              __syncwarp();
-            }
-          }
+          };
+          weights(o + 16);
+          load(0);
+          weights(o);
+          FTB_TMEM_ST32(s_tmem + side * 32, o);
           sum += (part[0] + part[1]) + (part[2] + part[3]);
-        } else if (lane == 0) {
-          mbar_arrive(&p_half[w]);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
         tc_fence_before();
         __syncwarp();
@@ -796,84 +841,81 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       }
       if (!ok) break;
       // ---- O ----
-      const uint32_t end[2] = {cnt[0] + count[0], cnt[1] + count[1]};
-      const bool both = alternate && count[0] > 0, mine = !alternate || w == 0;
-      float f[2] = {1.0f, 1.0f};  // factors of the halves' O
+      cnt0 += count0;
+      cnt1 += count1;
+      const bool both = alternate && count0 > 0, mine = !alternate || w == 0;
+      float f0 = 1.0f, f1 = 1.0f;  // factors of the halves' O
+      if (count > 0) {
+        if (!(ok = mbar_wait_warp(&pv_done[w], (done + count - 1) & 1u, abort_flag, p.err, 60))) break;
+        sum += exchange(sum);
+        meet();
+      }
       if (both && w == 1) {
-        // the first half has read those of the unit before
-        if (!(ok = mbar_wait_warp(&o_free[0], (oc & 1u) ^ 1u, abort_flag, p.err, 61))) break;
-        ml[quarter * 32 + lane] = make_float2(m, sum);
+        rows[warp * 32] = side ? sum : m;
         __syncwarp();
         if (lane == 0) mbar_arrive(ml_full);
         __syncwarp();
+        if (!(ok = mbar_wait_warp(ml_free, mc & 1u, abort_flag, p.err, 61))) break;
       }
       if (both && w == 0) {
         if (!(ok = mbar_wait_warp(ml_full, mc & 1u, abort_flag, p.err, 59))) break;
-        const float2 x = ml[quarter * 32 + lane];
-        const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top;
-        f[0] = ex2(m - base);
-        f[1] = ex2(x.x - base);
-        sum = sum * f[0] + x.y * f[1];
+        const float m1 = rows[(8 + quarter) * 32], sum1 = rows[(12 + quarter) * 32];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ml_free);
+        __syncwarp();
+        const float top = fmaxf(m, m1), base = top == -INFINITY ? 0.0f : top;
+        f0 = ex2(m - base);
+        f1 = ex2(m1 - base);
+        sum = sum * f0 + sum1 * f1;
         m = top;
       }
       if (both) ++mc;
       if (mine) {
-        for (int h = 0; h < 2 && ok; ++h)
-          if ((both || h == w) && count[h] > 0)
-            ok = mbar_wait_warp(&pv_done[h], (end[h] - 1) & 1u, abort_flag, p.err, 60);
-        if (!ok) break;
+        if (both && count1 > 0 && !(ok = mbar_wait_warp(&pv_done[1], (cnt1 - 1) & 1u, abort_flag, p.err, 63))) break;
         tc_fence_after();
         const bool bad = u.bad, dirty = u.dirty;
         const int g = u.r0 + r - tok * G;
         float* part = p.parts + (int64_t)max(u.slot, 0) * p.rows_bound * (2 + DH);
-        if (u.slot >= 0 && real) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, bad ? NAN : sum);
+        if (u.slot >= 0 && real && side == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, bad ? NAN : sum);
         part += 2 * p.rows_bound + (int64_t)r * DH;
         T* out = static_cast<T*>(a.out) + (int64_t)(u.tok0 + tok) * a.o_token + (int64_t)(u.kvh * G + g) * a.o_head;
         const float inv = 1.0f / sum;
         if (active) {
 #pragma unroll 1
-          for (int c = 0; c * 32 < a.dim; ++c) {
+          for (int c = side * (DH / 2); c < (side + 1) * (DH / 2) && c < a.dim; c += 32) {
             float v[32];
 #pragma unroll
             for (int k = 0; k < 32; ++k) v[k] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (!((both || h == w) && count[h] > 0)) continue;
+              if (!((both || h == w) && (h ? count1 : count0) > 0)) continue;
               uint32_t o[32];
               __syncwarp();
-              FTB_TMEM_LD32(tmem + 256 + h * 128 + lanes + c * 32, o);
+              FTB_TMEM_LD32(tmem + 256 + h * 128 + lanes + c, o);
               FTB_TMEM_WAIT_LD32(o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] = both ? __fmaf_rn(__uint_as_float(o[k]), f[h], v[k]) : __uint_as_float(o[k]);
+              for (int k = 0; k < 32; k += 2) fma2_to(v[k], v[k + 1], __uint_as_float(o[k]), __uint_as_float(o[k + 1]), h ? f1 : f0);
             }
-            if (dirty && real) {  // values that are not finite and that this row sees, in tiles seen in part
-              for (int key = (int)max((int64_t)u.tb * kPagedTile, a.window ? (int64_t)position - a.window + 1 : 0);
-                   key <= position && key < u.te * kPagedTile; ++key) {
-                if (!paged_masked(u, key / kPagedTile, a.window)) continue;
-                const int page = a.batch.page_table[u.seq * a.batch.table_ld + a.batch.by_page.of(key)];
-                if (page < 0 || page >= a.batch.pages) continue;
-                const T* x = static_cast<const T*>(a.values) + page * a.v_page + key % a.batch.page_size * a.v_token +
-                             (int64_t)u.kvh * a.v_head + c * 32;
+            if (dirty && real) {
+              const uint32_t bits = paged_marks<T>(p, u, position, c);
 #pragma unroll
-                for (int k = 0; k < 32; ++k)
-                  if (c * 32 + k < a.dim && !isfinite(to_f32(x[k]))) v[k] = NAN;
-              }
+              for (int k = 0; k < 32; ++k)
+                if (bits & (1u << k)) v[k] = NAN;
             }
             if (u.slot >= 0) {
               if (real) {
 #pragma unroll
                 for (int k = 0; k < 32; k += 4)
-                  *reinterpret_cast<float4*>(part + c * 32 + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                  *reinterpret_cast<float4*>(part + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
               }
             } else if (real) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] = bad ? NAN : position < 0 ? 0.0f : v[k] * inv;
+              const float by = bad ? NAN : position < 0 ? 0.0f : inv;
 #pragma unroll
               for (int k = 0; k < 32; k += 8)
-                if (c * 32 + k < a.dim)
-                  *reinterpret_cast<uint4*>(out + c * 32 + k) =
-                      make_uint4(pack2<T>(v[k], v[k + 1]), pack2<T>(v[k + 2], v[k + 3]), pack2<T>(v[k + 4], v[k + 5]),
-                                 pack2<T>(v[k + 6], v[k + 7]));
+                if (c + k < a.dim)
+                  *reinterpret_cast<uint4*>(out + c + k) =
+                      make_uint4(pack2<T>(v[k] * by, v[k + 1] * by), pack2<T>(v[k + 2] * by, v[k + 3] * by),
+                                 pack2<T>(v[k + 4] * by, v[k + 5] * by), pack2<T>(v[k + 6] * by, v[k + 7] * by));
             }
           }
         }
@@ -881,21 +923,18 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         __syncwarp();
         if (lane == 0) {
           for (int h = 0; h < 2; ++h)
-            if ((both || h == w) && count[h] > 0) mbar_arrive(&o_free[h]);
+            if ((both || h == w) && (h ? count1 : count0) > 0) mbar_arrive(&o_free[h]);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&u_empty[us]);
       __syncwarp();
-      cnt[0] = end[0];
-      cnt[1] = end[1];
-      oc += count[0] > 0;
       ++uc;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kPagedProducts) {
     __syncwarp();
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
