@@ -55,8 +55,8 @@ namespace ftb {
 constexpr int kPagedThreads = 640;
 constexpr int kPagedProducer = 16, kPagedProducts = 17, kPagedQueries = 18;  // warps
 constexpr int kPagedTile = 128;      // keys of a tile, rows of a half
-constexpr int kPagedUnitOver = 160;  // a unit's own cost, in keys
-constexpr int kPagedLeast = 448;     // keys (with it) that are worth a block
+constexpr int kPagedUnitOver = 256;  // a unit's own cost, in keys
+constexpr int kPagedLeast = 512;     // keys (with it) that are worth a block
 constexpr float kPagedRaise = 8.0f;  // log2
 constexpr int kPagedBlocks = 148;    // at most: B200's SMs
 
@@ -69,7 +69,8 @@ struct PagedTensorParams {
   PagedAttentionParams a;
   int group;         // query heads of a kv head
   FastDiv by_group;
-  int step;          // tokens in 256 rows
+  int capacity;      // tokens that a row of the page table has places for
+  int cost_shift, cost_step, cost_over, window_cap;  // see PagedCost
   int q_tma;         // Q has a TMA map: the group divides a tile's rows
   int box;           // tokens of a TMA box: in one page
   int negative;      // the scale is below 0 (a.scale is its absolute value)
@@ -86,28 +87,29 @@ struct PagedUnit {
   int lo, hi;          // keys that some row sees
   int first, last;     // positions of the first and the last row
   int alternate;       // the halves take the tiles in turn
+  int count0, count1;  // tiles that the halves take
   int slot;            // part of the workspace, -1: the whole unit
   int done;
   volatile int bad;    // a page outside of the pool
   volatile int dirty;  // a value that is not finite in a tile seen in part
 };
 
-// Cost of the first n tiles of rows of a sequence, in keys: tile i sees about
-// base + step (i + 1), at most `cap`.
+// Cost of the first n tiles of rows of a sequence, in keys (or, where the sum
+// over all sequences might not fit 31 bits, in 2^cost_shift of them): tile i sees
+// about base + step (i + 1) of them, at most `cap`.
 struct PagedCost {
-  int64_t base, step, cap;
-  __device__ __forceinline__ int64_t tile(int i) const { return min(cap, base + step * (i + 1)) + kPagedUnitOver; }
-  __device__ __forceinline__ int64_t first(int n) const {
-    int64_t k = n;  // tiles below the cap
-    if (cap < base + step * n) k = cap <= base ? 0 : min((int64_t)n, (int64_t)((uint32_t)(cap - base) / (uint32_t)step));
-    return k * base + step * (k * (k + 1) / 2) + (n - k) * cap + (int64_t)n * kPagedUnitOver;
+  int base, step, cap, over;
+  __device__ __forceinline__ int first(int n) const {
+    int k = n;  // about the tiles below the cap
+    if (cap - base < step * n) k = cap <= base ? 0 : min(n, (int)__fdividef((float)(cap - base), (float)step));
+    return k * base + step * (k * (k + 1) / 2) + (n - k) * cap + n * over;
   }
 };
 
 struct PagedSequence {
   int tok0, n, len, tiles;
   PagedCost cost;
-  int64_t head, whole;  // cost of a kv head, of all
+  int head, whole;  // cost of a kv head, of all
 };
 
 __device__ __forceinline__ PagedSequence paged_sequence(const PagedTensorParams& p, int b) {
@@ -117,20 +119,28 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedTensorParams&
   s.len = t.lengths[b];
   s.tok0 = max(0, min(start, p.a.tokens));
   s.n = max(0, min(stop, p.a.tokens) - s.tok0);
-  const int64_t rows = (int64_t)s.n * p.group;
-  s.tiles = rows == 0 ? 0 : rows <= kPagedTile ? 1 : (int)((rows + 255) >> 8);
-  const int64_t len = max((int64_t)0, min((int64_t)s.len, (int64_t)t.most_pages * t.page_size));
-  s.cost.base = max((int64_t)0, len - s.n);
-  s.cost.step = p.step;
-  s.cost.cap = len;
-  if (p.a.window) s.cost.cap = min(len, (int64_t)p.a.window + p.step);
+  // rows = n G below 2^27 2^12: tiles by the number of tokens
+  s.tiles = s.n == 0 ? 0 : (int64_t)s.n * p.group <= kPagedTile ? 1 : (int)(((int64_t)s.n * p.group + 255) >> 8);
+  const int len = max(0, min(s.len, p.capacity));
+  s.cost.base = max(0, len - s.n) >> p.cost_shift;
+  s.cost.step = p.cost_step;
+  s.cost.cap = (p.a.window ? min(len, p.window_cap) : len) >> p.cost_shift;
+  s.cost.over = p.cost_over;
   s.head = s.cost.first(s.tiles);
   s.whole = s.head * p.a.kv_heads;
   return s;
 }
 
-// floor(x / y) of whole numbers below 2^53
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) { return (int64_t)((double)x / (double)y); }
+// A bounded wait by a whole warp, with one outcome.  The long form is apart: the kernel has many waits, and what it
+// does between them is short, so that its code has to stay small (129 KB of it, with every wait written out, took
+// 684 us for a prompt of 8192 where XXXX KB take XXXX).
+__device__ __noinline__ bool paged_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  return mbar_wait_warp(bar, parity, abort_flag, err, code & 0xFF, (code & 0x100) != 0);
+}
+__device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return paged_wait_long(bar, parity, abort_flag, err, code);
+}
 
 template <int DH>
 struct PagedSmem {
@@ -199,19 +209,6 @@ __device__ __forceinline__ bool paged_masked(const PagedUnit& u, int t, int wind
   return (t + 1) * kPagedTile > u.first + 1 || (window && t * kPagedTile <= u.last - window);
 }
 
-// End of the tiles that half w of a unit sees.
-__device__ __forceinline__ int paged_end(const PagedUnit& u, int w, const FastDiv& by_group) {
-  if (u.alternate || w == 1) return u.te;
-  const int last = u.pos0 + by_group.of(u.r0 + min(u.rows, kPagedTile) - 1);
-  return max(u.tb, min(u.te, last < 0 ? 0 : last / kPagedTile + 1));
-}
-
-// Tiles of keys that half w takes.
-__device__ __forceinline__ int paged_count(const PagedUnit& u, int w, const FastDiv& by_group) {
-  if (u.alternate) return (u.te - u.tb + 1 - w) >> 1;
-  return w == 1 && u.rows <= kPagedTile ? 0 : paged_end(u, w, by_group) - u.tb;
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -251,6 +248,23 @@ __device__ __forceinline__ void fma2_to(float& x, float& y, float a, float b, fl
       "fma.rn.f32x2 p, q, r, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b), "f"(f));
+}
+
+// Transposes four pieces of four neighbouring lanes: lane l of them gets piece l of each, in order of the lanes.
+__device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, uint4& c, uint4& d, int lane) {
+  auto swap = [&](uint4& x, uint4& y, int by) {  // lanes apart by `by`: the lower keeps x and gets the other's x as y
+    const bool upper = lane & by;
+    uint4 give = upper ? x : y;
+    give.x = __shfl_xor_sync(0xffffffffu, give.x, by);
+    give.y = __shfl_xor_sync(0xffffffffu, give.y, by);
+    give.z = __shfl_xor_sync(0xffffffffu, give.z, by);
+    give.w = __shfl_xor_sync(0xffffffffu, give.w, by);
+    (upper ? x : y) = give;
+  };
+  swap(a, b, 1);
+  swap(c, d, 1);
+  swap(a, c, 2);
+  swap(b, d, 2);
 }
 
 // Of 32 elements from c on of a row's output, a bit for each in which a value of
@@ -360,66 +374,84 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     bool ok = true;
     uint32_t it = 0, uc = 0;
     const PagedBatchParams& bt = a.batch;
-    int64_t total = 0, mine = 0;
-    for (int b = lane; b < bt.seqs; b += 32) total += mine = paged_sequence(p, b).whole;
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    const int blocks = (int)max((int64_t)1, min((int64_t)gridDim.x, total / kPagedLeast));
-    const int64_t share = quotient(total, blocks) + 1;
-    const int64_t begin = min(total, (int64_t)blockIdx.x * share), end = min(total, begin + share);
-    PagedMeta meta{};
-    int64_t at = 0;  // offset of the sequence that `begin` lies in
+    // all sequences' cost, then the sequence that this block's share begins in
+    int total = 0, begin = 0, end = 0, share = 1, at = 0;  // at: offset of sequence seq
     int seq = 0;
-    if (begin < end) {
-      for (int b0 = 0;; b0 += 32) {
-        const int64_t c = b0 + lane >= bt.seqs ? 0 : bt.seqs <= 32 ? mine : paged_sequence(p, b0 + lane).whole;
-        int64_t sum = c;
+#pragma unroll 1
+    for (int pass = 0; pass < 2 && (pass == 0 || begin < end); ++pass) {
+      int sum = 0;
+#pragma unroll 1
+      for (int b0 = 0; b0 < bt.seqs; b0 += 32) {
+        const int c = b0 + lane < bt.seqs ? paged_sequence(p, b0 + lane).whole : 0;
+        int upto = c;
+#pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-          const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
-          if (lane >= d) sum += o;
+          const int o = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += o;
         }
-        const uint32_t beyond = __ballot_sync(0xffffffffu, at + sum > begin);
-        if (beyond || b0 + 32 >= bt.seqs) {
-          const int l = beyond ? __ffs(beyond) - 1 : 31;
-          seq = b0 + l;
-          at += __shfl_sync(0xffffffffu, sum - c, l);
-          break;
+        if (pass) {
+          const uint32_t beyond = __ballot_sync(0xffffffffu, sum + upto > begin);
+          if (beyond) {
+            const int l = __ffs(beyond) - 1;
+            seq = b0 + l;
+            at = sum + __shfl_sync(0xffffffffu, upto - c, l);
+            break;
+          }
         }
-        at += __shfl_sync(0xffffffffu, sum, 31);
+        sum += __shfl_sync(0xffffffffu, upto, 31);
+      }
+      if (pass == 0) {
+        total = sum;
+        const int blocks = max(1, min((int)gridDim.x, total / (p.cost_over * kPagedLeast / kPagedUnitOver)));
+        share = total / blocks + 1;
+        begin = min((int64_t)total, (int64_t)blockIdx.x * share);
+        end = min((int64_t)total, (int64_t)begin + share);
       }
     }
+    PagedMeta meta{};
     PagedSequence s{};
-    if (begin < end) s = paged_sequence(p, seq);
-    int64_t now = begin;  // offset of the next part
+    bool known = false;  // s is sequence seq
+    int now = begin;     // offset of the next part
     while (ok) {
       // the unit at `now`
       PagedUnit u{};
       u.done = 1;
       if (now < end) {
-        while (s.whole <= now - at) {
-          at += s.whole;
-          s = paged_sequence(p, ++seq);
+#pragma unroll 1
+        while (!known || s.whole <= now - at) {
+          if (known) {
+            at += s.whole;
+            ++seq;
+          }
+          if (seq >= bt.seqs) break;  // starts that fall may let the sum overflow
+          s = paged_sequence(p, seq);
+          known = true;
+        }
+        if (seq >= bt.seqs || s.head <= 0) {
+          now = end;
+          continue;
         }
         u.done = 0;
         u.seq = seq;
-        int64_t rest = now - at;
-        u.kvh = (int)quotient(rest, s.head);
+        int rest = now - at;
+        u.kvh = min(rest / s.head, a.kv_heads - 1);
         rest -= u.kvh * s.head;
         int lo = 0, hi = s.tiles - 1;  // the tile of rows: first(i) <= rest < first(i + 1)
+#pragma unroll 1
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
           if (s.cost.first(mid) <= rest) lo = mid;
           else hi = mid - 1;
         }
-        const int64_t cost = s.cost.tile(lo), u0 = now - (rest - s.cost.first(lo)), u1 = u0 + cost;
-        const int64_t rows = (int64_t)s.n * G;
+        const int before = s.cost.first(lo), cost = s.cost.first(lo + 1) - before, u0 = now - (rest - before), u1 = u0 + cost;
         u.r0 = lo * 256;
-        u.rows = (int)min((int64_t)256, rows - u.r0);
-        u.alternate = rows <= kPagedTile;
+        u.rows = (int)min((int64_t)256, (int64_t)s.n * G - u.r0);
+        u.alternate = lo == 0 && u.rows <= kPagedTile;
         u.tok0 = s.tok0;
-        u.pos0 = (int)max((int64_t)s.len - s.n, -((int64_t)1 << 30));
+        u.pos0 = max(s.len, -(1 << 30)) - s.n;
         u.first = u.pos0 + p.by_group.of(u.r0);
         u.last = u.pos0 + p.by_group.of(u.r0 + u.rows - 1);
-        if (s.len > (int64_t)bt.most_pages * bt.page_size) {
+        if (s.len > p.capacity) {
           u.bad = 1;
         } else {
           u.hi = max(0, u.last + 1);
@@ -427,8 +459,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         }
         const int tb = u.lo / kPagedTile, n = max(0, (u.hi + kPagedTile - 1) / kPagedTile - tb);
         // where a share's border cuts the unit, the same for the blocks on either side; not within two tiles of its ends
-        auto cut = [&](int64_t x) {
-          const int c = (int)((float)n * ((float)(x - u0) / (float)cost) + 0.5f);
+        const float per = __fdividef((float)n, (float)cost);
+        auto cut = [&](int x) {
+          const int c = (int)((float)(x - u0) * per + 0.5f);
           return c < 2 ? 0 : n - c < 2 ? n : c;
         };
         const int c1 = now > u0 ? cut(now) : 0, c2 = u1 > end ? cut(end) : n;
@@ -439,23 +472,32 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         if (u1 > end && c2 == 0) {  // the block behind does
           u.done = 1;
         } else {
-          u.tb = tb + c1;
+        u.tb = tb + c1;
           u.te = tb + c2;
+          if (u.alternate) {
+            u.count0 = (c2 - c1 + 1) >> 1;
+            u.count1 = (c2 - c1) >> 1;
+          } else {  // the first half's last row may see fewer
+            const int seen = u.pos0 + p.by_group.of(u.r0 + min(u.rows, kPagedTile) - 1);
+            u.count0 = max(0, min(u.te, seen < 0 ? 0 : seen / kPagedTile + 1) - u.tb);
+            u.count1 = u.rows <= kPagedTile ? 0 : c2 - c1;
+          }
           u.slot = c1 > 0 ? 2 * (int)blockIdx.x : c2 < n ? 2 * (int)blockIdx.x + 1 : -1;
           if (c1 == 0 && c2 < n) {
-            int last = (int)quotient(u1 - 1, share);
-            while (cut((int64_t)last * share) == n) --last;
+            int last = (u1 - 1) / share;
+#pragma unroll 1
+            while (cut(last * share) == n) --last;
             meta = PagedMeta{1, last, u.kvh, u.r0, u.rows, u.tok0, u.pos0, 0};
           }
         }
         now = min(u1, end);
       }
       const uint32_t us = uc % UNITS;
-      if (!(ok = mbar_wait_warp(&u_empty[us], ((uc / UNITS) & 1u) ^ 1u, abort_flag, p.err, 41))) break;
+      if (!(ok = paged_wait(&u_empty[us], ((uc / UNITS) & 1u) ^ 1u, abort_flag, p.err, 41))) break;
       if (lane == 0) {
         PagedUnit& d = units[us];
         d.seq = u.seq, d.kvh = u.kvh, d.r0 = u.r0, d.rows = u.rows, d.tok0 = u.tok0, d.pos0 = u.pos0;
-        d.first = u.first, d.last = u.last;
+        d.first = u.first, d.last = u.last, d.count0 = u.count0, d.count1 = u.count1;
         d.tb = u.tb, d.te = u.te, d.lo = u.lo, d.hi = u.hi, d.alternate = u.alternate, d.slot = u.slot;
         d.done = u.done, d.bad = u.bad, d.dirty = 0;
         mbar_arrive(&u_full[us]);
@@ -487,7 +529,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         ahead = page_of(j + 1);
         if (__any_sync(0xffffffffu, page == -2) && lane == 0) units[us].bad = 1;
         const uint32_t s = it % STAGES;
-        if (!(ok = mbar_wait_warp(&empty[s], ((it / STAGES) & 1u) ^ 1u, abort_flag, p.err, 42))) break;
+        if (!(ok = paged_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, abort_flag, p.err, 42))) break;
         const uint32_t boxes = (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0));
         if (lane == 0) mbar_arrive_expect_tx(&full[s], boxes * (uint32_t)p.box * DH * 2);
         __syncwarp();
@@ -505,121 +547,101 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     if (lane == 0) p.meta[blockIdx.x] = meta;
     if (!ok)  // the copies in flight land before the block leaves
       for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
-        mbar_wait_warp(&full[j % STAGES], (j / STAGES) & 1u, abort_flag, p.err, 43, /*ignore_abort=*/true);
+        paged_wait(&full[j % STAGES], (j / STAGES) & 1u, abort_flag, p.err, 0x100 | 43);
   } else if (warp == kPagedProducts) {
     // ---- products ----
     bool ok = true;
-    uint32_t it = 0, uc = 0, pc[2] = {0, 0}, oc[2] = {0, 0}, vc = 0;
+    uint32_t it = 0, uc = 0, vc = 0;
+    uint32_t p_phase = 0, o_phase = 3u;  // a bit of each half
     const uint32_t idesc_s = paged_idesc<T>(kPagedTile, false), idesc_o = paged_idesc<T>((a.dim + 15) / 16 * 16, true);
     const int steps = (a.dim + 15) / 16;
-    if (p.stall_test) ok = mbar_wait_warp(drain, 0, abort_flag, p.err, 44);
-    auto wait_tile = [&](uint32_t i) {
-      return mbar_wait_warp(&full[i % STAGES], (i / STAGES) & 1u, abort_flag, p.err, 45);
-    };
-    // S of half w from the K tile in stage s
-    auto product_s = [&](int w, int q_tile, uint32_t s) {
-      if (elect_one()) {
-        const uint32_t q = q_smem + q_tile * L::TILE, k = ring + s * L::TILE;
-        for (int i = 0; i < steps; ++i) {
-          const uint32_t off = (i >> 2) * (kPagedTile * 128) + (i & 3) * 32;
-          umma_f16(tmem + w * 128, paged_desc(q + off, 16), paged_desc(k + off, 16), idesc_s, i > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[w]);
-      }
-      __syncwarp();
-    };
-    auto product_o = [&](int w, uint32_t s, bool add) {
-      if (elect_one()) {
-        const uint32_t v = ring + s * L::TILE;
-#pragma unroll
-        for (int i = 0; i < kPagedTile / 16; ++i)
-          umma_f16_tmem_a(tmem + 256 + w * 128, tmem + w * 128 + i * 8, paged_desc(v + i * 2048, kPagedTile * 128), idesc_o,
-                          add || i > 0 ? 1u : 0u);
-        umma_commit(&pv_done[w]);
-      }
-      __syncwarp();
-    };
+    if (p.stall_test) ok = paged_wait(drain, 0, abort_flag, p.err, 44);
     auto commit = [&](uint64_t* bar) {
       if (elect_one()) umma_commit(bar);
       __syncwarp();
     };
     while (ok) {
       const uint32_t us = uc % UNITS;
-      if (!(ok = mbar_wait_warp(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 46))) break;
+      if (!(ok = paged_wait(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 46))) break;
       const PagedUnit& u = units[us];
       if (u.done) break;
-      const int n = u.te - u.tb, alternate = u.alternate, tb = u.tb;
-      const int count[2] = {paged_count(u, 0, p.by_group), paged_count(u, 1, p.by_group)};
-      if (!(ok = mbar_wait_warp(q_full, uc & 1u, abort_flag, p.err, 47))) break;
+      const int n = u.te - u.tb, alternate = u.alternate, tb = u.tb, count0 = u.count0, count1 = u.count1;
+      if (!(ok = paged_wait(q_full, uc & 1u, abort_flag, p.err, 47))) break;
       tc_fence_after();
-      if (n > 0) {
-        if (!(ok = wait_tile(it))) break;
-        tc_fence_after();
-        if (count[0] > 0) product_s(0, 0, it % STAGES);
-        if (!alternate && count[1] > 0) product_s(1, 1, it % STAGES);
-        commit(&empty[it % STAGES]);
-        ++it;
-        if (alternate && n > 1) {
-          if (!(ok = wait_tile(it))) break;
-          tc_fence_after();
-          product_s(1, 0, it % STAGES);
-          commit(&empty[it % STAGES]);
-          ++it;
-        }
-      }
-      if (n <= (alternate ? 2 : 1)) commit(q_empty);
-      for (int t = 0; t < n && ok; ++t) {
-        const uint32_t v = it++;
-        if (!(ok = wait_tile(v))) break;
-        if (paged_masked(u, tb + t, a.window)) {
-          if (lane == 0) mbar_arrive(v_seen);
-          __syncwarp();
-          if (!(ok = mbar_wait_warp(v_clean, vc & 1u, abort_flag, p.err, 48))) break;
-          ++vc;
-        }
-        const int ahead = t + (alternate ? 2 : 1);  // S of this tile of keys follows
-        const uint32_t k = it;
-        if (ahead < n) {
-          ++it;
-          if (!alternate && !(ok = wait_tile(k))) break;
-        }
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if (!ok || (alternate && w != (t & 1))) continue;
-          const int i = alternate ? t >> 1 : t;  // number of the tile among the half's
-          if (i >= count[w]) continue;
-          if (i == 0) {
-            if (!(ok = mbar_wait_warp(&o_free[w], (oc[w] & 1u) ^ 1u, abort_flag, p.err, 49))) break;
-            ++oc[w];
-          }
-          if (!(ok = mbar_wait_warp(&p_full[w], pc[w] & 1u, abort_flag, p.err, 50))) break;
-          ++pc[w];
-          tc_fence_after();
-          product_o(w, v % STAGES, i > 0);
-          if (alternate) commit(&empty[v % STAGES]);
-          if (i + 1 < count[w]) {
-            if (alternate) {
-              if (!(ok = wait_tile(k))) break;
-              tc_fence_after();
+      if (n == 0) commit(q_empty);
+      // Step q is P V of half w = q & 1 with its tile i, then its next S; the first
+      // two are the halves' first S.  Tiles of the unit: i, or 2 i + w.
+      int k_seen = 0, v_seen_to = 0;  // tiles of K and V that were waited for
+#pragma unroll 1
+      for (int q = -2; q < (alternate ? n : 2 * n); ++q) {
+        const int w = q & 1, i = q >> 1, count = w ? count1 : count0;
+        const int t = alternate ? q : i, ahead = t + (alternate ? 2 : 1);  // tile of P V, of the next S
+        const bool last_of_tile = alternate || w == 1;
+        if (q >= 0) {
+          const uint32_t v = it + (alternate ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1);
+          if (t >= v_seen_to) {
+            v_seen_to = t + 1;
+            if (!(ok = paged_wait(&full[v % STAGES], (v / STAGES) & 1u, abort_flag, p.err, 45))) break;
+            if (paged_masked(u, tb + t, a.window)) {
+              if (lane == 0) mbar_arrive(v_seen);
+              __syncwarp();
+              if (!(ok = paged_wait(v_clean, vc & 1u, abort_flag, p.err, 48))) break;
+              ++vc;
             }
-            product_s(w, alternate ? 0 : w, k % STAGES);
           }
+          if (i < count) {
+            if (i == 0) {
+              if (!(ok = paged_wait(&o_free[w], (o_phase >> w) & 1u, abort_flag, p.err, 49))) break;
+              o_phase ^= 1u << w;
+            }
+            if (!(ok = paged_wait(&p_full[w], (p_phase >> w) & 1u, abort_flag, p.err, 50))) break;
+            p_phase ^= 1u << w;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t vs = ring + (v % STAGES) * L::TILE, d = tmem + w * 128;
+#pragma unroll
+              for (int k = 0; k < kPagedTile / 16; ++k)
+                umma_f16_tmem_a(d + 256, d + (k >> 2) * 64 + (k & 3) * 8, paged_desc(vs + k * 2048, kPagedTile * 128), idesc_o,
+                                i > 0 || k > 0 ? 1u : 0u);
+              umma_commit(&pv_done[w]);
+            }
+            __syncwarp();
+          }
+          if (last_of_tile) commit(&empty[v % STAGES]);
         }
-        if (!ok) break;
-        if (!alternate) commit(&empty[v % STAGES]);
-        if (ahead < n) {
+        if (ahead >= n) continue;
+        const uint32_t k = it + (alternate ? (ahead == 0 ? 0 : 2 * ahead - 1) : 2 * ahead);
+        if (ahead >= k_seen) {
+          k_seen = ahead + 1;
+          if (!(ok = paged_wait(&full[k % STAGES], (k / STAGES) & 1u, abort_flag, p.err, 45))) break;
+          tc_fence_after();
+        }
+        if (i + 1 < count) {
+          if (elect_one()) {
+            const uint32_t qs = q_smem + (alternate ? 0 : w * L::TILE), ks = ring + (k % STAGES) * L::TILE;
+#pragma unroll 1
+            for (int c = 0; c < steps; ++c) {
+              const uint32_t off = (c >> 2) * (kPagedTile * 128) + (c & 3) * 32;
+              umma_f16(tmem + w * 128, paged_desc(qs + off, 16), paged_desc(ks + off, 16), idesc_s, c > 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[w]);
+          }
+          __syncwarp();
+        }
+        if (last_of_tile) {
           commit(&empty[k % STAGES]);
           if (ahead == n - 1) commit(q_empty);
         }
       }
       if (!ok) break;
+      it += 2 * n;
       if (lane == 0) mbar_arrive(&u_empty[us]);
       __syncwarp();
       ++uc;
     }
     if (!ok) {
       commit(drain);
-      mbar_wait_warp(drain, 0, abort_flag, p.err, 52, /*ignore_abort=*/true);
+      paged_wait(drain, 0, abort_flag, p.err, 0x100 | 52);
     }
   } else if (warp >= kPagedQueries) {
     // ---- Q, and values of tiles that are seen in part ----
@@ -628,10 +650,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     uint32_t it = 0, uc = 0, vc = 0;
     while (ok) {
       const uint32_t us = uc % UNITS;
-      if (!(ok = mbar_wait_warp(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 53))) break;
+      if (!(ok = paged_wait(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 53))) break;
       PagedUnit& u = units[us];
       if (u.done) break;
-      if (!(ok = mbar_wait_warp(q_empty, (uc & 1u) ^ 1u, abort_flag, p.err, 54))) break;
+      if (!(ok = paged_wait(q_empty, (uc & 1u) ^ 1u, abort_flag, p.err, 54))) break;
       if (p.q_tma) {  // G heads by 128 / G tokens: rows behind the unit's are other tokens', of which nothing is used
         if (elect_one()) {
           const int tiles = u.rows > kPagedTile ? 2 : 1;
@@ -651,7 +673,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         constexpr int CH = DH / 8;  // 16-byte pieces of a row
         const int c = lane % CH, rows = u.rows;
         const T* q = static_cast<const T*>(a.q) + (int64_t)u.tok0 * a.q_token + (int64_t)u.kvh * G * a.q_head + c * 8;
-#pragma unroll 4
+#pragma unroll 2
         for (int r = me * (32 / CH) + lane / CH; r < rows; r += 2 * (32 / CH)) {
           const int row = u.r0 + r, tok = p.by_group.of(row), g = row - tok * G;
           const uint32_t dst = q_smem + (r >> 7) * L::TILE + (c >> 3) * (kPagedTile * 128) + (r & 127) * 128 +
@@ -670,9 +692,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         if (!paged_masked(u, u.tb + t, a.window)) continue;
         const uint32_t v = it + (u.alternate ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1), s = v % STAGES;
         // the products wait at this tile: it has landed, and stays until it is clean
-        if (!(ok = mbar_wait_warp(v_seen, vc & 1u, abort_flag, p.err, 51))) break;
+        if (!(ok = paged_wait(v_seen, vc & 1u, abort_flag, p.err, 51))) break;
         ++vc;
-        if (!(ok = mbar_wait_warp(&full[s], (v / STAGES) & 1u, abort_flag, p.err, 55))) break;
+        if (!(ok = paged_wait(&full[s], (v / STAGES) & 1u, abort_flag, p.err, 55))) break;
         const int key0 = (u.tb + t) * kPagedTile;
         constexpr int CH = DH / 8;
         uint8_t* tile = smem + s * L::TILE;
@@ -680,32 +702,37 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         const int c = lane % CH, r_first = me * (32 / CH) + lane / CH;
         constexpr int STEP = 2 * (32 / CH);
         // keys outside of the unit's
+#pragma unroll 1
         for (int row = r_first; row < min(kPagedTile, u.lo - key0); row += STEP) *piece(row, c) = make_uint4(0, 0, 0, 0);
+#pragma unroll 2
         for (int row = max(r_first, r_first + (u.hi - key0 - r_first + STEP - 1) / STEP * STEP); row < kPagedTile; row += STEP)
           *piece(row, c) = make_uint4(0, 0, 0, 0);
         // keys that some rows see and others do not: the last ones, and those before the last row's window
         uint32_t found = 0;
-        auto scan = [&](int from, int to) {
-          from = max(from, max(0, u.lo - key0)), to = min(to, min(kPagedTile, u.hi - key0));
+        const int late = u.first + 1 - key0;
+#pragma unroll 1
+        for (int part = a.window ? 0 : 1; part < 2; ++part) {
+          const int from = max(part ? late : 0, max(0, u.lo - key0));
+          const int to = min(part ? kPagedTile : (int)min((int64_t)late, (int64_t)u.last - a.window - key0 + 1),
+                             min(kPagedTile, u.hi - key0));
+#pragma unroll 1
           for (int row0 = from + r_first; row0 < to; row0 += 4 * STEP) {
             uint4 x[4];
             uint32_t any = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = row0 + i * STEP < to ? *piece(row0 + i * STEP, c) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) any |= not_finite<T>(x[i].x) | not_finite<T>(x[i].y) | not_finite<T>(x[i].z) | not_finite<T>(x[i].w);
+            for (int i = 0; i < 4; ++i) {
+              x[i] = row0 + i * STEP < to ? *piece(row0 + i * STEP, c) : make_uint4(0, 0, 0, 0);
+              any |= not_finite<T>(x[i].x) | not_finite<T>(x[i].y) | not_finite<T>(x[i].z) | not_finite<T>(x[i].w);
+            }
             if (!(any & 0x80008000u)) continue;
             found = 1;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (row0 + i * STEP < to)
-                *piece(row0 + i * STEP, c) = make_uint4(finite_or_zero<T>(x[i].x), finite_or_zero<T>(x[i].y),
-                                                        finite_or_zero<T>(x[i].z), finite_or_zero<T>(x[i].w));
+#pragma unroll 1
+            for (int row = row0; row < min(to, row0 + 4 * STEP); row += STEP) {
+              const uint4 w = *piece(row, c);
+              *piece(row, c) = make_uint4(finite_or_zero<T>(w.x), finite_or_zero<T>(w.y), finite_or_zero<T>(w.z), finite_or_zero<T>(w.w));
+            }
           }
-        };
-        const int late = u.first + 1 - key0;
-        scan(late, kPagedTile);
-        if (a.window) scan(0, (int)min((int64_t)late, (int64_t)u.last - a.window - key0 + 1));
+        }
         if (found) u.dirty = 1;
         fence_proxy_async_smem();
         __syncwarp();
@@ -737,11 +764,11 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     uint32_t uc = 0, cnt0 = 0, cnt1 = 0, mc = 0;
     while (ok) {
       const uint32_t us = uc % UNITS;
-      if (!(ok = mbar_wait_warp(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 56))) break;
+      if (!(ok = paged_wait(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 56))) break;
       const PagedUnit& u = units[us];
       if (u.done) break;
       const int alternate = u.alternate, tb = u.tb;
-      const int count0 = paged_count(u, 0, p.by_group), count1 = paged_count(u, 1, p.by_group), count = w ? count1 : count0;
+      const int count0 = u.count0, count1 = u.count1, count = w ? count1 : count0;
       const uint32_t done = w ? cnt1 : cnt0;  // tiles of this half so far
       const int r = (alternate ? 0 : w * kPagedTile) + quarter * 32 + lane;  // row of the unit
       const bool real = r < u.rows, active = (alternate ? 0 : w * kPagedTile) + quarter * 32 < u.rows;
@@ -749,17 +776,21 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       float m = -INFINITY, sum = 0.0f;
       for (int i = 0; i < count && ok; ++i) {
         const int t = tb + (alternate ? 2 * i + w : i);
-        if (!(ok = mbar_wait_warp(&s_full[w], (done + i) & 1u, abort_flag, p.err, 57))) break;
+        if (!(ok = paged_wait(&s_full[w], (done + i) & 1u, abort_flag, p.err, 57))) break;
         tc_fence_after();
         if (active) {
           // columns that this row sees: low < column <= high
           const int high = position - t * kPagedTile - side * 64;
           const int low = a.window ? (int)max((int64_t)high - a.window, (int64_t)-1) : -1;
           const bool partly = __any_sync(0xffffffffu, real && (high < 63 || low >= 0));
-          // 32 scores; twice the first ones, since all 64 and what else a thread keeps do not fit its registers
-          // (spilled ones went to L2: 8700 cycles for two tiles instead of XXXX)
-          uint32_t x[32];
-          auto load = [&](int c) {
+          // The second 32 of the thread's scores, the first, and the second again: all 64 and what else a thread
+          // keeps do not fit its registers, and what is spilled goes to L2.  P of 32 goes over the first 16 columns
+          // of the scores, when both are done with.
+          float high_s = -INFINITY, base = 0.0f, part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+          for (int pass = 0; pass < 3; ++pass) {
+            const int c = (pass & 1) ^ 1;
+            uint32_t x[32];
             __syncwarp();
             FTB_TMEM_LD32(s_tmem + side * 64 + c * 32, x);
             FTB_TMEM_WAIT_LD32(x);
@@ -774,49 +805,42 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               for (int k = 0; k < 32; ++k)
                 if (!(seen & (1u << k))) x[k] = 0xFF800000u;
             }
-          };
-          auto largest = [&]() {
-            float top[2];
+            if (pass < 2) {
+              float top[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              top[c] = fmaxf(__uint_as_float(x[16 * c]), __uint_as_float(x[16 * c + 1]));
+              for (int k = 0; k < 2; ++k) {
+                top[k] = fmaxf(__uint_as_float(x[16 * k]), __uint_as_float(x[16 * k + 1]));
 #pragma unroll
-              for (int k = 2; k < 16; k += 2)
-                top[c] = max3(top[c], __uint_as_float(x[16 * c + k]), __uint_as_float(x[16 * c + k + 1]));
-            }
-            return fmaxf(top[0], top[1]);
-          };
-          load(0);
-          float high_s = largest();
-          load(1);
-          high_s = fmaxf(high_s, largest());
-          // after this both warps have their S, over which P goes
-          high_s = fmaxf(high_s, exchange(high_s)) * a.scale;
-          const bool raise = real && high_s > m + kPagedRaise;
-          if (__any_sync(0xffffffffu, raise)) {
-            float keep = 1.0f;
-            if (raise) {
-              keep = ex2(m - high_s);
-              sum *= keep;
-              m = high_s;
-            }
-            if (i > 0) {  // this S followed the last P V, so O is complete; each warp has half of its columns
-#pragma unroll 1
-              for (int c = side * (DH / 2); c < (side + 1) * (DH / 2) && c < a.dim; c += 32) {
-                uint32_t o[32];
-                __syncwarp();
-                FTB_TMEM_LD32(tmem + 256 + w * 128 + lanes + c, o);
-                FTB_TMEM_WAIT_LD32(o);
-#pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                FTB_TMEM_ST32(tmem + 256 + w * 128 + lanes + c, o);
+                for (int e = 2; e < 16; e += 2)
+                  top[k] = max3(top[k], __uint_as_float(x[16 * k + e]), __uint_as_float(x[16 * k + e + 1]));
               }
+              high_s = max3(high_s, top[0], top[1]);
             }
-          }
-          const float base = m == -INFINITY ? 0.0f : m;
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          uint32_t o[32];
-          auto weights = [&](uint32_t* to) {
+            if (pass == 0) continue;
+            if (pass == 1) {
+              high_s = fmaxf(high_s, exchange(high_s)) * a.scale;
+              const bool raise = real && high_s > m + kPagedRaise;
+              if (__any_sync(0xffffffffu, raise)) {
+                float keep = 1.0f;
+                if (raise) {
+                  keep = ex2(m - high_s);
+                  sum *= keep;
+                  m = high_s;
+                }
+                // this S followed the last P V, so O is complete; each of a row's warps has half of its columns
+#pragma unroll 1
+                for (int d = i > 0 ? side * (DH / 2) : a.dim; d < (side + 1) * (DH / 2) && d < a.dim; d += 16) {
+                  uint32_t o[16];
+                  __syncwarp();
+                  FTB_TMEM_LD16(tmem + 256 + w * 128 + lanes + d, o);
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                  FTB_TMEM_ST16(tmem + 256 + w * 128 + lanes + d, o);
+                }
+              }
+              base = m == -INFINITY ? 0.0f : m;
+            }
+            uint32_t o[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               float u = __uint_as_float(x[2 * k]), v = __uint_as_float(x[2 * k + 1]);
@@ -824,13 +848,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               u = ex2(u);
               v = ex2(v);
               add2(part[2 * (k & 1)], part[2 * (k & 1) + 1], u, v);
-              to[k] = pack2<T>(u, v);
+              o[k] = pack2<T>(u, v);
             }
-          };
-          weights(o + 16);
-          load(0);
-          weights(o);
-          FTB_TMEM_ST32(s_tmem + side * 32, o);
+            FTB_TMEM_ST16(s_tmem + side * 64 + c * 16, o);
+          }
           sum += (part[0] + part[1]) + (part[2] + part[3]);
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
@@ -846,7 +867,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       const bool both = alternate && count0 > 0, mine = !alternate || w == 0;
       float f0 = 1.0f, f1 = 1.0f;  // factors of the halves' O
       if (count > 0) {
-        if (!(ok = mbar_wait_warp(&pv_done[w], (done + count - 1) & 1u, abort_flag, p.err, 60))) break;
+        if (!(ok = paged_wait(&pv_done[w], (done + count - 1) & 1u, abort_flag, p.err, 60))) break;
         sum += exchange(sum);
         meet();
       }
@@ -855,10 +876,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(ml_full);
         __syncwarp();
-        if (!(ok = mbar_wait_warp(ml_free, mc & 1u, abort_flag, p.err, 61))) break;
+        if (!(ok = paged_wait(ml_free, mc & 1u, abort_flag, p.err, 61))) break;
       }
       if (both && w == 0) {
-        if (!(ok = mbar_wait_warp(ml_full, mc & 1u, abort_flag, p.err, 59))) break;
+        if (!(ok = paged_wait(ml_full, mc & 1u, abort_flag, p.err, 59))) break;
         const float m1 = rows[(8 + quarter) * 32], sum1 = rows[(12 + quarter) * 32];
         __syncwarp();
         if (lane == 0) mbar_arrive(ml_free);
@@ -871,30 +892,33 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       }
       if (both) ++mc;
       if (mine) {
-        if (both && count1 > 0 && !(ok = mbar_wait_warp(&pv_done[1], (cnt1 - 1) & 1u, abort_flag, p.err, 63))) break;
+        if (both && count1 > 0 && !(ok = paged_wait(&pv_done[1], (cnt1 - 1) & 1u, abort_flag, p.err, 63))) break;
         tc_fence_after();
         const bool bad = u.bad, dirty = u.dirty;
         const int g = u.r0 + r - tok * G;
+        // a part of the workspace: (m, sum) of each row, then O in quads of columns, each of them of all rows
         float* part = p.parts + (int64_t)max(u.slot, 0) * p.rows_bound * (2 + DH);
         if (u.slot >= 0 && real && side == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, bad ? NAN : sum);
-        part += 2 * p.rows_bound + (int64_t)r * DH;
-        T* out = static_cast<T*>(a.out) + (int64_t)(u.tok0 + tok) * a.o_token + (int64_t)(u.kvh * G + g) * a.o_head;
-        const float inv = 1.0f / sum;
+        const float by = u.slot >= 0 ? 1.0f : bad ? NAN : position < 0 ? 0.0f : 1.0f / sum;
+        f0 *= by;
+        f1 *= by;
+        const int64_t out = (int64_t)(u.tok0 + tok) * a.o_token + (int64_t)(u.kvh * G + g) * a.o_head;
         if (active) {
 #pragma unroll 1
           for (int c = side * (DH / 2); c < (side + 1) * (DH / 2) && c < a.dim; c += 32) {
             float v[32];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = 0.0f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (!((both || h == w) && (h ? count1 : count0) > 0)) continue;
+            for (int k = 0; k < 32; ++k) v[k] = by != by ? NAN : 0.0f;
+#pragma unroll 1
+            for (int h = both ? 0 : w; h < (both ? 2 : w + 1); ++h) {
+              if ((h ? count1 : count0) == 0) continue;
+              const float f = h && both ? f1 : f0;
               uint32_t o[32];
               __syncwarp();
               FTB_TMEM_LD32(tmem + 256 + h * 128 + lanes + c, o);
               FTB_TMEM_WAIT_LD32(o);
 #pragma unroll
-              for (int k = 0; k < 32; k += 2) fma2_to(v[k], v[k + 1], __uint_as_float(o[k]), __uint_as_float(o[k + 1]), h ? f1 : f0);
+              for (int k = 0; k < 32; k += 2) fma2_to(v[k], v[k + 1], __uint_as_float(o[k]), __uint_as_float(o[k + 1]), f);
             }
             if (dirty && real) {
               const uint32_t bits = paged_marks<T>(p, u, position, c);
@@ -906,16 +930,24 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               if (real) {
 #pragma unroll
                 for (int k = 0; k < 32; k += 4)
-                  *reinterpret_cast<float4*>(part + c + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                  *reinterpret_cast<float4*>(part + 2 * p.rows_bound + ((int64_t)((c + k) / 4) * p.rows_bound + r) * 4) =
+                      make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
               }
-            } else if (real) {
-              const float by = bad ? NAN : position < 0 ? 0.0f : inv;
+              continue;
+            }
+            // Four lanes exchange the 16-byte pieces of their rows, so that they store 64 bytes of one row at a time:
+            // a store of 32 rows takes as many turns of the memory pipe as it has lines.
+            uint4 o[4];
 #pragma unroll
-              for (int k = 0; k < 32; k += 8)
-                if (c + k < a.dim)
-                  *reinterpret_cast<uint4*>(out + c + k) =
-                      make_uint4(pack2<T>(v[k] * by, v[k + 1] * by), pack2<T>(v[k + 2] * by, v[k + 3] * by),
-                                 pack2<T>(v[k + 4] * by, v[k + 5] * by), pack2<T>(v[k + 6] * by, v[k + 7] * by));
+            for (int k = 0; k < 4; ++k)
+              o[k] = make_uint4(pack2<T>(v[8 * k], v[8 * k + 1]), pack2<T>(v[8 * k + 2], v[8 * k + 3]),
+                                pack2<T>(v[8 * k + 4], v[8 * k + 5]), pack2<T>(v[8 * k + 6], v[8 * k + 7]));
+            swap_pieces(o[0], o[1], o[2], o[3], lane);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // row 4 (lane / 4) + k, piece lane % 4
+              const int64_t to = __shfl_sync(0xffffffffu, real ? out : (int64_t)-1, (lane & 28) + k);
+              const int e = c + 8 * (lane & 3);
+              if (to >= 0 && e < a.dim) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to + e) = o[k];
             }
           }
         }
@@ -942,52 +974,44 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
 }
 
 // Units that several blocks worked on: block x of the grid joins the one that
-// block x of paged_attention_kernel began and did not finish, a warp a row.
+// block x of paged_attention_kernel began and did not finish; a thread has four
+// columns of a row, the rows side by side.
 // O = sum_k O_k 2^(m_k - m) / sum_k sum_k 2^(m_k - m), parts in order.
+constexpr int kPagedJoinThreads = 256;
+
 template <typename T, int DH>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedTensorParams p) {
+__global__ void __launch_bounds__(kPagedJoinThreads) paged_join_kernel(const PagedTensorParams p) {
   grid_dep_wait();
   grid_dep_trigger();
-  constexpr int E = DH / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PagedMeta u = p.meta[blockIdx.x];
   if (!u.open) return;
   const PagedAttentionParams& a = p.a;
+  const int rows = min(32, p.rows_bound), at = (int)(blockIdx.y * kPagedJoinThreads + threadIdx.x);
+  const int r = at % rows + at / (rows * (DH / 4)) * 32, quad = at / rows % (DH / 4);
+  if (r >= u.rows || 4 * quad >= a.dim) return;
   const int parts = u.last - (int)blockIdx.x + 1;
   const int64_t stride = (int64_t)p.rows_bound * (2 + DH);
   auto part = [&](int k) { return p.parts + (k == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + k)) * stride; };
-  for (int r = blockIdx.y * 32 + warp; r < min(u.rows, (int)blockIdx.y * 32 + 32); r += 8) {
-    float top = -INFINITY;
-    for (int k = lane; k < parts; k += 32) top = fmaxf(top, part(k)[2 * r]);
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+  float m = -INFINITY, sum = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-      const float2 x = *reinterpret_cast<const float2*>(part(k) + 2 * r);
-      const float* v = part(k) + 2 * p.rows_bound + (int64_t)r * DH + lane * E;
-      float t[E];
-      if constexpr (E == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(v);
-        t[0] = y.x, t[1] = y.y, t[2] = y.z, t[3] = y.w;
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(v);
-        t[0] = y.x, t[1] = y.y;
-      }
-      const float f = ex2(x.x - base);
-      sum = __fmaf_rn(x.y, f, sum);
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = lane * E + e < a.dim ? __fmaf_rn(t[e], f, o[e]) : 0.0f;
-    }
-    const int tok = p.by_group.of(u.r0 + r), g = u.r0 + r - tok * p.group;
-    T* out = static_cast<T*>(a.out) + (int64_t)(u.tok0 + tok) * a.o_token + (int64_t)(u.kvh * p.group + g) * a.o_head;
-    const bool nothing = u.pos0 + tok < 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (lane * E + e < a.dim) out[lane * E + e] = from_f32<T>(nothing ? 0.0f : o[e] / sum);
+  for (int k = 0; k < parts; ++k) {
+    const float2 x = *reinterpret_cast<const float2*>(part(k) + 2 * r);
+    const float4 v = *reinterpret_cast<const float4*>(part(k) + 2 * p.rows_bound + ((int64_t)quad * p.rows_bound + r) * 4);
+    const float top = fmaxf(m, x.x), base = top == -INFINITY ? 0.0f : top, f = ex2(m - base), g = ex2(x.x - base);
+    m = top;
+    sum = sum * f + x.y * g;
+    o.x = o.x * f + v.x * g;
+    o.y = o.y * f + v.y * g;
+    o.z = o.z * f + v.z * g;
+    o.w = o.w * f + v.w * g;
   }
+  const int tok = p.by_group.of(u.r0 + r), g = u.r0 + r - tok * p.group;
+  const float by = 1.0f / sum;
+  if (u.pos0 + tok < 0) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  else o = make_float4(o.x * by, o.y * by, o.z * by, o.w * by);
+  T* out = static_cast<T*>(a.out) + (int64_t)(u.tok0 + tok) * a.o_token + (int64_t)(u.kvh * p.group + g) * a.o_head + 4 * quad;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
 }
 
 // ---------------------------------------------------------------------------
@@ -1057,8 +1081,11 @@ cudaError_t launch_paged_as(PagedTensorParams& p, int type, int blocks, cudaStre
                            p.group, kPagedTile / p.group);
   cudaError_t e = pdl_launch(paged_attention_kernel<T, DH>, dim3((unsigned)blocks), dim3(kPagedThreads), PagedSmem<DH>::TOTAL, s,
                              map_k, map_v, map_q, p);
-  if (e == cudaSuccess)
-    e = pdl_launch(paged_join_kernel<T, DH>, dim3((unsigned)blocks, (unsigned)(p.rows_bound + 31) / 32), dim3(256), 0, s, p);
+  if (e == cudaSuccess) {
+    const int rows = std::min(32, p.rows_bound), threads = (p.rows_bound + rows - 1) / rows * rows * (DH / 4);
+    e = pdl_launch(paged_join_kernel<T, DH>, dim3((unsigned)blocks, (unsigned)((threads + kPagedJoinThreads - 1) / kPagedJoinThreads)),
+                   dim3(kPagedJoinThreads), 0, s, p);
+  }
   return e;
 }
 
@@ -1072,7 +1099,16 @@ inline cudaError_t launch_paged_attention(const PagedAttentionParams& a, int typ
   p.negative = a.scale < 0.0f;
   p.group = a.heads / a.kv_heads;
   p.by_group = FastDiv((uint32_t)p.group);
-  p.step = std::max(1, 256 / p.group);
+  // the largest sum of costs that tokens and page table allow fits 31 bits
+  p.capacity = (int)std::min<int64_t>((int64_t)a.batch.most_pages * a.batch.page_size, 0x7fffffff);
+  const int step = std::max(1, 256 / p.group);
+  const double tiles = (double)a.kv_heads * ((double)a.tokens * p.group / 256 + std::min(a.batch.seqs, a.tokens));
+  const double most = a.window ? std::min<double>(p.capacity, (double)a.window + step) : p.capacity;
+  while (tiles * (most / (1 << p.cost_shift) + std::max(1, kPagedUnitOver >> p.cost_shift) + 1) > 0x3fffffff && p.cost_shift < 20)
+    ++p.cost_shift;
+  p.cost_step = step >> p.cost_shift;
+  p.cost_over = std::max(1, kPagedUnitOver >> p.cost_shift);
+  p.window_cap = (int)std::min<int64_t>((int64_t)a.window + step, 0x7fffffff);
   p.box = 16;
   while (p.box < kPagedTile && a.batch.page_size % (2 * p.box) == 0) p.box *= 2;
   p.rows_bound = paged_rows_bound(a);

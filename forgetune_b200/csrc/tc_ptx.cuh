@@ -181,6 +181,23 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])                                   \
       : "memory")
 
+#define FTB_TMEM_ST16(taddr, r)                                                                                 \
+  asm volatile(                                                                                                 \
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), \
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),         \
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])                         \
+      : "memory")
+
+// 16 columns, waited for
+#define FTB_TMEM_LD16(taddr, r)                                                                                 \
+  asm volatile(                                                                                                 \
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t" \
+      "tcgen05.wait::ld.sync.aligned;"                                                                          \
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),         \
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])    \
+      : "r"(taddr)                                                                                              \
+      : "memory")
+
 // tcgen05.wait::ld for a load into r issued earlier: r is an operand, so the
 // compiler treats the registers as written here (the load fills them
 // asynchronously) and neither reads nor moves them before
