@@ -137,6 +137,13 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedTensorParams&
 __device__ __noinline__ bool paged_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
   return mbar_wait_warp(bar, parity, abort_flag, err, code & 0xFF, (code & 0x100) != 0);
 }
+// ... by a thread for itself.
+__device__ __noinline__ bool paged_wait_one_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  return mbar_wait(bar, parity, abort_flag, err, code & 0xFF, (code & 0x100) != 0);
+}
+__device__ __forceinline__ bool paged_wait_one(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  return mbar_try_wait(bar, parity) || paged_wait_one_long(bar, parity, abort_flag, err, code);
+}
 __device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return paged_wait_long(bar, parity, abort_flag, err, code);
@@ -150,7 +157,7 @@ struct PagedSmem {
   static constexpr int Q_OFF = STAGES * TILE;
   static constexpr int ROW_OFF = Q_OFF + 2 * TILE;  // [16 softmax warps][32]: a row's maximum or sum
   static constexpr int UNIT_OFF = ROW_OFF + 16 * 32 * 4;
-  static constexpr int UNITS = 2;
+  static constexpr int UNITS = 4;
   static constexpr int BAR_OFF = (UNIT_OFF + UNITS * (int)sizeof(PagedUnit) + 15) / 16 * 16;
   static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 4 + 5;
   static constexpr int TOTAL = BAR_OFF + 8 * NBAR + 16;
@@ -167,27 +174,26 @@ __device__ __forceinline__ uint32_t paged_idesc(int n, bool b_by_rows) {
 // Operand tiles of 128-byte rows in the 128-byte swizzle, 8-row groups 1024
 // bytes apart: K-major (Q, K: rows are M or N, 64 of the depth side by side) and
 // MN-major (V: rows are the depth, 64 of N side by side, the next 64 a tile of
-// 128 rows further).
-__device__ __forceinline__ uint64_t paged_desc(uint32_t saddr, uint32_t lead) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// 128 rows further).  The descriptor's upper word is the same for all; the lower has
+// the address and `lead`, both in units of 16 bytes.
+constexpr uint32_t kPagedDesc = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t paged_desc(uint32_t saddr, uint32_t lead) { return (saddr >> 4) | ((lead >> 4) << 16); }
 
-__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kPagedDesc)
       : "memory");
 }
 // A in tensor memory: a lane a row, eight columns 16 values of the depth
-__device__ __forceinline__ void umma_f16_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16_tmem_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kPagedDesc)
       : "memory");
 }
 
@@ -366,283 +372,115 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   tc_fence_after();
   grid_dep_wait();
   grid_dep_trigger();
+  // Costs of many sequences: each warp sums a run of them, in chunks of 32.
+  const int chunks = (a.batch.seqs + 31) / 32, run = (chunks + kPagedThreads / 32 - 1) / (kPagedThreads / 32);
+  int* warp_cost = reinterpret_cast<int*>(smem + L::ROW_OFF);
+  if (chunks > 2) {
+    int sum = 0;
+#pragma unroll 1
+    for (int c = warp * run; c < min(chunks, (warp + 1) * run); ++c)
+      sum += c * 32 + lane < a.batch.seqs ? paged_sequence(p, c * 32 + lane).whole : 0;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) warp_cost[warp] = sum;
+    __syncthreads();
+  }
   const uint32_t tmem = *tmem_slot;
   const uint32_t ring = smem_u32(smem), q_smem = smem_u32(smem + L::Q_OFF);
 
   if (warp == kPagedProducer) {
-    // ---- units, keys and values ----
-    bool ok = true;
-    uint32_t it = 0, uc = 0;
-    const PagedBatchParams& bt = a.batch;
-    // all sequences' cost, then the sequence that this block's share begins in
-    int total = 0, begin = 0, end = 0, share = 1, at = 0;  // at: offset of sequence seq
-    int seq = 0;
-#pragma unroll 1
-    for (int pass = 0; pass < 2 && (pass == 0 || begin < end); ++pass) {
-      int sum = 0;
-#pragma unroll 1
-      for (int b0 = 0; b0 < bt.seqs; b0 += 32) {
-        const int c = b0 + lane < bt.seqs ? paged_sequence(p, b0 + lane).whole : 0;
-        int upto = c;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int o = __shfl_up_sync(0xffffffffu, upto, d);
-          if (lane >= d) upto += o;
-        }
-        if (pass) {
-          const uint32_t beyond = __ballot_sync(0xffffffffu, sum + upto > begin);
-          if (beyond) {
-            const int l = __ffs(beyond) - 1;
-            seq = b0 + l;
-            at = sum + __shfl_sync(0xffffffffu, upto - c, l);
-            break;
-          }
-        }
-        sum += __shfl_sync(0xffffffffu, upto, 31);
-      }
-      if (pass == 0) {
-        total = sum;
-        const int blocks = max(1, min((int)gridDim.x, total / (p.cost_over * kPagedLeast / kPagedUnitOver)));
-        share = total / blocks + 1;
-        begin = min((int64_t)total, (int64_t)blockIdx.x * share);
-        end = min((int64_t)total, (int64_t)begin + share);
-      }
-    }
-    PagedMeta meta{};
-    PagedSequence s{};
-    bool known = false;  // s is sequence seq
-    int now = begin;     // offset of the next part
-    while (ok) {
-      // the unit at `now`
-      PagedUnit u{};
-      u.done = 1;
-      if (now < end) {
-#pragma unroll 1
-        while (!known || s.whole <= now - at) {
-          if (known) {
-            at += s.whole;
-            ++seq;
-          }
-          s = paged_sequence(p, seq);
-          known = true;
-        }
-        u.done = 0;
-        u.seq = seq;
-        int rest = now - at;
-        u.kvh = rest / s.head;
-        rest -= u.kvh * s.head;
-        int lo = 0, hi = s.tiles - 1;  // the tile of rows: first(i) <= rest < first(i + 1)
-#pragma unroll 1
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (s.cost.first(mid) <= rest) lo = mid;
-          else hi = mid - 1;
-        }
-        const int before = s.cost.first(lo), cost = s.cost.first(lo + 1) - before, u0 = now - (rest - before), u1 = u0 + cost;
-        u.r0 = lo * 256;
-        u.rows = (int)min((int64_t)256, (int64_t)s.n * G - u.r0);
-        u.alternate = lo == 0 && u.rows <= kPagedTile;
-        u.tok0 = s.tok0;
-        u.pos0 = max(s.len, -(1 << 30)) - s.n;
-        u.first = u.pos0 + p.by_group.of(u.r0);
-        u.last = u.pos0 + p.by_group.of(u.r0 + u.rows - 1);
-        if (s.len > p.capacity) {
-          u.bad = 1;
-        } else {
-          u.hi = max(0, u.last + 1);
-          u.lo = a.window ? (int)max((int64_t)0, (int64_t)u.first - a.window + 1) : 0;
-        }
-        const int tb = u.lo / kPagedTile, n = max(0, (u.hi + kPagedTile - 1) / kPagedTile - tb);
-        // where a share's border cuts the unit, the same for the blocks on either side; not within two tiles of its ends
-        const float per = __fdividef((float)n, (float)cost);
-        auto cut = [&](int x) {
-          const int c = (int)((float)(x - u0) * per + 0.5f);
-          return c < 2 ? 0 : n - c < 2 ? n : c;
-        };
-        const int c1 = now > u0 ? cut(now) : 0, c2 = u1 > end ? cut(end) : n;
-        if (c1 == n && n > 0) {  // the block before took all of it
-          now = min(u1, end);
-          continue;
-        }
-        if (u1 > end && c2 == 0) {  // the block behind does
-          u.done = 1;
-        } else {
-        u.tb = tb + c1;
-          u.te = tb + c2;
-          if (u.alternate) {
-            u.count0 = (c2 - c1 + 1) >> 1;
-            u.count1 = (c2 - c1) >> 1;
-          } else {  // the first half's last row may see fewer
-            const int seen = u.pos0 + p.by_group.of(u.r0 + min(u.rows, kPagedTile) - 1);
-            u.count0 = max(0, min(u.te, seen < 0 ? 0 : seen / kPagedTile + 1) - u.tb);
-            u.count1 = u.rows <= kPagedTile ? 0 : c2 - c1;
-          }
-          u.slot = c1 > 0 ? 2 * (int)blockIdx.x : c2 < n ? 2 * (int)blockIdx.x + 1 : -1;
-          if (c1 == 0 && c2 < n) {
-            int last = (u1 - 1) / share;
-#pragma unroll 1
-            while (cut(last * share) == n) --last;
-            meta = PagedMeta{1, last, u.kvh, u.r0, u.rows, u.tok0, u.pos0, 0};
-          }
-        }
-        now = min(u1, end);
-      }
-      const uint32_t us = uc % UNITS;
-      if (!(ok = paged_wait(&u_empty[us], ((uc / UNITS) & 1u) ^ 1u, abort_flag, p.err, 41))) break;
-      if (lane == 0) {
-        PagedUnit& d = units[us];
-        d.seq = u.seq, d.kvh = u.kvh, d.r0 = u.r0, d.rows = u.rows, d.tok0 = u.tok0, d.pos0 = u.pos0;
-        d.first = u.first, d.last = u.last, d.count0 = u.count0, d.count1 = u.count1;
-        d.tb = u.tb, d.te = u.te, d.lo = u.lo, d.hi = u.hi, d.alternate = u.alternate, d.slot = u.slot;
-        d.done = u.done, d.bad = u.bad, d.dirty = 0;
-        mbar_arrive(&u_full[us]);
-      }
-      __syncwarp();
-      ++uc;
-      if (u.done) break;
-      // K and V in the order of their products: K0 [K(i + 1)] V(i) where the
-      // halves alternate, K0 V(i) [K(i + 1)] where they share
-      const int n = u.te - u.tb;
-      const int* table = bt.page_table + u.seq * bt.table_ld;
-      // number j of them: its tile, and this lane's key and page (-1: none wanted, -2: none there)
-      auto tile_of = [&](int j) {
-        if (j == 0) return 0;
-        if (j == 2 * n - 1) return n - 1;
-        return u.alternate && !(j & 1) ? j / 2 - 1 : u.alternate ? (j + 1) / 2 : j / 2;
-      };
-      auto key_of = [&](int j) { return (u.tb + tile_of(j)) * kPagedTile + lane * p.box; };
-      auto page_of = [&](int j) {
-        const int key = key_of(j);
-        if (j >= 2 * n || lane * p.box >= kPagedTile || key >= u.hi || key + p.box <= u.lo) return -1;
-        const int page = table[bt.by_page.of(key)];
-        return page < 0 || page >= bt.pages ? -2 : page;
-      };
-      int ahead = page_of(0);
-      for (int j = 0; j < 2 * n; ++j, ++it) {
-        const bool is_v = j == 2 * n - 1 || (j > 0 && (u.alternate ? !(j & 1) : (j & 1)));
-        const int key = key_of(j), page = ahead;
-        ahead = page_of(j + 1);
-        if (__any_sync(0xffffffffu, page == -2) && lane == 0) units[us].bad = 1;
-        const uint32_t s = it % STAGES;
-        if (!(ok = paged_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, abort_flag, p.err, 42))) break;
-        const uint32_t boxes = (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0));
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], boxes * (uint32_t)p.box * DH * 2);
-        __syncwarp();
-        if (page >= 0) {
-          const CUtensorMap* map = is_v ? &map_v : &map_k;
-          const uint32_t dst = ring + s * L::TILE + (uint32_t)(lane * p.box) * 128u;
-          const int in = key - bt.by_page.of(key) * bt.page_size;
-#pragma unroll
-          for (int h = 0; h < HALVES; ++h)
-            tma_load_4d(dst + h * (kPagedTile * 128), map, h * 64, in, u.kvh, page, &full[s]);
-        }
-        __syncwarp();
-      }
-    }
-    if (lane == 0) p.meta[blockIdx.x] = meta;
-    if (!ok)  // the copies in flight land before the block leaves
-      for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
-        paged_wait(&full[j % STAGES], (j / STAGES) & 1u, abort_flag, p.err, 0x100 | 43);
   } else if (warp == kPagedProducts) {
-    // ---- products ----
-    bool ok = true;
-    uint32_t it = 0, uc = 0, vc = 0;
-    uint32_t p_phase = 0, o_phase = 3u;  // a bit of each half
-    const uint32_t idesc_s = paged_idesc<T>(kPagedTile, false), idesc_o = paged_idesc<T>((a.dim + 15) / 16 * 16, true);
-    const int steps = (a.dim + 15) / 16;
-    if (p.stall_test) ok = paged_wait(drain, 0, abort_flag, p.err, 44);
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) umma_commit(bar);
-      __syncwarp();
-    };
-    while (ok) {
-      const uint32_t us = uc % UNITS;
-      if (!(ok = paged_wait(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 46))) break;
-      const PagedUnit& u = units[us];
-      if (u.done) break;
-      const int n = u.te - u.tb, alternate = u.alternate, tb = u.tb, count0 = u.count0, count1 = u.count1;
-      if (!(ok = paged_wait(q_full, uc & 1u, abort_flag, p.err, 47))) break;
-      tc_fence_after();
-      if (n == 0) commit(q_empty);
-      // Step q is P V of half w = q & 1 with its tile i, then its next S; the first
-      // two are the halves' first S.  Tiles of the unit: i, or 2 i + w.
-      int k_seen = 0, v_seen_to = 0;  // tiles of K and V that were waited for
+    // ---- products, by one thread ----
+    if (elect_one()) {
+      bool ok = true;
+      uint32_t it = 0, uc = 0, vc = 0;
+      uint32_t p_phase = 0, o_phase = 3u;  // a bit of each half
+      const uint32_t idesc_s = paged_idesc<T>(kPagedTile, false), idesc_o = paged_idesc<T>((a.dim + 15) / 16 * 16, true);
+      const int steps = (a.dim + 15) / 16;
+      const uint32_t q_desc = paged_desc(q_smem, 16), k_desc = paged_desc(ring, 16), v_desc = paged_desc(ring, kPagedTile * 128);
+      if (p.stall_test) ok = paged_wait_one(drain, 0, abort_flag, p.err, 44);
+      while (ok) {
+        const uint32_t us = uc % UNITS;
+        if (!(ok = paged_wait_one(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 46))) break;
+        const PagedUnit& u = units[us];
+        if (u.done) break;
+        const int n = u.te - u.tb, alternate = u.alternate, count0 = u.count0, count1 = u.count1;
+        // tiles from here on are seen in part, and those before that
+        const int masked_from = (u.first + 1) / kPagedTile - u.tb;
+        const int masked_to = a.window ? (int)min((int64_t)n, ((int64_t)u.last - a.window + kPagedTile) / kPagedTile - u.tb) : 0;
+        if (!(ok = paged_wait_one(q_full, uc & 1u, abort_flag, p.err, 47))) break;
+        if (n == 0) umma_commit(q_empty);
+        // Step q is P V of half w = q & 1 with its tile i, then its next S; the first
+        // two are the halves' first S.  Tiles of the unit: i, or 2 i + w.
+        int k_seen = 0, v_seen_to = 0;  // tiles of K and V that were waited for
 #pragma unroll 1
-      for (int q = -2; q < (alternate ? n : 2 * n); ++q) {
-        const int w = q & 1, i = q >> 1, count = w ? count1 : count0;
-        const int t = alternate ? q : i, ahead = t + (alternate ? 2 : 1);  // tile of P V, of the next S
-        const bool last_of_tile = alternate || w == 1;
-        if (q >= 0) {
-          const uint32_t v = it + (alternate ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1);
-          if (t >= v_seen_to) {
-            v_seen_to = t + 1;
-            if (!(ok = paged_wait(&full[v % STAGES], (v / STAGES) & 1u, abort_flag, p.err, 45))) break;
-            if (paged_masked(u, tb + t, a.window)) {
-              if (lane == 0) mbar_arrive(v_seen);
-              __syncwarp();
-              if (!(ok = paged_wait(v_clean, vc & 1u, abort_flag, p.err, 48))) break;
-              ++vc;
+        for (int q = -2; q < (alternate ? n : 2 * n) && ok; ++q) {
+          const int w = q & 1, i = q >> 1, count = w ? count1 : count0;
+          const int t = alternate ? q : i, ahead = t + (alternate ? 2 : 1);  // tile of P V, of the next S
+          const bool last_of_tile = alternate || w == 1;
+          if (q >= 0) {
+            const uint32_t v = it + (alternate ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1), s = v % STAGES;
+            if (t >= v_seen_to) {
+              v_seen_to = t + 1;
+              if (!(ok = paged_wait_one(&full[s], (v / STAGES) & 1u, abort_flag, p.err, 45))) break;
+              if (t >= masked_from || t < masked_to) {
+                mbar_arrive(v_seen);
+                if (!(ok = paged_wait_one(v_clean, vc & 1u, abort_flag, p.err, 48))) break;
+                ++vc;
+              }
             }
-          }
-          if (i < count) {
-            if (i == 0) {
-              if (!(ok = paged_wait(&o_free[w], (o_phase >> w) & 1u, abort_flag, p.err, 49))) break;
-              o_phase ^= 1u << w;
-            }
-            if (!(ok = paged_wait(&p_full[w], (p_phase >> w) & 1u, abort_flag, p.err, 50))) break;
-            p_phase ^= 1u << w;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint32_t vs = ring + (v % STAGES) * L::TILE, d = tmem + w * 128;
+            if (i < count) {
+              if (i == 0) {
+                if (!(ok = paged_wait_one(&o_free[w], (o_phase >> w) & 1u, abort_flag, p.err, 49))) break;
+                o_phase ^= 1u << w;
+              }
+              const uint32_t vs = v_desc + s * (L::TILE / 16), d = tmem + w * 128;
+              if (!(ok = paged_wait_one(&p_full[w], (p_phase >> w) & 1u, abort_flag, p.err, 50))) break;
+              p_phase ^= 1u << w;
+              tc_fence_after();
 #pragma unroll
               for (int k = 0; k < kPagedTile / 16; ++k)
-                umma_f16_tmem_a(d + 256, d + (k >> 2) * 64 + (k & 3) * 8, paged_desc(vs + k * 2048, kPagedTile * 128), idesc_o,
-                                i > 0 || k > 0 ? 1u : 0u);
+                umma_f16_tmem_a(d + 256, d + (k >> 2) * 64 + (k & 3) * 8, vs + k * (2048 / 16), idesc_o, i > 0 || k > 0 ? 1u : 0u);
               umma_commit(&pv_done[w]);
             }
-            __syncwarp();
+            if (last_of_tile) umma_commit(&empty[s]);
           }
-          if (last_of_tile) commit(&empty[v % STAGES]);
-        }
-        if (ahead >= n) continue;
-        const uint32_t k = it + (alternate ? (ahead == 0 ? 0 : 2 * ahead - 1) : 2 * ahead);
-        if (ahead >= k_seen) {
-          k_seen = ahead + 1;
-          if (!(ok = paged_wait(&full[k % STAGES], (k / STAGES) & 1u, abort_flag, p.err, 45))) break;
-          tc_fence_after();
-        }
-        if (i + 1 < count) {
-          if (elect_one()) {
-            const uint32_t qs = q_smem + (alternate ? 0 : w * L::TILE), ks = ring + (k % STAGES) * L::TILE;
-#pragma unroll 1
-            for (int c = 0; c < steps; ++c) {
-              const uint32_t off = (c >> 2) * (kPagedTile * 128) + (c & 3) * 32;
-              umma_f16(tmem + w * 128, paged_desc(qs + off, 16), paged_desc(ks + off, 16), idesc_s, c > 0 ? 1u : 0u);
-            }
+          if (ahead >= n) continue;
+          const uint32_t k = it + (alternate ? (ahead == 0 ? 0 : 2 * ahead - 1) : 2 * ahead), s = k % STAGES;
+          if (ahead >= k_seen) {
+            k_seen = ahead + 1;
+            if (!(ok = paged_wait_one(&full[s], (k / STAGES) & 1u, abort_flag, p.err, 45))) break;
+          }
+          if (i + 1 < count) {
+            const uint32_t qs = q_desc + (alternate ? 0 : w * (L::TILE / 16)), ks = k_desc + s * (L::TILE / 16);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c)
+              if (c < steps)
+                umma_f16(tmem + w * 128, qs + ((c >> 2) * (kPagedTile * 128) + (c & 3) * 32) / 16,
+                         ks + ((c >> 2) * (kPagedTile * 128) + (c & 3) * 32) / 16, idesc_s, c > 0 ? 1u : 0u);
             umma_commit(&s_full[w]);
           }
-          __syncwarp();
+          if (last_of_tile) {
+            umma_commit(&empty[s]);
+            if (ahead == n - 1) umma_commit(q_empty);
+          }
         }
-        if (last_of_tile) {
-          commit(&empty[k % STAGES]);
-          if (ahead == n - 1) commit(q_empty);
-        }
+        if (!ok) break;
+        it += 2 * n;
+        mbar_arrive(&u_empty[us]);
+        ++uc;
       }
-      if (!ok) break;
-      it += 2 * n;
-      if (lane == 0) mbar_arrive(&u_empty[us]);
-      __syncwarp();
-      ++uc;
+      if (!ok) {
+        umma_commit(drain);
+        paged_wait_one(drain, 0, abort_flag, p.err, 0x100 | 52);
+      }
     }
-    if (!ok) {
-      commit(drain);
-      paged_wait(drain, 0, abort_flag, p.err, 0x100 | 52);
-    }
+    __syncwarp();
   } else if (warp >= kPagedQueries) {
     // ---- Q, and values of tiles that are seen in part ----
     const int me = warp - kPagedQueries;
     bool ok = true;
-    uint32_t it = 0, uc = 0, vc = 0;
+    uint32_t it = 0, uc = 0, vc = 0, sent = 0;  // sent: Q on its way by TMA, of so many units
     while (ok) {
       const uint32_t us = uc % UNITS;
       if (!(ok = paged_wait(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 53))) break;
@@ -650,6 +488,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       if (u.done) break;
       if (!(ok = paged_wait(q_empty, (uc & 1u) ^ 1u, abort_flag, p.err, 54))) break;
       if (p.q_tma) {  // G heads by 128 / G tokens: rows behind the unit's are other tokens', of which nothing is used
+        sent = uc + 1;
         if (elect_one()) {
           const int tiles = u.rows > kPagedTile ? 2 : 1;
           if (me == 0) {
@@ -740,6 +579,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       __syncwarp();
       ++uc;
     }
+    if (!ok && sent > 0 && me == 0) paged_wait(q_full, (sent - 1) & 1u, abort_flag, p.err, 0x100 | 54);  // it lands before the block leaves
   } else {
     // ---- softmax ----
     const int w = warp >> 3, side = (warp >> 2) & 1, quarter = warp & 3;
@@ -915,7 +755,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
 #pragma unroll
               for (int k = 0; k < 32; k += 2) fma2_to(v[k], v[k + 1], __uint_as_float(o[k]), __uint_as_float(o[k + 1]), f);
             }
-            if (false) {
+            if (dirty && real) {
               const uint32_t bits = paged_marks<T>(p, u, position, c);
 #pragma unroll
               for (int k = 0; k < 32; ++k)

@@ -137,6 +137,13 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedTensorParams&
 __device__ __noinline__ bool paged_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
   return mbar_wait_warp(bar, parity, abort_flag, err, code & 0xFF, (code & 0x100) != 0);
 }
+// ... by a thread for itself.
+__device__ __noinline__ bool paged_wait_one_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  return mbar_wait(bar, parity, abort_flag, err, code & 0xFF, (code & 0x100) != 0);
+}
+__device__ __forceinline__ bool paged_wait_one(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  return mbar_try_wait(bar, parity) || paged_wait_one_long(bar, parity, abort_flag, err, code);
+}
 __device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return paged_wait_long(bar, parity, abort_flag, err, code);
@@ -150,7 +157,7 @@ struct PagedSmem {
   static constexpr int Q_OFF = STAGES * TILE;
   static constexpr int ROW_OFF = Q_OFF + 2 * TILE;  // [16 softmax warps][32]: a row's maximum or sum
   static constexpr int UNIT_OFF = ROW_OFF + 16 * 32 * 4;
-  static constexpr int UNITS = 2;
+  static constexpr int UNITS = 4;
   static constexpr int BAR_OFF = (UNIT_OFF + UNITS * (int)sizeof(PagedUnit) + 15) / 16 * 16;
   static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 4 + 5;
   static constexpr int TOTAL = BAR_OFF + 8 * NBAR + 16;
@@ -167,27 +174,26 @@ __device__ __forceinline__ uint32_t paged_idesc(int n, bool b_by_rows) {
 // Operand tiles of 128-byte rows in the 128-byte swizzle, 8-row groups 1024
 // bytes apart: K-major (Q, K: rows are M or N, 64 of the depth side by side) and
 // MN-major (V: rows are the depth, 64 of N side by side, the next 64 a tile of
-// 128 rows further).
-__device__ __forceinline__ uint64_t paged_desc(uint32_t saddr, uint32_t lead) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// 128 rows further).  The descriptor's upper word is the same for all; the lower has
+// the address and `lead`, both in units of 16 bytes.
+constexpr uint32_t kPagedDesc = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t paged_desc(uint32_t saddr, uint32_t lead) { return (saddr >> 4) | ((lead >> 4) << 16); }
 
-__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kPagedDesc)
       : "memory");
 }
 // A in tensor memory: a lane a row, eight columns 16 values of the depth
-__device__ __forceinline__ void umma_f16_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16_tmem_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kPagedDesc)
       : "memory");
 }
 
@@ -366,6 +372,18 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   tc_fence_after();
   grid_dep_wait();
   grid_dep_trigger();
+  // Costs of many sequences: each warp sums a run of them, in chunks of 32.
+  const int chunks = (a.batch.seqs + 31) / 32, run = (chunks + kPagedThreads / 32 - 1) / (kPagedThreads / 32);
+  int* warp_cost = reinterpret_cast<int*>(smem + L::ROW_OFF);
+  if (chunks > 2) {
+    int sum = 0;
+#pragma unroll 1
+    for (int c = warp * run; c < min(chunks, (warp + 1) * run); ++c)
+      sum += c * 32 + lane < a.batch.seqs ? paged_sequence(p, c * 32 + lane).whole : 0;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) warp_cost[warp] = sum;
+    __syncthreads();
+  }
   const uint32_t tmem = *tmem_slot;
   const uint32_t ring = smem_u32(smem), q_smem = smem_u32(smem + L::Q_OFF);
 
@@ -379,11 +397,28 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     int seq = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 2 && (pass == 0 || begin < end); ++pass) {
-      int sum = 0;
+      int sum = 0, c = 0;
+      if (chunks > 2) {
+        const int mine = lane < kPagedThreads / 32 ? warp_cost[lane] : 0;
+        int upto = mine;
+        for (int d = 1; d < 32; d <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += o;
+        }
+        total = __shfl_sync(0xffffffffu, upto, 31);
+        if (pass) {  // the run that `begin` lies in
+          const int w = __ffs(__ballot_sync(0xffffffffu, upto > begin)) - 1;
+          sum = __shfl_sync(0xffffffffu, upto - mine, max(w, 0));
+          c = max(w, 0) * run;
+        } else {
+          c = chunks;
+          sum = total;
+        }
+      }
 #pragma unroll 1
-      for (int b0 = 0; b0 < bt.seqs; b0 += 32) {
-        const int c = b0 + lane < bt.seqs ? paged_sequence(p, b0 + lane).whole : 0;
-        int upto = c;
+      for (; c < chunks; ++c) {
+        const int mine = c * 32 + lane < bt.seqs ? paged_sequence(p, c * 32 + lane).whole : 0;
+        int upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const int o = __shfl_up_sync(0xffffffffu, upto, d);
@@ -393,8 +428,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           const uint32_t beyond = __ballot_sync(0xffffffffu, sum + upto > begin);
           if (beyond) {
             const int l = __ffs(beyond) - 1;
-            seq = b0 + l;
-            at = sum + __shfl_sync(0xffffffffu, upto - c, l);
+            seq = c * 32 + l;
+            at = sum + __shfl_sync(0xffffffffu, upto - mine, l);
             break;
           }
         }
@@ -549,105 +584,98 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; ++j)
         paged_wait(&full[j % STAGES], (j / STAGES) & 1u, abort_flag, p.err, 0x100 | 43);
   } else if (warp == kPagedProducts) {
-    // ---- products ----
-    bool ok = true;
-    uint32_t it = 0, uc = 0, vc = 0;
-    uint32_t p_phase = 0, o_phase = 3u;  // a bit of each half
-    const uint32_t idesc_s = paged_idesc<T>(kPagedTile, false), idesc_o = paged_idesc<T>((a.dim + 15) / 16 * 16, true);
-    const int steps = (a.dim + 15) / 16;
-    if (p.stall_test) ok = paged_wait(drain, 0, abort_flag, p.err, 44);
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) umma_commit(bar);
-      __syncwarp();
-    };
-    while (ok) {
-      const uint32_t us = uc % UNITS;
-      if (!(ok = paged_wait(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 46))) break;
-      const PagedUnit& u = units[us];
-      if (u.done) break;
-      const int n = u.te - u.tb, alternate = u.alternate, tb = u.tb, count0 = u.count0, count1 = u.count1;
-      if (!(ok = paged_wait(q_full, uc & 1u, abort_flag, p.err, 47))) break;
-      tc_fence_after();
-      if (n == 0) commit(q_empty);
-      // Step q is P V of half w = q & 1 with its tile i, then its next S; the first
-      // two are the halves' first S.  Tiles of the unit: i, or 2 i + w.
-      int k_seen = 0, v_seen_to = 0;  // tiles of K and V that were waited for
+    // ---- products, by one thread ----
+    if (elect_one()) {
+      bool ok = true;
+      uint32_t it = 0, uc = 0, vc = 0;
+      uint32_t p_phase = 0, o_phase = 3u;  // a bit of each half
+      const uint32_t idesc_s = paged_idesc<T>(kPagedTile, false), idesc_o = paged_idesc<T>((a.dim + 15) / 16 * 16, true);
+      const int steps = (a.dim + 15) / 16;
+      const uint32_t q_desc = paged_desc(q_smem, 16), k_desc = paged_desc(ring, 16), v_desc = paged_desc(ring, kPagedTile * 128);
+      if (p.stall_test) ok = paged_wait_one(drain, 0, abort_flag, p.err, 44);
+      while (ok) {
+        const uint32_t us = uc % UNITS;
+        if (!(ok = paged_wait_one(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 46))) break;
+        const PagedUnit& u = units[us];
+        if (u.done) break;
+        const int n = u.te - u.tb, alternate = u.alternate, count0 = u.count0, count1 = u.count1;
+        // tiles from here on are seen in part, and those before that
+        const int masked_from = (u.first + 1) / kPagedTile - u.tb;
+        const int masked_to = a.window ? (int)min((int64_t)n, ((int64_t)u.last - a.window + kPagedTile) / kPagedTile - u.tb) : 0;
+        if (!(ok = paged_wait_one(q_full, uc & 1u, abort_flag, p.err, 47))) break;
+        if (n == 0) umma_commit(q_empty);
+        // Step q is P V of half w = q & 1 with its tile i, then its next S; the first
+        // two are the halves' first S.  Tiles of the unit: i, or 2 i + w.
+        int k_seen = 0, v_seen_to = 0;  // tiles of K and V that were waited for
 #pragma unroll 1
-      for (int q = -2; q < (alternate ? n : 2 * n); ++q) {
-        const int w = q & 1, i = q >> 1, count = w ? count1 : count0;
-        const int t = alternate ? q : i, ahead = t + (alternate ? 2 : 1);  // tile of P V, of the next S
-        const bool last_of_tile = alternate || w == 1;
-        if (q >= 0) {
-          const uint32_t v = it + (alternate ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1);
-          if (t >= v_seen_to) {
-            v_seen_to = t + 1;
-            if (!(ok = paged_wait(&full[v % STAGES], (v / STAGES) & 1u, abort_flag, p.err, 45))) break;
-            if (paged_masked(u, tb + t, a.window)) {
-              if (lane == 0) mbar_arrive(v_seen);
-              __syncwarp();
-              if (!(ok = paged_wait(v_clean, vc & 1u, abort_flag, p.err, 48))) break;
-              ++vc;
+        for (int q = -2; q < (alternate ? n : 2 * n) && ok; ++q) {
+          const int w = q & 1, i = q >> 1, count = w ? count1 : count0;
+          const int t = alternate ? q : i, ahead = t + (alternate ? 2 : 1);  // tile of P V, of the next S
+          const bool last_of_tile = alternate || w == 1;
+          if (q >= 0) {
+            const uint32_t v = it + (alternate ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1), s = v % STAGES;
+            if (t >= v_seen_to) {
+              v_seen_to = t + 1;
+              if (!(ok = paged_wait_one(&full[s], (v / STAGES) & 1u, abort_flag, p.err, 45))) break;
+              if (t >= masked_from || t < masked_to) {
+                mbar_arrive(v_seen);
+                if (!(ok = paged_wait_one(v_clean, vc & 1u, abort_flag, p.err, 48))) break;
+                ++vc;
+              }
             }
-          }
-          if (i < count) {
-            if (i == 0) {
-              if (!(ok = paged_wait(&o_free[w], (o_phase >> w) & 1u, abort_flag, p.err, 49))) break;
-              o_phase ^= 1u << w;
-            }
-            if (!(ok = paged_wait(&p_full[w], (p_phase >> w) & 1u, abort_flag, p.err, 50))) break;
-            p_phase ^= 1u << w;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint32_t vs = ring + (v % STAGES) * L::TILE, d = tmem + w * 128;
+            if (i < count) {
+              if (i == 0) {
+                if (!(ok = paged_wait_one(&o_free[w], (o_phase >> w) & 1u, abort_flag, p.err, 49))) break;
+                o_phase ^= 1u << w;
+              }
+              const uint32_t vs = v_desc + s * (L::TILE / 16), d = tmem + w * 128;
+              if (!(ok = paged_wait_one(&p_full[w], (p_phase >> w) & 1u, abort_flag, p.err, 50))) break;
+              p_phase ^= 1u << w;
+              tc_fence_after();
 #pragma unroll
               for (int k = 0; k < kPagedTile / 16; ++k)
-                umma_f16_tmem_a(d + 256, d + (k >> 2) * 64 + (k & 3) * 8, paged_desc(vs + k * 2048, kPagedTile * 128), idesc_o,
-                                i > 0 || k > 0 ? 1u : 0u);
+                umma_f16_tmem_a(d + 256, d + (k >> 2) * 64 + (k & 3) * 8, vs + k * (2048 / 16), idesc_o, i > 0 || k > 0 ? 1u : 0u);
               umma_commit(&pv_done[w]);
             }
-            __syncwarp();
+            if (last_of_tile) umma_commit(&empty[s]);
           }
-          if (last_of_tile) commit(&empty[v % STAGES]);
-        }
-        if (ahead >= n) continue;
-        const uint32_t k = it + (alternate ? (ahead == 0 ? 0 : 2 * ahead - 1) : 2 * ahead);
-        if (ahead >= k_seen) {
-          k_seen = ahead + 1;
-          if (!(ok = paged_wait(&full[k % STAGES], (k / STAGES) & 1u, abort_flag, p.err, 45))) break;
-          tc_fence_after();
-        }
-        if (i + 1 < count) {
-          if (elect_one()) {
-            const uint32_t qs = q_smem + (alternate ? 0 : w * L::TILE), ks = ring + (k % STAGES) * L::TILE;
-#pragma unroll 1
-            for (int c = 0; c < steps; ++c) {
-              const uint32_t off = (c >> 2) * (kPagedTile * 128) + (c & 3) * 32;
-              umma_f16(tmem + w * 128, paged_desc(qs + off, 16), paged_desc(ks + off, 16), idesc_s, c > 0 ? 1u : 0u);
-            }
+          if (ahead >= n) continue;
+          const uint32_t k = it + (alternate ? (ahead == 0 ? 0 : 2 * ahead - 1) : 2 * ahead), s = k % STAGES;
+          if (ahead >= k_seen) {
+            k_seen = ahead + 1;
+            if (!(ok = paged_wait_one(&full[s], (k / STAGES) & 1u, abort_flag, p.err, 45))) break;
+          }
+          if (i + 1 < count) {
+            const uint32_t qs = q_desc + (alternate ? 0 : w * (L::TILE / 16)), ks = k_desc + s * (L::TILE / 16);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c)
+              if (c < steps)
+                umma_f16(tmem + w * 128, qs + ((c >> 2) * (kPagedTile * 128) + (c & 3) * 32) / 16,
+                         ks + ((c >> 2) * (kPagedTile * 128) + (c & 3) * 32) / 16, idesc_s, c > 0 ? 1u : 0u);
             umma_commit(&s_full[w]);
           }
-          __syncwarp();
+          if (last_of_tile) {
+            umma_commit(&empty[s]);
+            if (ahead == n - 1) umma_commit(q_empty);
+          }
         }
-        if (last_of_tile) {
-          commit(&empty[k % STAGES]);
-          if (ahead == n - 1) commit(q_empty);
-        }
+        if (!ok) break;
+        it += 2 * n;
+        mbar_arrive(&u_empty[us]);
+        ++uc;
       }
-      if (!ok) break;
-      it += 2 * n;
-      if (lane == 0) mbar_arrive(&u_empty[us]);
-      __syncwarp();
-      ++uc;
+      if (!ok) {
+        umma_commit(drain);
+        paged_wait_one(drain, 0, abort_flag, p.err, 0x100 | 52);
+      }
     }
-    if (!ok) {
-      commit(drain);
-      paged_wait(drain, 0, abort_flag, p.err, 0x100 | 52);
-    }
+    __syncwarp();
   } else if (warp >= kPagedQueries) {
     // ---- Q, and values of tiles that are seen in part ----
     const int me = warp - kPagedQueries;
     bool ok = true;
-    uint32_t it = 0, uc = 0, vc = 0;
+    uint32_t it = 0, uc = 0, vc = 0, sent = 0;  // sent: Q on its way by TMA, of so many units
     while (ok) {
       const uint32_t us = uc % UNITS;
       if (!(ok = paged_wait(&u_full[us], (uc / UNITS) & 1u, abort_flag, p.err, 53))) break;
@@ -655,6 +683,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       if (u.done) break;
       if (!(ok = paged_wait(q_empty, (uc & 1u) ^ 1u, abort_flag, p.err, 54))) break;
       if (p.q_tma) {  // G heads by 128 / G tokens: rows behind the unit's are other tokens', of which nothing is used
+        sent = uc + 1;
         if (elect_one()) {
           const int tiles = u.rows > kPagedTile ? 2 : 1;
           if (me == 0) {
@@ -745,6 +774,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       __syncwarp();
       ++uc;
     }
+    if (!ok && sent > 0 && me == 0) paged_wait(q_full, (sent - 1) & 1u, abort_flag, p.err, 0x100 | 54);  // it lands before the block leaves
   } else {
     // ---- softmax ----
     const int w = warp >> 3, side = (warp >> 2) & 1, quarter = warp & 3;
