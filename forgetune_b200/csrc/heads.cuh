@@ -13,10 +13,10 @@
 //
 // Bound by the bytes of x and y.  A lane holds V pairs of a head (two pieces
 // of V elements: either side of the half, or side by side where interleaved),
-// so no value crosses lanes but the sum of squares; LPH lanes share a head.  A
-// block takes HB heads per group of LPH lanes, loads them all, finds its
-// tokens' sequences and makes their cosines meanwhile, once per token for all
-// of its heads.
+// so no value crosses lanes but the sum of squares; up to 32 lanes share a head.
+// A block takes a few tokens: it begins to load their heads, finds their
+// sequences and pages and makes their cosines, once per token for all of its
+// heads, then goes through the heads with the next ones on their way.
 #pragma once
 
 #include <algorithm>
@@ -92,8 +92,9 @@ struct HeadsParams {
   int positions64;
   PagedBatchParams batch;
   int units, lanes;       // units of V pairs in a head, lanes that share them
-  int per_block;          // heads of a token that a block takes
+  FastDiv per_block;      // heads of a token that a block takes
   int tokens_per_block, blocks_per_token;
+  FastDiv by_pairs;
 };
 
 template <typename T, int V>
@@ -117,77 +118,88 @@ __device__ __forceinline__ void unit_at(const HeadsParams& p, int u, int* a, int
   }
 }
 
-template <typename T, typename O, int V, int UPL, int HB>
+template <typename T, typename O, int V, int UPL, int AHEAD>
 __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const HeadsParams p) {
   extern __shared__ float2 turn[];  // [tokens of the block][pairs]
   __shared__ int64_t where[64];     // position of a token
+  __shared__ int64_t slot[2][64];   // where its key and value go
   __shared__ int page_of[64];       // its page; -1: no place in the pool, -2: no sequence
   grid_dep_wait();
   grid_dep_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = (int)(blockIdx.x / p.blocks_per_token) * p.tokens_per_block;
-  const int h0 = (int)(blockIdx.x % p.blocks_per_token) * p.per_block;
+  const int h0 = (int)(blockIdx.x % p.blocks_per_token) * (int)p.per_block.d;
   const int all = p.heads[0] + p.heads[1] + p.heads[2];
   const int group = threadIdx.x / p.lanes, groups = kHeadsThreads / p.lanes, l = threadIdx.x % p.lanes;
+  const int tokens = min(p.tokens_per_block, p.tokens - t0), items = tokens * (int)p.per_block.d;
 
-  Piece<T, V> in[HB][UPL][2];
-  int tok[HB], kind[HB], head[HB];
-#pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    const int flat = i * groups + group;
-    tok[i] = flat / p.per_block;
-    int h = h0 + flat % p.per_block;
-    kind[i] = tok[i] < p.tokens_per_block && t0 + tok[i] < p.tokens && h < all ? 0 : -1;
-    if (kind[i] == 0 && h >= p.heads[0]) {
-      h -= p.heads[0];
-      kind[i] = 1;
-      if (h >= p.heads[1]) {
-        h -= p.heads[1];
-        kind[i] = 2;
+  // Item f is head h0 + f % per_block of token t0 + f / per_block.
+  struct Item {
+    int tok, kind, head;  // kind: q, k, v or -1
+  };
+  auto item = [&](int f) {
+    Item x;
+    x.tok = p.per_block.of(f);
+    x.head = h0 + f - x.tok * (int)p.per_block.d;
+    x.kind = f < items && x.head < all ? 0 : -1;
+    if (x.kind == 0 && x.head >= p.heads[0]) {
+      x.head -= p.heads[0];
+      x.kind = 1;
+      if (x.head >= p.heads[1]) {
+        x.head -= p.heads[1];
+        x.kind = 2;
       }
     }
-    head[i] = h;
-    const int k = max(kind[i], 0);
-    const T* x = static_cast<const T*>(p.x[k]) + (int64_t)(t0 + tok[i]) * p.x_token[k] + h * p.x_head[k];
+    return x;
+  };
+  Piece<T, V> in[AHEAD][UPL][2];
+  auto load = [&](Piece<T, V> (&to)[UPL][2], int f) {
+    const Item x = item(f);
+    const int k = max(x.kind, 0);
+    const T* src = static_cast<const T*>(p.x[k]) + (int64_t)(t0 + x.tok) * p.x_token[k] + x.head * p.x_head[k];
 #pragma unroll
     for (int j = 0; j < UPL; ++j) {
       const int u = l + j * p.lanes;
       int a, b;
       unit_at<V>(p, u, &a, &b);
-      memset(&in[i][j], 0, sizeof(in[i][j]));
-      if (kind[i] >= 0 && u < p.units) {
-        in[i][j][0] = *reinterpret_cast<const Piece<T, V>*>(x + a);
-        if (b < p.dim) in[i][j][1] = *reinterpret_cast<const Piece<T, V>*>(x + b);
+      memset(&to[j], 0, sizeof(to[j]));
+      if (x.kind >= 0 && u < p.units) {
+        to[j][0] = *reinterpret_cast<const Piece<T, V>*>(src + a);
+        if (b < p.dim) to[j][1] = *reinterpret_cast<const Piece<T, V>*>(src + b);
       }
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(in[i], i * groups + group);
 
-  for (int i = warp; i < p.tokens_per_block; i += kHeadsThreads / 32) {
+  for (int i = warp; i < tokens; i += kHeadsThreads / 32) {
     const int t = t0 + i;
-    int64_t position = 0;
+    int64_t position = 0, to = 0;
     int page = -2;
-    if (t < p.tokens) {
-      if (p.positions) {
-        position = p.positions64 ? static_cast<const int64_t*>(p.positions)[t] : static_cast<const int*>(p.positions)[t];
-        page = -1;
-      } else {
-        int seq;
-        if (place_of(p.batch, t, lane, &seq, &position)) {
-          const int n = position >= 0 ? p.batch.by_page.of((int)position) : p.batch.most_pages;
-          page = n < p.batch.most_pages ? p.batch.page_table[seq * p.batch.table_ld + n] : -1;
-          if (page < 0 || page >= p.batch.pages) page = -1;
-        }
+    if (p.positions) {
+      position = p.positions64 ? static_cast<const int64_t*>(p.positions)[t] : static_cast<const int*>(p.positions)[t];
+      page = -1;
+    } else {
+      int seq;
+      if (place_of(p.batch, t, lane, &seq, &position)) {
+        const int n = position >= 0 ? p.batch.by_page.of((int)position) : p.batch.most_pages;
+        page = n < p.batch.most_pages ? p.batch.page_table[seq * p.batch.table_ld + n] : -1;
+        if (page < 0 || page >= p.batch.pages) page = -1;
+        to = position - (int64_t)n * p.batch.page_size;
       }
     }
     if (lane == 0) {
       where[i] = position;
       page_of[i] = page;
+      slot[0][i] = page * p.y_page[1] + to * p.y_token[1];
+      slot[1][i] = page * p.y_page[2] + to * p.y_token[2];
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < p.tokens_per_block * p.pairs; i += kHeadsThreads) {
+  for (int i = threadIdx.x; i < tokens * p.pairs; i += kHeadsThreads) {
+    const int tok = p.by_pairs.of(i);
     // a / 2 pi in turns; what is left of whole turns is at most half a turn
-    double a = (double)where[i / p.pairs] * p.frequencies[i % p.pairs] * 0.15915494309189535;
+    double a = (double)where[tok] * p.frequencies[i - tok * p.pairs] * 0.15915494309189535;
     a -= rint(a);
     float s, c;
     sincospif((float)(2.0 * a), &s, &c);
@@ -195,107 +207,118 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const HeadsParams 
   }
   __syncthreads();
 
+#pragma unroll 1
+  for (int f0 = group; f0 - group < items; f0 += AHEAD * groups) {
 #pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    float v[UPL][2][V];
-    float sum = 0.0f;
+    for (int i = 0; i < AHEAD; ++i) {
+      const int f = f0 + i * groups;
+      if (f - group >= items) break;  // the same for all threads
+      const Item x = item(f);
+      float v[UPL][2][V];
+      float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < UPL; ++j)
+      for (int j = 0; j < UPL; ++j)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          v[j][s][e] = to_f32(in[i][j][s].v[e]);
-          sum = __fmaf_rn(v[j][s][e], v[j][s][e], sum);
-        }
-    if (p.norm) {  // whole warps: lanes of other kinds take part
-      for (int d = p.lanes >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    }
-    const int k = kind[i];
-    if (k < 0) continue;
-    const int page = page_of[tok[i]];
-    if (page == -2 || (k > 0 && page < 0)) continue;
-    const float r = p.norm ? 1.0f / sqrtf(sum / (float)p.dim + p.eps) : 1.0f;
-    const float* w = k < 2 ? p.weight[k] : nullptr;
-    O* y = static_cast<O*>(p.y[k]) + head[i] * p.y_head[k];
-    y += k == 0 ? (int64_t)(t0 + tok[i]) * p.y_token[0]
-                : (int64_t)page * p.y_page[k] + where[tok[i]] % p.batch.page_size * p.y_token[k];
-    const float2* cs = turn + tok[i] * p.pairs;
-#pragma unroll
-    for (int j = 0; j < UPL; ++j) {
-      const int u = l + j * p.lanes;
-      if (u >= p.units) continue;
-      int a, b;
-      unit_at<V>(p, u, &a, &b);
-      if (k < 2 && p.norm) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          v[j][0][e] *= r;
-          v[j][1][e] *= r;
-          if (w) {
-            v[j][0][e] *= w[a + e];
-            if (b + e < p.dim) v[j][1][e] *= w[b + e];
-          }
-        }
-      }
-      if (k < 2 && u < p.pairs / V) {
-        if (p.interleaved && V > 1) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {  // pair e of the unit: elements 2 e and 2 e + 1 of the two pieces
-            float& m = v[j][2 * e / V][2 * e % V];
-            float& n = v[j][2 * e / V][2 * e % V + 1 < V ? 2 * e % V + 1 : 0];
-            const float2 q = cs[u * V + e];
-            const float z = __fmaf_rn(m, q.x, -__fmul_rn(n, q.y));
-            n = __fmaf_rn(n, q.x, __fmul_rn(m, q.y));
-            m = z;
-          }
-        } else {
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float2 q = cs[u * V + e];
-            const float m = v[j][0][e], n = v[j][1][e];
-            v[j][0][e] = __fmaf_rn(m, q.x, -__fmul_rn(n, q.y));
-            v[j][1][e] = __fmaf_rn(n, q.x, __fmul_rn(m, q.y));
+            v[j][s][e] = to_f32(in[i][j][s].v[e]);
+            sum = __fmaf_rn(v[j][s][e], v[j][s][e], sum);
+          }
+      load(in[i], f + AHEAD * groups);
+      if (p.norm) {  // whole warps: lanes of other kinds take part
+        for (int d = p.lanes >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      }
+      const int k = x.kind;
+      if (k < 0) continue;
+      const int page = page_of[x.tok];
+      if (page == -2 || (k > 0 && page < 0)) continue;
+      const float r = p.norm ? 1.0f / sqrtf(sum / (float)p.dim + p.eps) : 1.0f;
+      const float* w = k < 2 ? p.weight[k] : nullptr;
+      O* y = static_cast<O*>(p.y[k]) + x.head * p.y_head[k] + (k == 0 ? (int64_t)(t0 + x.tok) * p.y_token[0] : slot[k - 1][x.tok]);
+      const float2* cs = turn + x.tok * p.pairs;
+#pragma unroll
+      for (int j = 0; j < UPL; ++j) {
+        const int u = l + j * p.lanes;
+        if (u >= p.units) continue;
+        int a, b;
+        unit_at<V>(p, u, &a, &b);
+        if (k < 2 && p.norm) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            v[j][0][e] *= r;
+            v[j][1][e] *= r;
+          }
+          if (w) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              v[j][0][e] *= w[a + e];
+              if (b + e < p.dim) v[j][1][e] *= w[b + e];
+            }
           }
         }
+        if (k < 2 && u < p.pairs / V) {
+          if (p.interleaved && V > 1) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {  // pair e of the unit: elements 2 e and 2 e + 1 of the two pieces
+              float& m = v[j][2 * e / V][2 * e % V];
+              float& n = v[j][2 * e / V][2 * e % V + 1 < V ? 2 * e % V + 1 : 0];
+              const float2 q = cs[u * V + e];
+              const float z = __fmaf_rn(m, q.x, -__fmul_rn(n, q.y));
+              n = __fmaf_rn(n, q.x, __fmul_rn(m, q.y));
+              m = z;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float2 q = cs[u * V + e];
+              const float m = v[j][0][e], n = v[j][1][e];
+              v[j][0][e] = __fmaf_rn(m, q.x, -__fmul_rn(n, q.y));
+              v[j][1][e] = __fmaf_rn(n, q.x, __fmul_rn(m, q.y));
+            }
+          }
+        }
+        Piece<O, V> out[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int e = 0; e < V; ++e) out[s].v[e] = from_f32<O>(v[j][s][e]);
+        *reinterpret_cast<Piece<O, V>*>(y + a) = out[0];
+        if (b < p.dim) *reinterpret_cast<Piece<O, V>*>(y + b) = out[1];
       }
-      Piece<O, V> out[2];
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[s].v[e] = from_f32<O>(v[j][s][e]);
-      *reinterpret_cast<Piece<O, V>*>(y + a) = out[0];
-      if (b < p.dim) *reinterpret_cast<Piece<O, V>*>(y + b) = out[1];
     }
   }
 }
 
-template <typename T, typename O, int V, int UPL, int HB>
-cudaError_t launch_heads_as(HeadsParams p, cudaStream_t s) {
+template <typename T, typename O, int V, int UPL, int AHEAD>
+cudaError_t launch_heads_as(HeadsParams p, int sm_count, cudaStream_t s) {
   p.units = p.pairs / V + (p.dim - 2 * p.pairs + 2 * V - 1) / (2 * V);
   p.lanes = 1;
   while (p.lanes < 32 && p.lanes < p.units) p.lanes *= 2;
-  const int slots = kHeadsThreads / p.lanes * HB, all = p.heads[0] + p.heads[1] + p.heads[2];
-  p.per_block = std::min(all, slots);
-  p.blocks_per_token = (all + slots - 1) / slots;
-  // tokens that share a block, their cosines in at most 16 KB
-  p.tokens_per_block = std::max(1, std::min({slots / p.per_block, 64, p.pairs ? 2048 / p.pairs : 64, p.tokens}));
+  const int groups = kHeadsThreads / p.lanes, all = p.heads[0] + p.heads[1] + p.heads[2];
+  // few heads: a turn of the groups each; else whole tokens, as many as leave eight blocks for each SM, with cosines
+  // in at most 16 KB
+  const bool few = (int64_t)p.tokens * ((all + groups - 1) / groups) <= 4 * sm_count;
+  const int per = few ? std::min(all, groups) : all;
+  p.per_block = FastDiv((uint32_t)per);
+  p.blocks_per_token = (all + per - 1) / per;
+  const int fill = std::max(1, groups / per);  // tokens that a turn of the groups takes
+  const int most = std::min(64, p.pairs ? std::max(1, 2048 / p.pairs) : 64);
+  p.tokens_per_block = std::min(most, few ? fill : std::max(fill, std::min(p.tokens / (8 * sm_count), 8 * fill)));
+  p.by_pairs = FastDiv((uint32_t)std::max(1, p.pairs));
   const int64_t blocks = ((int64_t)p.tokens + p.tokens_per_block - 1) / p.tokens_per_block * p.blocks_per_token;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return pdl_launch(heads_kernel<T, O, V, UPL, HB>, dim3((unsigned)blocks), dim3(kHeadsThreads),
+  return pdl_launch(heads_kernel<T, O, V, UPL, AHEAD>, dim3((unsigned)blocks), dim3(kHeadsThreads),
                     (size_t)p.tokens_per_block * p.pairs * sizeof(float2), s, p);
 }
 
 // `vec`: every base and stride is a multiple of four elements.  Vectors also
-// need dim and r in multiples of eight; four heads per lane group are loaded at
-// once where that leaves blocks for all SMs.
+// need dim and r in multiples of eight.
 template <typename T, typename O>
 cudaError_t launch_heads_types(const HeadsParams& p, bool vec, int sm_count, cudaStream_t s) {
-  if (!vec || p.dim % 8 || p.pairs % 4) return launch_heads_as<T, O, 1, 8, 1>(p, s);
-  if (p.dim > 256) return launch_heads_as<T, O, 4, 2, 1>(p, s);
-  const int64_t all = (int64_t)p.tokens * (p.heads[0] + p.heads[1] + p.heads[2]);
-  if (all * p.dim < (int64_t)sm_count * kHeadsThreads * 8 * 4) return launch_heads_as<T, O, 4, 1, 1>(p, s);
-  return launch_heads_as<T, O, 4, 1, 4>(p, s);
+  if (!vec || p.dim % 8 || p.pairs % 4) return launch_heads_as<T, O, 1, 8, 1>(p, sm_count, s);
+  if (p.dim > 256) return launch_heads_as<T, O, 4, 2, 1>(p, sm_count, s);
+  return launch_heads_as<T, O, 4, 1, 2>(p, sm_count, s);
 }
 
 inline cudaError_t launch_heads(const HeadsParams& p, int in, int out, bool vec, int sm_count, cudaStream_t s) {

@@ -30,8 +30,7 @@
 
 namespace ftb {
 
-constexpr int kLogprobsThreads = 512;
-constexpr int kLogprobsParts = kLogprobsThreads / 2;
+constexpr int kLogprobsThreads = 256;
 constexpr int kLogprobsMaxTop = 64;
 constexpr int kLogprobsCandidates = 1024;
 
@@ -64,12 +63,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 // Running sums of a part of a row; m stays finite from below.
 struct RowSums {
   float m, s, t;
   __device__ __forceinline__ void raise(float top) {
     const float d = m - top;  // <= 0
-    const float f = ex2(d * 1.4426950408889634f);
+    const float f = ex2(d * kLog2e);
     t = __fmaf_rn(s, fmaxf(d, -1e4f), t) * f;
     s *= f;
     m = top;
@@ -120,7 +121,7 @@ __device__ __forceinline__ void unpack(const uint4& u, float* f) {
 struct LogprobsSmem {
   unsigned long long found[kLogprobsCandidates];
   unsigned long long best[kLogprobsMaxTop];  // in order
-  uint32_t part[kLogprobsParts];
+  uint32_t part[kLogprobsThreads];
   RowSums sums[kLogprobsThreads / 32];
   RowSums total;
   int count, best_count;
@@ -198,8 +199,21 @@ __device__ __forceinline__ void rank_found(LogprobsSmem& sm, int k) {
   __syncthreads();
 }
 
+// (s, t) += (a, b) (c, d)
+__device__ __forceinline__ void row_fma2(float& s, float& t, float a, float b, float c, float d) {
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\t"
+      "fma.rn.f32x2 p, q, r, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(s), "+f"(t)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+}
+__device__ __forceinline__ float row_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kLogprobsThreads, 2) logprobs_kernel(const LogprobsParams p, const int split) {
+__global__ void __launch_bounds__(kLogprobsThreads, 4) logprobs_kernel(const LogprobsParams p, const int split) {
   constexpr int W = RowVectors<T>::W, U = 4;
   __shared__ LogprobsSmem sm;
   grid_dep_wait();
@@ -222,23 +236,41 @@ __global__ void __launch_bounds__(kLogprobsThreads, 2) logprobs_kernel(const Log
       memcpy(&u[i], t, 16);
       if (v + i * kLogprobsThreads < v1) u[i] = r.load(v + i * kLogprobsThreads);
     }
-    float f[U][W], high = -INFINITY;
+    float f[U][W], high[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       unpack<T>(u[i], f[i]);
 #pragma unroll
-      for (int k = 0; k < W; ++k) high = fmaxf(high, f[i][k]);
+      for (int k = 0; k < W; k += 4) {
+        high[0] = row_max3(high[0], f[i][k], f[i][k + 1]);
+        high[1] = row_max3(high[1], f[i][k + 2], f[i][k + 3]);
+      }
     }
-    top = fmaxf(top, high);
-    if (high > a.m) a.raise(high);
+    top = row_max3(top, high[0], high[1]);
+    if (top > a.m) a.raise(top);
+    float s[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const float d = f[i][k] - a.m, e = ex2(d * 1.4426950408889634f);
-        a.s += e;
-        a.t = __fmaf_rn(e, fmaxf(d, -1e4f), a.t);  // 0 for -inf
+      for (int k = 0; k < W; k += 2) {
+        add2(f[i][k], f[i][k + 1], -a.m, -a.m);
+        float x = f[i][k], y = f[i][k + 1];
+        mul2(x, y, kLog2e, kLog2e);
+        x = ex2(x);
+        y = ex2(y);
+        add2(s[0], s[1], x, y);
+        row_fma2(t[0], t[1], x, y, f[i][k], f[i][k + 1]);
       }
+    float more = t[0] + t[1];
+    if (more != more) {  // 0 times -inf, unless something was NaN before
+      more = 0.0f;
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int k = 0; k < W; ++k) more = __fmaf_rn(ex2(f[i][k] * kLog2e), fmaxf(f[i][k], -1e4f), more);
+    }
+    a.s += s[0] + s[1];
+    a.t += more;
   }
   const uint32_t mine = v0 + tid < v1 ? order_key(top) : 0u;
 
@@ -248,8 +280,11 @@ __global__ void __launch_bounds__(kLogprobsThreads, 2) logprobs_kernel(const Log
     a.add(b);
   }
   if (lane == 0) sm.sums[warp] = a;
-  const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-  if (!(tid & 1)) sm.part[tid >> 1] = max(mine, other);
+  // parts of four threads for up to 16 alternatives, of one for more
+  const int width = p.top <= 16 ? 4 : 1, parts = kLogprobsThreads / width;
+  uint32_t best = mine;
+  for (int d = 1; d < width; d <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
+  if (tid % width == 0) sm.part[tid / width] = best;
   if (tid == 0) sm.count = 0;
   __syncthreads();
   if (tid == 0) {
@@ -260,10 +295,16 @@ __global__ void __launch_bounds__(kLogprobsThreads, 2) logprobs_kernel(const Log
   const int e0 = max(0, r.first(v0)), e1 = min(p.n, r.first(v1)), k = min(p.top, e1 - e0);
   if (p.top > 0) {
     if (k > 0) {
-      if (tid < kLogprobsParts) {
+      if (tid < parts) {
         const uint32_t key = sm.part[tid];
+        const uint4* all = reinterpret_cast<const uint4*>(sm.part);
         int above = 0;
-        for (int j = 0; j < kLogprobsParts; ++j) above += sm.part[j] > key || (sm.part[j] == key && j < tid);
+#pragma unroll 4
+        for (int j = 0; j < parts / 4; ++j) {
+          const uint4 o = all[j];
+          above += (o.x > key || (o.x == key && 4 * j < tid)) + (o.y > key || (o.y == key && 4 * j + 1 < tid)) +
+                   (o.z > key || (o.z == key && 4 * j + 2 < tid)) + (o.w > key || (o.w == key && 4 * j + 3 < tid));
+        }
         if (above == k - 1) sm.bound = key;
       }
       __syncthreads();
@@ -312,8 +353,8 @@ __global__ void __launch_bounds__(kLogprobsThreads, 2) logprobs_kernel(const Log
       }
       __syncthreads();
       if (p.top > 0) {
-        const int c = tid / kLogprobsMaxTop, i = tid % kLogprobsMaxTop;  // eight lists of 64
-        if (c < split) {
+        const int i = tid % kLogprobsMaxTop;  // eight lists of 64
+        for (int c = tid / kLogprobsMaxTop; c < split; c += kLogprobsThreads / kLogprobsMaxTop) {
           int have;
           asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(have) : "r"(cluster_addr(&sm.best_count, c)) : "memory");
           if (i < have) {
@@ -332,24 +373,25 @@ __global__ void __launch_bounds__(kLogprobsThreads, 2) logprobs_kernel(const Log
     __syncthreads();
   }
   const float m = sm.total.m, logs = logf(sm.total.s);
+  auto logprob = [&](float x) { return (x - m) - logs; };
   if (tid == 0) {
     const int64_t at = row * p.token_stride;
     const int64_t token = p.tokens64 ? static_cast<const int64_t*>(p.tokens)[at] : static_cast<const int*>(p.tokens)[at];
-    p.logprobs[row] = token >= 0 && token < p.n ? (to_f32(r.row[token]) - m) - logs : __uint_as_float(0x7FC00000u);
+    p.logprobs[row] = token >= 0 && token < p.n ? logprob(to_f32(r.row[token])) : __uint_as_float(0x7FC00000u);
     p.entropy[row] = logs - sm.total.t / sm.total.s;
   }
   for (int i = tid; i < p.top; i += kLogprobsThreads) {
     const unsigned long long key = sm.best[i];
-    p.top_values[(int64_t)row * p.top + i] = (key_value((uint32_t)(key >> 32)) - m) - logs;
+    p.top_values[(int64_t)row * p.top + i] = logprob(key_value((uint32_t)(key >> 32)));
     p.top_tokens[(int64_t)row * p.top + i] = (int64_t)(0xFFFFFFFFu - (uint32_t)key);
   }
 }
 
-// Blocks per row: one where the rows fill the GPU (two blocks an SM), else as
-// many of up to eight as still find 8 KB each.
+// Blocks per row: one where the rows fill the GPU, else as many of up to eight
+// as still find 8 KB each.
 inline int logprobs_split(int64_t m, int64_t bytes, int sm_count) {
   int split = 1;
-  while (split < 8 && m * split * 2 <= 2 * sm_count && bytes / (2 * split) >= 8192) split *= 2;
+  while (split < 8 && m * split * 2 <= 8 * sm_count && bytes / (2 * split) >= 8192) split *= 2;
   return split;
 }
 
