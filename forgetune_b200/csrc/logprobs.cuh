@@ -7,11 +7,11 @@
 // t = sum exp(x - m) (x - m); when m grows by d, s and t become s e^-d and
 // (t - s d) e^-d.  Then L = m + log s and H = log s - t / s.
 //
-// The alternatives come from the same pass.  The maxima of 256 disjoint parts
-// of the row are values of the row, so the k-th largest of them is at most the
+// The alternatives come from the same pass.  The maxima of 64 disjoint parts
+// of the row are values of it, so the k-th largest of them is at most the
 // k-th largest value: only threads whose own maximum reaches it can hold one
-// of the top k, and only their vectors are read again (from L2), by whole
-// warps.  What reaches the bound is ordered by value and, where equal, by
+// of the top k, and only their vectors are read again (from L2), by all
+// threads at once.  What reaches the bound is ordered by value and, where equal, by
 // index, as one 64-bit number, and ranked by counting.  Where too many values
 // reach it (many equal ones), a bisection over the values finds the k-th.
 //
@@ -31,6 +31,7 @@
 namespace ftb {
 
 constexpr int kLogprobsThreads = 256;
+constexpr int kLogprobsParts = 64;  // at least the largest number of alternatives
 constexpr int kLogprobsMaxTop = 64;
 constexpr int kLogprobsCandidates = 1024;
 
@@ -121,10 +122,11 @@ __device__ __forceinline__ void unpack(const uint4& u, float* f) {
 struct LogprobsSmem {
   unsigned long long found[kLogprobsCandidates];
   unsigned long long best[kLogprobsMaxTop];  // in order
-  uint32_t part[kLogprobsThreads];
+  alignas(16) uint32_t part[kLogprobsParts];
   RowSums sums[kLogprobsThreads / 32];
   RowSums total;
-  int count, best_count;
+  int count, best_count, reach_count;
+  uint16_t reach[kLogprobsThreads];  // threads whose maximum reaches the bound
   uint32_t bound;
 };
 
@@ -213,7 +215,7 @@ __device__ __forceinline__ float row_max3(float a, float b, float c) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogprobsThreads, 4) logprobs_kernel(const LogprobsParams p, const int split) {
+__global__ void __launch_bounds__(kLogprobsThreads, 3) logprobs_kernel(const LogprobsParams p, const int split) {
   constexpr int W = RowVectors<T>::W, U = 4;
   __shared__ LogprobsSmem sm;
   grid_dep_wait();
@@ -225,17 +227,22 @@ __global__ void __launch_bounds__(kLogprobsThreads, 4) logprobs_kernel(const Log
 
   RowSums a{-FLT_MAX, 0.0f, 0.0f};
   float top = -INFINITY;
-  for (int v = v0 + tid; v < v1; v += U * kLogprobsThreads) {
-    uint4 u[U];
+  uint4 u[U], next[U];
+  auto load = [&](uint4 (&to)[U], int v) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const float none = -INFINITY;
       T t[W];
 #pragma unroll
-      for (int k = 0; k < W; ++k) t[k] = from_f32<T>(none);
-      memcpy(&u[i], t, 16);
-      if (v + i * kLogprobsThreads < v1) u[i] = r.load(v + i * kLogprobsThreads);
+      for (int k = 0; k < W; ++k) t[k] = from_f32<T>(-INFINITY);
+      memcpy(&to[i], t, 16);
+      if (v + i * kLogprobsThreads < v1) to[i] = r.load(v + i * kLogprobsThreads);
     }
+  };
+  load(next, v0 + tid);
+  for (int v = v0 + tid; v < v1; v += U * kLogprobsThreads) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) u[i] = next[i];
+    load(next, v + U * kLogprobsThreads);  // on their way meanwhile
     float f[U][W], high[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -280,12 +287,11 @@ __global__ void __launch_bounds__(kLogprobsThreads, 4) logprobs_kernel(const Log
     a.add(b);
   }
   if (lane == 0) sm.sums[warp] = a;
-  // parts of four threads for up to 16 alternatives, of one for more
-  const int width = p.top <= 16 ? 4 : 1, parts = kLogprobsThreads / width;
+  constexpr int WIDTH = kLogprobsThreads / kLogprobsParts;
   uint32_t best = mine;
-  for (int d = 1; d < width; d <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
-  if (tid % width == 0) sm.part[tid / width] = best;
-  if (tid == 0) sm.count = 0;
+  for (int d = 1; d < WIDTH; d <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
+  if (tid % WIDTH == 0) sm.part[tid / WIDTH] = best;
+  if (tid == 0) sm.count = sm.reach_count = 0;
   __syncthreads();
   if (tid == 0) {
     RowSums all = sm.sums[0];
@@ -295,12 +301,12 @@ __global__ void __launch_bounds__(kLogprobsThreads, 4) logprobs_kernel(const Log
   const int e0 = max(0, r.first(v0)), e1 = min(p.n, r.first(v1)), k = min(p.top, e1 - e0);
   if (p.top > 0) {
     if (k > 0) {
-      if (tid < parts) {
+      if (tid < kLogprobsParts) {
         const uint32_t key = sm.part[tid];
         const uint4* all = reinterpret_cast<const uint4*>(sm.part);
         int above = 0;
 #pragma unroll 4
-        for (int j = 0; j < parts / 4; ++j) {
+        for (int j = 0; j < kLogprobsParts / 4; ++j) {
           const uint4 o = all[j];
           above += (o.x > key || (o.x == key && 4 * j < tid)) + (o.y > key || (o.y == key && 4 * j + 1 < tid)) +
                    (o.z > key || (o.z == key && 4 * j + 2 < tid)) + (o.w > key || (o.w == key && 4 * j + 3 < tid));
@@ -309,22 +315,24 @@ __global__ void __launch_bounds__(kLogprobsThreads, 4) logprobs_kernel(const Log
       }
       __syncthreads();
       const uint32_t bound = sm.bound;
-      uint32_t todo = __ballot_sync(0xffffffffu, v0 + tid < v1 && mine >= bound);
-      while (todo) {
-        const int t = (warp << 5) + __ffs(todo) - 1;
-        todo &= todo - 1;
-        for (int v = v0 + t + lane * kLogprobsThreads; v < v1; v += 32 * kLogprobsThreads) {
-          float f[W];
-          unpack<T>(r.load(v), f);
+      // the vectors of all threads that reach the bound, spread over the block
+      if (v0 + tid < v1 && mine >= bound) sm.reach[atomicAdd(&sm.reach_count, 1)] = (uint16_t)tid;
+      __syncthreads();
+      const int each = (v1 - v0 + kLogprobsThreads - 1) / kLogprobsThreads, work = sm.reach_count * each;
+#pragma unroll 2
+      for (int w = tid; w < work; w += kLogprobsThreads) {
+        const int q = w / each, v = v0 + sm.reach[q] + (w - q * each) * kLogprobsThreads;
+        if (v >= v1) continue;
+        float f[W];
+        unpack<T>(r.load(v), f);
 #pragma unroll
-          for (int i = 0; i < W; ++i) {
-            const int e = r.first(v) + i;
-            const uint32_t key = order_key(f[i]);
-            if (key >= bound && e >= 0 && e < p.n) {
-              const int at = atomicAdd(&sm.count, 1);
-              if (at < kLogprobsCandidates)
-                sm.found[at] = (unsigned long long)key << 32 | (0xFFFFFFFFu - (uint32_t)e);
-            }
+        for (int i = 0; i < W; ++i) {
+          const int e = r.first(v) + i;
+          const uint32_t key = order_key(f[i]);
+          if (key >= bound && e >= 0 && e < p.n) {
+            const int at = atomicAdd(&sm.count, 1);
+            if (at < kLogprobsCandidates)
+              sm.found[at] = (unsigned long long)key << 32 | (0xFFFFFFFFu - (uint32_t)e);
           }
         }
       }
@@ -387,11 +395,11 @@ __global__ void __launch_bounds__(kLogprobsThreads, 4) logprobs_kernel(const Log
   }
 }
 
-// Blocks per row: one where the rows fill the GPU, else as many of up to eight
-// as still find 8 KB each.
+// Blocks per row: one where the rows fill the GPU (three blocks an SM), else as
+// many of up to eight as still find 8 KB each.
 inline int logprobs_split(int64_t m, int64_t bytes, int sm_count) {
   int split = 1;
-  while (split < 8 && m * split * 2 <= 8 * sm_count && bytes / (2 * split) >= 8192) split *= 2;
+  while (split < 8 && m * split * 2 <= 3 * sm_count && bytes / (2 * split) >= 8192) split *= 2;
   return split;
 }
 
