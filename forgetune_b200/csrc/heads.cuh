@@ -92,7 +92,7 @@ struct HeadsParams {
   int positions64;
   PagedBatchParams batch;
   int units, lanes;       // units of V pairs in a head, lanes that share them
-  FastDiv per_block;      // heads of a token that a block takes
+  int per_block;          // heads of a token that a block takes
   int tokens_per_block, blocks_per_token;
   FastDiv by_pairs;
 };
@@ -118,59 +118,81 @@ __device__ __forceinline__ void unit_at(const HeadsParams& p, int u, int* a, int
   }
 }
 
+// V cosines and sines, which for V = 4 lie on a 16-byte boundary (pairs are a multiple of four).
+template <int V>
+__device__ __forceinline__ void load_turns(const float2* from, float2 (&to)[V]) {
+  if constexpr (V == 4) {
+    const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
+    to[0] = make_float2(a.x, a.y), to[1] = make_float2(a.z, a.w), to[2] = make_float2(b.x, b.y), to[3] = make_float2(b.z, b.w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) to[e] = from[e];
+  }
+}
+
 template <typename T, typename O, int V, int UPL, int AHEAD>
-__global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const HeadsParams p) {
-  extern __shared__ float2 turn[];  // [tokens of the block][pairs]
-  __shared__ int64_t where[64];     // position of a token
-  __shared__ int64_t slot[2][64];   // where its key and value go
-  __shared__ int page_of[64];       // its page; -1: no place in the pool, -2: no sequence
+__global__ void __launch_bounds__(kHeadsThreads, UPL == 1 ? 4 : 1) heads_kernel(const HeadsParams p) {
+  extern __shared__ float4 turn4[];  // [tokens of the block][pairs] cosine and sine
+  float2* turn = reinterpret_cast<float2*>(turn4);
+  __shared__ int64_t where[64];      // position of a token
+  __shared__ int64_t slot[2][64];    // where its key and value go
+  __shared__ int page_of[64];        // its page; -1: no place in the pool, -2: no sequence
   grid_dep_wait();
   grid_dep_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = (int)(blockIdx.x / p.blocks_per_token) * p.tokens_per_block;
-  const int h0 = (int)(blockIdx.x % p.blocks_per_token) * (int)p.per_block.d;
+  const int h0 = (int)(blockIdx.x % p.blocks_per_token) * p.per_block;
   const int all = p.heads[0] + p.heads[1] + p.heads[2];
   const int group = threadIdx.x / p.lanes, groups = kHeadsThreads / p.lanes, l = threadIdx.x % p.lanes;
-  const int tokens = min(p.tokens_per_block, p.tokens - t0), items = tokens * (int)p.per_block.d;
+  const int tokens = min(p.tokens_per_block, p.tokens - t0);
+  // A group of lanes takes one head of every token, or of every side-th, and then its next head.
+  const int wide = min(p.per_block, groups), side = groups / wide, first = group / wide;
+  const int turns = (p.per_block + wide - 1) / wide, steps = (tokens + side - 1) / side;
 
-  // Item f is head h0 + f % per_block of token t0 + f / per_block.
-  struct Item {
-    int tok, kind, head;  // kind: q, k, v or -1
-  };
-  auto item = [&](int f) {
-    Item x;
-    x.tok = p.per_block.of(f);
-    x.head = h0 + f - x.tok * (int)p.per_block.d;
-    x.kind = f < items && x.head < all ? 0 : -1;
-    if (x.kind == 0 && x.head >= p.heads[0]) {
-      x.head -= p.heads[0];
-      x.kind = 1;
-      if (x.head >= p.heads[1]) {
-        x.head -= p.heads[1];
-        x.kind = 2;
+  // this lane's two pieces of each unit, in elements of the head; -1: none
+  int at[UPL][2];
+#pragma unroll
+  for (int j = 0; j < UPL; ++j) {
+    unit_at<V>(p, l + j * p.lanes, &at[j][0], &at[j][1]);
+    if (l + j * p.lanes >= p.units) at[j][0] = at[j][1] = -1;
+    else if (at[j][1] >= p.dim) at[j][1] = -1;
+  }
+  int kind = -1, head = 0, coming = 0;  // q, k, v or -1; the token of the next load
+  const T* src = nullptr;
+  int64_t stride = 0;
+  auto begin = [&](int n) {  // its n-th head
+    head = n * wide + group % wide;
+    kind = first < side && head < p.per_block && h0 + head < all ? 0 : -1;
+    head += h0;
+    if (kind == 0 && head >= p.heads[0]) {
+      head -= p.heads[0];
+      kind = 1;
+      if (head >= p.heads[1]) {
+        head -= p.heads[1];
+        kind = 2;
       }
     }
-    return x;
+    const int k = max(kind, 0);
+    src = static_cast<const T*>(p.x[k]) + (int64_t)(t0 + first) * p.x_token[k] + head * p.x_head[k];
+    stride = side * p.x_token[k];
+    coming = kind < 0 ? tokens : first;
+  };
+  auto load = [&](Piece<T, V> (&to)[UPL][2]) {  // of its next token; pieces that are not there stay zero
+    if (coming < tokens) {
+#pragma unroll
+      for (int j = 0; j < UPL; ++j)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          if (at[j][s] >= 0) to[j][s] = *reinterpret_cast<const Piece<T, V>*>(src + at[j][s]);
+    }
+    src += stride;
+    coming += side;
   };
   Piece<T, V> in[AHEAD][UPL][2];
-  auto load = [&](Piece<T, V> (&to)[UPL][2], int f) {
-    const Item x = item(f);
-    const int k = max(x.kind, 0);
-    const T* src = static_cast<const T*>(p.x[k]) + (int64_t)(t0 + x.tok) * p.x_token[k] + x.head * p.x_head[k];
+  memset(in, 0, sizeof(in));
+  begin(0);
 #pragma unroll
-    for (int j = 0; j < UPL; ++j) {
-      const int u = l + j * p.lanes;
-      int a, b;
-      unit_at<V>(p, u, &a, &b);
-      memset(&to[j], 0, sizeof(to[j]));
-      if (x.kind >= 0 && u < p.units) {
-        to[j][0] = *reinterpret_cast<const Piece<T, V>*>(src + a);
-        if (b < p.dim) to[j][1] = *reinterpret_cast<const Piece<T, V>*>(src + b);
-      }
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) load(in[i], i * groups + group);
+  for (int i = 0; i < AHEAD; ++i) load(in[i]);
 
   for (int i = warp; i < tokens; i += kHeadsThreads / 32) {
     const int t = t0 + i;
@@ -208,84 +230,89 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const HeadsParams 
   __syncthreads();
 
 #pragma unroll 1
-  for (int f0 = group; f0 - group < items; f0 += AHEAD * groups) {
+  for (int n = 0; n < turns; ++n) {
+    const bool turned = kind == 0 || kind == 1;
+    float w[UPL][2][V];  // the head's weights
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int f = f0 + i * groups;
-      if (f - group >= items) break;  // the same for all threads
-      const Item x = item(f);
+    for (int j = 0; j < UPL; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[j][s][e] = turned && p.weight[kind] && at[j][s] >= 0 ? p.weight[kind][at[j][s] + e] : 1.0f;
+    const int k = max(kind, 0);
+    O* y = static_cast<O*>(p.y[k]) + head * p.y_head[k];
+    if (kind == 0) y += (int64_t)(t0 + first) * p.y_token[0];
+    int tok = first;
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step, tok += side) {
       float v[UPL][2][V];
-      float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < UPL; ++j)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            v[j][s][e] = to_f32(in[i][j][s].v[e]);
-            sum = __fmaf_rn(v[j][s][e], v[j][s][e], sum);
-          }
-      load(in[i], f + AHEAD * groups);
+          for (int e = 0; e < V; ++e) v[j][s][e] = to_f32(in[0][j][s].v[e]);
+#pragma unroll
+      for (int i = 0; i + 1 < AHEAD; ++i) memcpy(&in[i], &in[i + 1], sizeof(in[0]));
+      load(in[AHEAD - 1]);
       if (p.norm) {  // whole warps: lanes of other kinds take part
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < UPL; ++j)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum = __fmaf_rn(v[j][s][e], v[j][s][e], sum);
         for (int d = p.lanes >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float r = turned ? rsqrtf(__fmaf_rn(sum, 1.0f / (float)p.dim, p.eps)) : 1.0f;
+#pragma unroll
+        for (int j = 0; j < UPL; ++j)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[j][s][e] = v[j][s][e] * r * w[j][s][e];
       }
-      const int k = x.kind;
-      if (k < 0) continue;
-      const int page = page_of[x.tok];
-      if (page == -2 || (k > 0 && page < 0)) continue;
-      const float r = p.norm ? 1.0f / sqrtf(sum / (float)p.dim + p.eps) : 1.0f;
-      const float* w = k < 2 ? p.weight[k] : nullptr;
-      O* y = static_cast<O*>(p.y[k]) + x.head * p.y_head[k] + (k == 0 ? (int64_t)(t0 + x.tok) * p.y_token[0] : slot[k - 1][x.tok]);
-      const float2* cs = turn + x.tok * p.pairs;
+      if (kind < 0 || tok >= tokens) continue;
+      const int page = page_of[tok];
+      if (page == -2 || (kind > 0 && page < 0)) continue;
+      O* to = kind == 0 ? y + (int64_t)(step * side) * p.y_token[0] : y + slot[kind - 1][tok];
 #pragma unroll
       for (int j = 0; j < UPL; ++j) {
         const int u = l + j * p.lanes;
-        if (u >= p.units) continue;
-        int a, b;
-        unit_at<V>(p, u, &a, &b);
-        if (k < 2 && p.norm) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            v[j][0][e] *= r;
-            v[j][1][e] *= r;
-          }
-          if (w) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              v[j][0][e] *= w[a + e];
-              if (b + e < p.dim) v[j][1][e] *= w[b + e];
-            }
-          }
-        }
-        if (k < 2 && u < p.pairs / V) {
+        if (turned && u < p.pairs / V) {
+          float2 q[V];
+          load_turns<V>(turn + tok * p.pairs + u * V, q);
           if (p.interleaved && V > 1) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {  // pair e of the unit: elements 2 e and 2 e + 1 of the two pieces
               float& m = v[j][2 * e / V][2 * e % V];
-              float& n = v[j][2 * e / V][2 * e % V + 1 < V ? 2 * e % V + 1 : 0];
-              const float2 q = cs[u * V + e];
-              const float z = __fmaf_rn(m, q.x, -__fmul_rn(n, q.y));
-              n = __fmaf_rn(n, q.x, __fmul_rn(m, q.y));
-              m = z;
+              float& z = v[j][2 * e / V][2 * e % V + 1 < V ? 2 * e % V + 1 : 0];
+              const float x = __fmaf_rn(m, q[e].x, -__fmul_rn(z, q[e].y));
+              z = __fmaf_rn(z, q[e].x, __fmul_rn(m, q[e].y));
+              m = x;
             }
           } else {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              const float2 q = cs[u * V + e];
-              const float m = v[j][0][e], n = v[j][1][e];
-              v[j][0][e] = __fmaf_rn(m, q.x, -__fmul_rn(n, q.y));
-              v[j][1][e] = __fmaf_rn(n, q.x, __fmul_rn(m, q.y));
+              const float m = v[j][0][e], z = v[j][1][e];
+              v[j][0][e] = __fmaf_rn(m, q[e].x, -__fmul_rn(z, q[e].y));
+              v[j][1][e] = __fmaf_rn(z, q[e].x, __fmul_rn(m, q[e].y));
             }
           }
         }
-        Piece<O, V> out[2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s) {
+          Piece<O, V> out;
 #pragma unroll
-          for (int e = 0; e < V; ++e) out[s].v[e] = from_f32<O>(v[j][s][e]);
-        *reinterpret_cast<Piece<O, V>*>(y + a) = out[0];
-        if (b < p.dim) *reinterpret_cast<Piece<O, V>*>(y + b) = out[1];
+          for (int e = 0; e < V; ++e) out.v[e] = from_f32<O>(v[j][s][e]);
+          if (at[j][s] >= 0) *reinterpret_cast<Piece<O, V>*>(to + at[j][s]) = out;
+        }
       }
+    }
+    if (n + 1 < turns) {
+      begin(n + 1);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) load(in[i]);
     }
   }
 }
@@ -299,17 +326,16 @@ cudaError_t launch_heads_as(HeadsParams p, int sm_count, cudaStream_t s) {
   // few heads: a turn of the groups each; else whole tokens, as many as leave eight blocks for each SM, with cosines
   // in at most 16 KB
   const bool few = (int64_t)p.tokens * ((all + groups - 1) / groups) <= 4 * sm_count;
-  const int per = few ? std::min(all, groups) : all;
-  p.per_block = FastDiv((uint32_t)per);
-  p.blocks_per_token = (all + per - 1) / per;
-  const int fill = std::max(1, groups / per);  // tokens that a turn of the groups takes
+  p.per_block = few ? std::min(all, groups) : all;
+  p.blocks_per_token = (all + p.per_block - 1) / p.per_block;
+  const int fill = std::max(1, groups / p.per_block);  // tokens that a turn of the groups takes
   const int most = std::min(64, p.pairs ? std::max(1, 2048 / p.pairs) : 64);
   p.tokens_per_block = std::min(most, few ? fill : std::max(fill, std::min(p.tokens / (8 * sm_count), 8 * fill)));
   p.by_pairs = FastDiv((uint32_t)std::max(1, p.pairs));
   const int64_t blocks = ((int64_t)p.tokens + p.tokens_per_block - 1) / p.tokens_per_block * p.blocks_per_token;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   return pdl_launch(heads_kernel<T, O, V, UPL, AHEAD>, dim3((unsigned)blocks), dim3(kHeadsThreads),
-                    (size_t)p.tokens_per_block * p.pairs * sizeof(float2), s, p);
+                    ((size_t)p.tokens_per_block * p.pairs * sizeof(float2) + 15) / 16 * 16, s, p);
 }
 
 // `vec`: every base and stride is a multiple of four elements.  Vectors also

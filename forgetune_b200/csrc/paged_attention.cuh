@@ -55,7 +55,9 @@ namespace ftb {
 constexpr int kPagedThreads = 640;
 constexpr int kPagedProducer = 16, kPagedProducts = 17, kPagedQueries = 18;  // warps
 constexpr int kPagedTile = 128;      // keys of a tile, rows of a half
-constexpr int kPagedUnitOver = 256;  // a unit's own cost, in keys
+// A unit's own cost, in keys; twice that where it is all of a sequence's rows, whose keys cost less (160, 256, 512 and
+// 700 for all: 64 sequences of one token 191, 184, 172 and 174 us, a prompt of 8192 586, 552, 562 and 573).
+constexpr int kPagedUnitOver = 256;
 constexpr int kPagedLeast = 512;     // keys (with it) that are worth a block
 constexpr float kPagedRaise = 8.0f;  // log2
 constexpr int kPagedBlocks = 148;    // at most: B200's SMs
@@ -125,7 +127,7 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedTensorParams&
   s.cost.base = max(0, len - s.n) >> p.cost_shift;
   s.cost.step = p.cost_step;
   s.cost.cap = (p.a.window ? min(len, p.window_cap) : len) >> p.cost_shift;
-  s.cost.over = p.cost_over;
+  s.cost.over = s.tiles == 1 ? 2 * p.cost_over : p.cost_over;
   s.head = s.cost.first(s.tiles);
   s.whole = s.head * p.a.kv_heads;
   return s;
@@ -1134,7 +1136,7 @@ inline cudaError_t launch_paged_attention(const PagedAttentionParams& a, int typ
   const int step = std::max(1, 256 / p.group);
   const double tiles = (double)a.kv_heads * ((double)a.tokens * p.group / 256 + std::min(a.batch.seqs, a.tokens));
   const double most = a.window ? std::min<double>(p.capacity, (double)a.window + step) : p.capacity;
-  while (tiles * (most / (1 << p.cost_shift) + std::max(1, kPagedUnitOver >> p.cost_shift) + 1) > 0x3fffffff && p.cost_shift < 20)
+  while (tiles * (most / (1 << p.cost_shift) + 2 * std::max(1, kPagedUnitOver >> p.cost_shift) + 1) > 0x3fffffff && p.cost_shift < 20)
     ++p.cost_shift;
   p.cost_step = step >> p.cost_shift;
   p.cost_over = std::max(1, kPagedUnitOver >> p.cost_shift);
