@@ -271,6 +271,7 @@ static int check_attention(const char* fn, const ftb_attention_args& a) {
   if (a.tokens < 0 || a.tokens > kMaxTokens || a.heads < 1 || a.heads > kMaxHeads)
     return refuse(fn, "needs 0 <= tokens and 1 <= heads (at most 4096)");
   std::string why = check(c);
+  if (why.empty() && a.tokens * a.heads > 0x7fffffff) why = "tokens times heads must be below 2^31";
   if (why.empty() && a.heads % c.kv_heads) why = "heads must be a multiple of kv_heads";
   if (why.empty()) why = check(a.batch);
   if (why.empty()) why = check("q", a.q, a.tokens, a.heads, c.dim);

@@ -161,7 +161,7 @@ struct PagedSmem {
   static constexpr int UNIT_OFF = ROW_OFF + 16 * 32 * 4;
   static constexpr int UNITS = 4;
   static constexpr int BAR_OFF = (UNIT_OFF + UNITS * (int)sizeof(PagedUnit) + 15) / 16 * 16;
-  static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 4 + 5;
+  static constexpr int NBAR = 2 * STAGES + 2 * UNITS + 2 + 2 * 4 + 13;
   static constexpr int TOTAL = BAR_OFF + 8 * NBAR + 16;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
 };
@@ -324,7 +324,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   uint64_t* v_clean = v_seen + 1;        // ... and clean
   uint64_t* ml_full = v_clean + 1;       // m and sum of the second half
   uint64_t* ml_free = ml_full + 1;       // ... read
-  uint64_t* drain = ml_free + 1;         // products retired after an abort
+  uint64_t* pairs = ml_free + 1;         // [8] the two warps of 32 rows have met
+  uint64_t* drain = pairs + 8;           // products retired after an abort
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 1) + 1;
 
@@ -353,6 +354,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     mbar_init(v_clean, 2);
     mbar_init(ml_full, 8);
     mbar_init(ml_free, 8);
+    for (int s = 0; s < 8; ++s) mbar_init(&pairs[s], 2);
     mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -784,13 +786,24 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     const uint32_t s_tmem = tmem + w * 128 + lanes;
     // the warp with the other scores of the same rows, and where the two leave theirs
     float* rows = reinterpret_cast<float*>(smem + L::ROW_OFF) + lane;
-    // what the two warps of a row have, for both.  A place is written again only when its
-    // reader is known to be past this: behind a barrier of theirs or the next S.
-    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + w * 4 + quarter) : "memory"); };
-    auto exchange = [&](float x) {
+    // What the two warps of a row have, for both.  A place is written again only when its
+    // reader is known to be past this: behind a meeting of theirs or the next S.  Meetings
+    // are bounded waits too: one warp may have given up where the other went on.
+    uint64_t* pair = pairs + w * 4 + quarter;
+    uint32_t met = 0;
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair);
+      __syncwarp();
+      const bool both_here = paged_wait(pair, met & 1u, abort_flag, p.err, 62);
+      ++met;
+      return both_here;
+    };
+    auto exchange = [&](float x, float* y) {
       rows[warp * 32] = x;
-      meet();
-      return rows[(warp ^ 4) * 32];
+      const bool both_here = meet();
+      *y = rows[(warp ^ 4) * 32];
+      return both_here;
     };
     bool ok = true;
     uint32_t uc = 0, cnt0 = 0, cnt1 = 0, mc = 0;
@@ -850,7 +863,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
             }
             if (pass == 0) continue;
             if (pass == 1) {
-              high_s = fmaxf(high_s, exchange(high_s)) * a.scale;
+              float other;
+              if (!(ok = exchange(high_s, &other))) break;
+              high_s = fmaxf(high_s, other) * a.scale;
               const bool raise = real && high_s > m + kPagedRaise;
               if (__any_sync(0xffffffffu, raise)) {
                 float keep = 1.0f;
@@ -884,6 +899,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
             }
             FTB_TMEM_ST16(s_tmem + side * 64 + c * 16, o);
           }
+          if (!ok) break;
           sum += (part[0] + part[1]) + (part[2] + part[3]);
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
@@ -900,8 +916,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       float f0 = 1.0f, f1 = 1.0f;  // factors of the halves' O
       if (count > 0) {
         if (!(ok = paged_wait(&pv_done[w], (done + count - 1) & 1u, abort_flag, p.err, 60))) break;
-        sum += exchange(sum);
-        meet();
+        float other;
+        if (!(ok = exchange(sum, &other))) break;
+        sum += other;
+        if (!(ok = meet())) break;
       }
       if (both && w == 1) {
         rows[warp * 32] = side ? sum : m;
@@ -1066,13 +1084,17 @@ inline bool make_map_heads(CUtensorMap* map, const void* base, int type, int64_t
 }
 
 // Whether the tensor-core kernel takes a call: 16-bit types, heads of up to 128
-// in eights, pages of whole 16 tokens, and 16-byte boundaries throughout.
+// in eights, pages of whole 16 tokens, and 16-byte boundaries throughout.  (A
+// pool that repeats itself, with strides of 0, has no TMA map.)
 inline bool paged_on_tensor_cores(const PagedAttentionParams& p, int type) {
   if (type == FTB_F32 || p.dim > 128 || p.dim % 8 || p.batch.page_size % 16) return false;
   for (const void* x : {p.q, (const void*)p.out, p.keys, p.values})
     if (reinterpret_cast<uintptr_t>(x) & 15) return false;
   for (int64_t s : {p.q_token, p.q_head, p.o_token, p.o_head, p.k_page, p.k_token, p.k_head, p.v_page, p.v_token, p.v_head})
     if (s % 8) return false;
+  if ((p.batch.pages > 1 && !(p.k_page && p.v_page)) || (p.batch.page_size > 1 && !(p.k_token && p.v_token)) ||
+      (p.kv_heads > 1 && !(p.k_head && p.v_head)))
+    return false;
   return true;
 }
 

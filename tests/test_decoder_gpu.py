@@ -580,3 +580,102 @@ def test_outputs_count_as_changed():
     paged_attention(q, *b.args(), out=saved.detach())
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.backward()
+
+
+def test_a_wait_that_runs_out_is_reported_once():
+    """The failure-detection hook: a kernel whose products never come leaves, the next call says so, later ones work."""
+    from forgetune_b200 import ForgeTuneRuntimeError, _native
+    b = ref.Batch([1, 300], [500, 300], 16, 2, 128, BF16)
+    q = randn(b.tokens, 8, 128, dtype=BF16)
+    want = paged_attention(q, *b.args())
+    torch.cuda.synchronize()
+    try:
+        _native.lib().ftb_fp8_set_fault_injection(1)
+        paged_attention(q, *b.args())
+        torch.cuda.synchronize()
+    finally:
+        _native.lib().ftb_fp8_set_fault_injection(0)
+    with pytest.raises(ForgeTuneRuntimeError, match="gave up"):
+        rotate_heads(q, torch.zeros(b.tokens, dtype=torch.int32, device="cuda"), rope_frequencies(128))
+    assert torch.equal(paged_attention(q, *b.args()), want)
+
+
+def test_pools_with_strides_of_their_own():
+    """A pool that repeats one page, one of rows apart, and one whose pages lie backwards in memory order."""
+    b = ref.Batch([3, 20], [64, 40], 16, 2, 64, F16)
+    q = randn(b.tokens, 4, 64, dtype=F16)
+    for change in (lambda x: x[:1].expand(x.shape), lambda x: torch.cat([x, x], 3)[..., :64],
+                   lambda x: x.permute(2, 1, 0, 3).contiguous().permute(2, 1, 0, 3)):
+        b.keys, b.values = change(b.keys), change(b.values)
+        want, tol, inside = ref.attention(q, b)
+        within(paged_attention(q, *b.args()), want, tol)
+
+
+def test_python_refusals():
+    b = ref.Batch([2, 3], [4, 9], 16, 2, 64, BF16)
+    q, k, v = randn(5, 8, 64, dtype=BF16).split((4, 2, 2), 1)
+    f, positions = rope_frequencies(64), torch.arange(5, device="cuda")
+    keys, values, table, starts, lengths = b.args()
+    from forgetune_b200 import InvalidShapeError
+    x = randn(5, 4, 64)
+
+    def attend(**over):
+        a = dict(q=q, keys=keys, values=values, page_table=table, starts=starts, lengths=lengths)
+        a.update(over)
+        return lambda: paged_attention(**a)
+
+    def append(**over):
+        a = dict(q=q, k=k, v=v, keys=keys, values=values, page_table=table, starts=starts, lengths=lengths, frequencies=f)
+        a.update(over)
+        return lambda: append_heads(**a)
+    logits, tokens = randn(3, 100), torch.zeros(3, dtype=torch.int64, device="cuda")
+    grad = torch.zeros(5, 4, 64, device="cuda", requires_grad=True)
+    cases = [
+        (TypeError, lambda: rotate_heads(x.double(), positions, f)), (TypeError, lambda: rotate_heads(x, positions.float(), f)),
+        (TypeError, lambda: rotate_heads(x, positions, f.float())), (InvalidShapeError, lambda: rotate_heads(x[0], positions, f)),
+        (InvalidShapeError, lambda: rotate_heads(x, positions[:4], f)), (InvalidShapeError, lambda: rotate_heads(x, positions, rope_frequencies(66))),
+        (ValueError, lambda: rotate_heads(x, positions, f, weight=torch.ones(64, device="cuda"))),
+        (InvalidShapeError, lambda: rotate_heads(x, positions, f, weight=torch.ones(32, device="cuda"), norm=True)),
+        (TypeError, lambda: rotate_heads(x, positions, f, out=torch.empty_like(x).half())),
+        (InvalidShapeError, lambda: rotate_heads(x, positions, f, out=torch.empty(5, 4, 128, device="cuda")[..., ::2])),
+        (ValueError, lambda: rotate_heads(x, positions.cpu(), f)), (ValueError, lambda: rotate_heads(x, positions, f, out=grad)),
+        (TypeError, append(k=k.float())), (TypeError, append(q=q.half(), k=k.half(), v=v.half())), (InvalidShapeError, append(k=q)),
+        (InvalidShapeError, append(q=q[:4])), (TypeError, append(values=values.half())), (InvalidShapeError, append(values=values[:1])),
+        (InvalidShapeError, append(keys=torch.empty(3, 16, 2, 128, dtype=BF16, device="cuda")[..., ::2])),
+        (TypeError, append(lengths=lengths.long())), (InvalidShapeError, append(starts=starts[1:])), (ValueError, append(page_table=table.cpu())),
+        (TypeError, attend(q=q.float())), (InvalidShapeError, attend(q=q[:, :3])), (InvalidShapeError, attend(q=q[..., :32])),
+        (ValueError, attend(window=-1)), (InvalidShapeError, attend(lengths=lengths[:1])), (TypeError, attend(page_table=table.float())),
+        (TypeError, attend(window="all")), (InvalidShapeError, attend(out=torch.empty(5, 4, 32, dtype=BF16, device="cuda"))),
+        (TypeError, lambda: token_logprobs(logits.double(), tokens)), (InvalidShapeError, lambda: token_logprobs(logits, tokens[:2])),
+        (ValueError, lambda: token_logprobs(logits, tokens, top=65)), (ValueError, lambda: token_logprobs(logits[:, :5], tokens, top=6)),
+        (TypeError, lambda: token_logprobs(logits, tokens.float())), (ValueError, lambda: token_logprobs(logits, tokens, top=-1)),
+    ]
+    for i, (error, call) in enumerate(cases):
+        with pytest.raises(error):
+            call()
+            pytest.fail("case %d was taken" % i)
+    from forgetune_b200 import ForgeTuneRuntimeError
+    inside = keys[0, :5]  # heads that lie in the pool that is written
+    for call in (attend(out=q), append(k=inside, q=torch.cat([q, q], 1)), append(values=keys)):
+        with pytest.raises(ForgeTuneRuntimeError, match="overlap"):
+            call()
+
+
+def test_no_gradients_and_no_tangents():
+    import torch.autograd.forward_ad as ad
+    x = torch.randn(3, 2, 64, device="cuda", requires_grad=True)
+    positions, f = torch.arange(3, device="cuda"), rope_frequencies(64)
+    assert not rotate_heads(x, positions, f).requires_grad
+    with ad.dual_level():
+        with pytest.raises(ValueError, match="tangent"):
+            rotate_heads(ad.make_dual(x.detach(), torch.ones_like(x)), positions, f)
+    with torch.no_grad():
+        assert rotate_heads(x, positions, f, out=x) is not None
+
+
+def test_a_negated_view_is_taken_as_what_it_stands_for():
+    x = torch.randn(3, 2, 64, dtype=torch.complex64, device="cuda")
+    neg = x.conj().imag
+    assert neg.is_neg()
+    positions, f = torch.arange(3, device="cuda"), rope_frequencies(64)
+    assert torch.equal(rotate_heads(neg, positions, f), rotate_heads(neg.resolve_neg(), positions, f))
