@@ -4,8 +4,10 @@
 //
 // in one pass over the keys: a row keeps its reference m and its sum, and O
 // lies in tensor memory.  m is raised (and O rescaled) only where a tile's
-// maximum is above it by more than 2^8: any reference gives the same quotient,
-// and weights up to 2^8 are as exact as weights up to 1.
+// largest weight would be above 2^8: any reference gives the same quotient, and
+// weights up to 2^8 are as exact as weights up to 1.  Scores, m, sums and O are
+// fp32; a weight is rounded once, to the type of the values that the tensor
+// cores multiply it by, while the sum takes it as it was.
 //
 // Rows.  The queries that share a kv head are the rows of one matrix, row r =
 // (token r / G, head r % G), so that one token of G heads costs one row of
@@ -40,6 +42,17 @@
 // Shared memory: Q of two tiles, and a ring of 128-token tiles of K or V,
 // 128-byte swizzle, in columns of 64.  Tensor memory: S and P of both halves at
 // [0, 256), O at [256, 512).
+//
+// What bounds it.  Few rows: the cache's bytes; a tile of 64 KB takes an SM 1.36
+// us (47 GB/s, 6.9 TB/s over all).  Many rows: a pair of tiles takes 2.1 us; the
+// tensor cores need 1.25 of it (82 cycles for 128 x 128 x 16 of Q K^T, whose
+// operands come from shared memory, 74 of P V), the exponentials 1.05.  The rest
+// is latency: a half's next S waits for its P V, since P lies over S.  Tiles of
+// 80 keys leave room for S beside P, and S and P V then had threads of their own;
+// but N = 80 costs 97 cycles, and 128 keys took 2.5 us.  Scores in one thread a
+// row (eight softmax warps) took 2.3 with the registers of twelve warps, of which
+// some were spilled: local memory has 28 KB of L1 beside this much shared memory.
+// A unit costs 3 to 5 us beside its tiles: Q, the first tile, the last P V and O.
 #pragma once
 
 #include <algorithm>
@@ -133,9 +146,9 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedTensorParams&
   return s;
 }
 
-// A bounded wait by a whole warp, with one outcome.  The long form is apart: the kernel has many waits, and what it
-// does between them is short, so that its code has to stay small (129 KB of it, with every wait written out, took
-// 684 us for a prompt of 8192 where XXXX KB take XXXX).
+// A bounded wait by a whole warp, with one outcome.  The long form is apart: the roles are many and what they do
+// between waits is short, so that instructions have to come from near (a prompt of 4096: 218 us with 129 KB of code,
+// 171 with 78).
 __device__ __noinline__ bool paged_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
   return mbar_wait_warp(bar, parity, abort_flag, err, code & 0xFF, (code & 0x100) != 0);
 }
@@ -832,7 +845,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           // keeps do not fit its registers, and what is spilled goes to L2.  P of 32 goes over the first 16 columns
           // of the scores, when both are done with.
           float high_s = -INFINITY, base = 0.0f, part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
+#pragma unroll  // rolled up: 578 us for a prompt of 8192 in place of 545
           for (int pass = 0; pass < 3; ++pass) {
             const int c = (pass & 1) ^ 1;
             uint32_t x[32];
