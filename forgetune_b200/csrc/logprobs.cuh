@@ -215,8 +215,8 @@ __device__ __forceinline__ float row_max3(float a, float b, float c) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogprobsThreads, 3) logprobs_kernel(const LogprobsParams p, const int split) {
-  constexpr int W = RowVectors<T>::W, U = 4;
+__global__ void __launch_bounds__(kLogprobsThreads, 5) logprobs_kernel(const LogprobsParams p, const int split) {
+  constexpr int W = RowVectors<T>::W, U = 2;
   __shared__ LogprobsSmem sm;
   grid_dep_wait();
   grid_dep_trigger();
@@ -228,7 +228,14 @@ __global__ void __launch_bounds__(kLogprobsThreads, 3) logprobs_kernel(const Log
   RowSums a{-FLT_MAX, 0.0f, 0.0f};
   float top = -INFINITY;
   uint4 u[U], next[U];
+  const int whole0 = r.off ? 1 : 0, whole1 = min(v1, (r.n + r.off) / W);  // vectors inside of the row
   auto load = [&](uint4 (&to)[U], int v) {
+    if (v >= whole0 && v + (U - 1) * kLogprobsThreads < whole1) {
+      const uint4* from = reinterpret_cast<const uint4*>(r.row - r.off) + v;
+#pragma unroll
+      for (int i = 0; i < U; ++i) to[i] = __ldg(from + i * kLogprobsThreads);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       T t[W];
