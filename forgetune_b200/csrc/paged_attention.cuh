@@ -43,16 +43,17 @@
 // 128-byte swizzle, in columns of 64.  Tensor memory: S and P of both halves at
 // [0, 256), O at [256, 512).
 //
-// What bounds it.  Few rows: the cache's bytes; a tile of 64 KB takes an SM 1.36
-// us (47 GB/s, 6.9 TB/s over all).  Many rows: a pair of tiles takes 2.1 us; the
-// tensor cores need 1.25 of it (82 cycles for 128 x 128 x 16 of Q K^T, whose
-// operands come from shared memory, 74 of P V), the exponentials 1.05.  The rest
-// is latency: a half's next S waits for its P V, since P lies over S.  Tiles of
-// 80 keys leave room for S beside P, and S and P V then had threads of their own;
-// but N = 80 costs 97 cycles, and 128 keys took 2.5 us.  Scores in one thread a
-// row (eight softmax warps) took 2.3 with the registers of twelve warps, of which
-// some were spilled: local memory has 28 KB of L1 beside this much shared memory.
-// A unit costs 3 to 5 us beside its tiles: Q, the first tile, the last P V and O.
+// What bounds it.  Few rows: the cache's bytes; a tile of 64 KB takes an SM 1.38
+// us (47 GB/s, 7.0 TB/s over all).  Many rows: a pair of tiles takes 2.16 us, of
+// which the tensor cores are busy 44 % and the exponentials' unit 44 % (prompt of
+// 4096); neither is full because a half's next S waits for its P V, since P lies
+// over S.  Tiles of 80 keys leave room for S beside P, and S and P V then had
+// threads of their own; but an N = 80 product takes about 97 cycles (N = 128: 82), and
+// 128 keys took 2.5 us.  A row's scores in one thread had spilled registers, for
+// which 227 KB of shared memory leave little L1: 262 us for a prompt of 4096 where
+// two threads a row took 218 (167 now).  A unit costs 4 to 5.5 us beside its
+// tiles: Q, the first tile, the last P V and O (1480 sequences against 296: 7.6 us
+// for each further unit of 256 rows and one tile, 5.5 for one of a single token).
 #pragma once
 
 #include <algorithm>
