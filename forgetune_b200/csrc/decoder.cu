@@ -277,7 +277,7 @@ static int check_attention(const char* fn, const ftb_attention_args& a) {
   if (why.empty()) why = check("q", a.q, a.tokens, a.heads, c.dim);
   if (why.empty()) why = check("out", a.out, a.tokens, a.heads, c.dim);
   if (why.empty() && (a.q.type != c.type || a.out.type != c.type)) why = "q, out and the cache must have one type";
-  if (why.empty() && !std::isfinite(a.scale)) why = "scale must be finite";
+  if (why.empty() && !(std::fabs(a.scale) * 1.4426950408889634 < 3.4e38)) why = "scale must be finite in float32, times log2(e) too";
   if (why.empty() && (a.window < 0 || a.window > 0x7fffffff)) why = "window must not be negative";
   if (why.empty()) {
     const Span in[6] = {span(a.q, a.tokens, a.heads, c.dim), flat(c.keys, cache_bytes(c, c.k_page, c.k_token, c.k_head)),

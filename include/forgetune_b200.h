@@ -332,7 +332,7 @@ FORGETUNE_EXPORT int ftb_fp8_set_kernel(int nt, int split);
  * (starts[b + 1] - starts[b]) + i.  The token at position j lies in page
  * page_table[b][j / page_size], at j % page_size.  starts, lengths and
  * page_table are read on the device when the kernels run.  starts must not
- * fall.  Rows in no sequence are left as they were. */
+ * fall, nor pass the number of tokens.  Rows in no sequence are left as they were. */
 typedef struct {
   void* data;
   int64_t token, head; /* strides in elements */

@@ -110,7 +110,8 @@ def test_attention_refusals():
         for over in (dict(tokens=-1), dict(heads=0), dict(heads=3), dict(type=1), dict(q_type=0), dict(o_type=1), dict(o=B),
                      dict(o=20 * B), dict(o=30 * B + 64), dict(o=40 * B), dict(o=41 * B), dict(o=42 * B), dict(window=-1),
                      dict(scale=math.nan), dict(scale=math.inf), dict(q_head=60), dict(o_token=0), dict(dim=513), dict(seqs=0),
-                     dict(lengths=3), dict(keys=20 * B + 1), dict(window=1 << 31), dict(tokens=1 << 28)):
+                     dict(lengths=3), dict(keys=20 * B + 1), dict(window=1 << 31), dict(tokens=1 << 28), dict(scale=1e300),
+                     dict(scale=-2.9e38)):
             refused(ATTENTION, name, **over)
     assert ATTENTION.call("ftb_paged_attention_workspace") >= 0
     assert _native.lib().ftb_paged_attention(None, None) == -1 and _native.lib().ftb_paged_attention_workspace(None) == -1
