@@ -4,10 +4,10 @@
 //
 // in one pass over the keys: a row keeps its reference m and its sum, and O
 // lies in tensor memory.  m is raised (and O rescaled) only where a tile's
-// largest weight would be above 2^8: any reference gives the same quotient, and
-// weights up to 2^8 are as exact as weights up to 1.  Scores, m, sums and O are
-// fp32; a weight is rounded once, to the type of the values that the tensor
-// cores multiply it by, while the sum takes it as it was.
+// largest weight would be above 2^7 times the reference's: any reference gives
+// the same quotient, and weights up to 2^7 are as exact as weights up to 1.
+// Scores, m, sums and O are fp32; a weight is rounded once, to the type of the
+// values that the tensor cores multiply it by, while the sum takes it as it was.
 //
 // Rows.  The queries that share a kv head are the rows of one matrix, row r =
 // (token r / G, head r % G), so that one token of G heads costs one row of
@@ -73,7 +73,13 @@ constexpr int kPagedTile = 128;      // keys of a tile, rows of a half
 // 700 for all: 64 sequences of one token 191, 184, 172 and 174 us, a prompt of 8192 586, 552, 562 and 573).
 constexpr int kPagedUnitOver = 256;
 constexpr int kPagedLeast = 512;     // keys (with it) that are worth a block
-constexpr float kPagedRaise = 8.0f;  // log2
+constexpr float kPagedRaise = 7.0f;  // log2
+// float16 weights are taken relative to 2^-7 of a row's reference (sums and O alike, so that the factor cancels): up to
+// 2^15, below the largest number, and off by at most 2^-32 of the reference's where they are below the smallest normal
+// number.  Relative to the reference itself, what lay 2^-25 below it became 0 in P V and counted in the sum: of 4096 keys
+// 17.5 nats below one nothing was left, and 17 nats below came out 44 % too large.  bfloat16 has float32's exponents.
+template <typename T>
+constexpr float kPagedLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;  // log2
 constexpr int kPagedBlocks = 148;    // at most: B200's SMs
 
 // What the blocks leave for the join: for each block whose last unit others go on with.
@@ -880,7 +886,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               float other;
               if (!(ok = exchange(high_s, &other))) break;
               high_s = fmaxf(high_s, other) * a.scale;
-              const bool raise = real && high_s > m + kPagedRaise;
+              const bool raise = real && high_s - m > kPagedRaise;  // (their sum might round up to high_s)
               if (__any_sync(0xffffffffu, raise)) {
                 float keep = 1.0f;
                 if (raise) {
@@ -899,7 +905,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
                   FTB_TMEM_ST16(tmem + 256 + w * 128 + lanes + d, o);
                 }
               }
-              base = m == -INFINITY ? 0.0f : m;
+              base = m == -INFINITY ? 0.0f : m - kPagedLift<T>;
             }
             uint32_t o[16];
 #pragma unroll

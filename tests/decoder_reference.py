@@ -73,8 +73,9 @@ class Batch:
         return self.page_table[b].long()[positions // self.page], positions % self.page
 
 
-def attention(q, batch, scale=None, window=0):
-    """float64 result, its tolerance, and which rows belong to a sequence."""
+def attention(q, batch, scale=None, window=0, least=2.0 ** -25):
+    """float64 result, its tolerance, and which rows belong to a sequence.  float16: a weight below the smallest normal
+    number is off by at most `least`, relative to the row's largest."""
     tokens, heads, dim = q.shape
     kv = batch.keys.shape[2]
     scale = dim ** -0.5 if scale is None else scale
@@ -110,7 +111,7 @@ def attention(q, batch, scale=None, window=0):
             out[at:at + n] = o
             tol[at:at + n] = half * o.abs() + (half + 2 * off + whole * 2.0 ** -23) * mean
             if q.dtype == torch.float16:
-                tol[at:at + n] += (whole + 1) * 2.0 ** -25 * max(1.0, float(v.abs().max()))
+                tol[at:at + n] += (whole + 1) * least * max(1.0, float(v.abs().max()))
         at += n
     return out, tol + 1e-30, inside
 
