@@ -106,13 +106,13 @@ struct PagedTensorParams {
 struct PagedUnit {
   int seq, kvh, r0, rows, tok0, pos0;
   int tb, te;          // tiles of keys of this part
-  int lo, hi;          // keys that some row sees
+  int lo, hi;          // keys that some row sees and the table has places for
   int first, last;     // positions of the first and the last row
   int alternate;       // the halves take the tiles in turn
   int count0, count1;  // tiles that the halves take
   int slot;            // part of the workspace, -1: the whole unit
   int done;
-  volatile int bad;    // a page outside of the pool
+  volatile int bad;    // a page outside of the pool, in tiles that have come
   volatile int dirty;  // a value that is not finite in a tile seen in part
 };
 
@@ -303,8 +303,9 @@ __device__ __forceinline__ uint32_t paged_marks(const PagedTensorParams& p, cons
   const PagedAttentionParams& a = p.a;
   uint32_t bits = 0;
   const int64_t from = a.window ? (int64_t)position - a.window + 1 : 0;
+  const int end = min(min(position + 1, u.hi), u.te * kPagedTile);  // within the table
 #pragma unroll 1
-  for (int key = (int)max((int64_t)u.tb * kPagedTile, from); key <= position && key < u.te * kPagedTile; ++key) {
+  for (int key = (int)max((int64_t)u.tb * kPagedTile, from); key < end; ++key) {
     if (!paged_masked(u, key / kPagedTile, a.window)) continue;
     const int page = a.batch.page_table[u.seq * a.batch.table_ld + a.batch.by_page.of(key)];
     if (page < 0 || page >= a.batch.pages) continue;
@@ -315,6 +316,22 @@ __device__ __forceinline__ uint32_t paged_marks(const PagedTensorParams& p, cons
       if (!isfinite(to_f32(x[k]))) bits |= 1u << k;
   }
   return bits;
+}
+
+// Whether the row at `position` sees a key of this part whose page is outside of the pool.  By the table and not by what
+// the block has come to: the answer is the same for any split and at any time.  (In a tile that other rows see in part
+// such keys have a weight of 0 for the rows that do not see them, and finite values: cleaned.)
+__device__ __forceinline__ bool paged_lost(const PagedTensorParams& p, const PagedUnit& u, int position) {
+  const PagedAttentionParams& a = p.a;
+  const int64_t from = a.window ? (int64_t)position - a.window + 1 : 0;
+  const int end = min(min(position + 1, u.hi), u.te * kPagedTile);
+#pragma unroll 1
+  for (int64_t key = max((int64_t)u.tb * kPagedTile, from); key < end;) {
+    const int n = a.batch.by_page.of((int)key), page = a.batch.page_table[u.seq * a.batch.table_ld + n];
+    if (page < 0 || page >= a.batch.pages) return true;
+    key = (int64_t)(n + 1) * a.batch.page_size;
+  }
+  return false;
 }
 
 template <typename T, int DH>
@@ -510,12 +527,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         u.pos0 = max(s.len, -(1 << 30)) - s.n;
         u.first = u.pos0 + p.by_group.of(u.r0);
         u.last = u.pos0 + p.by_group.of(u.r0 + u.rows - 1);
-        if (s.len > p.capacity) {
-          u.bad = 1;
-        } else {
-          u.hi = max(0, u.last + 1);
-          u.lo = a.window ? (int)max((int64_t)0, (int64_t)u.first - a.window + 1) : 0;
-        }
+        u.hi = max(0, min(u.last + 1, p.capacity));
+        u.lo = a.window ? (int)max((int64_t)0, (int64_t)u.first - a.window + 1) : 0;
         const int tb = u.lo / kPagedTile, n = max(0, (u.hi + kPagedTile - 1) / kPagedTile - tb);
         // where a share's border cuts the unit, the same for the blocks on either side; not within two tiles of its ends
         const float per = __fdividef((float)n, (float)cost);
@@ -558,7 +571,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         d.seq = u.seq, d.kvh = u.kvh, d.r0 = u.r0, d.rows = u.rows, d.tok0 = u.tok0, d.pos0 = u.pos0;
         d.first = u.first, d.last = u.last, d.count0 = u.count0, d.count1 = u.count1;
         d.tb = u.tb, d.te = u.te, d.lo = u.lo, d.hi = u.hi, d.alternate = u.alternate, d.slot = u.slot;
-        d.done = u.done, d.bad = u.bad, d.dirty = 0;
+        d.done = u.done, d.bad = 0, d.dirty = 0;
         mbar_arrive(&u_full[us]);
       }
       __syncwarp();
@@ -964,7 +977,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       if (mine) {
         if (both && count1 > 0 && !(ok = paged_wait(&pv_done[1], (cnt1 - 1) & 1u, abort_flag, p.err, 63))) break;
         tc_fence_after();
-        const bool bad = u.bad, dirty = u.dirty;
+        const bool dirty = u.dirty, bad = position >= p.capacity || (u.bad && real && paged_lost(p, u, position));
         const int g = u.r0 + r - tok * G;
         // a part of the workspace: (m, sum) of each row, then O in quads of columns, each of them of all rows
         float* part = p.parts + (int64_t)max(u.slot, 0) * p.rows_bound * (2 + DH);

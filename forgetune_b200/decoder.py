@@ -127,8 +127,9 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, p
     ``scale`` (default ``dim ** -0.5``) multiplies the scores.  A token at a
     negative position (a length below its number of new tokens) sees nothing
     and gets zeros.  What a token does not see does not change its output,
-    whatever it holds (infinities and NaN too).  ``out`` receives the result in place of a new tensor; it may
-    not be ``q``.
+    whatever it holds (infinities and NaN too).  A token that sees one whose page
+    number is outside of the pool, or whose own position is beyond the table, gets
+    NaN.  ``out`` receives the result in place of a new tensor; it may not be ``q``.
 
     Softmax statistics and sums are float32; a weight is rounded to the
     cache's type where the tensor cores multiply it by the values.

@@ -1,14 +1,19 @@
-"""Attention over the paged cache at its edges: far tails in float16."""
+"""Attention over the paged cache at its edges: far tails in float16, pages outside of the pool, lengths beyond the
+table."""
 
 import pytest
 import torch
 
-from forgetune_b200 import paged_attention
+from forgetune_b200 import append_heads, paged_attention
 
 from . import decoder_reference as ref
-from .test_decoder_gpu import BF16, F16, randn, within
+from .test_decoder_gpu import BF16, F16, F32, randn, within
 
 pytestmark = pytest.mark.gpu
+
+# kernel by type and head size: tensor cores, tensor cores, a key at a time, a key at a time
+KINDS = [(BF16, 128), (F16, 80), (F32, 64), (BF16, 136)]
+
 
 # ---------------------------------------------------------------------------
 # float16 weights
@@ -47,3 +52,72 @@ def test_equal_values_come_out_as_they_are(dtype):
         q = (spread * randn(new, 8, 128)).to(dtype)
         want, tol, _ = ref.attention(q, b, least=2.0 ** -32)
         within(paged_attention(q, *b.args()), want, tol)
+
+
+# ---------------------------------------------------------------------------
+# pages outside of the pool, lengths beyond the table
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,dim", KINDS, ids=str)
+@pytest.mark.parametrize("page", [16, 48, 128])
+@pytest.mark.parametrize("new,length,window,group", [(300, 300, 0, 1), (300, 1000, 0, 2), (100, 700, 0, 4), (40, 90, 20, 2),
+                                                     (700, 700, 130, 1), (1, 500, 60, 4), (1, 3000, 0, 4), (5, 5, 0, 1)])
+def test_only_rows_that_see_a_bad_page_are_nan(dtype, dim, page, new, length, window, group):
+    b = ref.Batch([3, new, 2], [40, length, 9], page, 2, dim, dtype)
+    q = randn(b.tokens, 2 * group, dim, dtype=dtype)
+    clean = paged_attention(q, *b.args(), window=window)
+    position = torch.arange(length - new, length, device="cuda")
+    pages = -(-length // page)
+    for bad in sorted({0, pages // 2, max(0, pages - 2), pages - 1}):
+        for number in (-1, b.keys.shape[0], 2 ** 31 - 1):
+            kept = int(b.page_table[1, bad])
+            b.page_table[1, bad] = number
+            got = paged_attention(q, *b.args(), window=window)
+            b.page_table[1, bad] = kept
+            sees = position >= bad * page
+            if window:
+                sees &= position - window < (bad + 1) * page - 1
+            assert got[3:3 + new][sees].isnan().all()
+            assert torch.equal(got[3:3 + new][~sees], clean[3:3 + new][~sees])
+            assert torch.equal(got[:3], clean[:3]) and torch.equal(got[3 + new:], clean[3 + new:])
+    for bad in (slice(0, pages), slice(pages // 2, pages)):  # several
+        kept = b.page_table[1, bad].clone()
+        b.page_table[1, bad] = -5
+        got = paged_attention(q, *b.args(), window=window)[3:3 + new]
+        b.page_table[1, bad] = kept
+        sees = position >= (bad.start or 0) * page
+        assert got[sees].isnan().all() and torch.equal(got[~sees], clean[3:3 + new][~sees])
+
+
+@pytest.mark.parametrize("dtype,dim", KINDS, ids=str)
+@pytest.mark.parametrize("new,length,places,window", [(200, 300, 160, 0), (200, 300, 112, 0), (300, 300, 16, 0), (600, 1500, 1008, 100),
+                                                      (1, 300, 160, 0), (2, 161, 160, 0), (200, 300, 160, 30), (500, 900, 128, 0)])
+def test_rows_beyond_the_table_are_nan_and_others_are_not(dtype, dim, new, length, places, window):
+    b = ref.Batch([new, 2], [length, 9], 16, 2, dim, dtype)
+    q = randn(b.tokens, 4, dim, dtype=dtype)
+    want, tol, _ = ref.attention(q, b, window=window)
+    b.page_table = b.page_table[:, :places // 16].contiguous()
+    got = paged_attention(q, *b.args(), window=window)
+    beyond = torch.arange(length - new, length, device="cuda") >= places
+    assert got[:new][beyond].isnan().all()
+    within(got[:new][~beyond], want[:new][~beyond], tol[:new][~beyond])
+    within(got[new:], want[new:], tol[new:])
+
+
+@pytest.mark.parametrize("dtype,dim", KINDS, ids=str)
+def test_bad_rows_are_the_same_every_time(dtype, dim):
+    """The halves of a block come to a bad page at different times; a full machine makes them differ more."""
+    b = ref.Batch([400] * 20, [500 + 7 * i for i in range(20)], 16, 2, dim, dtype)
+    q = randn(b.tokens, 2, dim, dtype=dtype)
+    b.page_table[torch.arange(20), torch.arange(20) + 10] = -1
+    first = paged_attention(q, *b.args())
+    for _ in range(20):
+        assert torch.equal(paged_attention(q, *b.args()).nan_to_num(123.0), first.nan_to_num(123.0))
+
+
+def test_tokens_before_the_end_of_the_table_are_stored():
+    b = ref.Batch([40], [60], 16, 1, 64, BF16)
+    b.page_table = b.page_table[:, :2].contiguous()
+    q, k, v = randn(40, 3, 64, dtype=BF16).split((1, 1, 1), 1)
+    append_heads(q, k, v, *b.args())
+    page, col = b.slots(0, torch.arange(20, 32, device="cuda"))
+    assert torch.equal(b.keys[page, col], k[:12]) and torch.equal(b.values[page, col], v[:12])
