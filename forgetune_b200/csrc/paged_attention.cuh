@@ -37,7 +37,7 @@
 //   warps 18-19      Q of the next unit; tiles that some row sees in part:
 //                    values outside of the unit's keys become 0, and so do
 //                    values that are not finite (0 weights would make them
-//                    NaN); rows that do see one are marked at the end
+//                    NaN); rows that do see one get it added at the end
 //
 // Shared memory: Q of two tiles, and a ring of 128-token tiles of K or V,
 // 128-byte swizzle, in columns of 64.  Tensor memory: S and P of both halves at
@@ -296,12 +296,15 @@ __device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, uint4& c, uint4&
 }
 
 // Of 32 elements from c on of a row's output, a bit for each in which a value of
-// a tile seen in part is not finite and the row, at `position`, sees it.  Such
-// values were left out of the products.
+// a tile seen in part is +inf or -inf (NaN: both) and the row, at `position`,
+// sees it.  Such values were left out of the products.
+struct PagedMarks {
+  uint32_t plus, minus;
+};
 template <typename T>
-__device__ __forceinline__ uint32_t paged_marks(const PagedTensorParams& p, const PagedUnit& u, int position, int c) {
+__device__ __forceinline__ PagedMarks paged_marks(const PagedTensorParams& p, const PagedUnit& u, int position, int c) {
   const PagedAttentionParams& a = p.a;
-  uint32_t bits = 0;
+  PagedMarks bits{0, 0};
   const int64_t from = a.window ? (int64_t)position - a.window + 1 : 0;
   const int end = min(min(position + 1, u.hi), u.te * kPagedTile);  // within the table
 #pragma unroll 1
@@ -312,8 +315,11 @@ __device__ __forceinline__ uint32_t paged_marks(const PagedTensorParams& p, cons
     const T* x = static_cast<const T*>(a.values) + page * a.v_page + key % a.batch.page_size * a.v_token +
                  (int64_t)u.kvh * a.v_head + c;
 #pragma unroll 1
-    for (int k = 0; k < 32 && c + k < a.dim; ++k)
-      if (!isfinite(to_f32(x[k]))) bits |= 1u << k;
+    for (int k = 0; k < 32 && c + k < a.dim; ++k) {
+      const float v = to_f32(x[k]);
+      if (!(v < INFINITY)) bits.plus |= 1u << k;
+      if (!(v > -INFINITY)) bits.minus |= 1u << k;
+    }
   }
   return bits;
 }
@@ -1004,10 +1010,12 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
               for (int k = 0; k < 32; k += 2) fma2_to(v[k], v[k + 1], __uint_as_float(o[k]), __uint_as_float(o[k + 1]), f);
             }
             if (dirty && real) {
-              const uint32_t bits = paged_marks<T>(p, u, position, c);
+              const PagedMarks bits = paged_marks<T>(p, u, position, c);
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (bits & (1u << k)) v[k] = NAN;
+              for (int k = 0; k < 32; ++k) {
+                if (bits.plus & (1u << k)) v[k] += INFINITY;
+                if (bits.minus & (1u << k)) v[k] -= INFINITY;
+              }
             }
             if (u.slot >= 0) {
               if (real) {

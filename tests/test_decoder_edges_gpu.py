@@ -1,5 +1,7 @@
 """Attention over the paged cache at its edges: far tails in float16, pages outside of the pool, lengths beyond the
-table."""
+table, infinities that are seen."""
+
+import math
 
 import pytest
 import torch
@@ -121,3 +123,38 @@ def test_tokens_before_the_end_of_the_table_are_stored():
     append_heads(q, k, v, *b.args())
     page, col = b.slots(0, torch.arange(20, 32, device="cuda"))
     assert torch.equal(b.keys[page, col], k[:12]) and torch.equal(b.values[page, col], v[:12])
+
+
+# ---------------------------------------------------------------------------
+# infinities that are seen
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,dim", KINDS, ids=str)
+@pytest.mark.parametrize("new,length,window", [(1, 100, 0), (20, 400, 0), (300, 300, 0), (300, 700, 140), (1, 5000, 0)])
+def test_an_infinite_value_makes_an_infinite_output(dtype, dim, new, length, window):
+    """In tiles that all rows see and in those that some see in part; two of unlike signs, and NaN, give NaN."""
+    b = ref.Batch([new], [length], 16, 1, dim, dtype)
+    q = (0.1 * randn(new, 4, dim)).to(dtype)
+    clean = paged_attention(q, *b.args(), window=window)
+    p = torch.arange(length - new, length, device="cuda")
+    for position in {length - 1, max(0, length - new - 3), length // 2}:
+        page, col = b.slots(0, torch.tensor([position], device="cuda"))
+        kept = b.values[page, col].clone()
+        b.values[page, col, 0, 0] = math.inf
+        b.values[page, col, 0, 1] = -math.inf
+        b.values[page, col, 0, dim - 1] = math.nan
+        got = paged_attention(q, *b.args(), window=window)
+        sees = p >= position
+        if window:
+            sees &= p - window < position
+        assert torch.equal(got[~sees], clean[~sees]) and torch.equal(got[..., 2:dim - 1], clean[..., 2:dim - 1])
+        assert (got[sees][..., 0] == math.inf).all() and (got[sees][..., 1] == -math.inf).all()
+        assert got[sees][..., dim - 1].isnan().all()
+        b.values[page, col] = kept
+    if length > 1:
+        at = torch.tensor([max(0, length - new - 1), length - 1], device="cuda")
+        page, col = b.slots(0, at)
+        b.values[page, col, 0, 5] = torch.tensor([math.inf, -math.inf], device="cuda", dtype=dtype)
+        got = paged_attention(q, *b.args(), window=window)
+        first = (p >= at[0]) & (not window or p - window < at[0])
+        both = first & (p >= at[1])
+        assert (got[first & ~both][..., 5] == math.inf).all() and got[both][..., 5].isnan().all()
