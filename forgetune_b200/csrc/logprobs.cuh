@@ -91,6 +91,15 @@ struct RowSums {
   }
 };
 
+// A plain load, after grid_dep_wait: the kernel before may have written the row after this one began, which the
+// read-only loads do not allow.  (Written as a C++ load the compiler spilled 20 bytes a thread in place of 4:
+// 4096 x 131072 with 8 alternatives 249 us in place of 240.)
+__device__ __forceinline__ uint4 load_row(const uint4* p) {
+  uint4 u;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
+}
+
 template <typename T>
 struct RowVectors {
   static constexpr int W = 16 / (int)sizeof(T);
@@ -105,7 +114,7 @@ struct RowVectors {
   // Vector v; what lies outside of the row reads as -inf.
   __device__ __forceinline__ uint4 load(int v) const {
     const int e = first(v);
-    if (whole(v)) return __ldg(reinterpret_cast<const uint4*>(row + e));
+    if (whole(v)) return load_row(reinterpret_cast<const uint4*>(row + e));
     T t[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) t[i] = e + i >= 0 && e + i < n ? row[e + i] : from_f32<T>(-INFINITY);
@@ -238,7 +247,7 @@ __global__ void __launch_bounds__(kLogprobsThreads, 5) logprobs_kernel(const Log
     if (v >= whole0 && v + (U - 1) * kLogprobsThreads < whole1) {
       const uint4* from = reinterpret_cast<const uint4*>(r.row - r.off) + v;
 #pragma unroll
-      for (int i = 0; i < U; ++i) to[i] = __ldg(from + i * kLogprobsThreads);
+      for (int i = 0; i < U; ++i) to[i] = load_row(from + i * kLogprobsThreads);
       return;
     }
 #pragma unroll

@@ -39,3 +39,13 @@ def test_a_box_stored_by_rows_is_fenced_before_the_copy_engine_writes_it():
     lanes that made them, then the warp barrier before the lane that sends the load."""
     body = re.search(r"void store_box_rows\(.*?\n\}", code("fp8_pair.cuh"), re.S).group(0)
     assert re.search(r"fence_proxy_async_smem\(\);\s*__syncwarp\(\);\s*\}$", body)
+
+
+@pytest.mark.parametrize("name", ["heads.cuh", "logprobs.cuh", "paged_attention.cuh", "paged_rows.cuh", "fp8_gemm.cuh",
+                                  "fp8_pair.cuh", "fp8_rows.cuh"])
+def test_programmatic_launches_read_by_plain_loads(name):
+    """A kernel that may begin before the one in front of it is done: what that one writes is written during this one's
+    life, which the read-only loads do not allow (nor pointers marked as the only ones to their memory)."""
+    text = code(name)
+    assert "grid_dep_wait();" in text
+    assert not re.search(r"__ldg|ld\.global\.nc|__restrict__|__ldlu", text)
