@@ -79,7 +79,7 @@ __device__ __forceinline__ uint32_t conv_gather4(float4& v, const int4* ktab_s, 
     const int ih = ih0 + e.y, iw = iw0 + e.z;
     const bool in = live && k < K && ih >= 0 && ih < H && iw >= 0 && iw < W;
     const float* a = in ? xb + ((ptrdiff_t)ih0 * W + iw0 + e.x) : xb;
-    t[j] = __ldg(a);
+    t[j] = *a;  // plain: the kernel before may write it during this one's life (see grid_dep_wait)
     ok |= (in ? 1u : 0u) << j;
   }
   v = make_float4(t[0], t[1], t[2], t[3]);
