@@ -74,6 +74,11 @@ constexpr int kPagedTile = 128;      // keys of a tile, rows of a half
 constexpr int kPagedUnitOver = 256;
 constexpr int kPagedLeast = 512;     // keys (with it) that are worth a block
 constexpr float kPagedRaise = 7.0f;  // log2
+// The exponent score scale - m is one fused product, of which m is rounded: the difference of the largest score itself is
+// up to half a step of float32 at m, from 2^28 on more than float16's weights hold and from 2^31 on more than any.  Rows
+// whose m is beyond this round the product as m was, before the difference.  (A prompt of 8192 takes 617 us with it, 606
+// without, and 650 with the scale in a register that such rows set to 1; out of line on tensor memory 618 to 643.)
+__device__ __forceinline__ bool paged_far(float m) { return fabsf(m) > 16777216.0f && m != -INFINITY; }
 // float16 weights are taken relative to 2^-7 of a row's reference (sums and O alike, so that the factor cancels): up to
 // 2^15, below the largest number, and off by at most 2^-32 of the reference's where they are below the smallest normal
 // number.  Relative to the reference itself, what lay 2^-25 below it became 0 in P V and counted in the sum: of 4096 keys
@@ -858,6 +863,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       const bool real = r < u.rows, active = (alternate ? 0 : w * kPagedTile) + quarter * 32 < u.rows;
       const int tok = p.by_group.of(u.r0 + r), position = u.pos0 + tok;
       float m = -INFINITY, sum = 0.0f;
+      bool far = false;  // some row's m is far
       for (int i = 0; i < count && ok; ++i) {
         const int t = tb + (alternate ? 2 * i + w : i);
         if (!(ok = paged_wait(&s_full[w], (done + i) & 1u, abort_flag, p.err, 57))) break;
@@ -913,6 +919,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
                   sum *= keep;
                   m = high_s;
                 }
+                far = __any_sync(0xffffffffu, paged_far(m));
                 // this S followed the last P V, so O is complete; each of a row's warps has half of its columns
 #pragma unroll 1
                 for (int d = i > 0 ? side * (DH / 2) : a.dim; d < (side + 1) * (DH / 2) && d < a.dim; d += 16) {
@@ -925,6 +932,16 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
                 }
               }
               base = m == -INFINITY ? 0.0f : m - kPagedLift<T>;
+            }
+            if (far) [[unlikely]] {
+              if (paged_far(m)) {  // of this row alone: other rows' scores do not change its bits
+                const float back = __frcp_rn(a.scale);
+                base = -kPagedLift<T>;
+#pragma unroll
+                for (int k = 0; k < 32; ++k)  // (a packed product and sum were made one operation again)
+                  x[k] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[k]), a.scale), m) * back);
+              }
+              __syncwarp();
             }
             uint32_t o[16];
 #pragma unroll

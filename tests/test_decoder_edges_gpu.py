@@ -1,5 +1,5 @@
 """Attention over the paged cache at its edges: far tails in float16, pages outside of the pool, lengths beyond the
-table, infinities that are seen."""
+table, infinities that are seen, scores whose steps are large."""
 
 import math
 
@@ -158,3 +158,27 @@ def test_an_infinite_value_makes_an_infinite_output(dtype, dim, new, length, win
         first = (p >= at[0]) & (not window or p - window < at[0])
         both = first & (p >= at[1])
         assert (got[first & ~both][..., 5] == math.inf).all() and got[both][..., 5].isnan().all()
+
+
+# ---------------------------------------------------------------------------
+# scores of every size
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,dim,step", [(F16, 128, 4.0), (F16, 64, 4.0), (BF16, 128, 2.0 ** 13), (BF16, 64, 2.0 ** 40),
+                                            (F32, 64, 2.0 ** 13), (BF16, 136, 2.0 ** 13)], ids=str)
+@pytest.mark.parametrize("new,length", [(1, 100), (100, 100), (120, 120), (3, 1000)])
+@pytest.mark.parametrize("falling", [False, True])
+def test_scores_whose_steps_are_larger_than_one(dtype, dim, step, new, length, falling):
+    """Of keys so far apart each row takes the largest that it sees alone, though no float32 near the scores is exact."""
+    b = ref.Batch([new], [length], 16, 1, dim, dtype)
+    n = min(length, 120)  # the last ones; those before score 0
+    at = torch.arange(n, device="cuda")
+    page, col = b.slots(0, length - n + at)
+    base = 1250 if dtype == F16 else 128
+    b.keys[:] = 0
+    b.keys[page, col] = ((base + (n - 1 - at if falling else at)) * step).to(dtype)[:, None, None]
+    q = torch.full((new, 2, dim), base * step, dtype=dtype, device="cuda")
+    p = torch.arange(length - new, length, device="cuda")
+    page, col = b.slots(0, torch.full_like(p, length - n) if falling else p)
+    for scale, sign in ((None, 1), (-1.0, -1)):
+        got = paged_attention(sign * q, *b.args(), scale=scale)
+        assert torch.equal(got, b.values[page, col].expand(new, 2, dim))
