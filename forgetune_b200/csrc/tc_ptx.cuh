@@ -188,11 +188,6 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])                         \
       : "memory")
 
-#define FTB_TMEM_ST8(taddr, r)                                                                                  \
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),            \
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])           \
-               : "memory")
-
 // 16 columns, waited for
 #define FTB_TMEM_LD16(taddr, r)                                                                                 \
   asm volatile(                                                                                                 \

@@ -54,3 +54,9 @@ def test_programmatic_launches_read_by_plain_loads(name):
         assert constant in text
         text = text.replace(constant, "")
     assert not re.search(r"__ldg|ld\.global\.nc", text)
+
+
+def test_every_macro_is_used():
+    text = "\n".join(code(f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh", ".cpp", ".h", ".hpp")))
+    made = set(re.findall(r"#define (FTB_TMEM_\w+)", text))
+    assert made and not [m for m in made if len(re.findall(r"\b%s\b" % m, text)) < 2]
