@@ -102,7 +102,7 @@ static std::string check(const ftb_paged_batch& b) {
 }
 
 static std::string check(const ftb_rotation& r, int64_t dim) {
-  if (r.pairs < 0 || 2 * r.pairs > dim) return "more frequencies than pairs in a head";
+  if (r.pairs < 0 || r.pairs > dim / 2) return "more frequencies than pairs in a head";
   if (r.pairs > 0 && !r.frequencies) return "frequencies is null";
   if (!aligned(r.frequencies, 8)) return "frequencies is not aligned to its type";
   if (!(r.eps >= 0.0)) return "eps must not be negative";
