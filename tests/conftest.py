@@ -27,3 +27,11 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip)
+
+
+@pytest.fixture(autouse=True)
+def same_numbers_every_time():
+    """torch seeds its CPU generator anew for each process; tests that draw from it without a seed of their own get the
+    same numbers in every run."""
+    import torch
+    torch.default_generator.manual_seed(0)
