@@ -111,7 +111,8 @@ def attention(q, batch, scale=None, window=0, least=2.0 ** -25):
             out[at:at + n] = o
             tol[at:at + n] = half * o.abs() + (half + 2 * off + whole * 2.0 ** -23) * mean
             if q.dtype == torch.float16:
-                tol[at:at + n] += (whole + 1) * least * max(1.0, float(v.abs().max()))
+                # and of the result below the smallest normal number: half of float16's smallest step, 2^-25
+                tol[at:at + n] += (whole * least + 2.0 ** -25) * max(1.0, float(v.abs().max()))
         at += n
     return out, tol + 1e-30, inside
 
