@@ -17,10 +17,11 @@
 // A block takes a few tokens: it begins to load their heads, finds their
 // sequences and pages and makes their cosines, once per token for all of its
 // heads, then goes through the heads with the next ones on their way.
-// 16384 x 16 x 128 f32 with the norm: 55 us (4.9 TB/s).  12725 tokens of 32 + 8 +
-// 8 heads of 128 bf16 appended with the norm: 108 us (2.9 TB/s): 16-bit values
-// are bound by issue slots (70 % used at 122 us, about 150 warp instructions for
-// a head), which a head's 256 bytes share as 512 do of fp32.
+// In a graph of ten calls (calls in Python in brackets): 16384 x 16 x 128 f32 with
+// the norm 55 us (59; 4.9 TB/s), 12725 tokens of 32 + 8 + 8 heads of 128 bf16
+// appended with the norm 108 (108; 2.9 TB/s).  Both use two thirds of the issue
+// slots, about 140 and 130 warp instructions for a head, which a head's 256 bytes
+// in 16 bits need as 512 do in fp32.
 #pragma once
 
 #include <algorithm>
@@ -134,7 +135,8 @@ __device__ __forceinline__ void load_turns(const float2* from, float2 (&to)[V]) 
   }
 }
 
-// AHEAD heads are on their way.  Two, four blocks an SM: 55 us for the rotation above, 108 for the append; three: 58 and
+// AHEAD heads are on their way (and 28 bytes of a lane in fp32, 4 in bf16 are
+// spilled for it).  Two, four blocks an SM: 55 us for the rotation above, 108 for the append; three: 58 and
 // 106; two with five blocks 65 and 140; three with three 57 and 128; four with three 57 and 127.
 template <typename T, typename O, int V, int UPL, int AHEAD>
 __global__ void __launch_bounds__(kHeadsThreads, UPL == 1 ? 4 : 1) heads_kernel(const HeadsParams p) {
@@ -346,7 +348,9 @@ cudaError_t launch_heads_as(HeadsParams p, int sm_count, cudaStream_t s) {
 }
 
 // `vec`: every base and stride is a multiple of four elements.  Vectors also
-// need dim and r in multiples of eight.
+// need dim and r in multiples of eight.  The form without them has the room for
+// any head: 16384 x 16 x 128 bf16 off by one element takes 250 us, on a boundary
+// 52; heads of 72 with 36 turned 236.
 template <typename T, typename O>
 cudaError_t launch_heads_types(const HeadsParams& p, bool vec, int sm_count, cudaStream_t s) {
   if (!vec || p.dim % 8 || p.pairs % 4) return launch_heads_as<T, O, 1, 8, 1>(p, sm_count, s);

@@ -18,8 +18,11 @@
 // Bound by the logits' bytes, read once, and next to it by issue slots.  A block
 // takes a row; of few rows a cluster of up to eight blocks takes one, and the
 // first joins their sums and lists over distributed shared memory.
-// 4096 x 131072 bf16: 197 us (5.5 TB/s), 226 with 8 alternatives, 264 with 20;
-// 333 x 50001 f16: 12.1, and 16.8 with 20 (the ranking).  Two vectors on their
+// In a graph of ten calls: 4096 x 131072 bf16 197 us (5.5 TB/s), 226 with 8
+// alternatives (calls for longer, at the power limit, 250), 264 with 20; 333 x
+// 50001 f16 12.1, and 17 with 20 (the ranking).  Rows of which four values are
+// finite: 313 us without alternatives (0 times -inf sends every vector through the
+// second sum), 307 with 3, 16 ms with 8 (the bisection).  Two vectors on their
 // way and five blocks an SM took 268 us with 8 where four and three took 286 (two
 // and four: 292); vectors inside of the row loaded without a check each, 226.
 // 64 parts: with 256, 333 x 50001 with 20 took 34 us (17.8), by counting them.

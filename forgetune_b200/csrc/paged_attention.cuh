@@ -44,16 +44,20 @@
 // [0, 256), O at [256, 512).
 //
 // What bounds it.  Few rows: the cache's bytes; a tile of 64 KB takes an SM 1.38
-// us (47 GB/s, 7.0 TB/s over all).  Many rows: a pair of tiles takes 2.16 us, of
-// which the tensor cores are busy 44 % and the exponentials' unit 44 % (prompt of
+// us (47 GB/s, 7.0 TB/s over all).  Many rows: a pair of tiles takes 2.20 us, of
+// which the tensor cores are busy 42 % and the exponentials' unit 42 % (prompt of
 // 4096); neither is full because a half's next S waits for its P V, since P lies
 // over S.  Tiles of 80 keys leave room for S beside P, and S and P V then had
 // threads of their own; but an N = 80 product takes about 97 cycles (N = 128: 82), and
 // 128 keys took 2.5 us.  A row's scores in one thread had spilled registers, for
 // which 227 KB of shared memory leave little L1: 262 us for a prompt of 4096 where
-// two threads a row took 218 (167 now).  A unit costs 4 to 5.5 us beside its
-// tiles: Q, the first tile, the last P V and O (1480 sequences against 296: 7.6 us
-// for each further unit of 256 rows and one tile, 5.5 for one of a single token).
+// two threads a row took 218 (171 now).  A unit costs 4 to 4.5 us beside its
+// tiles: Q, the first tile, the last P V and O (1480 units against 296: 6.7 us for
+// each further unit of 256 rows and one tile, 5.4 for one of a single token).  A
+// group that does not divide 128 has its Q by 16-byte copies, which the two warps
+// wait for: 14 heads take 73 us where 16, with more work, take 61 (chunks of up to
+// 1000 tokens, heads of 80).  Times of a graph of ten calls; calls for longer run
+// at the power limit (a prompt of 8192 617 to 634 us, in a graph 561).
 #pragma once
 
 #include <algorithm>
@@ -877,7 +881,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           // keeps do not fit its registers, and what is spilled goes to L2.  P of 32 goes over the first 16 columns
           // of the scores, when both are done with.
           float high_s = -INFINITY, base = 0.0f, part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll  // rolled up: 578 us for a prompt of 8192 in place of 545
+#pragma unroll  // rolled up: 578 us for a prompt of 8192 where it took 545
           for (int pass = 0; pass < 3; ++pass) {
             const int c = (pass & 1) ^ 1;
             uint32_t x[32];

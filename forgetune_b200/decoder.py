@@ -60,7 +60,8 @@ def rope_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] = N
     ``scaling`` changes them for contexts ``scale`` times as long as the ``original`` one a model was trained on:
     ``"linear"`` divides all by ``scale``; ``"base"`` raises the base so that the slowest is divided by it and the
     fastest is kept; ``"parts"`` keeps those that turn at least ``fast`` times in the original context, divides those
-    that turn at most ``slow`` times, and goes over between them in proportion to their turns.
+    that turn at most ``slow`` times, and goes over between them in proportion to their turns.  Frequencies of any
+    other rule are a tensor of the caller's.
     """
     if dim < 2 or dim % 2:
         raise ValueError("rope_frequencies: dim must be even and positive")

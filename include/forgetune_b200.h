@@ -392,9 +392,10 @@ FORGETUNE_EXPORT int ftb_append_heads(const ftb_append_args* args, void* stream)
 /* out[t, h] = sum_j softmax_j(scale q[t, h] . key_j) value_j over the tokens j of t's sequence up to t's own
  * position, and with window > 0 the last `window` of them only; head h reads kv head h / (heads / kv_heads).  A
  * token at a negative position sees nothing and gets zeros.  Keys and values that a token does not see do not
- * change its output, whatever they hold; an infinite value makes its element of the outputs that see it infinite (with
- * one of the other sign NaN), a NaN makes it NaN.  Outputs that see a token whose page number is outside the pool, and those of tokens at positions
- * beyond the table, are NaN; the others are what they would be without it, and nothing outside is read.  q, out and the cache have one type.
+ * change its output, whatever they hold; an infinite value makes its element of the outputs that see it infinite
+ * (with one of the other sign NaN), a NaN makes it NaN.  Outputs that see a token whose page number is outside the
+ * pool, and those of tokens at positions beyond the table, are NaN; the others are what they would be without it, and
+ * nothing outside is read.  q, out and the cache have one type.
  *
  * `workspace` holds ftb_paged_attention_workspace(args) bytes on 16-byte boundaries (0: may be null), which no
  * other call may use until this one's kernels are done; its contents do not matter. */
